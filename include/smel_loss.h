@@ -1,5 +1,5 @@
-/* C-ABI of the single-pass chunked cross-entropy (libsmel_moe.so, HIP for gfx950): both GEMMs of every
- * (token pass, vocabulary chunk) step on MFMA, the online softmax in the logits GEMM's epilogue, no [tokens, vocab]
+/* C-ABI of the losses (libsmel_moe.so, HIP for gfx950): the single-pass chunked cross-entropy, and the router's balance
+ * loss (at the end). The cross-entropy: both GEMMs of every (token pass, vocabulary chunk) step on MFMA, the online softmax in the logits GEMM's epilogue, no [tokens, vocab]
  * logits in memory. Replaces _ce_chunk / _ChunkedCE of smel/loss.py:50-146.
  *
  * Same conventions as smel_moe.h. `dtype` is that of the token rows h, the head rows and the softmax terms: 0 bf16,
@@ -93,6 +93,29 @@ int smel_ce_transpose(const void* src, int64_t R, int64_t C, int64_t lds, void* 
  * smel_ce_grad in one pass. */
 int smel_ce_dequant8(const int8_t* q, const void* scale, int64_t R, int64_t C, int32_t dtype, void* rows, void* wt,
                      int64_t ldt, hipStream_t stream);
+
+/* The router's balance loss. A sequence s holds the tokens [offsets[s], offsets[s + 1]) (offsets null: one sequence of all T
+ * tokens; int64 or int32 by off_i64, ascending; values outside [0, T] are clamped to it), of which those with mask[t] != 0
+ * count (mask null: all). With n_s such tokens, c[s][e] of their K picks topi[t][k] = e (ids outside [0, E) count nowhere),
+ * p = softmax of the logits' row, S' the sequences with n_s > 0:
+ *   loss = coef / S' * sum_s E sum_e c[s][e] / (K n_s) * mean_t p[t][e]
+ * (0 without any token). Rows that do not count are not read.
+ * `dtype` of the logits [T][ldl]: 0 bf16, 1 fp32, 2 fp16; topi [T][K] contiguous, int64 or int32 by topi_i64.
+ * 0 <= T <= 2^25, 1 <= E <= 512, 1 <= K <= 64, 1 <= S <= 2^24.
+ * Writes loss (fp32), counts (int64 [S][E]) and, for the backward, row_stats (fp32 [T][2]: a counted row's maximum and
+ * 1 / its sum of exponentials; may be null without one) and weights (fp32 [S][E] and one more: coef E / (K n_s^2) (c[s][e] - sum_e c[s][e] / E), then
+ * 1 / S'). ws: smel_balance_ws_bytes bytes, 16-byte aligned. */
+int64_t smel_balance_ws_bytes(int64_t T, int64_t E, int64_t S);
+int smel_balance_fwd(const void* logits, int64_t ldl, int32_t dtype, const void* topi, int32_t topi_i64, int64_t T,
+                     int64_t E, int64_t K, const uint8_t* mask, const void* offsets, int32_t off_i64, int64_t S,
+                     float coef, float* loss, int64_t* counts, float* row_stats, float* weights, void* ws,
+                     int64_t ws_bytes, hipStream_t stream);
+
+/* dlogits [T][E] contiguous, in the logits' dtype: go / S' p[t][e] (v[e] - sum_j p[t][j] v[j]) with v = weights of the token's
+ * sequence (the counts are constants); zero rows for tokens that do not count. go: one fp32 on the device. */
+int smel_balance_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, const uint8_t* mask,
+                     const void* offsets, int32_t off_i64, int64_t S, const float* row_stats, const float* weights,
+                     const float* go, void* dlogits, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,11 +1,12 @@
-"""ctypes binding of libsmel_moe.so (the C-ABI declared in include/smel_moe.h, smel_f32.h, smel_norm.h, smel_stream.h and
-smel_loss.h).
+"""ctypes binding of libsmel_moe.so (the C-ABI declared in include/smel_moe.h, smel_f32.h, smel_norm.h, smel_stream.h,
+smel_loss.h and smel_ortho.h).
 
 The library is the only compute path: if it is missing, or no GPU is visible, calls raise instead of falling back to
 anything else. Tensors go in as raw device pointers; every call runs on torch's current HIP stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -24,9 +25,9 @@ WSET_MERGE_SHORT = 8 # smel_wset.flags: gate_up forward, a full int4 tile also t
 WSET_MERGED_LIST = 16 # smel_wset.flags: gate_up forward on smel_dispatch's merged tile list (int4 tiles up to 160 rows)
 WSET_TILE32 = 32     # smel_wset.flags: a tile list of at most 32 rows a tile
 WSET_COL_CHUNK = 64  # smel_wset.flags: column blocks, not tiles, are spread over the XCDs
-ABI_VERSION = 24
+ABI_VERSION = 25
 
-vp, i64, i32, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
+vp, i64, i32, f32, f64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_double
 
 
 class WSet(ctypes.Structure):
@@ -146,6 +147,9 @@ SIGNATURES = {
     "smel_add_rmsnorm_fwd": (i32, [vp, vp, i64, i64, vp, i32, f32, i32, vp, vp, vp, vp]),
     "smel_gated_rmsnorm_fwd": (i32, [vp, vp, i64, i64, vp, f32, i32, vp, vp, vp]),
     "smel_gated_rmsnorm_bwd": (i32, [vp, vp, vp, i64, i64, vp, vp, i32, vp, vp, vp]),
+    "smel_layernorm_fwd": (i32, [vp, vp, i64, i64, i64, vp, vp, f32, i32, i32, vp, vp, vp, vp]),
+    "smel_layernorm_bwd_ws_floats": (i64, [i64, i64]),
+    "smel_layernorm_bwd": (i32, [vp, vp, i64, i64, i64, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64, vp]),
     # include/smel_stream.h
     "smel_event_create": (i32, [ctypes.POINTER(vp)]),
     "smel_event_destroy": (i32, [vp]),
@@ -166,6 +170,12 @@ SIGNATURES = {
     "smel_ce_loss_sum": (i32, [vp, i64, f32, i32, vp, vp]),
     "smel_ce_scale": (i32, [vp, i64, i32, vp, vp]),
     "smel_ce_transpose": (i32, [vp, i64, i64, i64, vp, i64, i32, vp]),
+    "smel_balance_ws_bytes": (i64, [i64, i64, i64]),
+    "smel_balance_fwd": (i32, [vp, i64, i32, vp, i32, i64, i64, i64, vp, vp, i32, i64, f32, vp, vp, vp, vp, vp, i64, vp]),
+    "smel_balance_bwd": (i32, [vp, i64, i32, i64, i64, vp, vp, i32, i64, vp, vp, vp, vp, vp]),
+    # include/smel_ortho.h
+    "smel_orthogonalize_ws": (i64, [vp, i32]),
+    "smel_orthogonalize": (i32, [vp, i32, i32, f64, f64, f64, f64, vp, i64, vp]),
     # include/smel_probe.h
     "smel_probe_mfma": (i32, [vp, i32, i32, vp]),
     "smel_probe_read": (i32, [vp, i64, vp, i32, vp]),
@@ -300,3 +310,22 @@ def require_device(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError("smel MoE kernels run on the GPU: every tensor must be on a cuda device")
+
+
+def one_device(first: torch.Tensor, *others):
+    """Every tensor on first's GPU, or ValueError."""
+    if not first.is_cuda:
+        raise ValueError("smel kernels run on the GPU: every tensor must be on a cuda device")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors of one call on {first.device} and {t.device}")
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """``with on_device_of(t):`` launches and allocates on t's GPU and its current stream."""
+    if _device is not None and t.device.index == _device():
+        return _HERE
+    return torch.cuda.device(t.device)

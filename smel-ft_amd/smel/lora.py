@@ -4,17 +4,21 @@ B_up, A_down, B_down in that order, fp32, A [.., r, in] uniform in +-1/sqrt(in) 
 B [.., out, r] zero), so adapters written by either load into the other.
 
 The MoE layer never multiplies these factors in Python: smel.moe lays them out as a 32-wide K-extension of the
-grouped-GEMM kernels. ``lora_linear`` / ``lora_gate_up`` are the dense helpers of the API (torch ops).
+grouped-GEMM kernels. ``lora_linear`` / ``lora_gate_up`` are the dense helpers of the API (torch ops);
+``orthogonalize`` makes the factors' updates orthogonal on the GPU (include/smel_ortho.h).
 """
 from __future__ import annotations
 
 import json
 import math
 import os
+from array import array
 
 import torch
 import torch.nn.functional as F
 from torch import nn
+
+from . import _lib
 
 _PROJ = ("gate", "up", "down")
 
@@ -106,6 +110,71 @@ def lora_gate_up(x, w_gate_up, A_gate, B_gate, A_up, B_up, scale):
         xa = x2 @ torch.cat((A_gate, A_up)).to(x.dtype).t()
         g, u = _add_low_rank(g, xa[:, :r], B_gate, scale), _add_low_rank(u, xa[:, r:], B_up, scale)
     return g.reshape(*lead, I), u.reshape(*lead, I)
+
+
+# ------------------------------------------------------------------------------------------------ updates
+
+_ORTHO_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+ORTHO_MAX_RANK = 128   # of the shorter side
+
+
+def _ortho_operand(t: torch.Tensor):
+    """t [..., m, n] as [batch, m, n] with unit stride along one side: a view where there is one, else a copy."""
+    if t.dim() > 3:
+        try:
+            t = t.view(-1, *t.shape[-2:])
+        except RuntimeError:
+            t = t.reshape(-1, *t.shape[-2:]).contiguous()
+    elif t.dim() == 2:
+        t = t.unsqueeze(0)
+    _, m, n = t.shape
+    if not (n == 1 or t.stride(2) == 1 or m == 1 or t.stride(1) == 1):
+        t = t.contiguous()
+    return t
+
+
+def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
+    """Orthogonalised updates by Newton-Schulz products, as the Muon optimiser makes them of its momentum: for every matrix
+    G of the last two dimensions, X = G / (|G|_F + eps), then ``steps`` times
+
+        X <- a X + b (X X^T) X + c (X X^T)^2 X
+
+    which moves every singular value towards 1 and keeps the singular vectors. ``update``: a tensor [..., m, n] (bf16,
+    fp16, fp32; a factor's gradient or momentum) or a sequence of them, e.g. every factor's of a block, which go through
+    few launches together; the shorter side (a LoRA's rank) is at most 128. Returns the same shapes and dtypes,
+    contiguous, without gradients. The products run on the rank's r x r matrices in 64 bits, so small singular values keep
+    their directions (include/smel_ortho.h)."""
+    single = isinstance(update, torch.Tensor)
+    ts = [update] if single else list(update)
+    a, b, c = (float(v) for v in coeffs)
+    if not 0 <= int(steps) <= 64:
+        raise ValueError(f"orthogonalize takes 0 to 64 steps, got {steps}")
+    if not eps >= 0:
+        raise ValueError(f"orthogonalize: eps must not be negative, got {eps}")
+    if not ts:
+        return []
+    _lib.one_device(ts[0], *ts[1:])
+    jobs, outs, keep = array("q"), [], []
+    with torch.no_grad(), _lib.on_device_of(ts[0]):
+        for t in ts:
+            if t.dtype not in _ORTHO_DTYPES or t.dim() < 2:
+                raise ValueError(f"orthogonalize takes bf16, fp16 or fp32 matrices, got {tuple(t.shape)} {t.dtype}")
+            if min(t.shape[-2:]) > ORTHO_MAX_RANK:
+                raise ValueError(f"orthogonalize takes matrices whose shorter side is at most {ORTHO_MAX_RANK}, got "
+                                 f"{tuple(t.shape)}")
+            y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            outs.append(y)
+            if t.numel() == 0:
+                continue
+            x = _ortho_operand(t)
+            keep.append(x)
+            jobs.extend((x.data_ptr(), y.data_ptr(), *x.shape, *x.stride(), _ORTHO_DTYPES[t.dtype]))
+        lib = _lib.load()
+        addr, n = jobs.buffer_info()[0], len(keep)
+        need = lib.smel_orthogonalize_ws(addr, n)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=ts[0].device)
+        _lib.call("smel_orthogonalize", addr, n, int(steps), a, b, c, float(eps), _lib.ptr(ws), need, _lib.stream())
+    return outs[0] if single else outs
 
 
 class LayerLoRA(nn.Module):

@@ -25,6 +25,7 @@ The gradient is computed in the forward (lm_head is frozen) and handed back by t
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .quant import dequant_int8_rows, quantize_int8_rows
@@ -377,3 +378,113 @@ def chunked_ce(h, head: LMHead, tgt, denom: float, token_chunk: int = TOKEN_CHUN
     grad = need_grad and h.requires_grad
     with torch.set_grad_enabled(grad and torch.is_grad_enabled()):
         return _ChunkedCE.apply(h, head, tgt, float(denom), rows, max_rows, grad)
+
+
+# ------------------------------------------------------------------------------------------------ the router's balance
+
+
+def _balance_check(logits, topi, mask, offsets):
+    L.one_device(logits, topi, mask, offsets)
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError(f"balance_loss takes bf16, fp16 or fp32 logits [T, E], got {tuple(logits.shape)} {logits.dtype}")
+    if topi.dim() != 2 or topi.shape[0] != logits.shape[0] or topi.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"balance_loss takes int64 or int32 picks [T, K] of the logits' {logits.shape[0]} tokens, got "
+                         f"{tuple(topi.shape)} {topi.dtype}")
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (logits.shape[0],)):
+        raise ValueError(f"balance_loss takes a bool mask [{logits.shape[0]}], got {tuple(mask.shape)} {mask.dtype}")
+    if offsets is not None and (offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int64, torch.int32)):
+        raise ValueError(f"balance_loss takes int64 or int32 offsets [S + 1], got {tuple(offsets.shape)} {offsets.dtype}")
+
+
+class _Balance:
+    """One call's operands, and the launches."""
+
+    __slots__ = ("z", "T", "E", "ldl", "mask", "off", "S", "keep", "stats", "weights")
+
+    def __init__(self, logits, mask, offsets):
+        T, E = logits.shape
+        if logits.stride(1) != 1 and E > 1 or T > 1 and logits.stride(0) < E:
+            logits = logits.contiguous()
+        self.z, self.T, self.E = logits, T, E
+        self.ldl = logits.stride(0) if T > 1 else E
+        self.mask = mask.contiguous() if mask is not None else None
+        self.off = offsets.contiguous() if offsets is not None else None
+        self.S = 1 if offsets is None else offsets.numel() - 1
+
+    def _common(self):
+        p = L.ptr
+        return p(self.mask), p(self.off), int(self.off is not None and self.off.dtype == torch.int64), self.S
+
+    def forward(self, topi, coef: float, need_grad: bool):
+        dev, T, E, S = self.z.device, self.T, self.E, self.S
+        topi = topi.contiguous()
+        mem = L.Carve()     # kept for the backward
+        self.weights = mem.take(4 * (S * E + 1))
+        self.stats = mem.take(8 * T) if need_grad else None
+        self.keep = mem
+        ws_n = L.load().smel_balance_ws_bytes(T, E, S)
+        tmp = L.Carve()
+        ws = (tmp if need_grad else mem).take(ws_n)
+        mem.alloc(dev)
+        if need_grad:
+            tmp.alloc(dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty((E,) if self.off is None else (S, E), dtype=torch.int64, device=dev)
+        p = L.ptr
+        L.call("smel_balance_fwd", p(self.z), self.ldl, _DT[self.z.dtype], p(topi), int(topi.dtype == torch.int64), T, E,
+               topi.shape[1], *self._common(), float(coef), p(loss), p(counts), p(self.stats), p(self.weights), p(ws), ws_n,
+               L.stream())
+        return loss, counts
+
+    def backward(self, go):
+        dz = torch.empty(self.T, self.E, dtype=self.z.dtype, device=self.z.device)
+        go = go.to(device=self.z.device, dtype=torch.float32).contiguous()
+        p = L.ptr
+        L.call("smel_balance_bwd", p(self.z), self.ldl, _DT[self.z.dtype], self.T, self.E, *self._common(), p(self.stats),
+               p(self.weights), p(go), p(dz), L.stream())
+        return dz
+
+
+class _BalanceFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topi, mask, offsets, coef):
+        b = _Balance(logits, mask, offsets)
+        with L.on_device_of(logits):
+            loss, counts = b.forward(topi, coef, True)
+        ctx.save_for_backward(b.z, b.mask, b.off)     # autograd reports a change in place
+        ctx.b = b
+        b.z = b.mask = b.off = None
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go, _):
+        if go is None:
+            return None, None, None, None, None
+        b = ctx.b
+        b.z, b.mask, b.off = ctx.saved_tensors
+        dz = b.backward(go)
+        b.z = b.mask = b.off = None
+        return dz, None, None, None, None
+
+
+def balance_loss(logits, topi, mask=None, offsets=None, coef: float = 1.0):
+    """Balance loss of a router and its picks per expert: (loss fp32, counts int64 [E], or [S, E] with ``offsets``).
+
+    logits [T, E] (bf16, fp16, fp32; ``smel.moe.route(..., with_logits=True)`` gives them), topi [T, K] the picked experts.
+    Over the n tokens that count, with c_e picks of expert e and P_e the mean of softmax(logits)_e:
+
+        loss = coef E sum_e c_e / (K n) P_e                    (coef for an even router)
+
+    ``mask`` [T] bool: the tokens that count (rows of others are not read: they may hold anything). ``offsets`` [S + 1]
+    (ascending, on the GPU): sequence s is the tokens offsets[s] to offsets[s + 1]; the loss is the mean of the losses of
+    the sequences that have tokens, and tokens outside all of them count nowhere. Without any token the loss is 0. Picks
+    outside [0, E) count nowhere. The gradient goes to the logits (zero rows where a token does not count); the counts
+    are constants to it."""
+    _balance_check(logits, topi, mask, offsets)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _BalanceFn.apply(logits, topi, mask, offsets, float(coef))
+    with L.on_device_of(logits):
+        return _Balance(logits, mask, offsets).forward(topi, coef, False)

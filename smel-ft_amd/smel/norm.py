@@ -1,12 +1,15 @@
-"""RMSNorm family of the frozen layers around the MoE block, on the HIP kernels of libsmel_moe.so
-(include/smel_norm.h): one launch forward, one backward.
+"""RMSNorm family of the frozen layers around the MoE block, and layer norm with trained weights, on the HIP kernels of
+libsmel_moe.so (include/smel_norm.h): one launch forward, one backward (layer norm: two, the second adds up the weights'
+gradients).
 
   rmsnorm(x, w, eps, plus_one)          y = x * rstd * (1 + w) (Qwen3.5/3.6), x * rstd * w (Gemma 4), x * rstd (w None)
   add_rmsnorm(h, x, w, eps, plus_one)   s = h + x (the residual add), y = rmsnorm(s)
   gated_rmsnorm(x, z, w, eps)           y = w * norm(x) * silu(z)  (output norm of Gated DeltaNet)
+  layernorm(x, w, b, eps)               y = (x - mean) * rstd * w + b
+  add_layernorm(h, x, w, b, eps)        s = h + x, y = layernorm(s)
 
-The API is the reference's smel/norm.py:252-275 (``supported``, ``ENABLED``, ``MAX_COLS`` and the three functions,
-same arguments and return values). The norm weights are frozen, so backward gives dx (and dz) only, as there.
+Of the RMSNorm functions the API is the reference's smel/norm.py:252-275 (``supported``, ``ENABLED``, ``MAX_COLS`` and the three functions,
+same arguments and return values). Their weights are frozen, so backward gives dx (and dz) only, as there.
 fp32 math with the reference's rounding points (the residual sum rounded to the stream's dtype, the gated norm's
 ``n`` and ``w n`` rounded); saved for backward: the rows the norm read and one fp32 rstd per row:
 
@@ -20,6 +23,7 @@ columns), so a caller that routes other cases to its own torch code keeps doing 
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -161,3 +165,107 @@ def add_rmsnorm(h, x, w, eps, plus_one):
 
 def gated_rmsnorm(x, z, w, eps):
     return _NormFn.apply(_GATED, eps, 1, w, x, z)
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+
+_LN_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _ln_check(x, h, w, b):
+    _lib.one_device(x, h, w, b)
+    if x.dtype not in _LN_DTYPES:
+        raise ValueError(f"layer norm takes bf16, fp16 or fp32 rows, got {x.dtype}")
+    if x.dim() == 0 or not 1 <= x.shape[-1] <= MAX_COLS:
+        raise ValueError(f"layer norm takes rows of 1 to {MAX_COLS} columns, got shape {tuple(x.shape)}")
+    if h is not None and (h.shape != x.shape or h.dtype != x.dtype):
+        raise ValueError(f"the two addends differ: {tuple(h.shape)} {h.dtype} and {tuple(x.shape)} {x.dtype}")
+    for t in (w, b):
+        if t is not None and (t.dtype not in (x.dtype, torch.float32) or tuple(t.shape) != (x.shape[-1],)
+                              or not t.is_contiguous()):
+            raise ValueError(f"layer norm weights must be contiguous [{x.shape[-1]}] tensors of {x.dtype} or float32")
+    if w is not None and b is not None and w.dtype != b.dtype:
+        raise ValueError(f"layer norm's weight is {w.dtype} and its bias {b.dtype}")
+
+
+def _ln_wtype(x, w, b) -> int:
+    t = w if w is not None else b
+    return _LN_DTYPES[x.dtype if t is None else t.dtype]
+
+
+def _ln_forward(x, h, w, b, eps):
+    """(rows the norm read, their pitch, s or None, y, stats)."""
+    if h is None:
+        x2, pitch = _row_layout(x)
+        h2 = s = None
+    else:
+        x2, h2 = _packed(x), _packed(h)
+        pitch = x2.shape[1]
+        s = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    R, n = x2.shape
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    stats = torch.empty(R, 2, device=x.device, dtype=torch.float32)
+    p = _lib.ptr
+    _lib.call("smel_layernorm_fwd", p(x2), p(h2), R, n, pitch, p(w), p(b), float(eps), _LN_DTYPES[x.dtype],
+              _ln_wtype(x, w, b), p(s), p(y), p(stats), _lib.stream())
+    return (x2 if h is None else s), pitch, s, y, stats
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """forward(x, h, w, b, eps): y, or (s, y) with the residual addend h. Saved: the rows that the norm read and two fp32
+    numbers a row."""
+
+    @staticmethod
+    def forward(ctx, x, h, w, b, eps):
+        with _lib.on_device_of(x):
+            rows, ctx.pitch, s, y, stats = _ln_forward(x, h, w, b, eps)
+        ctx.save_for_backward(rows, w, stats)
+        ctx.add, ctx.wtype, ctx.like_b = h is not None, _ln_wtype(x, w, b), b is not None
+        ctx.set_materialize_grads(False)
+        return y if h is None else (s, y)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        ds, dy = grads if ctx.add else (None, grads[0])
+        if dy is None:      # the sum alone was used (or nothing)
+            return ds, ds if ctx.add else None, None, None, None
+        rows, w, stats = ctx.saved_tensors
+        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        want_w, want_b = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        n = rows.shape[-1]
+        R = stats.shape[0]
+        dev, p = rows.device, _lib.ptr
+        dy2 = _packed(dy)
+        ds2 = _packed(ds) if ds is not None and want_x else None
+        dx = torch.empty(dy.shape, device=dev, dtype=rows.dtype) if want_x else None
+        wdt = torch.float32 if ctx.wtype == 2 else rows.dtype
+        dw = torch.empty(n, device=dev, dtype=wdt) if want_w else None
+        db = torch.empty(n, device=dev, dtype=wdt) if want_b else None
+        ws, ws_n = None, 0
+        if want_w or want_b:
+            ws_n = _lib.load().smel_layernorm_bwd_ws_floats(R, n)
+            ws = torch.empty(max(ws_n, 1), device=dev, dtype=torch.float32)
+        _lib.call("smel_layernorm_bwd", p(dy2), p(rows), R, n, ctx.pitch, p(w), p(stats), p(ds2),
+                  _LN_DTYPES[rows.dtype], ctx.wtype, p(dx), p(dw), p(db), p(ws), ws_n, _lib.stream())
+        return dx, dx if ctx.add else None, dw, db, None
+
+
+def _ln(x, h, w, b, eps):
+    _ln_check(x, h, w, b)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, h, w, b)):
+        return _LayerNormFn.apply(x, h, w, b, eps)
+    with _lib.on_device_of(x):
+        _, _, s, y, _ = _ln_forward(x, h, w, b, eps)
+    return y if h is None else (s, y)
+
+
+def layernorm(x, w, b, eps):
+    """(x - mean) rstd w + b over the last dimension: bf16, fp16 or fp32 rows of any stride; w and b (either may be None: 1
+    and 0) of the rows' dtype or fp32, trained: backward gives dx, dw and db. fp32 math, one rounding."""
+    return _ln(x, None, w, b, eps)
+
+
+def add_layernorm(h, x, w, b, eps):
+    """(h + x, layernorm(h + x)): the residual add, rounded to the stream's dtype, and the norm after it."""
+    return _ln(x, h, w, b, eps)
