@@ -669,10 +669,11 @@ def _bank_sources(fz):
 
 
 class _RouteFn(torch.autograd.Function):
-    """route (smel/moe.py:162-167) with topv differentiable w.r.t. x through the router softmax."""
+    """route (smel/moe.py:162-167) with topv differentiable w.r.t. x through the router softmax; with_logits: the rounded
+    logits as a fourth result, differentiable too (their gradient joins topv's before the router GEMM's backward)."""
 
     @staticmethod
-    def forward(ctx, x, gate_w, top_k):
+    def forward(ctx, x, gate_w, top_k, with_logits=False):
         T, H = x.shape
         E = gate_w.shape[0]
         dev = x.device
@@ -685,24 +686,30 @@ class _RouteFn(torch.autograd.Function):
                L.ptr(topi), L.ptr(topi32), None, L.ptr(lg), L.stream())
         ctx.save_for_backward(probs, topi32, gate_w)
         ctx.mark_non_differentiable(probs, topi)
-        return probs, topv, topi
+        ctx.set_materialize_grads(not with_logits)   # either gradient may be missing then
+        return (probs, topv, topi, lg[:, :E]) if with_logits else (probs, topv, topi)
 
     @staticmethod
-    def backward(ctx, dprobs, dtopv, dtopi):
+    def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
         probs, topi32, gate_w = ctx.saved_tensors
         T, E = probs.shape
         K = topi32.shape[1]
         dev = probs.device
-        if dtopv is None:
-            return None, None, None
-        dwp = dtopv.float().contiguous().reshape(-1, 1)
+        if dtopv is None and dlogits is None:
+            return None, None, None, None
         wr = _router_ext_weight(gate_w, None)
         Epad = wr.R
-        dl = torch.empty(T, Epad, dtype=torch.bfloat16, device=dev)
-        L.call("smel_route_bwd", L.ptr(dwp), 1, None, L.ptr(probs), L.ptr(topi32), None, None, 0, T, K, E, T * K,
-               L.ptr(dl), Epad, None, None, L.stream())
+        if dtopv is None:
+            dl = torch.zeros(T, Epad, dtype=torch.bfloat16, device=dev)
+        else:
+            dwp = dtopv.float().contiguous().reshape(-1, 1)
+            dl = torch.empty(T, Epad, dtype=torch.bfloat16, device=dev)
+            L.call("smel_route_bwd", L.ptr(dwp), 1, None, L.ptr(probs), L.ptr(topi32), None, None, 0, T, K, E, T * K,
+                   L.ptr(dl), Epad, None, None, L.stream())
+        if dlogits is not None:
+            dl[:, :E] += dlogits
         dx = _router_dx(dl, wr, T, dev, L.stream())
-        return dx, None, None
+        return dx, None, None, None
 
 
 def _router_dx(dl, wr: PackedW, T: int, dev, st, dx=None):
@@ -719,16 +726,17 @@ def _router_dx(dl, wr: PackedW, T: int, dev, st, dx=None):
     return dx
 
 
-def route(x2d, gate_w, top_k):
+def route(x2d, gate_w, top_k, with_logits=False):
     """smel/moe.py:162-167 -> (probs fp32 [T,E], topv [T,K] renormalised in the logits' dtype, topi int64 [T,K]).
-    bf16 or fp32 activations (the fp32 path: every product an fp32 MFMA)."""
+    bf16 or fp32 activations (the fp32 path: every product an fp32 MFMA). with_logits: (..., logits [T,E] in the
+    activations' dtype), differentiable w.r.t. x2d, for losses on the router (``smel.loss.balance_loss``)."""
     L.require_device(x2d, gate_w)
     if x2d.dtype == torch.float32:
-        return F32.RouteFn.apply(F32.f32(x2d), F32.f32(gate_w, "gate_w"), int(top_k))
+        return F32.RouteFn.apply(F32.f32(x2d), F32.f32(gate_w, "gate_w"), int(top_k), bool(with_logits))
     if _bf16_limit(x2d.shape[-1]) is not None:
-        probs, topv, topi = F32.RouteFn.apply(x2d.float(), _f32_of(_bf16(gate_w)), int(top_k))
-        return probs, topv.to(x2d.dtype), topi
-    return _RouteFn.apply(_bf16(x2d), _bf16(gate_w), int(top_k))
+        probs, topv, topi, *lg = F32.RouteFn.apply(x2d.float(), _f32_of(_bf16(gate_w)), int(top_k), bool(with_logits))
+        return (probs, topv.to(x2d.dtype), topi, *(t.to(x2d.dtype) for t in lg))
+    return _RouteFn.apply(_bf16(x2d), _bf16(gate_w), int(top_k), bool(with_logits))
 
 
 class _RouteGemma4Fn(torch.autograd.Function):

@@ -240,10 +240,10 @@ def mlp_core_bwd(sv: _Saved, dy, tl, I: int, w_gu, w_dn, gu_split, lora_w, s: fl
 
 class RouteFn(torch.autograd.Function):
     """route (smel/moe.py:162-167) on fp32 tensors: logits = x W_r^T (fp32 MFMA), softmax, top-k, renorm; topv fp32
-    (the logits' dtype), differentiable w.r.t. x."""
+    (the logits' dtype), differentiable w.r.t. x; with_logits: the logits as a fourth result, differentiable too."""
 
     @staticmethod
-    def forward(ctx, x, gate_w, top_k):
+    def forward(ctx, x, gate_w, top_k, with_logits=False):
         T, H = x.shape
         E = gate_w.shape[0]
         dev = x.device
@@ -258,24 +258,30 @@ class RouteFn(torch.autograd.Function):
                L.ptr(topi32), L.stream(), tag="route_f32")
         ctx.save_for_backward(probs, topi32, gate_w)
         ctx.mark_non_differentiable(probs, topi)
-        return probs, topv, topi
+        ctx.set_materialize_grads(not with_logits)   # either gradient may be missing then
+        return (probs, topv, topi, logits) if with_logits else (probs, topv, topi)
 
     @staticmethod
-    def backward(ctx, dprobs, dtopv, dtopi):
-        if dtopv is None:
-            return None, None, None
+    def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
+        if dtopv is None and dlogits is None:
+            return None, None, None, None
         probs, topi32, gate_w = ctx.saved_tensors
-        return _router_bwd(dtopv, probs, topi32, gate_w, None), None, None
+        return _router_bwd(dtopv, probs, topi32, gate_w, None, dlogits), None, None, None
 
 
-def _router_bwd(dtopv, probs, topi32, w, pes):
+def _router_bwd(dtopv, probs, topi32, w, pes, dlogits=None):
     T, E = probs.shape
     K = topi32.shape[1]
     dev = probs.device
-    dl = torch.empty(T, E, dtype=torch.float32, device=dev)
-    dtv = dtopv.float().contiguous()
-    L.call("smel_route_bwd_f32", L.ptr(dtv), L.ptr(probs), L.ptr(topi32), L.ptr(pes), T, K, E, L.ptr(dl), L.stream(),
-           tag="route_f32_bwd")
+    if dtopv is None:
+        dl = dlogits.contiguous()
+    else:
+        dl = torch.empty(T, E, dtype=torch.float32, device=dev)
+        dtv = dtopv.float().contiguous()
+        L.call("smel_route_bwd_f32", L.ptr(dtv), L.ptr(probs), L.ptr(topi32), L.ptr(pes), T, K, E, L.ptr(dl), L.stream(),
+               tag="route_f32_bwd")
+        if dlogits is not None:
+            dl += dlogits
     tl, _, _ = dense_tiles(T, dev)
     dx = torch.empty(T, w.shape[1], dtype=torch.float32, device=dev)
     gmm(_dense(w), 1, tl, dl, E, dx, w.shape[1], tag="route_f32_bwd")
