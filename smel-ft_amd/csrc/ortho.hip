@@ -13,9 +13,13 @@
 // the operand B at step m of a 16-long contraction, and of the operand A of a symmetric matrix: results are the next
 // product's operands as they are.
 //
-// Kernels: gram (a block per slice of columns: the slice's part of A0's upper tiles), iterate (a block per matrix: sums
-// the parts in slice order, runs the steps, writes Q's tiles), apply (a block per slice: Q G). Nothing is atomic: results
-// repeat bit for bit.
+// Kernels: gram (a block per part of a matrix's columns: the part's upper tiles of A0), then for r <= 32 apply with the steps
+// inside (every block of a matrix runs them again: two launches in all), for r <= 64 iterate (a block per matrix) and apply,
+// and above that the products as launches of their own, a wave per tile (a block per matrix would leave most CUs idle: 128 x 128
+// products of 17 cost 130 us of one CU's matrix units). Nothing is atomic: results repeat bit for bit.
+#include <algorithm>
+#include <utility>
+
 #include "../../include/smel_ortho.h"
 #include "abi_util.h"
 #include "common.h"
@@ -26,7 +30,7 @@ typedef double f64x4_t __attribute__((ext_vector_type(4)));
 SMEL_DEV f64x4_t mfma64(double a, double b, f64x4_t c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 
 constexpr int MAX_R = 128;
-constexpr int MAX_JOBS = 40;   // of one launch: the jobs travel as kernel arguments (under 4 KiB)
+constexpr int MAX_JOBS = 36;   // of one launch: the jobs travel as kernel arguments (under 4 KiB)
 constexpr int WAVES = 8;       // of a gram or apply block
 
 struct Job {
@@ -37,12 +41,13 @@ struct Job {
   int32_t batch, r, n;
   int32_t blk0, mat0;  // first block (gram, apply) and first matrix (iterate, Q)
   int32_t slices;      // of a matrix
+  int32_t gblk0, parts;   // gram: first block, blocks of a matrix (each takes js.per slices)
   int32_t x_tall;      // 1: the short side has the unit stride in x
   int32_t y_tall;      // 1: the short side is y's last
 };
 struct Jobs {
   int32_t n, slice;    // jobs; columns of a slice (a multiple of 64)
-  int64_t pad_;
+  int32_t per, pad_;   // slices of a gram block
   Job j[MAX_JOBS];
 };
 static_assert(sizeof(Jobs) <= 3584, "kernel arguments");
@@ -87,37 +92,100 @@ SMEL_DEV void st_elem(typename Elem<DT>::T* p, double v) {
   if constexpr (DT == 2) *p = __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-// the job of block (or matrix) b; uniform
-template <bool MAT>
+// the job of block (gram, apply) or matrix b; uniform
+enum { BY_GRAM, BY_APPLY, BY_MATRIX };
+template <int BY>
 SMEL_DEV int find_job(const Jobs& js, int b) {
   int k = 0;
-  while (k + 1 < js.n && b >= (MAT ? js.j[k + 1].mat0 : js.j[k + 1].blk0)) ++k;
+  while (k + 1 < js.n && b >= (BY == BY_GRAM ? js.j[k + 1].gblk0 : BY == BY_APPLY ? js.j[k + 1].blk0 : js.j[k + 1].mat0)) ++k;
   return k;
 }
 
-// columns [j0, j0 + slice) of a matrix as fp32 X[i][j] in LDS, rows [r, 16 NT) and columns past n zero
+typedef u32x4_t __attribute__((aligned(2))) u32x4_a2;
+typedef f32x4_t __attribute__((aligned(4))) f32x4_a4;
+// N (4 or 8) consecutive elements, `left` of them in range: 8- or 16-byte stores at any alignment
+typedef uint32_t __attribute__((ext_vector_type(2), aligned(2))) u32x2_a2;
+template <int DT, int N>
+SMEL_DEV void st_run(typename Elem<DT>::T* p, int left, const double* v) {
+  if (left >= N) {
+    if constexpr (DT == 1) {
+#pragma unroll
+      for (int k = 0; k < N; k += 4) *(f32x4_a4*)(p + k) = f32x4_t{(float)v[k], (float)v[k + 1], (float)v[k + 2], (float)v[k + 3]};
+    } else {
+      uint32_t w[N / 2];
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) {
+        if constexpr (DT == 0)
+          w[k] = pack2bf((float)v[2 * k], (float)v[2 * k + 1]);
+        else
+          w[k] = __builtin_bit_cast(uint16_t, (_Float16)(float)v[2 * k]) |
+                 (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)v[2 * k + 1]) << 16;
+      }
+      if constexpr (N == 8)
+        *(u32x4_a2*)p = u32x4_t{w[0], w[1], w[2], w[3]};
+      else
+        *(u32x2_a2*)p = u32x2_a2{w[0], w[1]};
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (k < left) st_elem<DT>(p + k, v[k]);
+}
+
+// V consecutive elements as floats: one 16-byte load at any alignment, element by element where fewer than V are left
 template <int DT>
-SMEL_DEV void load_slice(const Job& J, int mat, int j0, int slice, int rp, float* X, int pitch) {
+struct Vec {
+  static constexpr int V = DT == 1 ? 4 : 8;
+};
+template <int DT>
+SMEL_DEV void ld_vec(const typename Elem<DT>::T* p, int left, float v[Vec<DT>::V]) {
+  constexpr int V = Vec<DT>::V;
+  if (left >= V) {
+    if constexpr (DT == 1) {
+      const f32x4_t q = *(const f32x4_a4*)p;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = q[k];
+    } else {
+      const u32x4_t q = *(const u32x4_a2*)p;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = to_f<DT>((k & 1) ? q[k >> 1] >> 16 : q[k >> 1] & 0xffffu);
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = k < left ? ld_elem<DT>(p + k) : 0.f;
+}
+
+// columns [j0, j0 + slice) of a matrix as fp32 X[i][j] in LDS, rows [r, 16 NT) and columns past n zero. The pitch of slice + 20
+// floats (20 mod 64 banks) keeps the 16 rows of a gram operand and the 16 columns x 4 chunks of a transposed store apart.
+template <int NT, int DT>
+SMEL_DEV void load_slice(const Job& J, int mat, int j0, int slice, float* X, int pitch) {
   typedef typename Elem<DT>::T T;
+  constexpr int V = Vec<DT>::V, RP = 16 * NT;
   const T* const x = (const T*)J.x + mat * J.xb;
   const int nc = min(slice, J.n - j0);
-  for (int e = threadIdx.x; e < rp * slice; e += blockDim.x) {
-    int i, j;
-    if (J.x_tall) {
-      j = e / rp;
-      i = e % rp;
+  const int chunks = RP * slice / V;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
+    float v[V];
+    if (J.x_tall) {   // lines along i: 16 lanes take a chunk of 16 lines
+      constexpr int Q = RP / V;
+      const int j = e / (16 * Q) * 16 + (e & 15), i = (e >> 4) % Q * V;
+      ld_vec<DT>(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) X[(i + k) * pitch + j] = v[k];
     } else {
-      i = e / slice;
-      j = e % slice;
+      const int c = slice / V, i = e / c, j = e % c * V;
+      ld_vec<DT>(x + i * J.ld + j0 + j, i < J.r ? nc - j : 0, v);
+#pragma unroll
+      for (int k = 0; k < V; k += 4) *(f32x4_t*)(X + i * pitch + j + k) = f32x4_t{v[k], v[k + 1], v[k + 2], v[k + 3]};
     }
-    float v = 0.f;
-    if (i < J.r && j < nc) v = ld_elem<DT>(x + (J.x_tall ? (j0 + j) * J.ld + i : i * J.ld + j0 + j));
-    X[i * pitch + j] = v;
   }
 }
 
 // columns of a slice at most: two blocks on a CU
-constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt == 2 ? 512 : nt == 4 ? 256 : 128; }
+constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt <= 4 ? 256 : 128; }
 constexpr int slice_bytes(int nt) { return 16 * nt * (max_slice(nt) + 20) * 4; }
 
 template <int NT, int DT>
@@ -129,25 +197,32 @@ __global__ __launch_bounds__(64 * WAVES) void gram_kernel(Jobs js, double* __res
   static_assert(TPW * TG == NTL, "tiles per wave");
   float* const X = (float*)smem;
   const int pitch = js.slice + 20;
-  const Job& J = js.j[find_job<false>(js, blockIdx.x)];
-  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, sl = lb % J.slices;
-  load_slice<DT>(J, mat, sl * js.slice, js.slice, 16 * NT, X, pitch);
-  __syncthreads();
+  const Job& J = js.j[find_job<BY_GRAM>(js, blockIdx.x)];
+  const int lb = blockIdx.x - J.gblk0, mat = lb / J.parts, s0 = lb % J.parts * js.per;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int tg = wave % TG, kg = wave / TG;
   f64x4_t acc[TPW];
+  int ra[TPW], rb[TPW];
 #pragma unroll
   for (int k = 0; k < TPW; ++k) {
     acc[k] = f64x4_t{0, 0, 0, 0};
     int t, u;
     tile_of(tg * TPW + k, NT, t, u);
+    ra[k] = (16 * t + lo) * pitch + 4 * hi;
+    rb[k] = (16 * u + lo) * pitch + 4 * hi;
+  }
+  for (int sl = s0; sl < min(s0 + js.per, J.slices); ++sl) {
+    if (sl > s0) __syncthreads();
+    load_slice<NT, DT>(J, mat, sl * js.slice, js.slice, X, pitch);
+    __syncthreads();
     // 16 columns a step, four to a lane: which columns make one instruction's contraction does not matter
-    for (int j = 16 * kg; j < js.slice; j += 16 * KG) {
-      const f32x4_t a = *(const f32x4_t*)(X + (16 * t + lo) * pitch + j + 4 * hi);
-      const f32x4_t b = *(const f32x4_t*)(X + (16 * u + lo) * pitch + j + 4 * hi);
+    for (int j = 16 * kg; j < js.slice; j += 16 * KG)
 #pragma unroll
-      for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
-    }
+      for (int k = 0; k < TPW; ++k) {
+        const f32x4_t a = *(const f32x4_t*)(X + ra[k] + j), b = *(const f32x4_t*)(X + rb[k] + j);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
+      }
   }
   // the column groups' sums, in group order
   f64x4_t* const red = (f64x4_t*)smem;   // [TG][TPW][64]
@@ -175,7 +250,7 @@ struct Steps {
 constexpr int TP = 17;   // doubles between the rows of a tile in LDS
 
 // waves of an iterate block, one to three upper tiles each
-constexpr int it_waves(int nt) { return nt == 8 ? 12 : nt == 4 ? 10 : nt == 2 ? 3 : 1; }
+constexpr int it_waves(int nt) { return nt == 4 ? 10 : 3; }
 
 // element (16 u + 4 m + l / 16, 16 t + l % 16) of a symmetric matrix in upper tiles: at + m * step
 SMEL_DEV int frag_at(int u, int t, int nt, int lo, int hi, int& step) {
@@ -193,7 +268,7 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
   constexpr int NTL = ntiles(NT), W = it_waves(NT), TPW = NTL / W;
   static_assert(TPW * W == NTL, "tiles per wave");
   __shared__ double buf0[NTL * 16 * TP], buf1[NTL * 16 * TP], trs[NT];
-  const Job& J = js.j[find_job<true>(js, blockIdx.x)];
+  const Job& J = js.j[find_job<BY_MATRIX>(js, blockIdx.x)];
   const int mat = blockIdx.x - J.mat0;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   int tt[TPW], uu[TPW];
@@ -202,8 +277,8 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
   for (int k = 0; k < TPW; ++k) {
     tile_of(wave * TPW + k, NT, tt[k], uu[k]);
     A[k] = f64x4_t{0, 0, 0, 0};
-    const double* p = part + (J.part0 + (int64_t)mat * J.slices) * (NTL * 256) + ((wave * TPW + k) * 64 + lane) * 4;
-    for (int s = 0; s < J.slices; ++s) A[k] += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
+    const double* p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + ((wave * TPW + k) * 64 + lane) * 4;
+    for (int s = 0; s < J.parts; ++s) A[k] += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
     if (tt[k] == uu[k]) {   // the tile's trace: row 4 m + hi, column lo
       double d = 0;
 #pragma unroll
@@ -284,44 +359,257 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
   }
 }
 
-template <int NT, int DT>
-__global__ __launch_bounds__(64 * WAVES) void apply_kernel(Jobs js, const double* __restrict__ Qin) {
+// ------------------------------------------------------------------------------------------------ steps of r <= 32, in a block
+
+// A0 (scaled) and the steps, wave w < NT^2 holding tile (w / NT, w % NT) of every matrix; Q's tiles to bQ. All waves of the
+// block call it. Tiles lie in LDS as they lie in the registers (64 lanes x 4), which is the operand layout.
+template <int NT>
+SMEL_DEV void steps_small(const Job& J, int mat, const Steps& st, const double* __restrict__ part, f64x4_t (*bA)[64],
+                          f64x4_t (*bP)[64], f64x4_t (*bT)[64], f64x4_t (*bQ)[64], double* tr) {
+  constexpr int NTL = ntiles(NT);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+  const bool mine = wave < NT * NT;
+  const int t = wave / NT, u = wave % NT;
+  f64x4_t A = {0, 0, 0, 0}, Q = {0, 0, 0, 0}, P = {0, 0, 0, 0}, S;
+  f64x4_t eye;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) eye[m] = t == u && 4 * m + hi == lo ? 1.0 : 0.0;
+  if (mine) {
+    // a lower tile is its mirror's transpose: element (4 m + hi, lo) is register lo / 4 of lane (lo % 4, 4 m + hi)
+    const int k = t <= u ? tile_at(t, u, NT) : tile_at(u, t, NT);
+    const double* const p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + k * 256;
+#pragma unroll 4
+    for (int s = 0; s < J.parts; ++s) {
+      const double* const q = p + (int64_t)s * (NTL * 256);
+      if (t <= u) {
+        A += *(const f64x4_t*)(q + lane * 4);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) A[m] += q[((lo & 3) * 16 + 4 * m + hi) * 4 + (lo >> 2)];
+      }
+    }
+    double d = 0;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) d += eye[m] != 0 ? A[m] : 0.0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) d += __shfl_xor(d, o, 64);
+    if (t == u && lane == 0) tr[t] = d;
+  }
+  __syncthreads();
+  double sum = tr[0];
+#pragma unroll
+  for (int k = 1; k < NT; ++k) sum += tr[k];
+  const double s = 1.0 / (sqrt(sum) + st.eps);
+  A = A * s * s;
+  Q = eye * s;
+  auto product = [&](f64x4_t (*M)[64], f64x4_t (*N)[64]) {
+    f64x4_t acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const f64x4_t a = M[k * NT + t][lane], b = N[k * NT + u][lane];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) acc = mfma64(a[m], b[m], acc);
+    }
+    return acc;
+  };
+  auto own = [&](f64x4_t a, f64x4_t b) {   // NT = 1: the operands are the wave's own registers
+    f64x4_t acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc = mfma64(a[m], b[m], acc);
+    return acc;
+  };
+  for (int it = 0; it < st.steps; ++it) {
+    const bool first = it == 0, last = it + 1 == st.steps;
+    if constexpr (NT == 1) {
+      if (mine) {
+        P = st.b * A + st.c * own(A, A) + st.a * eye;
+        if (!last) S = own(A, P);
+        Q = first ? P * s : own(P, Q);
+        if (!last) A = own(S, P);
+      }
+    } else {
+      if (mine) bA[wave][lane] = A;
+      lds_barrier();
+      if (mine) {
+        P = st.b * A + st.c * product(bA, bA) + st.a * eye;
+        bP[wave][lane] = P;
+        bQ[wave][lane] = Q;
+      }
+      lds_barrier();
+      if (mine) {
+        if (!last) bT[wave][lane] = product(bA, bP);
+        Q = first ? P * s : product(bP, bQ);
+      }
+      lds_barrier();
+      if (mine && !last) A = product(bT, bP);
+    }
+  }
+  if (mine) bQ[wave][lane] = Q;
+  __syncthreads();
+}
+
+// Q G for a slice. SMALL: the steps run here, from the parts; else Q's tiles are read. A wave owns one tile of rows and every
+// CG-th pair of 16-column blocks. The columns of a pair (or, for a result whose short side is last, the rows of a tile) are
+// dealt to the instruction's rows so that a lane's registers are neighbours in memory.
+template <int NT, int DT, bool SMALL>
+__global__ __launch_bounds__(64 * WAVES) void apply_kernel(Jobs js, Steps st, const double* __restrict__ in) {
   __shared__ __attribute__((aligned(16))) char smem[slice_bytes(NT)];
   typedef typename Elem<DT>::T T;
-  constexpr int CG = WAVES / NT;   // column groups; a wave owns one tile of rows
+  constexpr int CG = WAVES / NT;
   float* const X = (float*)smem;
   const int pitch = js.slice + 20;
-  const Job& J = js.j[find_job<false>(js, blockIdx.x)];
+  const Job& J = js.j[find_job<BY_APPLY>(js, blockIdx.x)];
   const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = lb % J.slices * js.slice;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int t = wave % NT, cg = wave / NT;
+  const int perm = 4 * (lo & 3) + (lo >> 2);   // row 4 m + hi of the result <- index 4 hi + m
+  const int qlane = J.y_tall ? hi * 16 + perm : lane;
+  load_slice<NT, DT>(J, mat, j0, js.slice, X, pitch);
   f64x4_t q[NT];
+  if constexpr (SMALL) {
+    __shared__ f64x4_t b[4][NT * NT][64];
+    __shared__ double tr[NT];
+    steps_small<NT>(J, mat, st, in, b[0], b[1], b[2], b[3], tr);   // ends with a barrier: X and b[3] are there
 #pragma unroll
-  for (int u = 0; u < NT; ++u)
-    q[u] = *(const f64x4_t*)(Qin + (int64_t)(J.mat0 + mat) * (NT * NT * 256) + ((u * NT + t) * 64 + lane) * 4);
-  load_slice<DT>(J, mat, j0, js.slice, 16 * NT, X, pitch);
-  __syncthreads();
-  const int nc = min(js.slice, J.n - j0);
-  T* const y = (T*)J.y + (int64_t)mat * J.r * J.n;
-  for (int j = 16 * cg; j < nc; j += 16 * CG) {
-    f64x4_t acc = {0, 0, 0, 0};
+    for (int u = 0; u < NT; ++u) q[u] = b[3][u * NT + t][qlane];
+  } else {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
+      q[u] = *(const f64x4_t*)(in + (int64_t)(J.mat0 + mat) * (NT * NT * 256) + ((u * NT + t) * 64 + qlane) * 4);
+    __syncthreads();
+  }
+  const int nc = min(js.slice, J.n - j0);
+  T* const y = (T*)J.y + (int64_t)mat * J.r * J.n;
+  if (J.y_tall) {
+    for (int j = 16 * cg; j < nc; j += 16 * CG) {
+      f64x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const double x = X[(16 * u + 4 * m + hi) * pitch + j + lo];
-        acc = J.y_tall ? mfma64(x, q[u][m], acc) : mfma64(q[u][m], x, acc);
-      }
+      for (int u = 0; u < NT; ++u)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      if (J.y_tall) {   // row: column j + 4 m + hi of the matrix, column: row 16 t + lo
-        const int c = j + 4 * m + hi, i = 16 * t + lo;
-        if (c < nc && i < J.r) st_elem<DT>(y + (int64_t)(j0 + c) * J.r + i, acc[m]);
-      } else {
-        const int c = j + lo, i = 16 * t + 4 * m + hi;
-        if (c < nc && i < J.r) st_elem<DT>(y + (int64_t)i * J.n + j0 + c, acc[m]);
-      }
+        for (int m = 0; m < 4; ++m) acc = mfma64(q[u][m], (double)X[(16 * u + 4 * m + hi) * pitch + j + lo], acc);
+      const int i = 16 * t + 4 * hi;   // rows i + m, column j + lo
+      if (j + lo < nc) st_run<DT, 4>(y + (int64_t)(j0 + j + lo) * J.r + i, J.r - i, (const double*)&acc);
     }
+  } else {
+    for (int j = 32 * cg; j < nc; j += 32 * CG) {
+      f64x4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      const int c = j + 8 * (lo & 3) + (lo >> 2);   // the pair: columns 8 hi + m and 8 hi + 4 + m
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float* const x = X + (16 * u + 4 * m + hi) * pitch + c;
+          acc[0] = mfma64((double)x[0], q[u][m], acc[0]);
+          acc[1] = mfma64((double)x[4], q[u][m], acc[1]);
+        }
+      const int i = 16 * t + lo, k = j + 8 * hi;   // row i, columns k to k + 7
+      if (i < J.r) st_run<DT, 8>(y + (int64_t)i * J.n + j0 + k, nc - k, (const double*)acc);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ steps of r > 64, as launches
+
+constexpr int BIG = 8, BIG_MAT = BIG * BIG * 256;   // doubles of a matrix: 64 tiles in the operand layout
+struct BigArgs {
+  const double* part;
+  double *A, *P, *T, *Q, *Q2, *tr;   // [mats][BIG_MAT] (tr: [mats][8])
+  int mats;
+  int first, last;
+  Steps st;
+};
+// blocks of a matrix to one XCD, whose L2 then holds its tiles: block b -> matrix, index among the matrix's `n` blocks
+SMEL_DEV bool big_map(int mats, int n, int& mat, int& k) {
+  const int x = blockIdx.x % NXCD, j = blockIdx.x / NXCD;
+  mat = j / n * NXCD + x;
+  k = j % n;
+  return mat < mats;
+}
+
+// the parts' sum: both mirrored tiles of A0, and the diagonal tiles' traces; a wave per upper tile
+__global__ __launch_bounds__(256) void big_sum_kernel(Jobs js, BigArgs g) {
+  constexpr int NTL = ntiles(BIG);
+  __shared__ double tile[4][16 * TP];
+  int mat, kb;
+  if (!big_map(g.mats, NTL / 4, mat, kb)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+  const Job& J = js.j[find_job<BY_MATRIX>(js, mat)];
+  int t, u;
+  tile_of(kb * 4 + wave, BIG, t, u);
+  const double* const p = g.part + (J.part0 + (int64_t)(mat - J.mat0) * J.parts) * (NTL * 256) + ((kb * 4 + wave) * 64 + lane) * 4;
+  f64x4_t a = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < J.parts; ++s) a += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
+  double* const A = g.A + (int64_t)mat * BIG_MAT;
+  *(f64x4_t*)(A + ((t * BIG + u) * 64 + lane) * 4) = a;
+  if (t == u) {
+    double d = 0;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) d += 4 * m + hi == lo ? a[m] : 0.0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) d += __shfl_xor(d, o, 64);
+    if (lane == 0) g.tr[mat * BIG + t] = d;
+    return;
+  }
+  double* const l = tile[wave];   // the wave's own: its LDS accesses are in order
+#pragma unroll
+  for (int m = 0; m < 4; ++m) l[(4 * m + hi) * TP + lo] = a[m];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  f64x4_t b;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) b[m] = l[lo * TP + 4 * m + hi];
+  *(f64x4_t*)(A + ((u * BIG + t) * 64 + lane) * 4) = b;
+}
+
+// tile (t, u) of M N for symmetric M and N that commute
+SMEL_DEV f64x4_t big_product(const double* M, const double* N, int t, int u, int lane) {
+  f64x4_t a[BIG], b[BIG], acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < BIG; ++k) {
+    a[k] = *(const f64x4_t*)(M + ((k * BIG + t) * 64 + lane) * 4);
+    b[k] = *(const f64x4_t*)(N + ((k * BIG + u) * 64 + lane) * 4);
+  }
+#pragma unroll
+  for (int k = 0; k < BIG; ++k)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc = mfma64(a[k][m], b[k][m], acc);
+  return acc;
+}
+
+// 1: P = a I + b A + c A A (first: of the scaled A, and Q = s P);  2: T = A P and Q2 = P Q;  3: A = T P
+enum { BIG_P, BIG_TQ, BIG_A };
+template <int WHAT>
+__global__ __launch_bounds__(256) void big_kernel(BigArgs g) {
+  int mat, kb;
+  if (!big_map(g.mats, 16, mat, kb)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+  const int k = kb * 4 + wave, t = k / BIG, u = k % BIG;
+  const int64_t base = (int64_t)mat * BIG_MAT, at = base + (k * 64 + lane) * 4;
+  double s = 1.0;
+  if (g.first) {   // the trace is the squared norm
+    double tr = 0;
+#pragma unroll
+    for (int i = 0; i < BIG; ++i) tr += g.tr[mat * BIG + i];
+    s = 1.0 / (sqrt(tr) + g.st.eps);
+  }
+  const double s2 = s * s;
+  if constexpr (WHAT == BIG_P) {
+    f64x4_t p;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) p[m] = t == u && 4 * m + hi == lo ? 1.0 : 0.0;
+    if (g.st.steps > 0) {
+      const f64x4_t aa = big_product(g.A + base, g.A + base, t, u, lane);
+      p = g.st.a * p + g.st.b * (*(const f64x4_t*)(g.A + at) * s2) + g.st.c * (aa * s2 * s2);
+      *(f64x4_t*)(g.P + at) = p;
+    }
+    if (g.first) *(f64x4_t*)(g.Q + at) = p * s;
+  } else if constexpr (WHAT == BIG_TQ) {
+    if (blockIdx.y == 0 && !g.last) *(f64x4_t*)(g.T + at) = big_product(g.A + base, g.P + base, t, u, lane) * s2;
+    if (blockIdx.y == 1 || g.last) {
+      if (!g.first) *(f64x4_t*)(g.Q2 + at) = big_product(g.P + base, g.Q + base, t, u, lane);
+    }
+  } else {
+    *(f64x4_t*)(g.A + at) = big_product(g.T + base, g.P + base, t, u, lane);
   }
 }
 
@@ -353,37 +641,58 @@ int check(const smel_ortho_job* jobs, int32_t n) {
 
 struct Plan {
   Jobs js;
-  int64_t blocks, mats, parts;   // blocks of gram and apply, matrices, tile sets of the parts
+  int64_t blocks, gblocks, mats;   // apply's and gram's blocks, matrices
 };
+struct Cursor {
+  int job;
+  int64_t mat;
+};
+constexpr int64_t MAX_MATS = 65536, BIG_MATS = 256;   // of a launch; its workspace is 0.6 MB a matrix above r = 64
+constexpr int64_t GRAM_BLOCKS = 512;                  // two a CU
 
-// the jobs of one (tiles a side, dtype), MAX_JOBS at a time from `from`; returns the index behind the last job taken
-int fill(const smel_ortho_job* jobs, int32_t n, int from, int nt, int dt, Plan& p) {
+// the next jobs of one (tiles a side, dtype) from `at` on, as many as a launch takes (a job's batch may be split)
+Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Plan& p) {
   p.js.n = 0;
-  p.blocks = p.mats = p.parts = 0;
-  int end = from;
+  p.blocks = p.gblocks = p.mats = 0;
+  struct Taken {
+    int job;
+    int64_t mat, count;
+  } taken[MAX_JOBS];
   int64_t cols = 0;
-  int taken[MAX_JOBS];
-  for (; end < n && p.js.n < MAX_JOBS; ++end) {
-    const smel_ortho_job& j = jobs[end];
-    if (j.batch == 0 || j.rows == 0 || j.cols == 0 || j.dtype != dt) continue;
+  const int64_t most = nt == 8 ? BIG_MATS : MAX_MATS;
+  while (at.job < n && p.js.n < MAX_JOBS && p.mats < most) {
+    const smel_ortho_job& j = jobs[at.job];
     const int64_t r = j.rows < j.cols ? j.rows : j.cols;
-    if (nt_of(r) != nt) continue;
-    taken[p.js.n++] = end;
-    cols += j.batch * (j.rows < j.cols ? j.cols : j.rows);
+    if (j.batch == 0 || r == 0 || j.dtype != dt || nt_of(r) != nt) {
+      at = Cursor{at.job + 1, 0};
+      continue;
+    }
+    const int64_t take = j.batch - at.mat < most - p.mats ? j.batch - at.mat : most - p.mats;
+    taken[p.js.n++] = Taken{at.job, at.mat, take};
+    p.mats += take;
+    cols += take * (j.rows < j.cols ? j.cols : j.rows);
+    at.mat += take;
+    if (at.mat == j.batch) at = Cursor{at.job + 1, 0};
   }
+  // the largest slices that give two blocks to a CU, but at least 128 columns (each wave a block of 16)
   int slice = max_slice(nt);
   while (slice > 128 && cols / slice < 512) slice /= 2;
   p.js.slice = slice;
+  p.js.per = 1;
+  // the parts of A0 cost 2 KB a tile: above r = 64 (72 KB) a gram block takes several slices
+  if (nt == 8) p.js.per = (int)std::max<int64_t>(1, cols / slice / GRAM_BLOCKS);
+  int64_t mats = 0;
   for (int k = 0; k < p.js.n; ++k) {
-    const smel_ortho_job& j = jobs[taken[k]];
+    const smel_ortho_job& j = jobs[taken[k].job];
     Job& o = p.js.j[k];
     const bool wide = j.rows <= j.cols;   // the short side is the rows
-    o.x = j.x;
-    o.y = j.y;
+    const int64_t es = dt == 1 ? 4 : 2;
+    o.x = (const char*)j.x + taken[k].mat * j.x_batch * es;
+    o.y = (char*)j.y + taken[k].mat * j.rows * j.cols * es;
     o.xb = j.x_batch;
     o.r = (int32_t)(wide ? j.rows : j.cols);
     o.n = (int32_t)(wide ? j.cols : j.rows);
-    o.batch = (int32_t)j.batch;
+    o.batch = (int32_t)taken[k].count;
     o.y_tall = !wide;
     const bool last = j.cols == 1 || j.x_col == 1;   // lines run along the last side
     if (last && !(j.cols == 1 && j.rows > 1 && j.x_row == 1)) {
@@ -394,28 +703,68 @@ int fill(const smel_ortho_job* jobs, int32_t n, int from, int nt, int dt, Plan& 
       o.x_tall = wide;
     }
     o.slices = (o.n + slice - 1) / slice;
+    o.parts = (o.slices + p.js.per - 1) / p.js.per;
     o.blk0 = (int32_t)p.blocks;
-    o.mat0 = (int32_t)p.mats;
-    o.part0 = p.blocks;
-    p.blocks += j.batch * o.slices;
-    p.mats += j.batch;
-    if (p.blocks >= (int64_t)1 << 22) return -1;   // 768 threads each: a launch takes fewer than 2^32
+    o.gblk0 = (int32_t)p.gblocks;
+    o.mat0 = (int32_t)mats;
+    o.part0 = p.gblocks;
+    mats += o.batch;
+    p.blocks += (int64_t)o.batch * o.slices;
+    p.gblocks += (int64_t)o.batch * o.parts;
+    if (p.blocks >= (int64_t)1 << 22) return Cursor{-1, 0};   // 512 threads each: a launch takes fewer than 2^32
   }
-  p.parts = p.blocks;
-  return end;
+  return at;
 }
 
-int64_t part_bytes(const Plan& p, int nt) { return p.parts * ntiles(nt) * 2048; }
-int64_t q_bytes(const Plan& p, int nt) { return p.mats * nt * nt * 2048; }
+int64_t part_bytes(const Plan& p, int nt) { return p.gblocks * ntiles(nt) * 2048; }
+int64_t ws_bytes_of(const Plan& p, int nt) {
+  const int64_t parts = part_bytes(p, nt);
+  if (nt <= 2) return parts;
+  if (nt == 4) return parts + p.mats * nt * nt * 2048;
+  return parts + p.mats * (5 * BIG_MAT + BIG) * 8;
+}
+
+// the steps above r = 64; returns where Q's tiles are
+const double* run_big(const Plan& p, const Steps& st, const double* part, double* ws, hipStream_t stream) {
+  BigArgs g{};
+  const int64_t m = p.mats * BIG_MAT;
+  g.part = part;
+  g.A = ws;
+  g.P = ws + m;
+  g.T = ws + 2 * m;
+  g.Q = ws + 3 * m;
+  g.Q2 = ws + 4 * m;
+  g.tr = ws + 5 * m;
+  g.mats = (int)p.mats;
+  g.st = st;
+  const unsigned groups = (unsigned)((p.mats + NXCD - 1) / NXCD * NXCD);
+  big_sum_kernel<<<groups * (ntiles(BIG) / 4), 256, 0, stream>>>(p.js, g);
+  for (int it = 0; it == 0 || it < st.steps; ++it) {
+    g.first = it == 0;
+    g.last = it + 1 >= st.steps;
+    big_kernel<BIG_P><<<groups * 16, 256, 0, stream>>>(g);
+    if (g.first && g.last) break;
+    big_kernel<BIG_TQ><<<dim3(groups * 16, g.first || g.last ? 1 : 2), 256, 0, stream>>>(g);
+    if (!g.first) std::swap(g.Q, g.Q2);
+    if (!g.last) big_kernel<BIG_A><<<groups * 16, 256, 0, stream>>>(g);
+  }
+  return g.Q;
+}
 
 template <int NT, int DT>
 int run(const Plan& p, const Steps& st, void* ws, hipStream_t stream) {
   const Jobs& js = p.js;
   double* const part = (double*)ws;
-  double* const Q = (double*)((char*)ws + part_bytes(p, NT));
-  gram_kernel<NT, DT><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(js, part);
-  iterate_kernel<NT><<<(unsigned)p.mats, 64 * it_waves(NT), 0, stream>>>(js, st, part, Q);
-  apply_kernel<NT, DT><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(js, Q);
+  double* const rest = (double*)((char*)ws + part_bytes(p, NT));
+  gram_kernel<NT, DT><<<(unsigned)p.gblocks, 64 * WAVES, 0, stream>>>(js, part);
+  if constexpr (NT <= 2) {
+    apply_kernel<NT, DT, true><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(js, st, part);
+  } else {
+    const double* Q = rest;
+    if constexpr (NT == 4) iterate_kernel<NT><<<(unsigned)p.mats, 64 * it_waves(NT), 0, stream>>>(js, st, part, rest);
+    else Q = run_big(p, st, part, rest, stream);
+    apply_kernel<NT, DT, false><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(js, st, Q);
+  }
   return smel::launch_status();
 }
 template <int NT>
@@ -426,12 +775,17 @@ int run_dt(const Plan& p, int dt, const Steps& st, void* ws, hipStream_t stream)
 // f(plan, nt, dt) for every launch group, in order; stops at the first non-zero result
 template <class F>
 int each(const smel_ortho_job* jobs, int32_t n, F f) {
+  bool any[9][3] = {};
+  for (int k = 0; k < n; ++k) {
+    const int64_t r = jobs[k].rows < jobs[k].cols ? jobs[k].rows : jobs[k].cols;
+    if (jobs[k].batch && r) any[nt_of(r)][jobs[k].dtype] = true;
+  }
   for (int nt = 1; nt <= 8; nt *= 2)
     for (int dt = 0; dt < 3; ++dt)
-      for (int at = 0; at < n;) {
+      for (Cursor at{0, 0}; any[nt][dt] && at.job < n;) {
         Plan p;
         at = fill(jobs, n, at, nt, dt, p);
-        SMEL_REQUIRE(at >= 0, SMEL_EUNSUPPORTED, "orthogonalize: too many matrices in one call");
+        SMEL_REQUIRE(at.job >= 0, SMEL_EUNSUPPORTED, "orthogonalize: too many columns in one call");
         if (p.js.n == 0) continue;
         const int rc = f(p, nt, dt);
         if (rc) return rc;
@@ -442,8 +796,7 @@ int each(const smel_ortho_job* jobs, int32_t n, F f) {
 int64_t ws_need(const smel_ortho_job* jobs, int32_t n, int& rc) {
   int64_t need = 0;   // the groups run one after the other on one stream and share the workspace
   rc = each(jobs, n, [&](const Plan& p, int nt, int) {
-    const int64_t b = part_bytes(p, nt) + q_bytes(p, nt);
-    if (b > need) need = b;
+    need = std::max(need, ws_bytes_of(p, nt));
     return 0;
   });
   return need;

@@ -54,7 +54,7 @@ def test_orthogonalize_refusals():
     assert f(x=18) == -1 and f(y=17, dt=0) == -1 and f(xr=-64) == -1 and f(xr=2, xc=64 * 3) == -1
     assert f(steps=-1) == -1 and f(steps=65) == -1 and f(eps=-1.0) == -1 and f(eps=float("nan")) == -1
     assert f(ws=None) == -1 and f(ws=24) == -1 and f(n=100) == -1 and b"workspace" in L.smel_last_error()
-    assert f(cols=1 << 31) == -2 and f(batch=1 << 23) == -2
+    assert f(cols=1 << 31) == -2 and f(batch=1 << 31) == -2
     assert f(batch=0, ws=None, n=0) == 0 and f(rows=0, ws=None, n=0) == 0
     assert L.smel_orthogonalize(None, 0, 5, 1.0, 1.0, 1.0, 0.0, None, 0, None) == 0
     assert L.smel_orthogonalize(None, 1, 5, 1.0, 1.0, 1.0, 0.0, None, 0, None) == -1
