@@ -189,7 +189,7 @@ constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt <= 4 ? 256 : 128; }
 constexpr int slice_bytes(int nt) { return 16 * nt * (max_slice(nt) + 20) * 4; }
 
 template <int NT, int DT>
-__global__ __launch_bounds__(64 * WAVES) void gram_kernel(Jobs js, double* __restrict__ part) {
+__global__ __launch_bounds__(64 * WAVES, 4) void gram_kernel(Jobs js, double* __restrict__ part) {
   constexpr int NTL = ntiles(NT);
   __shared__ __attribute__((aligned(16))) char smem[slice_bytes(NT)];
   static_assert(slice_bytes(NT) >= NTL * 2048, "room for the column groups' sums");
@@ -222,6 +222,7 @@ __global__ __launch_bounds__(64 * WAVES) void gram_kernel(Jobs js, double* __res
         const f32x4_t a = *(const f32x4_t*)(X + ra[k] + j), b = *(const f32x4_t*)(X + rb[k] + j);
 #pragma unroll
         for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
+        if (k % 3 == 2) __builtin_amdgcn_sched_barrier(0);   // no more operands ahead than registers for two blocks a CU
       }
   }
   // the column groups' sums, in group order
@@ -247,6 +248,10 @@ struct Steps {
   double a, b, c, eps;
 };
 
+// Q carries 1 / (|G|_F + eps) = s. Above 2^64 (only an update of tiny norm with eps near 0) a power of two stays out of it, so
+// that Q's bf16 parts stay in range; the last product multiplies it back in. exp_of(s): that power's exponent.
+SMEL_DEV int exp_of(double s) { return s > 0x1p64 && s < 0x1p1000 ? ilogb(s) - 64 : 0; }
+
 constexpr int TP = 17;   // doubles between the rows of a tile in LDS
 
 // waves of an iterate block, one to three upper tiles each
@@ -264,7 +269,7 @@ SMEL_DEV int frag_at(int u, int t, int nt, int lo, int hi, int& step) {
 
 template <int NT>
 __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Steps st, const double* __restrict__ part,
-                                                                   double* __restrict__ Qout) {
+                                                                   double* __restrict__ Qout, double* __restrict__ qscale) {
   constexpr int NTL = ntiles(NT), W = it_waves(NT), TPW = NTL / W;
   static_assert(TPW * W == NTL, "tiles per wave");
   __shared__ double buf0[NTL * 16 * TP], buf1[NTL * 16 * TP], trs[NT];
@@ -298,8 +303,9 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       A[k][m] = A[k][m] * s * s;
-      Q[k][m] = tt[k] == uu[k] && 4 * m + hi == lo ? s : 0.0;
+      Q[k][m] = tt[k] == uu[k] && 4 * m + hi == lo ? ldexp(s, -exp_of(s)) : 0.0;
     }
+  if (threadIdx.x == 0) qscale[blockIdx.x] = ldexp(1.0, exp_of(s));
   auto put = [&](double* buf, const f64x4_t* M) {
 #pragma unroll
     for (int k = 0; k < TPW; ++k)
@@ -362,9 +368,10 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
 // ------------------------------------------------------------------------------------------------ steps of r <= 32, in a block
 
 // A0 (scaled) and the steps, wave w < NT^2 holding tile (w / NT, w % NT) of every matrix; Q's tiles to bQ. All waves of the
-// block call it. Tiles lie in LDS as they lie in the registers (64 lanes x 4), which is the operand layout.
+// block call it; returns the power of two that is not in Q. Tiles lie in LDS as they lie in the registers (64 lanes x 4), which
+// is the operand layout.
 template <int NT>
-SMEL_DEV void steps_small(const Job& J, int mat, const Steps& st, const double* __restrict__ part, f64x4_t (*bA)[64],
+SMEL_DEV double steps_small(const Job& J, int mat, const Steps& st, const double* __restrict__ part, f64x4_t (*bA)[64],
                           f64x4_t (*bP)[64], f64x4_t (*bT)[64], f64x4_t (*bQ)[64], double* tr) {
   constexpr int NTL = ntiles(NT);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
@@ -400,8 +407,10 @@ SMEL_DEV void steps_small(const Job& J, int mat, const Steps& st, const double* 
 #pragma unroll
   for (int k = 1; k < NT; ++k) sum += tr[k];
   const double s = 1.0 / (sqrt(sum) + st.eps);
+  const int ex = exp_of(s);
+  const double sq = ldexp(s, -ex);
   A = A * s * s;
-  Q = eye * s;
+  Q = eye * sq;
   auto product = [&](f64x4_t (*M)[64], f64x4_t (*N)[64]) {
     f64x4_t acc = {0, 0, 0, 0};
 #pragma unroll
@@ -424,7 +433,7 @@ SMEL_DEV void steps_small(const Job& J, int mat, const Steps& st, const double* 
       if (mine) {
         P = st.b * A + st.c * own(A, A) + st.a * eye;
         if (!last) S = own(A, P);
-        Q = first ? P * s : own(P, Q);
+        Q = first ? P * sq : own(P, Q);
         if (!last) A = own(S, P);
       }
     } else {
@@ -438,7 +447,7 @@ SMEL_DEV void steps_small(const Job& J, int mat, const Steps& st, const double* 
       lds_barrier();
       if (mine) {
         if (!last) bT[wave][lane] = product(bA, bP);
-        Q = first ? P * s : product(bP, bQ);
+        Q = first ? P * sq : product(bP, bQ);
       }
       lds_barrier();
       if (mine && !last) A = product(bT, bP);
@@ -446,13 +455,16 @@ SMEL_DEV void steps_small(const Job& J, int mat, const Steps& st, const double* 
   }
   if (mine) bQ[wave][lane] = Q;
   __syncthreads();
+  return ldexp(1.0, ex);
 }
 
 // Q G for a slice. SMALL: the steps run here, from the parts; else Q's tiles are read. A wave owns one tile of rows and every
 // CG-th pair of 16-column blocks. The columns of a pair (or, for a result whose short side is last, the rows of a tile) are
 // dealt to the instruction's rows so that a lane's registers are neighbours in memory.
 template <int NT, int DT, bool SMALL>
-__global__ __launch_bounds__(64 * WAVES) void apply_kernel(Jobs js, Steps st, const double* __restrict__ in) {
+__global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st, const double* __restrict__ in,
+                                                        const double* __restrict__ qscale) {
+  static_assert(DT == 1, "16-bit types: apply16_kernel");
   __shared__ __attribute__((aligned(16))) char smem[slice_bytes(NT)];
   typedef typename Elem<DT>::T T;
   constexpr int CG = WAVES / NT;
@@ -466,18 +478,22 @@ __global__ __launch_bounds__(64 * WAVES) void apply_kernel(Jobs js, Steps st, co
   const int qlane = J.y_tall ? hi * 16 + perm : lane;
   load_slice<NT, DT>(J, mat, j0, js.slice, X, pitch);
   f64x4_t q[NT];
+  double scale;
   if constexpr (SMALL) {
     __shared__ f64x4_t b[4][NT * NT][64];
     __shared__ double tr[NT];
-    steps_small<NT>(J, mat, st, in, b[0], b[1], b[2], b[3], tr);   // ends with a barrier: X and b[3] are there
+    scale = steps_small<NT>(J, mat, st, in, b[0], b[1], b[2], b[3], tr);   // ends with a barrier: X and b[3] are there
 #pragma unroll
     for (int u = 0; u < NT; ++u) q[u] = b[3][u * NT + t][qlane];
   } else {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
       q[u] = *(const f64x4_t*)(in + (int64_t)(J.mat0 + mat) * (NT * NT * 256) + ((u * NT + t) * 64 + qlane) * 4);
+    scale = qscale[J.mat0 + mat];
     __syncthreads();
   }
+#pragma unroll
+  for (int u = 0; u < NT; ++u) q[u] = q[u] * scale;
   const int nc = min(js.slice, J.n - j0);
   T* const y = (T*)J.y + (int64_t)mat * J.r * J.n;
   if (J.y_tall) {
@@ -508,12 +524,181 @@ __global__ __launch_bounds__(64 * WAVES) void apply_kernel(Jobs js, Steps st, co
   }
 }
 
+// The same for 16-bit results, whose rounding (2^-9, 2^-12) leaves room for fp32 sums: Q as three bf16 parts (24 bits), G's
+// bf16 values as they are and fp16 values as two bf16 parts, products on v_mfma_f32_16x16x16_bf16: 36 x 128 x 2816 bf16 took
+// 80 us on the f64 instruction. The parts' products are added in fp32: off by at most 3 r 2^-24 of sum |q| |g|.
+// G's slice lies in LDS as pairs of rows: word [i / 2][j] = (i, i + 1), the operand's neighbours. Pitch slice + 8: the four
+// row pairs that 64 lanes read at 16 columns take the banks twice at most.
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+SMEL_DEV f32x4_t mfma16(s16x4_t a, s16x4_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
+SMEL_DEV s16x4_t words(uint32_t a, uint32_t b) { return __builtin_bit_cast(s16x4_t, (u32x2_t{a, b})); }
+
+// 8 consecutive 16-bit elements as stored, zeros past `left`
+SMEL_DEV u32x4_t ld_raw8(const uint16_t* p, int left) {
+  if (left >= 8) return *(const u32x4_a2*)p;
+  uint32_t v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : 0u;
+  return u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+}
+template <int NT>
+SMEL_DEV void load_pairs(const Job& J, int mat, int j0, int slice, uint32_t* X, int pitch) {
+  constexpr int RP = 16 * NT;
+  const uint16_t* const x = (const uint16_t*)J.x + mat * J.xb;
+  const int nc = min(slice, J.n - j0);
+  if (J.x_tall) {
+    constexpr int Q = RP / 8;
+    const int chunks = RP * slice / 8;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
+      const int j = e / (16 * Q) * 16 + (e & 15), i = (e >> 4) % Q * 8;
+      const u32x4_t v = ld_raw8(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) X[(i / 2 + k) * pitch + j] = v[k];
+    }
+  } else {
+    const int c = slice / 8, chunks = RP / 2 * c;
+#pragma unroll 2
+    for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
+      const int p = e / c, j = e % c * 8;
+      const uint16_t* const row = x + 2 * p * J.ld + j0 + j;
+      const u32x4_t a = ld_raw8(row, 2 * p < J.r ? nc - j : 0), b = ld_raw8(row + J.ld, 2 * p + 1 < J.r ? nc - j : 0);
+      u32x4_t w[2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k >> 1][2 * (k & 1)] = (a[k] & 0xffffu) | b[k] << 16;
+        w[k >> 1][2 * (k & 1) + 1] = a[k] >> 16 | (b[k] & 0xffff0000u);
+      }
+      *(u32x4_t*)(X + p * pitch + j) = w[0];
+      *(u32x4_t*)(X + p * pitch + j + 4) = w[1];
+    }
+  }
+}
+
+template <int DT, int N>
+SMEL_DEV void st_run16(uint16_t* p, int left, const float* v) {
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) {
+    if constexpr (DT == 0)
+      w[k] = pack2bf(v[2 * k], v[2 * k + 1]);
+    else
+      w[k] = __builtin_bit_cast(uint16_t, (_Float16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k + 1]) << 16;
+  }
+  if (left >= N) {
+    if constexpr (N == 8)
+      *(u32x4_a2*)p = u32x4_t{w[0], w[1], w[2], w[3]};
+    else
+      *(u32x2_a2*)p = u32x2_a2{w[0], w[1]};
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (k < left) p[k] = (uint16_t)((k & 1) ? w[k >> 1] >> 16 : w[k >> 1]);
+}
+
+template <int NT, int DT, bool SMALL>
+__global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps st, const double* __restrict__ in,
+                                                          const double* __restrict__ qscale) {
+  constexpr int CG = WAVES / NT;
+  __shared__ __attribute__((aligned(16))) uint32_t X[8 * NT * (max_slice(NT) + 8)];
+  const int pitch = js.slice + 8;
+  const Job& J = js.j[find_job<BY_APPLY>(js, blockIdx.x)];
+  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = lb % J.slices * js.slice;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+  const int t = wave % NT, cg = wave / NT;
+  load_pairs<NT>(J, mat, j0, js.slice, X, pitch);
+  float scale;
+  s16x4_t q[NT][3];   // parts of Q[16 t + lo][16 u + 4 hi + 0..3]
+  auto parts = [&](int u, const double (&v)[4]) {
+    float r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = (float)v[k];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t a = pack2bf(r[0], r[1]), b = pack2bf(r[2], r[3]);
+      q[u][p] = words(a, b);
+      r[0] -= bf_lo(a);
+      r[1] -= bf_hi(a);
+      r[2] -= bf_lo(b);
+      r[3] -= bf_hi(b);
+    }
+  };
+  // element (4 hi + k, lo) of tile (u, t): register hi of lane (k, lo)
+  if constexpr (SMALL) {
+    __shared__ f64x4_t b[4][NT * NT][64];
+    __shared__ double tr[NT];
+    scale = (float)steps_small<NT>(J, mat, st, in, b[0], b[1], b[2], b[3], tr);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const double* const f = (const double*)b[3][u * NT + t];
+      parts(u, {f[lo * 4 + hi], f[(16 + lo) * 4 + hi], f[(32 + lo) * 4 + hi], f[(48 + lo) * 4 + hi]});
+    }
+  } else {
+    scale = (float)qscale[J.mat0 + mat];
+    const double* const Q = in + (int64_t)(J.mat0 + mat) * (NT * NT * 256);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const double* const f = Q + (u * NT + t) * 256;
+      parts(u, {f[lo * 4 + hi], f[(16 + lo) * 4 + hi], f[(32 + lo) * 4 + hi], f[(48 + lo) * 4 + hi]});
+    }
+    __syncthreads();
+  }
+  const int nc = min(js.slice, J.n - j0);
+  uint16_t* const y = (uint16_t*)J.y + (int64_t)mat * J.r * J.n;
+  // acc += Q G (or its transpose) for column c of the lane
+  auto dot = [&](int u, int c, bool tall, f32x4_t acc) {
+    const uint32_t* const x = X + (8 * u + 2 * hi) * pitch + c;
+    const uint32_t w0 = x[0], w1 = x[pitch];
+    s16x4_t g, g2;
+    if constexpr (DT == 0) {
+      g = words(w0, w1);
+    } else {
+      const float f0 = to_f<2>(w0 & 0xffffu), f1 = to_f<2>(w0 >> 16), f2 = to_f<2>(w1 & 0xffffu), f3 = to_f<2>(w1 >> 16);
+      const uint32_t a = pack2bf(f0, f1), b = pack2bf(f2, f3);
+      g = words(a, b);
+      g2 = words(pack2bf(f0 - bf_lo(a), f1 - bf_hi(a)), pack2bf(f2 - bf_lo(b), f3 - bf_hi(b)));
+    }
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+      if (DT == 2 && p < 2) acc = tall ? mfma16(q[u][p], g2, acc) : mfma16(g2, q[u][p], acc);
+      acc = tall ? mfma16(q[u][p], g, acc) : mfma16(g, q[u][p], acc);
+    }
+    return acc;
+  };
+  if (J.y_tall) {
+    for (int j = 16 * cg; j < nc; j += 16 * CG) {
+      f32x4_t acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < NT; ++u) acc = dot(u, j + lo, true, acc);
+      acc = acc * scale;
+      const int i = 16 * t + 4 * hi;   // rows i + m, column j + lo
+      if (j + lo < nc) st_run16<DT, 4>(y + (int64_t)(j0 + j + lo) * J.r + i, J.r - i, (const float*)&acc);
+    }
+  } else {
+    for (int j = 32 * cg; j < nc; j += 32 * CG) {
+      f32x4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      const int c = j + 8 * (lo >> 2) + (lo & 3);   // row 4 hi + m of the pair's results: columns 8 hi + m and 8 hi + 4 + m
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        acc[0] = dot(u, c, false, acc[0]);
+        acc[1] = dot(u, c + 4, false, acc[1]);
+      }
+      acc[0] = acc[0] * scale;
+      acc[1] = acc[1] * scale;
+      const int i = 16 * t + lo, k = j + 8 * hi;   // row i, columns k to k + 7
+      if (i < J.r) st_run16<DT, 8>(y + (int64_t)i * J.n + j0 + k, nc - k, (const float*)acc);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ steps of r > 64, as launches
 
 constexpr int BIG = 8, BIG_MAT = BIG * BIG * 256;   // doubles of a matrix: 64 tiles in the operand layout
 struct BigArgs {
   const double* part;
-  double *A, *P, *T, *Q, *Q2, *tr;   // [mats][BIG_MAT] (tr: [mats][8])
+  double *A, *P, *T, *Q, *Q2;   // [mats][BIG_MAT]
+  double *tr, *qscale;          // [mats][8], [mats]
   int mats;
   int first, last;
   Steps st;
@@ -526,7 +711,37 @@ SMEL_DEV bool big_map(int mats, int n, int& mat, int& k) {
   return mat < mats;
 }
 
-// the parts' sum: both mirrored tiles of A0, and the diagonal tiles' traces; a wave per upper tile
+// tile (t, u) of M N for symmetric M and N that commute
+SMEL_DEV f64x4_t big_product(const double* M, const double* N, int t, int u, int lane) {
+  f64x4_t a[BIG], b[BIG], acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < BIG; ++k) {
+    a[k] = *(const f64x4_t*)(M + ((k * BIG + t) * 64 + lane) * 4);
+    b[k] = *(const f64x4_t*)(N + ((k * BIG + u) * 64 + lane) * 4);
+  }
+  __builtin_amdgcn_sched_barrier(0);   // every load is on its way before the first product
+#pragma unroll
+  for (int k = 0; k < BIG; ++k)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc = mfma64(a[k][m], b[k][m], acc);
+  return acc;
+}
+
+// tile (t, u), t <= u, and its mirror (through the wave's own LDS tile, in the wave's order)
+SMEL_DEV void big_store(double* M, int t, int u, int lane, f64x4_t v, double* l) {
+  const int lo = lane & 15, hi = lane >> 4;
+  *(f64x4_t*)(M + ((t * BIG + u) * 64 + lane) * 4) = v;
+  if (t == u) return;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) l[(4 * m + hi) * TP + lo] = v[m];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  f64x4_t b;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) b[m] = l[lo * TP + 4 * m + hi];
+  *(f64x4_t*)(M + ((u * BIG + t) * 64 + lane) * 4) = b;
+}
+
+// the parts' sum as A0, and the diagonal tiles' traces; here and below a wave per upper tile
 __global__ __launch_bounds__(256) void big_sum_kernel(Jobs js, BigArgs g) {
   constexpr int NTL = ntiles(BIG);
   __shared__ double tile[4][16 * TP];
@@ -540,8 +755,7 @@ __global__ __launch_bounds__(256) void big_sum_kernel(Jobs js, BigArgs g) {
   f64x4_t a = {0, 0, 0, 0};
 #pragma unroll 4
   for (int s = 0; s < J.parts; ++s) a += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
-  double* const A = g.A + (int64_t)mat * BIG_MAT;
-  *(f64x4_t*)(A + ((t * BIG + u) * 64 + lane) * 4) = a;
+  big_store(g.A + (int64_t)mat * BIG_MAT, t, u, lane, a, tile[wave]);
   if (t == u) {
     double d = 0;
 #pragma unroll
@@ -549,42 +763,21 @@ __global__ __launch_bounds__(256) void big_sum_kernel(Jobs js, BigArgs g) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) d += __shfl_xor(d, o, 64);
     if (lane == 0) g.tr[mat * BIG + t] = d;
-    return;
   }
-  double* const l = tile[wave];   // the wave's own: its LDS accesses are in order
-#pragma unroll
-  for (int m = 0; m < 4; ++m) l[(4 * m + hi) * TP + lo] = a[m];
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  f64x4_t b;
-#pragma unroll
-  for (int m = 0; m < 4; ++m) b[m] = l[lo * TP + 4 * m + hi];
-  *(f64x4_t*)(A + ((u * BIG + t) * 64 + lane) * 4) = b;
 }
 
-// tile (t, u) of M N for symmetric M and N that commute
-SMEL_DEV f64x4_t big_product(const double* M, const double* N, int t, int u, int lane) {
-  f64x4_t a[BIG], b[BIG], acc = {0, 0, 0, 0};
-#pragma unroll
-  for (int k = 0; k < BIG; ++k) {
-    a[k] = *(const f64x4_t*)(M + ((k * BIG + t) * 64 + lane) * 4);
-    b[k] = *(const f64x4_t*)(N + ((k * BIG + u) * 64 + lane) * 4);
-  }
-#pragma unroll
-  for (int k = 0; k < BIG; ++k)
-#pragma unroll
-    for (int m = 0; m < 4; ++m) acc = mfma64(a[k][m], b[k][m], acc);
-  return acc;
-}
-
-// 1: P = a I + b A + c A A (first: of the scaled A, and Q = s P);  2: T = A P and Q2 = P Q;  3: A = T P
+// BIG_P: P = a I + b A + c A A (first: of the scaled A, and Q = s P);  BIG_TQ: T = A P and Q2 = P Q;  BIG_A: A = T P
 enum { BIG_P, BIG_TQ, BIG_A };
 template <int WHAT>
-__global__ __launch_bounds__(256) void big_kernel(BigArgs g) {
+__global__ __launch_bounds__(256, 2) void big_kernel(BigArgs g) {
+  constexpr int NTL = ntiles(BIG);
+  __shared__ double tile[4][16 * TP];
   int mat, kb;
-  if (!big_map(g.mats, 16, mat, kb)) return;
+  if (!big_map(g.mats, NTL / 4, mat, kb)) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
-  const int k = kb * 4 + wave, t = k / BIG, u = k % BIG;
-  const int64_t base = (int64_t)mat * BIG_MAT, at = base + (k * 64 + lane) * 4;
+  int t, u;
+  tile_of(kb * 4 + wave, BIG, t, u);
+  const int64_t base = (int64_t)mat * BIG_MAT, at = base + ((t * BIG + u) * 64 + lane) * 4;
   double s = 1.0;
   if (g.first) {   // the trace is the squared norm
     double tr = 0;
@@ -600,16 +793,19 @@ __global__ __launch_bounds__(256) void big_kernel(BigArgs g) {
     if (g.st.steps > 0) {
       const f64x4_t aa = big_product(g.A + base, g.A + base, t, u, lane);
       p = g.st.a * p + g.st.b * (*(const f64x4_t*)(g.A + at) * s2) + g.st.c * (aa * s2 * s2);
-      *(f64x4_t*)(g.P + at) = p;
+      big_store(g.P + base, t, u, lane, p, tile[wave]);
     }
-    if (g.first) *(f64x4_t*)(g.Q + at) = p * s;
+    if (g.first) {
+      const int ex = exp_of(s);
+      big_store(g.Q + base, t, u, lane, p * ldexp(s, -ex), tile[wave]);
+      if (kb == 0 && threadIdx.x == 0) g.qscale[mat] = ldexp(1.0, ex);
+    }
   } else if constexpr (WHAT == BIG_TQ) {
-    if (blockIdx.y == 0 && !g.last) *(f64x4_t*)(g.T + at) = big_product(g.A + base, g.P + base, t, u, lane) * s2;
-    if (blockIdx.y == 1 || g.last) {
-      if (!g.first) *(f64x4_t*)(g.Q2 + at) = big_product(g.P + base, g.Q + base, t, u, lane);
-    }
+    if (blockIdx.y == 0 && !g.last) big_store(g.T + base, t, u, lane, big_product(g.A + base, g.P + base, t, u, lane) * s2, tile[wave]);
+    if (!g.first && (blockIdx.y == 1 || g.last))
+      big_store(g.Q2 + base, t, u, lane, big_product(g.P + base, g.Q + base, t, u, lane), tile[wave]);
   } else {
-    *(f64x4_t*)(g.A + at) = big_product(g.T + base, g.P + base, t, u, lane);
+    big_store(g.A + base, t, u, lane, big_product(g.T + base, g.P + base, t, u, lane), tile[wave]);
   }
 }
 
@@ -720,12 +916,13 @@ int64_t part_bytes(const Plan& p, int nt) { return p.gblocks * ntiles(nt) * 2048
 int64_t ws_bytes_of(const Plan& p, int nt) {
   const int64_t parts = part_bytes(p, nt);
   if (nt <= 2) return parts;
-  if (nt == 4) return parts + p.mats * nt * nt * 2048;
-  return parts + p.mats * (5 * BIG_MAT + BIG) * 8;
+  if (nt == 4) return parts + p.mats * (nt * nt * 256 + 1) * 8;
+  return parts + p.mats * (5 * BIG_MAT + BIG + 1) * 8;
 }
 
 // the steps above r = 64; returns where Q's tiles are
-const double* run_big(const Plan& p, const Steps& st, const double* part, double* ws, hipStream_t stream) {
+const double* run_big(const Plan& p, const Steps& st, const double* part, double* ws, const double*& qscale,
+                      hipStream_t stream) {
   BigArgs g{};
   const int64_t m = p.mats * BIG_MAT;
   g.part = part;
@@ -735,6 +932,7 @@ const double* run_big(const Plan& p, const Steps& st, const double* part, double
   g.Q = ws + 3 * m;
   g.Q2 = ws + 4 * m;
   g.tr = ws + 5 * m;
+  qscale = g.qscale = g.tr + p.mats * BIG;
   g.mats = (int)p.mats;
   g.st = st;
   const unsigned groups = (unsigned)((p.mats + NXCD - 1) / NXCD * NXCD);
@@ -742,15 +940,20 @@ const double* run_big(const Plan& p, const Steps& st, const double* part, double
   for (int it = 0; it == 0 || it < st.steps; ++it) {
     g.first = it == 0;
     g.last = it + 1 >= st.steps;
-    big_kernel<BIG_P><<<groups * 16, 256, 0, stream>>>(g);
+    big_kernel<BIG_P><<<groups * (ntiles(BIG) / 4), 256, 0, stream>>>(g);
     if (g.first && g.last) break;
-    big_kernel<BIG_TQ><<<dim3(groups * 16, g.first || g.last ? 1 : 2), 256, 0, stream>>>(g);
+    big_kernel<BIG_TQ><<<dim3(groups * (ntiles(BIG) / 4), g.first || g.last ? 1 : 2), 256, 0, stream>>>(g);
     if (!g.first) std::swap(g.Q, g.Q2);
-    if (!g.last) big_kernel<BIG_A><<<groups * 16, 256, 0, stream>>>(g);
+    if (!g.last) big_kernel<BIG_A><<<groups * (ntiles(BIG) / 4), 256, 0, stream>>>(g);
   }
   return g.Q;
 }
 
+template <int NT, int DT, bool SMALL>
+void run_apply(const Plan& p, const Steps& st, const double* in, const double* qscale, hipStream_t stream) {
+  if constexpr (DT == 1) apply_kernel<NT, DT, SMALL><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, st, in, qscale);
+  else apply16_kernel<NT, DT, SMALL><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, st, in, qscale);
+}
 template <int NT, int DT>
 int run(const Plan& p, const Steps& st, void* ws, hipStream_t stream) {
   const Jobs& js = p.js;
@@ -758,12 +961,15 @@ int run(const Plan& p, const Steps& st, void* ws, hipStream_t stream) {
   double* const rest = (double*)((char*)ws + part_bytes(p, NT));
   gram_kernel<NT, DT><<<(unsigned)p.gblocks, 64 * WAVES, 0, stream>>>(js, part);
   if constexpr (NT <= 2) {
-    apply_kernel<NT, DT, true><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(js, st, part);
+    run_apply<NT, DT, true>(p, st, part, nullptr, stream);
+  } else if constexpr (NT == 4) {
+    double* const qscale = rest + p.mats * NT * NT * 256;
+    iterate_kernel<NT><<<(unsigned)p.mats, 64 * it_waves(NT), 0, stream>>>(js, st, part, rest, qscale);
+    run_apply<NT, DT, false>(p, st, rest, qscale, stream);
   } else {
-    const double* Q = rest;
-    if constexpr (NT == 4) iterate_kernel<NT><<<(unsigned)p.mats, 64 * it_waves(NT), 0, stream>>>(js, st, part, rest);
-    else Q = run_big(p, st, part, rest, stream);
-    apply_kernel<NT, DT, false><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(js, st, Q);
+    const double* qscale = nullptr;
+    const double* const Q = run_big(p, st, part, rest, qscale, stream);
+    run_apply<NT, DT, false>(p, st, Q, qscale, stream);
   }
   return smel::launch_status();
 }
