@@ -41,13 +41,13 @@ struct Job {
   int32_t batch, r, n;
   int32_t blk0, mat0;  // first block (gram, apply) and first matrix (iterate, Q)
   int32_t slices;      // of a matrix
-  int32_t gblk0, parts;   // gram: first block, blocks of a matrix (each takes js.per slices)
+  int32_t gblk0, gslices, parts;   // gram: first block, slices and blocks of a matrix (each takes js.per slices)
   int32_t x_tall;      // 1: the short side has the unit stride in x
   int32_t y_tall;      // 1: the short side is y's last
 };
 struct Jobs {
-  int32_t n, slice;    // jobs; columns of a slice (a multiple of 64)
-  int32_t per, pad_;   // slices of a gram block
+  int32_t n, lg;      // jobs; log2 of the columns of an apply block's slice (64 at least)
+  int32_t glg, per;   // log2 of the columns of a gram slice; slices of a gram block
   Job j[MAX_JOBS];
 };
 static_assert(sizeof(Jobs) <= 3584, "kernel arguments");
@@ -77,13 +77,6 @@ template <>
 struct Elem<1> {
   typedef float T;
 };
-template <int DT>
-SMEL_DEV float ld_elem(const typename Elem<DT>::T* p) {
-  if constexpr (DT == 1)
-    return *p;
-  else
-    return to_f<DT>(*p);
-}
 template <int DT>
 SMEL_DEV void st_elem(typename Elem<DT>::T* p, double v) {
   const float f = (float)v;
@@ -133,72 +126,112 @@ SMEL_DEV void st_run(typename Elem<DT>::T* p, int left, const double* v) {
     if (k < left) st_elem<DT>(p + k, v[k]);
 }
 
-// V consecutive elements as floats: one 16-byte load at any alignment, element by element where fewer than V are left
 template <int DT>
 struct Vec {
-  static constexpr int V = DT == 1 ? 4 : 8;
+  static constexpr int V = DT == 1 ? 4 : 8;   // elements of 16 bytes
 };
+// V consecutive elements as stored (16 bytes), zeros past `left`; 16-byte loads at any alignment
 template <int DT>
-SMEL_DEV void ld_vec(const typename Elem<DT>::T* p, int left, float v[Vec<DT>::V]) {
+SMEL_DEV u32x4_t ld_raw(const typename Elem<DT>::T* p, int left) {
   constexpr int V = Vec<DT>::V;
   if (left >= V) {
-    if constexpr (DT == 1) {
-      const f32x4_t q = *(const f32x4_a4*)p;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = q[k];
-    } else {
-      const u32x4_t q = *(const u32x4_a2*)p;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = to_f<DT>((k & 1) ? q[k >> 1] >> 16 : q[k >> 1] & 0xffffu);
-    }
-    return;
+    if constexpr (DT == 1)
+      return __builtin_bit_cast(u32x4_t, (f32x4_t)*(const f32x4_a4*)p);
+    else
+      return *(const u32x4_a2*)p;
   }
+  if (left <= 0) return u32x4_t{0, 0, 0, 0};
+  uint32_t v[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = k < left ? ld_elem<DT>(p + k) : 0.f;
+  for (int k = 0; k < V; ++k) {
+    const auto e = p[min(k, left - 1)];   // in range; dropped past it
+    if constexpr (DT == 1)
+      v[k] = k < left ? __float_as_uint(e) : 0u;
+    else
+      v[k] = k < left ? (uint32_t)e : 0u;
+  }
+  if constexpr (DT == 1)
+    return u32x4_t{v[0], v[1], v[2], v[3]};
+  else
+    return u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+}
+template <int DT>
+SMEL_DEV float raw_at(const u32x4_t& r, int k) {
+  if constexpr (DT == 1)
+    return __uint_as_float(r[k]);
+  else
+    return to_f<DT>((k & 1) ? r[k >> 1] >> 16 : r[k >> 1] & 0xffffu);
 }
 
-// columns [j0, j0 + slice) of a matrix as fp32 X[i][j] in LDS, rows [r, 16 NT) and columns past n zero. The pitch of slice + 20
-// floats (20 mod 64 banks) keeps the 16 rows of a gram operand and the 16 columns x 4 chunks of a transposed store apart.
-template <int NT, int DT>
-SMEL_DEV void load_slice(const Job& J, int mat, int j0, int slice, float* X, int pitch) {
-  typedef typename Elem<DT>::T T;
-  constexpr int V = Vec<DT>::V, RP = 16 * NT;
-  const T* const x = (const T*)J.x + mat * J.xb;
-  const int nc = min(slice, J.n - j0);
-  const int chunks = RP * slice / V;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
-    float v[V];
-    if (J.x_tall) {   // lines along i: 16 lanes take a chunk of 16 lines
-      constexpr int Q = RP / V;
-      const int j = e / (16 * Q) * 16 + (e & 15), i = (e >> 4) % Q * V;
-      ld_vec<DT>(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0, v);
+// Columns [j0, j0 + slice) of a matrix on the way to LDS, where they lie as fp32 X[i][j], rows [r, 16 NT) and columns past n
+// zero: fetch issues the loads, put converts and writes. W waves; slice <= S. The pitch of slice + 20 floats (20 mod 64
+// banks) keeps the 16 rows of a gram operand and the 16 columns x 4 chunks of a transposed store apart.
+template <int NT, int DT, int W, int S>
+struct Slice {
+  static constexpr int V = Vec<DT>::V, RP = 16 * NT, CH = (RP * S / V + 64 * W - 1) / (64 * W);
+  static constexpr int LV = V == 4 ? 2 : 3;
+  u32x4_t raw[CH];
+
+  // row and column of chunk e (lines along i: 16 lanes take a chunk of 16 lines)
+  SMEL_DEV static int row(bool tall, int e, int lg) { return tall ? (e >> 4) % (RP / V) * V : e >> (lg - LV); }
+  SMEL_DEV static int col(bool tall, int e, int lg) { return tall ? e / (16 * RP / V) * 16 + (e & 15) : (e << LV) & ((1 << lg) - 1); }
+  SMEL_DEV void fetch(const Job& J, int mat, int j0, int lg) {
+    const int slice = 1 << lg;
+    typedef typename Elem<DT>::T T;
+    const T* const x = (const T*)J.x + mat * J.xb;
+    const int nc = min(slice, J.n - j0);
 #pragma unroll
-      for (int k = 0; k < V; ++k) X[(i + k) * pitch + j] = v[k];
-    } else {
-      const int c = slice / V, i = e / c, j = e % c * V;
-      ld_vec<DT>(x + i * J.ld + j0 + j, i < J.r ? nc - j : 0, v);
-#pragma unroll
-      for (int k = 0; k < V; k += 4) *(f32x4_t*)(X + i * pitch + j + k) = f32x4_t{v[k], v[k + 1], v[k + 2], v[k + 3]};
+    for (int q = 0; q < CH; ++q) {
+      const int e = threadIdx.x + q * 64 * W;
+      const int i = row(J.x_tall, e, lg), j = col(J.x_tall, e, lg);
+      if (e >= (RP << lg) / V) continue;
+      if (J.x_tall)
+        raw[q] = ld_raw<DT>(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0);
+      else
+        raw[q] = ld_raw<DT>(x + i * J.ld + j0 + j, i < J.r ? nc - j : 0);
     }
   }
-}
+  SMEL_DEV void put(bool tall, int lg, float* X, int pitch) const {
+#pragma unroll
+    for (int q = 0; q < CH; ++q) {
+      const int e = threadIdx.x + q * 64 * W;
+      const int i = row(tall, e, lg), j = col(tall, e, lg);
+      if (e >= (RP << lg) / V) continue;
+      if (tall) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) X[(i + k) * pitch + j] = raw_at<DT>(raw[q], k);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k += 4)
+          *(f32x4_t*)(X + i * pitch + j + k) = f32x4_t{raw_at<DT>(raw[q], k), raw_at<DT>(raw[q], k + 1), raw_at<DT>(raw[q], k + 2),
+                                                       raw_at<DT>(raw[q], k + 3)};
+      }
+    }
+  }
+};
 
-// columns of a slice at most: two blocks on a CU
+// columns of an apply block's slice at most: two blocks on a CU
 constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt <= 4 ? 256 : 128; }
 constexpr int slice_bytes(int nt) { return 16 * nt * (max_slice(nt) + 20) * 4; }
 
+// A gram block takes `per` slices, the next one on its way while one is multiplied (two buffers). Waves of a block: the
+// upper tiles in TG groups, a group's columns dealt to the others. Three tiles a wave at r = 128: nine leave registers for two
+// waves a SIMD, too few to cover the operands' latencies (36 x 128 x 2816: 65 us, three: 55; one round of blocks with the
+// loads ahead: see the plan's `per`).
+constexpr int gram_slice(int nt) { return nt == 1 ? 512 : nt == 2 ? 256 : nt == 4 ? 128 : 64; }
+constexpr int gram_waves(int nt) { return nt == 8 ? 12 : WAVES; }
+constexpr int gram_tg(int nt) { return nt == 8 ? 12 : nt == 4 ? 2 : 1; }
+
 template <int NT, int DT>
-__global__ __launch_bounds__(64 * WAVES, 4) void gram_kernel(Jobs js, double* __restrict__ part) {
-  constexpr int NTL = ntiles(NT);
-  __shared__ __attribute__((aligned(16))) char smem[slice_bytes(NT)];
-  static_assert(slice_bytes(NT) >= NTL * 2048, "room for the column groups' sums");
-  constexpr int TG = NT == 8 ? 4 : NT == 4 ? 2 : 1, KG = WAVES / TG, TPW = NTL / TG;
-  static_assert(TPW * TG == NTL, "tiles per wave");
-  float* const X = (float*)smem;
-  const int pitch = js.slice + 20;
+__global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, double* __restrict__ part) {
+  constexpr int NTL = ntiles(NT), W = gram_waves(NT), TG = gram_tg(NT), KG = W / TG, TPW = NTL / TG;
+  constexpr int S = gram_slice(NT), BUF = 16 * NT * (S + 20);
+  static_assert(TPW * TG == NTL && KG * TG == W, "tiles per wave");
+  static_assert(2 * BUF * 4 >= NTL * 2048 || KG == 1, "room for the column groups' sums");
+  __shared__ __attribute__((aligned(16))) float X[2 * BUF];
+  const int lg = js.glg, slice = 1 << lg, pitch = slice + 20;
   const Job& J = js.j[find_job<BY_GRAM>(js, blockIdx.x)];
-  const int lb = blockIdx.x - J.gblk0, mat = lb / J.parts, s0 = lb % J.parts * js.per;
+  const int lb = blockIdx.x - J.gblk0, mat = lb / J.parts, s0 = lb % J.parts * js.per, s1 = min(s0 + js.per, J.gslices);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int tg = wave % TG, kg = wave / TG;
   f64x4_t acc[TPW];
@@ -211,25 +244,29 @@ __global__ __launch_bounds__(64 * WAVES, 4) void gram_kernel(Jobs js, double* __
     ra[k] = (16 * t + lo) * pitch + 4 * hi;
     rb[k] = (16 * u + lo) * pitch + 4 * hi;
   }
-  for (int sl = s0; sl < min(s0 + js.per, J.slices); ++sl) {
-    if (sl > s0) __syncthreads();
-    load_slice<NT, DT>(J, mat, sl * js.slice, js.slice, X, pitch);
-    __syncthreads();
+  Slice<NT, DT, W, S> in;
+  in.fetch(J, mat, s0 << lg, lg);
+  in.put(J.x_tall, lg, X, pitch);
+  __syncthreads();
+  for (int sl = s0; sl < s1; ++sl) {
+    const float* const x = X + ((sl - s0) & 1) * BUF;
+    if (sl + 1 < s1) in.fetch(J, mat, (sl + 1) << lg, lg);
     // 16 columns a step, four to a lane: which columns make one instruction's contraction does not matter
-    for (int j = 16 * kg; j < js.slice; j += 16 * KG)
+    for (int j = 16 * kg; j < slice; j += 16 * KG)
 #pragma unroll
       for (int k = 0; k < TPW; ++k) {
-        const f32x4_t a = *(const f32x4_t*)(X + ra[k] + j), b = *(const f32x4_t*)(X + rb[k] + j);
+        const f32x4_t a = *(const f32x4_t*)(x + ra[k] + j), b = *(const f32x4_t*)(x + rb[k] + j);
 #pragma unroll
         for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
-        if (k % 3 == 2) __builtin_amdgcn_sched_barrier(0);   // no more operands ahead than registers for two blocks a CU
       }
+    if (sl + 1 < s1) in.put(J.x_tall, lg, X + ((sl + 1 - s0) & 1) * BUF, pitch);
+    __syncthreads();
   }
   // the column groups' sums, in group order
-  f64x4_t* const red = (f64x4_t*)smem;   // [TG][TPW][64]
+  f64x4_t* const red = (f64x4_t*)X;   // [TG][TPW][64]
   double* const out = part + (J.part0 + lb) * (int64_t)(NTL * 256);
   for (int g = 1; g < KG; ++g) {
-    __syncthreads();
+    if (g > 1) __syncthreads();
     if (kg == g)
 #pragma unroll
       for (int k = 0; k < TPW; ++k) red[(tg * TPW + k) * 64 + lane] = acc[k];
@@ -283,6 +320,7 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
     tile_of(wave * TPW + k, NT, tt[k], uu[k]);
     A[k] = f64x4_t{0, 0, 0, 0};
     const double* p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + ((wave * TPW + k) * 64 + lane) * 4;
+#pragma unroll 8
     for (int s = 0; s < J.parts; ++s) A[k] += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
     if (tt[k] == uu[k]) {   // the tile's trace: row 4 m + hi, column lo
       double d = 0;
@@ -372,8 +410,9 @@ __global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Ste
 // is the operand layout.
 template <int NT>
 SMEL_DEV double steps_small(const Job& J, int mat, const Steps& st, const double* __restrict__ part, f64x4_t (*bA)[64],
-                          f64x4_t (*bP)[64], f64x4_t (*bT)[64], f64x4_t (*bQ)[64], double* tr) {
-  constexpr int NTL = ntiles(NT);
+                            double* tr) {
+  constexpr int NTL = ntiles(NT), N2 = NT * NT;
+  f64x4_t(*const bP)[64] = bA + N2, (*const bT)[64] = bA + 2 * N2, (*const bQ)[64] = bA + 3 * N2;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const bool mine = wave < NT * NT;
   const int t = wave / NT, u = wave % NT;
@@ -381,18 +420,29 @@ SMEL_DEV double steps_small(const Job& J, int mat, const Steps& st, const double
   f64x4_t eye;
 #pragma unroll
   for (int m = 0; m < 4; ++m) eye[m] = t == u && 4 * m + hi == lo ? 1.0 : 0.0;
+  // the parts' sum: GR groups of waves take every GR-th part of an upper tile each, then the groups in order
+  constexpr int GR = NT == 1 ? 4 : 2;
+  static_assert(GR * NTL <= 4 * NT * NT && GR * NTL <= WAVES, "slots and waves of the sum");
+  if (wave < GR * NTL) {
+    const int g = wave / NTL;
+    const double* const p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + (wave % NTL) * 256 + lane * 4;
+#pragma unroll 8
+    for (int s = g; s < J.parts; s += GR) A += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
+    bA[wave][lane] = A;     // bA to bQ are one array
+  }
+  __syncthreads();
   if (mine) {
     // a lower tile is its mirror's transpose: element (4 m + hi, lo) is register lo / 4 of lane (lo % 4, 4 m + hi)
     const int k = t <= u ? tile_at(t, u, NT) : tile_at(u, t, NT);
-    const double* const p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + k * 256;
-#pragma unroll 4
-    for (int s = 0; s < J.parts; ++s) {
-      const double* const q = p + (int64_t)s * (NTL * 256);
+    A = f64x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const f64x4_t(&q)[64] = bA[g * NTL + k];
       if (t <= u) {
-        A += *(const f64x4_t*)(q + lane * 4);
+        A += q[lane];
       } else {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) A[m] += q[((lo & 3) * 16 + 4 * m + hi) * 4 + (lo >> 2)];
+        for (int m = 0; m < 4; ++m) A[m] += ((const double*)q)[((lo & 3) * 16 + 4 * m + hi) * 4 + (lo >> 2)];
       }
     }
     double d = 0;
@@ -469,22 +519,26 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
   typedef typename Elem<DT>::T T;
   constexpr int CG = WAVES / NT;
   float* const X = (float*)smem;
-  const int pitch = js.slice + 20;
+  const int slice = 1 << js.lg, pitch = slice + 20;
   const Job& J = js.j[find_job<BY_APPLY>(js, blockIdx.x)];
-  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = lb % J.slices * js.slice;
+  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = (lb % J.slices) << js.lg;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int t = wave % NT, cg = wave / NT;
   const int perm = 4 * (lo & 3) + (lo >> 2);   // row 4 m + hi of the result <- index 4 hi + m
   const int qlane = J.y_tall ? hi * 16 + perm : lane;
-  load_slice<NT, DT>(J, mat, j0, js.slice, X, pitch);
+  {
+    Slice<NT, DT, WAVES, max_slice(NT)> in;
+    in.fetch(J, mat, j0, js.lg);
+    in.put(J.x_tall, js.lg, X, pitch);
+  }
   f64x4_t q[NT];
   double scale;
   if constexpr (SMALL) {
-    __shared__ f64x4_t b[4][NT * NT][64];
+    __shared__ f64x4_t b[4 * NT * NT][64];
     __shared__ double tr[NT];
-    scale = steps_small<NT>(J, mat, st, in, b[0], b[1], b[2], b[3], tr);   // ends with a barrier: X and b[3] are there
+    scale = steps_small<NT>(J, mat, st, in, b, tr);   // ends with a barrier: X and Q's tiles are there
 #pragma unroll
-    for (int u = 0; u < NT; ++u) q[u] = b[3][u * NT + t][qlane];
+    for (int u = 0; u < NT; ++u) q[u] = b[(3 * NT + u) * NT + t][qlane];
   } else {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -494,7 +548,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
   }
 #pragma unroll
   for (int u = 0; u < NT; ++u) q[u] = q[u] * scale;
-  const int nc = min(js.slice, J.n - j0);
+  const int nc = min(slice, J.n - j0);
   T* const y = (T*)J.y + (int64_t)mat * J.r * J.n;
   if (J.y_tall) {
     for (int j = 16 * cg; j < nc; j += 16 * CG) {
@@ -533,17 +587,10 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 SMEL_DEV f32x4_t mfma16(s16x4_t a, s16x4_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
 SMEL_DEV s16x4_t words(uint32_t a, uint32_t b) { return __builtin_bit_cast(s16x4_t, (u32x2_t{a, b})); }
 
-// 8 consecutive 16-bit elements as stored, zeros past `left`
-SMEL_DEV u32x4_t ld_raw8(const uint16_t* p, int left) {
-  if (left >= 8) return *(const u32x4_a2*)p;
-  uint32_t v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : 0u;
-  return u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
-}
 template <int NT>
-SMEL_DEV void load_pairs(const Job& J, int mat, int j0, int slice, uint32_t* X, int pitch) {
+SMEL_DEV void load_pairs(const Job& J, int mat, int j0, int lg, uint32_t* X, int pitch) {
   constexpr int RP = 16 * NT;
+  const int slice = 1 << lg;
   const uint16_t* const x = (const uint16_t*)J.x + mat * J.xb;
   const int nc = min(slice, J.n - j0);
   if (J.x_tall) {
@@ -552,17 +599,17 @@ SMEL_DEV void load_pairs(const Job& J, int mat, int j0, int slice, uint32_t* X, 
 #pragma unroll 4
     for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
       const int j = e / (16 * Q) * 16 + (e & 15), i = (e >> 4) % Q * 8;
-      const u32x4_t v = ld_raw8(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0);
+      const u32x4_t v = ld_raw<0>(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k) X[(i / 2 + k) * pitch + j] = v[k];
     }
   } else {
-    const int c = slice / 8, chunks = RP / 2 * c;
+    const int chunks = RP / 2 << (lg - 3);
 #pragma unroll 2
     for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
-      const int p = e / c, j = e % c * 8;
+      const int p = e >> (lg - 3), j = (e << 3) & (slice - 1);
       const uint16_t* const row = x + 2 * p * J.ld + j0 + j;
-      const u32x4_t a = ld_raw8(row, 2 * p < J.r ? nc - j : 0), b = ld_raw8(row + J.ld, 2 * p + 1 < J.r ? nc - j : 0);
+      const u32x4_t a = ld_raw<0>(row, 2 * p < J.r ? nc - j : 0), b = ld_raw<0>(row + J.ld, 2 * p + 1 < J.r ? nc - j : 0);
       u32x4_t w[2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -602,12 +649,12 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps s
                                                           const double* __restrict__ qscale) {
   constexpr int CG = WAVES / NT;
   __shared__ __attribute__((aligned(16))) uint32_t X[8 * NT * (max_slice(NT) + 8)];
-  const int pitch = js.slice + 8;
+  const int slice = 1 << js.lg, pitch = slice + 8;
   const Job& J = js.j[find_job<BY_APPLY>(js, blockIdx.x)];
-  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = lb % J.slices * js.slice;
+  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = (lb % J.slices) << js.lg;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int t = wave % NT, cg = wave / NT;
-  load_pairs<NT>(J, mat, j0, js.slice, X, pitch);
+  load_pairs<NT>(J, mat, j0, js.lg, X, pitch);
   float scale;
   s16x4_t q[NT][3];   // parts of Q[16 t + lo][16 u + 4 hi + 0..3]
   auto parts = [&](int u, const double (&v)[4]) {
@@ -626,12 +673,12 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps s
   };
   // element (4 hi + k, lo) of tile (u, t): register hi of lane (k, lo)
   if constexpr (SMALL) {
-    __shared__ f64x4_t b[4][NT * NT][64];
+    __shared__ f64x4_t b[4 * NT * NT][64];
     __shared__ double tr[NT];
-    scale = (float)steps_small<NT>(J, mat, st, in, b[0], b[1], b[2], b[3], tr);
+    scale = (float)steps_small<NT>(J, mat, st, in, b, tr);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const double* const f = (const double*)b[3][u * NT + t];
+      const double* const f = (const double*)b[(3 * NT + u) * NT + t];
       parts(u, {f[lo * 4 + hi], f[(16 + lo) * 4 + hi], f[(32 + lo) * 4 + hi], f[(48 + lo) * 4 + hi]});
     }
   } else {
@@ -644,7 +691,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps s
     }
     __syncthreads();
   }
-  const int nc = min(js.slice, J.n - j0);
+  const int nc = min(slice, J.n - j0);
   uint16_t* const y = (uint16_t*)J.y + (int64_t)mat * J.r * J.n;
   // acc += Q G (or its transpose) for column c of the lane
   auto dot = [&](int u, int c, bool tall, f32x4_t acc) {
@@ -753,7 +800,7 @@ __global__ __launch_bounds__(256) void big_sum_kernel(Jobs js, BigArgs g) {
   tile_of(kb * 4 + wave, BIG, t, u);
   const double* const p = g.part + (J.part0 + (int64_t)(mat - J.mat0) * J.parts) * (NTL * 256) + ((kb * 4 + wave) * 64 + lane) * 4;
   f64x4_t a = {0, 0, 0, 0};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < J.parts; ++s) a += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
   big_store(g.A + (int64_t)mat * BIG_MAT, t, u, lane, a, tile[wave]);
   if (t == u) {
@@ -844,7 +891,6 @@ struct Cursor {
   int64_t mat;
 };
 constexpr int64_t MAX_MATS = 65536, BIG_MATS = 256;   // of a launch; its workspace is 0.6 MB a matrix above r = 64
-constexpr int64_t GRAM_BLOCKS = 512;                  // two a CU
 
 // the next jobs of one (tiles a side, dtype) from `at` on, as many as a launch takes (a job's batch may be split)
 Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Plan& p) {
@@ -870,13 +916,28 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
     at.mat += take;
     if (at.mat == j.batch) at = Cursor{at.job + 1, 0};
   }
-  // the largest slices that give two blocks to a CU, but at least 128 columns (each wave a block of 16)
+  // the largest slices that give most CUs a block, but at least 128 columns (each wave a block of 16); up to r = 32 every
+  // block runs the steps, and two on a CU get in each other's way (a layer's 84 updates: 20.7 us with 780 blocks, 14.4 with 195)
   int slice = max_slice(nt);
-  while (slice > 128 && cols / slice < 512) slice /= 2;
-  p.js.slice = slice;
-  p.js.per = 1;
-  // the parts of A0 cost 2 KB a tile: above r = 64 (72 KB) a gram block takes several slices
-  if (nt == 8) p.js.per = (int)std::max<int64_t>(1, cols / slice / GRAM_BLOCKS);
+  while (slice > 128 && cols / slice < 192) slice /= 2;
+  p.js.lg = __builtin_ctz(slice);
+  // gram: likewise, down to 64 columns at r > 64; then one round of blocks (two on a CU, one at r > 64, whose blocks fill it
+  // and whose parts are 72 KB each)
+  int gs = gram_slice(nt);
+  while (gs > 128 && cols / gs < 512) gs /= 2;
+  p.js.glg = __builtin_ctz(gs);
+  const int64_t round = nt == 8 ? 256 : 512;
+  p.js.per = (int)std::max<int64_t>(1, cols / gs / round);
+  for (;;) {
+    int64_t blocks = 0;
+    for (int k = 0; k < p.js.n; ++k) {
+      const smel_ortho_job& j = jobs[taken[k].job];
+      const int64_t n = j.rows < j.cols ? j.cols : j.rows;
+      blocks += taken[k].count * ((n + gs * p.js.per - 1) / (gs * p.js.per));
+    }
+    if (blocks <= round || blocks <= p.mats) break;   // or a block a matrix
+    ++p.js.per;
+  }
   int64_t mats = 0;
   for (int k = 0; k < p.js.n; ++k) {
     const smel_ortho_job& j = jobs[taken[k].job];
@@ -899,7 +960,8 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
       o.x_tall = wide;
     }
     o.slices = (o.n + slice - 1) / slice;
-    o.parts = (o.slices + p.js.per - 1) / p.js.per;
+    o.gslices = (o.n + gs - 1) / gs;
+    o.parts = (o.gslices + p.js.per - 1) / p.js.per;
     o.blk0 = (int32_t)p.blocks;
     o.gblk0 = (int32_t)p.gblocks;
     o.mat0 = (int32_t)mats;
@@ -907,7 +969,7 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
     mats += o.batch;
     p.blocks += (int64_t)o.batch * o.slices;
     p.gblocks += (int64_t)o.batch * o.parts;
-    if (p.blocks >= (int64_t)1 << 22) return Cursor{-1, 0};   // 512 threads each: a launch takes fewer than 2^32
+    if (p.blocks >= (int64_t)1 << 22) return Cursor{-1, 0};   // 768 threads each at most: a launch takes fewer than 2^32
   }
   return at;
 }
@@ -959,7 +1021,7 @@ int run(const Plan& p, const Steps& st, void* ws, hipStream_t stream) {
   const Jobs& js = p.js;
   double* const part = (double*)ws;
   double* const rest = (double*)((char*)ws + part_bytes(p, NT));
-  gram_kernel<NT, DT><<<(unsigned)p.gblocks, 64 * WAVES, 0, stream>>>(js, part);
+  gram_kernel<NT, DT><<<(unsigned)p.gblocks, 64 * gram_waves(NT), 0, stream>>>(js, part);
   if constexpr (NT <= 2) {
     run_apply<NT, DT, true>(p, st, part, nullptr, stream);
   } else if constexpr (NT == 4) {
