@@ -10,9 +10,12 @@
 // alignment, which the hardware takes at any address, so odd row lengths and views at any offset run the same code; only
 // a row's last, partial chunk goes element by element.
 //
-// Backward: blocks walk over the rows with a stride, each thread keeping the dw and db sums of its columns in registers;
-// the block's row groups are joined through LDS in a tree, the blocks' sums go to the workspace and a second kernel adds
-// them in block order. No atomics: every result repeats bit for bit. HBM-bound.
+// Backward: blocks walk over the rows with a stride, each thread keeping the weights and the dw and db sums of its columns in
+// registers and four rows (16-bit) on their way; the block's row groups are joined through LDS in a tree, the blocks' sums go
+// to the workspace and a second kernel adds them in block order. No atomics: every result repeats bit for bit. A chunk per
+// thread and a block per row, not a wave per row with four chunks: 209 registers there let two waves on a SIMD and every row
+// read the weights twice more (32749 x 2048 bf16: 119 us; a block per row 108, with four rows on their way 91).
+// HBM-bound: forward 4.9 TB/s, backward 4.4 TB/s at 32749 x 2048 bf16 (a copy reaches 5.55).
 #include "../../include/smel_norm.h"
 #include "abi_util.h"
 #include "common.h"
@@ -147,22 +150,22 @@ SMEL_DEV void weight8(const void* p, int e0, int n, float one, float v[8]) {
   for (int j = 0; j < 8; ++j) v[j] = r.at(j);
 }
 
-// sums over the lpr threads of a row: xor butterfly over its lanes, then (a block per row) the waves in order
+// sums over the lpr threads of a row: xor butterfly over its lanes, then the row's waves in order. red: 16 floats a value
 template <int N>
 SMEL_DEV void row_sums(float (&v)[N], int lpr, float* red) {
   for (int o = 1; o < lpr && o < 64; o <<= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
   if (lpr > 64) {
-    const int nw = blockDim.x >> 6;
+    const int wave = threadIdx.x >> 6, nw = lpr >> 6, w0 = wave & ~(nw - 1);
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) red[i * 16 + (threadIdx.x >> 6)] = v[i];
-    __syncthreads();
+      for (int i = 0; i < N; ++i) red[i * 16 + wave] = v[i];
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = red[i * 16];
-      for (int k = 1; k < nw; ++k) v[i] += red[i * 16 + k];
+      v[i] = red[i * 16 + w0];
+      for (int k = 1; k < nw; ++k) v[i] += red[i * 16 + w0 + k];
     }
   }
 }
@@ -236,41 +239,48 @@ template <int DT, int WT, int CPL, int BS, bool WG>
 __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
   typedef typename El<DT>::T T;
   __shared__ float red[2][32];
-  __shared__ float join[WG && BS == 256 ? BS / 2 * CPL * 16 : 1];   // a 1024-thread block is one row's
+  __shared__ float join[WG && BS == 256 ? BS / 2 * CPL * 16 : 1];   // larger blocks are one row's
   const int lpr = p.lpr, n = p.cols, nch = (n + 7) >> 3;
   const int groups = BS / lpr, grp = threadIdx.x / lpr, li = threadIdx.x & (lpr - 1);
-  float dw[WG ? CPL * 8 : 1], db[WG ? CPL * 8 : 1];
+  float w[CPL][8], dw[WG ? CPL * 8 : 1], db[WG ? CPL * 8 : 1];
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) {
+    const int ck = li + lpr * k;
+    weight8<WT>(ck < nch ? p.w : nullptr, 8 * ck, n, 1.f, w[k]);
+  }
   if constexpr (WG)
 #pragma unroll
     for (int i = 0; i < CPL * 8; ++i) dw[i] = db[i] = 0.f;
-  int par = 0;
-  // every thread of the block takes the same number of turns (row_sums has barriers)
-  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < p.rows; r0 += (int64_t)gridDim.x * groups) {
-    const int64_t row = r0 + grp;
-    const bool live = row < p.rows;
-    const int64_t in = (live ? row : 0) * p.stride, out = (live ? row : 0) * (int64_t)n;
-    const float mean = live ? p.stats[2 * row] : 0.f, rstd = live ? p.stats[2 * row + 1] : 0.f;
-    Raw<DT> X[CPL], D[CPL];
+  // PF rows on their way: buffer f is refilled as soon as its row is done with, PF - 1 rows before it is used again
+  constexpr int PF = CPL == 2 ? 1 : DT == 2 ? 2 : 4;
+  struct Row {
+    Raw<DT> x[CPL], d[CPL];
+    float mean, rstd;
+  } buf[PF];
+  auto fetch = [&](Row& b, int64_t row) {
+    const bool ok = row < p.rows;
+    const int64_t in = (ok ? row : 0) * p.stride, out = (ok ? row : 0) * (int64_t)n;
+    b.mean = ok ? p.stats[2 * row] : 0.f;
+    b.rstd = ok ? p.stats[2 * row + 1] : 0.f;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) {
       const int ck = li + lpr * k;
-      X[k] = D[k] = Raw<DT>{};
-      if (live && ck < nch) {
-        X[k] = load8<DT>((const T*)p.x + in, 8 * ck, n);
-        D[k] = load8<DT>((const T*)p.dy + out, 8 * ck, n);
+      b.x[k] = b.d[k] = Raw<DT>{};
+      if (ok && ck < nch) {
+        b.x[k] = load8<DT>((const T*)p.x + in, 8 * ck, n);
+        b.d[k] = load8<DT>((const T*)p.dy + out, 8 * ck, n);
       }
     }
+  };
+  auto one = [&](Row& b, int64_t row, float* rd) {
+    const bool live = row < p.rows;
     float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      const int ck = li + lpr * k;
-      if (!(live && ck < nch)) continue;
-      float w[8];
-      weight8<WT>(p.w, 8 * ck, n, 1.f, w);
+    for (int k = 0; k < CPL; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = D[k].at(j), xhat = (X[k].at(j) - mean) * rstd;   // d is zero past the row
-        const float g = d * w[j];
+      for (int j = 0; j < 8; ++j) {   // d is zero past the row and past the last row
+        const float d = b.d[k].at(j), xhat = (b.x[k].at(j) - b.mean) * b.rstd;
+        const float g = d * w[k][j];
         sums[0] += g;
         sums[1] = fmaf(g, xhat, sums[1]);
         if constexpr (WG) {
@@ -278,21 +288,19 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
           db[k * 8 + j] += d;
         }
       }
-    }
-    row_sums(sums, lpr, red[par]);   // two buffers in turn: a row's readers are done before the next but one writes
-    par ^= 1;
-    if (!live || !p.dx) continue;
+    row_sums(sums, lpr, rd);
+    if (!live || !p.dx) return;
+    const int64_t out = row * (int64_t)n;
     const float mg = sums[0] / (float)n, mgx = sums[1] / (float)n;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) {
       const int ck = li + lpr * k;
       if (ck >= nch) continue;
-      float w[8], v[8];
-      weight8<WT>(p.w, 8 * ck, n, 1.f, w);
+      float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float xhat = (X[k].at(j) - mean) * rstd;
-        v[j] = rstd * (D[k].at(j) * w[j] - mg - xhat * mgx);
+        const float xhat = (b.x[k].at(j) - b.mean) * b.rstd;
+        v[j] = b.rstd * (b.d[k].at(j) * w[k][j] - mg - xhat * mgx);
       }
       if (p.ds) {
         const Raw<DT> S = load8<DT>((const T*)p.ds + out, 8 * ck, n);
@@ -303,7 +311,22 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
       o.set(v);
       store8<DT>((T*)p.dx + out, 8 * ck, n, o);
     }
-  }
+  };
+  const int64_t step = (int64_t)gridDim.x * groups, r1 = (int64_t)blockIdx.x * groups;
+#pragma unroll
+  for (int f = 0; f < PF; ++f) fetch(buf[f], r1 + f * step + grp);
+  // every thread of the block takes the same number of turns (row_sums has a barrier); the sums' buffers alternate: a row's
+  // readers are done before the next but one writes
+  int par = 0;
+  for (int64_t r0 = r1; r0 < p.rows; r0 += PF * step)
+#pragma unroll
+    for (int f = 0; f < PF; ++f) {
+      const int64_t row = r0 + f * step;
+      if (row >= p.rows) break;
+      one(buf[f], row + grp, red[par]);
+      par ^= 1;
+      fetch(buf[f], row + PF * step + grp);
+    }
   if constexpr (WG) {
     for (int half = groups / 2; half >= 1; half /= 2) {
       __syncthreads();
@@ -327,15 +350,18 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
     if (grp == 0) {
       float* const o = p.part + (int64_t)blockIdx.x * 2 * n;
 #pragma unroll
-      for (int k = 0; k < CPL; ++k)
+      for (int k = 0; k < CPL; ++k) {
+        const int e = 8 * (li + lpr * k);
+        if (e >= n) continue;
+        Raw<2> a, b;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int e = 8 * (li + lpr * k) + j;
-          if (e < n) {
-            o[e] = dw[k * 8 + j];
-            o[n + e] = db[k * 8 + j];
-          }
+          a.q[j >> 2][j & 3] = __float_as_uint(dw[k * 8 + j]);
+          b.q[j >> 2][j & 3] = __float_as_uint(db[k * 8 + j]);
         }
+        store8<2>(o, e, n, a);
+        store8<2>(o + n, e, n, b);
+      }
     }
   }
 }
@@ -348,6 +374,7 @@ __global__ __launch_bounds__(1024) void ln_wsum_kernel(const float* __restrict__
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
   float v = 0.f;
   if (c < 2 * n)
+#pragma unroll 8
     for (int r = wave; r < blocks; r += 16) v += part[(int64_t)r * 2 * n + c];
   red[wave][threadIdx.x & 63] = v;
   __syncthreads();
@@ -376,11 +403,23 @@ Shape shape_of(int64_t cols) {
   while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 4
   return s;
 }
+// backward: a chunk per thread where 1024 threads reach (the weights, their sums and the next row stay in registers)
+Shape bwd_shape(int64_t cols) {
+  const int nch = (int)((cols + 7) / 8);
+  Shape s{1, 1, 256};
+  while (s.lpr < nch && s.lpr < 1024) s.lpr *= 2;
+  if (s.lpr > 256) s.bs = s.lpr;
+  while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 2
+  return s;
+}
 // blocks of the backward: its weight sums cost 16 bytes a column and block
 int64_t bwd_blocks(int64_t rows, int64_t cols) {
-  const Shape s = shape_of(cols);
+  const Shape s = bwd_shape(cols);
   const int64_t turns = (rows + s.bs / s.lpr - 1) / (s.bs / s.lpr);
-  return turns < 512 ? turns : 512;
+  // three blocks a CU of 256 threads, two of 512, one of 1024, with two rows each at least. 32749 x 2048 bf16: 114 us with 512
+  // blocks, 93 with 768, 93 with 1024 (and 1 us more for their sums); 4092 x 2816 fp32: 36 with 384, 33 with 512, 44 with 640
+  const int64_t most = s.bs == 256 ? 768 : s.bs == 512 ? 512 : 256, g = (turns + 1) / 2;
+  return g < most ? g : most;
 }
 
 template <int DT, int WT, int CPL, int BS>
@@ -400,16 +439,16 @@ int launch_bwd(const LnArgs& p, hipStream_t stream) {
 }
 template <bool FWD, int DT, int WT>
 int launch_w(LnArgs& p, hipStream_t st) {
-  const Shape s = shape_of(p.cols);
+  const Shape s = FWD ? shape_of(p.cols) : bwd_shape(p.cols);
   p.lpr = s.lpr;
   if constexpr (FWD) {
     if (s.bs == 1024) return launch_fwd<DT, WT, 2, 1024>(p, st);
     return s.cpl == 1 ? launch_fwd<DT, WT, 1, 256>(p, st) : s.cpl == 2 ? launch_fwd<DT, WT, 2, 256>(p, st)
                                                                        : launch_fwd<DT, WT, 4, 256>(p, st);
   } else {
-    if (s.bs == 1024) return launch_bwd<DT, WT, 2, 1024>(p, st);
-    return s.cpl == 1 ? launch_bwd<DT, WT, 1, 256>(p, st) : s.cpl == 2 ? launch_bwd<DT, WT, 2, 256>(p, st)
-                                                                       : launch_bwd<DT, WT, 4, 256>(p, st);
+    if (s.bs == 256) return launch_bwd<DT, WT, 1, 256>(p, st);
+    if (s.bs == 512) return launch_bwd<DT, WT, 1, 512>(p, st);
+    return s.cpl == 1 ? launch_bwd<DT, WT, 1, 1024>(p, st) : launch_bwd<DT, WT, 2, 1024>(p, st);
   }
 }
 template <bool FWD>
