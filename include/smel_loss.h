@@ -99,11 +99,12 @@ int smel_ce_dequant8(const int8_t* q, const void* scale, int64_t R, int64_t C, i
  * count (mask null: all). With n_s such tokens, c[s][e] of their K picks topi[t][k] = e (ids outside [0, E) count nowhere),
  * p = softmax of the logits' row, S' the sequences with n_s > 0:
  *   loss = coef / S' * sum_s E sum_e c[s][e] / (K n_s) * mean_t p[t][e]
- * (0 without any token). Rows that do not count are not read.
+ * (0 without any token). Rows that do not count may hold anything.
  * `dtype` of the logits [T][ldl]: 0 bf16, 1 fp32, 2 fp16; topi [T][K] contiguous, int64 or int32 by topi_i64.
- * 0 <= T <= 2^25, 1 <= E <= 512, 1 <= K <= 64, 1 <= S <= 2^24.
- * Writes loss (fp32), counts (int64 [S][E]) and, for the backward, row_stats (fp32 [T][2]: a counted row's maximum and
- * 1 / its sum of exponentials; may be null without one) and weights (fp32 [S][E] and one more: coef E / (K n_s^2) (c[s][e] - sum_e c[s][e] / E), then
+ * 0 <= T <= 2^24, 1 <= E <= 512, 1 <= K <= 64, 1 <= S <= 2^24.
+ * Writes loss (fp32), counts (int64 [S][E]) and, for the backward, row_stats ([T] of 16 bytes, aligned to them: the row's
+ * maximum and 1 / its sum of exponentials (fp32), its sequence (int32, -1 where it does not count); may be null without a
+ * backward) and weights (fp32 [S][E] and one more: coef E / (K n_s^2) (c[s][e] - sum_e c[s][e] / E), then
  * 1 / S'). ws: smel_balance_ws_bytes bytes, 16-byte aligned. */
 int64_t smel_balance_ws_bytes(int64_t T, int64_t E, int64_t S);
 int smel_balance_fwd(const void* logits, int64_t ldl, int32_t dtype, const void* topi, int32_t topi_i64, int64_t T,
@@ -113,9 +114,8 @@ int smel_balance_fwd(const void* logits, int64_t ldl, int32_t dtype, const void*
 
 /* dlogits [T][E] contiguous, in the logits' dtype: go / S' p[t][e] (v[e] - sum_j p[t][j] v[j]) with v = weights of the token's
  * sequence (the counts are constants); zero rows for tokens that do not count. go: one fp32 on the device. */
-int smel_balance_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, const uint8_t* mask,
-                     const void* offsets, int32_t off_i64, int64_t S, const float* row_stats, const float* weights,
-                     const float* go, void* dlogits, hipStream_t stream);
+int smel_balance_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t S,
+                     const float* row_stats, const float* weights, const float* go, void* dlogits, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -4,12 +4,16 @@
 // v only enters through differences, so its mean is taken out first: c_e - (sum c) / E is formed from whole numbers, and a
 // balanced router's gradient is zero instead of the rounding of two equal terms.
 //
-// Forward: a block takes a chunk of tokens and walks through the sequences in it; per sequence, each wave's lanes sum the
-// softmax of its rows per expert in registers (lane: experts l, l + 64, ...), the picks are counted by integer adds in LDS,
-// and the block writes both to slot (chunk + sequence) of the workspace: along the tokens either number grows at every
-// step, so slots are distinct and a sequence's are consecutive. A second kernel (a block per sequence) adds a sequence's
-// slots in order; a third joins the sequences' losses where there are several. Sums have a fixed order, integer adds have
-// none that shows: results repeat bit for bit. Backward: one pass, a row per wave.
+// Forward: a block of 16 waves takes a chunk of tokens and walks through the sequences in it; per sequence, each wave takes four
+// tokens at a time (their loads together: a chunk is short, so a row's latency counts), its lanes sum the softmax of NE
+// neighbouring experts each in registers, the picks are counted by integer adds in LDS, and the block writes both to slot
+// (chunk + sequence) of the workspace: along the tokens either number grows at every step, so slots are distinct and a
+// sequence's are consecutive. A second kernel (a block per sequence) adds a sequence's slots, a fixed set of them per thread in
+// order; a third joins the sequences' losses where there are several. A short batch of one sequence is one block's, and one
+// launch. Sums have a fixed order, integer adds have none that shows: results repeat bit for bit. The forward leaves with every
+// token what the backward needs to take it up again (maximum, 1 / sum, sequence or none): one pass, four rows a wave.
+#include <algorithm>
+
 #include "../../include/smel_loss.h"
 #include "abi_util.h"
 #include "common.h"
@@ -19,11 +23,66 @@ namespace {
 constexpr int MAX_E = 512, MAX_K = 64;
 
 template <int DT>
-SMEL_DEV float ld_logit(const void* p, int64_t i) {
-  if constexpr (DT == 1) return ((const float*)p)[i];
-  const uint32_t b = ((const uint16_t*)p)[i];
-  if constexpr (DT == 0) return __uint_as_float(b << 16);
-  return (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+struct El {
+  typedef uint16_t T;
+};
+template <>
+struct El<1> {
+  typedef float T;
+};
+template <int DT>
+SMEL_DEV float cvt(typename El<DT>::T b) {
+  if constexpr (DT == 1) return b;
+  else if constexpr (DT == 0) return __uint_as_float((uint32_t)b << 16);
+  else return (float)__builtin_bit_cast(_Float16, b);
+}
+// N neighbouring values of a row of E from e0 on, `none` past it; one access of element alignment (the hardware takes any address)
+template <class T, int N>
+struct Run {
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef V U __attribute__((aligned(sizeof(T))));
+};
+template <class T>
+struct Run<T, 1> {
+  typedef T V;
+  typedef T U;
+};
+template <int DT, int N>
+SMEL_DEV void ld_run(const typename El<DT>::T* row, int e0, int E, float none, float (&v)[N]) {
+  typedef typename El<DT>::T T;
+  if constexpr (N > 1) {
+    if (e0 + N <= E) {
+      const typename Run<T, N>::V q = *(const typename Run<T, N>::U*)(row + e0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = cvt<DT>(q[i]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = e0 + i < E ? cvt<DT>(row[e0 + i]) : none;
+}
+template <int DT, int N>
+SMEL_DEV void st_run(typename El<DT>::T* row, int e0, int E, const float (&v)[N]) {
+  typedef typename El<DT>::T T;
+  T o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (DT == 1) o[i] = v[i];
+    else if constexpr (DT == 0) o[i] = f2bf(v[i]);
+    else o[i] = __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+  }
+  if constexpr (N > 1) {
+    if (e0 + N <= E) {
+      typename Run<T, N>::V q;
+#pragma unroll
+      for (int i = 0; i < N; ++i) q[i] = o[i];
+      *(typename Run<T, N>::U*)(row + e0) = q;
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (e0 + i < E) row[e0 + i] = o[i];
 }
 
 // e^x (x <= 0 or NaN) on v_exp_f32: x log2(e) in two parts, so that the product's rounding does not grow with |x|; an expert
@@ -33,6 +92,29 @@ SMEL_DEV float exp_acc(float x) {
   const float hi = x * 1.4426950408889634f;
   const float lo = fmaf(x, 1.4426950408889634f, -hi) + x * 1.9259629911266175e-8f;
   return __builtin_amdgcn_exp2f(hi) * fmaf(lo, 0.6931471805599453f, 1.f);
+}
+
+// Sum and maximum over the wave by DPP moves (six of about 8 cycles, where a shuffle through the LDS unit is about 64): rows of
+// 16 lanes, then across them; lane 63 holds the result. Lanes without a source add 0, or meet themselves.
+#define BAL_DPP(v, old, ctrl, rows) \
+  __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), ctrl, rows, 0xf, false))
+SMEL_DEV float sum64(float v) {
+  v += BAL_DPP(v, 0.f, 0x111, 0xf);   // row_shr:1, 2, 4, 8
+  v += BAL_DPP(v, 0.f, 0x112, 0xf);
+  v += BAL_DPP(v, 0.f, 0x114, 0xf);
+  v += BAL_DPP(v, 0.f, 0x118, 0xf);
+  v += BAL_DPP(v, 0.f, 0x142, 0xa);   // row_bcast:15 into rows 1 and 3
+  v += BAL_DPP(v, 0.f, 0x143, 0xc);   // row_bcast:31 into rows 2 and 3
+  return lane_get(v, 63);
+}
+SMEL_DEV float max64(float v) {
+  v = fmaxf(v, BAL_DPP(v, v, 0x111, 0xf));
+  v = fmaxf(v, BAL_DPP(v, v, 0x112, 0xf));
+  v = fmaxf(v, BAL_DPP(v, v, 0x114, 0xf));
+  v = fmaxf(v, BAL_DPP(v, v, 0x118, 0xf));
+  v = fmaxf(v, BAL_DPP(v, v, 0x142, 0xa));
+  v = fmaxf(v, BAL_DPP(v, v, 0x143, 0xc));
+  return lane_get(v, 63);
 }
 
 struct Seqs {
@@ -57,18 +139,24 @@ struct Seqs {
   }
 };
 
+struct Row {      // what the backward takes a token up with
+  float m, r;     // its maximum, 1 / its sum of exponentials
+  int seq, pad;   // its sequence, -1 where it does not count
+};
+
 struct BalArgs {
   const void* z;
   int64_t ldl, T;
   const void* topi;
   int topi_i64;
-  int E, K, chunk, nchunk;
+  int E, K, chunk;
   const uint8_t* mask;
   Seqs q;
   float coef;
-  float* row_stats;
+  Row* rows;       // null: no backward
   float* P;        // [slots][E]
-  int32_t* C;      // [slots][E + 1]: picks, then counted tokens
+  int32_t* C;      // [slots][E]
+  int32_t* N;      // [slots] counted tokens
   float* loss;
   int64_t* counts;
   float* weights;
@@ -76,112 +164,177 @@ struct BalArgs {
   int32_t* seq_n;  // [S]
 };
 
-template <int DT, int NE>
-__global__ __launch_bounds__(256) void bal_fwd_kernel(BalArgs a) {
-  __shared__ float sp[4][MAX_E];
-  __shared__ int sc[MAX_E + 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+template <int NE>
+constexpr int TB = NE == 8 ? 2 : 4;   // tokens of a wave at a time
+
+// A sequence's counts, weights and loss from expert x's picks c and sum P of the softmax, x < E in thread x; the sums over
+// the experts go through red and tot (a slot a wave). All threads of the block call it; the result is thread 0's.
+SMEL_DEV float finish_seq(const BalArgs& a, int s, int x, int64_t c, int64_t n, float P, float* red, long long* tot) {
+  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
+  const bool mine = x < a.E;
+  if (mine) a.counts[(int64_t)s * a.E + x] = c;
+  long long ct = mine ? c : 0;   // picks in range, over all experts
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) ct += __shfl_xor(ct, o, 64);
+  if ((threadIdx.x & 63) == 0) tot[wave] = ct;
+  __syncthreads();
+  ct = 0;
+  for (int k = 0; k < waves; ++k) ct += tot[k];
+  float l = 0.f;
+  if (mine) {
+    const double scale = n > 0 ? (double)a.coef / ((double)a.K * (double)n * (double)n) : 0.0;
+    a.weights[(int64_t)s * a.E + x] = (float)((double)(c * a.E - ct) * scale);
+    l = n > 0 ? (float)((double)(c * a.E) * scale) * P : 0.f;
+  }
+  l = wave_sum(l);
+  if ((threadIdx.x & 63) == 0) red[wave] = l;
+  __syncthreads();
+  for (int k = 1; k < waves; ++k) l = k == 1 ? red[0] + red[1] : l + red[k];
+  return l;
+}
+
+// W waves. ONE: all tokens are this block's and one sequence: no slots, the loss at once
+template <int DT, int NE, int W, bool ONE>
+__global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
+  typedef typename El<DT>::T T;
+  __shared__ float sp[W][64 * NE];
+  __shared__ int sc[MAX_E], sn;
+  __shared__ float red[W];
+  __shared__ long long tot[W];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e0 = lane * NE;
   const int64_t c0 = (int64_t)blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, a.T);
-  int s = max(a.q.find(c0), 0);
-  for (; s < a.q.S; ++s) {
-    const int64_t b = max(a.q.at(s), c0), e = min(a.q.at(s + 1), c1);
-    if (a.q.at(s) >= c1) break;
-    if (b >= e) continue;
-    for (int i = threadIdx.x; i <= a.E; i += 256) sc[i] = 0;
+  if (a.rows && a.q.off) {   // tokens of no sequence
+    for (int64_t t = c0 + threadIdx.x; t < c1; t += 64 * W) a.rows[t].seq = -1;
     __syncthreads();
+  }
+  int s = ONE ? 0 : max(a.q.find(c0), 0);
+  int64_t begin = a.q.at(s), end = a.q.at(s + 1), next;
+  for (; s < a.q.S; ++s, begin = end, end = next) {
+    const int64_t b = max(begin, c0), e = min(end, c1);
+    next = a.q.at(min(s + 2, a.q.S));
+    if (!ONE) {
+      if (begin >= c1) break;
+      if (b >= e) continue;
+    }
+    for (int i = threadIdx.x; i < a.E; i += 64 * W) sc[i] = 0;
+    if (threadIdx.x == 0) sn = 0;
+    __syncthreads();
+    auto pick = [&](int64_t i) -> int64_t {   // pick i of the block's, -1 where it counts nowhere
+      if (i >= e * a.K || (a.mask && !a.mask[(uint32_t)i / (uint32_t)a.K])) return -1;   // T K < 2^31
+      return a.topi_i64 ? ((const int64_t*)a.topi)[i] : (int64_t)((const int32_t*)a.topi)[i];
+    };
+    int64_t i0 = b * a.K + threadIdx.x;
+    int64_t id = pick(i0);   // on its way while the rows are summed
     float acc[NE];
+    int n = 0;
 #pragma unroll
     for (int i = 0; i < NE; ++i) acc[i] = 0.f;
-    for (int64_t t = b + wave; t < e; t += 4) {
-      if (a.mask && !a.mask[t]) continue;
-      float z[NE], m = -INFINITY, sum = 0.f;
+    constexpr int B = TB<NE>;
+    for (int64_t t0 = b + wave * B; t0 < e; t0 += W * B) {
+      float z[B][NE];
+      bool keep[B];
 #pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int x = lane + 64 * i;
-        z[i] = x < a.E ? ld_logit<DT>(a.z, t * a.ldl + x) : -INFINITY;
-        m = fmaxf(m, z[i]);
+      for (int k = 0; k < B; ++k) {   // a row that does not count may be read; nothing of it is used
+        const int64_t t = min(t0 + k, e - 1);
+        keep[k] = t0 + k < e && !(a.mask && !a.mask[t]);
+        ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, -INFINITY, z[k]);
       }
-      m = wave_max(m);
 #pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        z[i] = lane + 64 * i < a.E ? exp_acc(z[i] - m) : 0.f;
-        sum += z[i];
-      }
-      const float r = 1.f / wave_sum(sum);
+      for (int k = 0; k < B; ++k) {
+        float m = z[k][0], sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < NE; ++i) acc[i] = fmaf(z[i], r, acc[i]);
-      if (lane == 0) {
-        if (a.row_stats) {
-          a.row_stats[2 * t] = m;
-          a.row_stats[2 * t + 1] = r;
+        for (int i = 1; i < NE; ++i) m = fmaxf(m, z[k][i]);
+        m = max64(m);
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          z[k][i] = e0 + i < a.E ? exp_acc(z[k][i] - m) : 0.f;
+          sum += z[k][i];
         }
-        atomicAdd(&sc[a.E], 1);
+        const float r = 1.f / sum64(sum);
+#pragma unroll
+        for (int i = 0; i < NE; ++i) acc[i] = keep[k] ? fmaf(z[k][i], r, acc[i]) : acc[i];
+        n += keep[k];
+        if (a.rows && lane == 0 && t0 + k < e) a.rows[t0 + k] = Row{m, r, keep[k] ? s : -1, 0};
       }
     }
-    for (int64_t i = b * a.K + threadIdx.x; i < e * a.K; i += 256) {
-      if (a.mask && !a.mask[i / a.K]) continue;
-      const int64_t id = a.topi_i64 ? ((const int64_t*)a.topi)[i] : (int64_t)((const int32_t*)a.topi)[i];
+    while (i0 < e * a.K) {
       if (id >= 0 && id < a.E) atomicAdd(&sc[id], 1);
+      i0 += 64 * W;
+      id = pick(i0);
     }
+    if (lane == 0) atomicAdd(&sn, n);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) sp[wave][lane + 64 * i] = acc[i];
+    for (int i = 0; i < NE; ++i) sp[wave][e0 + i] = acc[i];
     __syncthreads();
-    const int64_t slot = (int64_t)blockIdx.x + s;
-    for (int x = threadIdx.x; x <= a.E; x += 256) {
-      if (x < a.E) a.P[slot * a.E + x] = ((sp[0][x] + sp[1][x]) + sp[2][x]) + sp[3][x];
-      a.C[slot * (a.E + 1) + x] = sc[x];
+    auto share = [&](int x) {
+      float P = sp[0][x];
+#pragma unroll
+      for (int k = 1; k < W; ++k) P += sp[k][x];
+      return P;
+    };
+    if constexpr (ONE) {
+      const int x = threadIdx.x;
+      const float l = finish_seq(a, 0, x, x < a.E ? sc[x] : 0, sn, x < a.E ? share(x) : 0.f, red, tot);
+      if (x == 0) {
+        *a.loss = l;
+        a.weights[a.E] = 1.f;
+      }
+      return;
     }
+    const int64_t slot = (int64_t)blockIdx.x + s;
+    for (int x = threadIdx.x; x < a.E; x += 64 * W) {
+      a.P[slot * a.E + x] = share(x);
+      a.C[slot * a.E + x] = sc[x];
+    }
+    if (threadIdx.x == 0) a.N[slot] = sn;
     __syncthreads();
   }
 }
 
-// one sequence: its slots' sums, counts, gradient weights and loss
-__global__ __launch_bounds__(512) void bal_seq_kernel(BalArgs a) {
-  __shared__ float red[8];
-  __shared__ long long tot[8];
-  const int s = blockIdx.x, x = threadIdx.x;   // an expert per thread
+// One sequence: its slots' sums, counts, weights and loss. Threads: columns of `1 << lgc` experts, the groups take every
+// group-th slot each.
+template <int BS>
+__global__ __launch_bounds__(BS) void bal_seq_kernel(BalArgs a, int lgc) {
+  __shared__ float sp[BS], red[BS / 64];
+  __shared__ int sc[BS];
+  __shared__ long long tot[BS / 64];
+  __shared__ int sn;
+  const int s = blockIdx.x;
   const int64_t b = a.q.at(s), e = a.q.at(s + 1);
-  int64_t c = 0;
-  int64_t n = 0;
+  const int cols = 1 << lgc, groups = BS >> lgc, x = threadIdx.x & (cols - 1), g = threadIdx.x >> lgc;
+  const int64_t k0 = b / a.chunk + s, k1 = b < e ? (e - 1) / a.chunk + s : k0 - 1;
   float P = 0.f;
-  if (b < e) {
-    const int64_t k0 = b / a.chunk + s, k1 = (e - 1) / a.chunk + s;
-    for (int64_t k = k0; k <= k1; ++k) {
-      n += a.C[k * (a.E + 1) + a.E];
-      if (x < a.E) {
-        P += a.P[k * a.E + x];
-        c += a.C[k * (a.E + 1) + x];
-      }
+  int c = 0;   // K T < 2^31
+  if (x < a.E)
+#pragma unroll 8
+    for (int64_t k = k0 + g; k <= k1; k += groups) {
+      P += a.P[k * a.E + x];
+      c += a.C[k * a.E + x];
     }
-  }
-  if (x < a.E) a.counts[(int64_t)s * a.E + x] = c;
-  // picks in range, over all experts
-  long long ct = c;
+  if (threadIdx.x < 64) {
+    int n = 0;
+    for (int64_t k = k0 + threadIdx.x; k <= k1; k += 64) n += a.N[k];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) ct += __shfl_xor(ct, o, 64);
-  if ((x & 63) == 0) tot[x >> 6] = ct;
-  __syncthreads();
-  ct = 0;
-  for (int k = 0; k < 8; ++k) ct += tot[k];
-  float l = 0.f;
-  if (x < a.E && n > 0) {
-    const double scale = (double)a.coef / ((double)a.K * (double)n * (double)n);
-    a.weights[(int64_t)s * a.E + x] = (float)((double)(c * a.E - ct) * scale);
-    l = (float)((double)c * a.E * scale) * P;
-  } else if (x < a.E) {
-    a.weights[(int64_t)s * a.E + x] = 0.f;
+    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (threadIdx.x == 0) sn = n;
   }
-  l = wave_sum(l);
-  if ((x & 63) == 0) red[x >> 6] = l;
+  sp[threadIdx.x] = P;
+  sc[threadIdx.x] = c;
   __syncthreads();
-  if (x == 0) {
-    for (int k = 1; k < 8; ++k) l += red[k];
+  if (g == 0)
+    for (int k = 1; k < groups; ++k) {
+      P += sp[(k << lgc) + x];
+      c += sc[(k << lgc) + x];
+    }
+  const int mine = g == 0 ? x : MAX_E;
+  const float l = finish_seq(a, s, mine, c, sn, P, red, tot);
+  if (threadIdx.x == 0) {
     if (a.q.S == 1) {
       *a.loss = l;
       a.weights[a.E] = 1.f;
     } else {
       a.seq_loss[s] = l;
-      a.seq_n[s] = n > 0;
+      a.seq_n[s] = sn > 0;
     }
   }
 }
@@ -216,65 +369,77 @@ __global__ __launch_bounds__(1024) void bal_join_kernel(BalArgs a) {
 
 template <int DT, int NE>
 __global__ __launch_bounds__(256) void bal_bwd_kernel(BalArgs a, const float* __restrict__ go, void* __restrict__ dz) {
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (t >= a.T) return;
-  const int s = a.q.find(t);
-  const bool counts = s >= 0 && s < a.q.S && t < a.q.at(s + 1) && !(a.mask && !a.mask[t]);
-  float p[NE], d[NE];
-  if (counts) {
-    const float m = a.row_stats[2 * t], r = a.row_stats[2 * t + 1];
-    const float g = *go * a.weights[(int64_t)a.q.S * a.E];
-    float dot = 0.f;
+  typedef typename El<DT>::T T;
+  constexpr int B = TB<NE>;
+  const int lane = threadIdx.x & 63, e0 = lane * NE;
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * B;
+  if (t0 >= a.T) return;
+  const float g = *go * a.weights[(int64_t)a.q.S * a.E];
+  float z[B][NE], v[B][NE];
+  Row row[B];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int x = lane + 64 * i;
-      p[i] = x < a.E ? exp_acc(ld_logit<DT>(a.z, t * a.ldl + x) - m) * r : 0.f;
-      d[i] = x < a.E ? a.weights[(int64_t)s * a.E + x] : 0.f;
-      dot = fmaf(p[i], d[i], dot);
-    }
-    dot = wave_sum(dot);
+  for (int k = 0; k < B; ++k) {
+    const int64_t t = min(t0 + k, a.T - 1);
+    row[k] = a.rows[t];
+    ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, 0.f, z[k]);
+  }
+  if (a.q.S == 1) {
+    ld_run<1, NE>(a.weights, e0, a.E, 0.f, v[0]);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) d[i] = g * (p[i] * (d[i] - dot));
+    for (int k = 1; k < B; ++k)
+#pragma unroll
+      for (int i = 0; i < NE; ++i) v[k][i] = v[0][i];
   } else {
 #pragma unroll
-    for (int i = 0; i < NE; ++i) d[i] = 0.f;
+    for (int k = 0; k < B; ++k) ld_run<1, NE>(a.weights + (int64_t)max(row[k].seq, 0) * a.E, e0, a.E, 0.f, v[k]);
   }
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int x = lane + 64 * i;
-    if (x >= a.E) continue;
-    if constexpr (DT == 1) ((float*)dz)[t * a.E + x] = d[i];
-    if constexpr (DT == 0) ((uint16_t*)dz)[t * a.E + x] = f2bf(d[i]);
-    if constexpr (DT == 2) ((uint16_t*)dz)[t * a.E + x] = __builtin_bit_cast(uint16_t, (_Float16)d[i]);
+  for (int k = 0; k < B; ++k) {
+    if (t0 + k >= a.T) break;
+    float p[NE], d[NE], dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      p[i] = exp_acc(z[k][i] - row[k].m) * row[k].r;
+      dot = e0 + i < a.E ? fmaf(p[i], v[k][i], dot) : dot;
+    }
+    dot = sum64(dot);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) d[i] = row[k].seq >= 0 ? g * (p[i] * (v[k][i] - dot)) : 0.f;
+    st_run<DT, NE>((T*)dz + (t0 + k) * a.E, e0, a.E, d);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 
-int chunk_of(int64_t T) {
-  int64_t c = (T + 255) / 256;
-  return (int)(c < 16 ? 16 : c);
+// Sequences of under 64 tokens on average: blocks of four waves and about four sequences (each costs a block a few round
+// trips to memory, so many blocks have to be under way: 131072 tokens in 4096 sequences 129 -> 40 us).
+bool short_seqs(int64_t T, int64_t S) { return S > 1 && S * 64 > T; }
+// tokens of a forward block: up to 256 blocks, 64 tokens at least (four for a wave)
+int chunk_of(int64_t T, int64_t S) {
+  if (short_seqs(T, S)) return (int)std::max<int64_t>(4, 4 * T / S);
+  return (int)std::max<int64_t>((T + 255) / 256, 64);
 }
-int64_t chunks_of(int64_t T) { return T ? (T + chunk_of(T) - 1) / chunk_of(T) : 0; }
+int64_t chunks_of(int64_t T, int64_t S) { return T ? (T + chunk_of(T, S) - 1) / chunk_of(T, S) : 0; }
+constexpr int64_t ONE_BLOCK = 192;   // tokens of one sequence that a block takes alone
 
 struct Ws {
-  int64_t P, C, loss, n, bytes;
+  int64_t P, C, N, loss, n, bytes;
 };
 Ws ws_of(int64_t T, int64_t E, int64_t S) {
   auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
-  const int64_t slots = chunks_of(T) + S;
+  const int64_t slots = chunks_of(T, S) + S;
   Ws w;
   w.P = 0;
   w.C = up(slots * E * 4);
-  w.loss = w.C + up(slots * (E + 1) * 4);
+  w.N = w.C + up(slots * E * 4);
+  w.loss = w.N + up(slots * 4);
   w.n = w.loss + up(S * 4);
   w.bytes = w.n + up(S * 4);
   return w;
 }
 
 int check(const char* name, const void* z, int64_t ldl, int dtype, int64_t T, int64_t E, int64_t S, const void* off) {
-  SMEL_REQUIRE(T >= 0 && T <= (int64_t)1 << 25, SMEL_EUNSUPPORTED, "%s: T=%lld tokens, 0 to 2^25", name, (long long)T);
+  SMEL_REQUIRE(T >= 0 && T <= (int64_t)1 << 24, SMEL_EUNSUPPORTED, "%s: T=%lld tokens, 0 to 2^24", name, (long long)T);
   SMEL_REQUIRE(E >= 1 && E <= MAX_E, SMEL_EUNSUPPORTED, "%s: E=%lld experts, 1 to %d", name, (long long)E, MAX_E);
   SMEL_REQUIRE(S >= 1 && S <= (int64_t)1 << 24, SMEL_EUNSUPPORTED, "%s: S=%lld sequences, 1 to 2^24", name, (long long)S);
   SMEL_REQUIRE(off || S == 1, SMEL_EINVAL, "%s: %lld sequences without offsets", name, (long long)S);
@@ -284,23 +449,22 @@ int check(const char* name, const void* z, int64_t ldl, int dtype, int64_t T, in
   return 0;
 }
 
-// f<DT, NE> of the call's type and experts per lane
-#define BAL_PICK(F, ...)                                                                        \
-  [&](auto dt) {                                                                                \
-    if (a.E <= 64) F<decltype(dt)::value, 1> __VA_ARGS__;                                       \
-    else if (a.E <= 128) F<decltype(dt)::value, 2> __VA_ARGS__;                                 \
-    else if (a.E <= 256) F<decltype(dt)::value, 4> __VA_ARGS__;                                 \
-    else F<decltype(dt)::value, 8> __VA_ARGS__;                                                 \
-  }
 template <int V>
 struct Int {
   static constexpr int value = V;
 };
+// f(dtype, experts a lane) as constants
 template <class F>
-void by_dtype(int dtype, F f) {
-  if (dtype == 0) f(Int<0>{});
-  else if (dtype == 1) f(Int<1>{});
-  else f(Int<2>{});
+void pick(int dtype, int64_t E, F f) {
+  auto by_e = [&](auto dt) {
+    if (E <= 64) f(dt, Int<1>{});
+    else if (E <= 128) f(dt, Int<2>{});
+    else if (E <= 256) f(dt, Int<4>{});
+    else f(dt, Int<8>{});
+  };
+  if (dtype == 0) by_e(Int<0>{});
+  else if (dtype == 1) by_e(Int<1>{});
+  else by_e(Int<2>{});
 }
 
 }  // namespace
@@ -322,6 +486,7 @@ extern "C" int smel_balance_fwd(const void* logits, int64_t ldl, int32_t dtype, 
   SMEL_REQUIRE(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= w.bytes, SMEL_EINVAL,
                "balance_fwd: a workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", (long long)w.bytes,
                (long long)ws_bytes);
+  SMEL_REQUIRE((uintptr_t)row_stats % 16 == 0, SMEL_EINVAL, "balance_fwd: row_stats must be 16-byte aligned");
   char* const base = (char*)ws;
   BalArgs a{};
   a.z = logits;
@@ -331,42 +496,60 @@ extern "C" int smel_balance_fwd(const void* logits, int64_t ldl, int32_t dtype, 
   a.topi_i64 = topi_i64;
   a.E = (int)E;
   a.K = (int)K;
-  a.chunk = chunk_of(T);
-  a.nchunk = (int)chunks_of(T);
   a.mask = mask;
   a.q = Seqs{offsets, off_i64, (int)S, T};
   a.coef = coef;
-  a.row_stats = row_stats;
-  a.P = (float*)(base + w.P);
-  a.C = (int32_t*)(base + w.C);
+  a.rows = (Row*)row_stats;
   a.loss = loss;
   a.counts = counts;
   a.weights = weights;
+  if (S == 1 && T <= ONE_BLOCK) {
+    a.chunk = ONE_BLOCK;
+    pick(dtype, E, [&](auto dt, auto ne) {
+      bal_fwd_kernel<decltype(dt)::value, decltype(ne)::value, 16, true><<<1, 1024, 0, stream>>>(a);
+    });
+    return smel::launch_status();
+  }
+  a.chunk = chunk_of(T, S);
+  a.P = (float*)(base + w.P);
+  a.C = (int32_t*)(base + w.C);
+  a.N = (int32_t*)(base + w.N);
   a.seq_loss = (float*)(base + w.loss);
   a.seq_n = (int32_t*)(base + w.n);
-  if (a.nchunk) by_dtype(dtype, BAL_PICK(bal_fwd_kernel, <<<a.nchunk, 256, 0, stream>>>(a)));
-  bal_seq_kernel<<<(unsigned)S, 512, 0, stream>>>(a);
+  if (T)
+    pick(dtype, E, [&](auto dt, auto ne) {
+      constexpr int d = decltype(dt)::value, m = decltype(ne)::value;
+      const unsigned n = (unsigned)chunks_of(T, S);
+      if (short_seqs(T, S)) bal_fwd_kernel<d, m, 4, false><<<n, 256, 0, stream>>>(a);
+      else bal_fwd_kernel<d, m, 16, false><<<n, 1024, 0, stream>>>(a);
+    });
+  int lgc = 6;
+  while ((1 << lgc) < E) ++lgc;
+  if (S <= 512) bal_seq_kernel<1024><<<(unsigned)S, 1024, 0, stream>>>(a, lgc);
+  else bal_seq_kernel<512><<<(unsigned)S, 512, 0, stream>>>(a, lgc);
   if (S > 1) bal_join_kernel<<<1, 1024, 0, stream>>>(a);
   return smel::launch_status();
 }
 
-extern "C" int smel_balance_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E,
-                                const uint8_t* mask, const void* offsets, int32_t off_i64, int64_t S,
+extern "C" int smel_balance_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t S,
                                 const float* row_stats, const float* weights, const float* go, void* dlogits,
                                 hipStream_t stream) {
-  const int rc = check("balance_bwd", logits, ldl, dtype, T, E, S, offsets);
+  const int rc = check("balance_bwd", logits, ldl, dtype, T, E, S, weights);
   if (rc) return rc;
   if (T == 0) return 0;
   SMEL_REQUIRE(row_stats && weights && go && dlogits, SMEL_EINVAL, "balance_bwd: null pointer");
+  SMEL_REQUIRE((uintptr_t)row_stats % 16 == 0, SMEL_EINVAL, "balance_bwd: row_stats must be 16-byte aligned");
   BalArgs a{};
   a.z = logits;
   a.ldl = ldl;
   a.T = T;
   a.E = (int)E;
-  a.mask = mask;
-  a.q = Seqs{offsets, off_i64, (int)S, T};
-  a.row_stats = const_cast<float*>(row_stats);
+  a.q = Seqs{nullptr, 0, (int)S, T};
+  a.rows = (Row*)const_cast<float*>(row_stats);
   a.weights = const_cast<float*>(weights);
-  by_dtype(dtype, BAL_PICK(bal_bwd_kernel, <<<(unsigned)((T + 3) / 4), 256, 0, stream>>>(a, go, dlogits)));
+  pick(dtype, E, [&](auto dt, auto ne) {
+    constexpr int tokens = 4 * TB<decltype(ne)::value>;
+    bal_bwd_kernel<decltype(dt)::value, decltype(ne)::value><<<(unsigned)((T + tokens - 1) / tokens), 256, 0, stream>>>(a, go, dlogits);
+  });
   return smel::launch_status();
 }

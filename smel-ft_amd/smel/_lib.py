@@ -172,7 +172,7 @@ SIGNATURES = {
     "smel_ce_transpose": (i32, [vp, i64, i64, i64, vp, i64, i32, vp]),
     "smel_balance_ws_bytes": (i64, [i64, i64, i64]),
     "smel_balance_fwd": (i32, [vp, i64, i32, vp, i32, i64, i64, i64, vp, vp, i32, i64, f32, vp, vp, vp, vp, vp, i64, vp]),
-    "smel_balance_bwd": (i32, [vp, i64, i32, i64, i64, vp, vp, i32, i64, vp, vp, vp, vp, vp]),
+    "smel_balance_bwd": (i32, [vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp]),
     # include/smel_ortho.h
     "smel_orthogonalize_ws": (i64, [vp, i32]),
     "smel_orthogonalize": (i32, [vp, i32, i32, f64, f64, f64, f64, vp, i64, vp]),

@@ -420,7 +420,7 @@ class _Balance:
         topi = topi.contiguous()
         mem = L.Carve()     # kept for the backward
         self.weights = mem.take(4 * (S * E + 1))
-        self.stats = mem.take(8 * T) if need_grad else None
+        self.stats = mem.take(16 * T) if need_grad else None
         self.keep = mem
         ws_n = L.load().smel_balance_ws_bytes(T, E, S)
         tmp = L.Carve()
@@ -440,7 +440,7 @@ class _Balance:
         dz = torch.empty(self.T, self.E, dtype=self.z.dtype, device=self.z.device)
         go = go.to(device=self.z.device, dtype=torch.float32).contiguous()
         p = L.ptr
-        L.call("smel_balance_bwd", p(self.z), self.ldl, _DT[self.z.dtype], self.T, self.E, *self._common(), p(self.stats),
+        L.call("smel_balance_bwd", p(self.z), self.ldl, _DT[self.z.dtype], self.T, self.E, self.S, p(self.stats),
                p(self.weights), p(go), p(dz), L.stream())
         return dz
 
@@ -451,7 +451,7 @@ class _BalanceFn(torch.autograd.Function):
         b = _Balance(logits, mask, offsets)
         with L.on_device_of(logits):
             loss, counts = b.forward(topi, coef, True)
-        ctx.save_for_backward(b.z, b.mask, b.off)     # autograd reports a change in place
+        ctx.save_for_backward(b.z)     # autograd reports a change in place
         ctx.b = b
         b.z = b.mask = b.off = None
         ctx.mark_non_differentiable(counts)
@@ -464,9 +464,9 @@ class _BalanceFn(torch.autograd.Function):
         if go is None:
             return None, None, None, None, None
         b = ctx.b
-        b.z, b.mask, b.off = ctx.saved_tensors
+        b.z, = ctx.saved_tensors
         dz = b.backward(go)
-        b.z = b.mask = b.off = None
+        b.z = None
         return dz, None, None, None, None
 
 
