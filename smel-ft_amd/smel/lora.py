@@ -145,7 +145,7 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
     contiguous, without gradients. The products run on the rank's r x r matrices in 64 bits, so small singular values keep
     their directions (include/smel_ortho.h)."""
     single = isinstance(update, torch.Tensor)
-    ts = [update] if single else list(update)
+    ts = (update,) if single else tuple(update)
     a, b, c = (float(v) for v in coeffs)
     if not 0 <= int(steps) <= 64:
         raise ValueError(f"orthogonalize takes 0 to 64 steps, got {steps}")
@@ -153,27 +153,39 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
         raise ValueError(f"orthogonalize: eps must not be negative, got {eps}")
     if not ts:
         return []
-    _lib.one_device(ts[0], *ts[1:])
-    jobs, outs, keep = array("q"), [], []
+    if not ts[0].is_cuda:
+        _lib.one_device(ts[0])
+    jobs, outs, keep, n = array("q"), [], [], 0
+    dev = ts[0].device
     with torch.no_grad(), _lib.on_device_of(ts[0]):
-        for t in ts:
-            if t.dtype not in _ORTHO_DTYPES or t.dim() < 2:
+        for t in ts:     # a layer has a dozen: about three microseconds each
+            code = _ORTHO_DTYPES.get(t.dtype)
+            *lead, rows, cols = t.shape if t.dim() > 1 else (0, 0)
+            if code is None or t.dim() < 2:
                 raise ValueError(f"orthogonalize takes bf16, fp16 or fp32 matrices, got {tuple(t.shape)} {t.dtype}")
-            if min(t.shape[-2:]) > ORTHO_MAX_RANK:
+            if rows > ORTHO_MAX_RANK and cols > ORTHO_MAX_RANK:
                 raise ValueError(f"orthogonalize takes matrices whose shorter side is at most {ORTHO_MAX_RANK}, got "
                                  f"{tuple(t.shape)}")
-            y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            if t.device != dev:
+                _lib.one_device(ts[0], t)
+            size = rows * cols
+            if t.is_contiguous():
+                y = torch.empty_like(t)
+                if t.numel():
+                    jobs.extend((t.data_ptr(), y.data_ptr(), t.numel() // size, rows, cols, size, cols, 1, code))
+                    n += 1
+            else:
+                y = t.new_empty(t.shape)
+                if t.numel():
+                    x = _ortho_operand(t)
+                    keep.append(x)
+                    jobs.extend((x.data_ptr(), y.data_ptr(), *x.shape, *x.stride(), code))
+                    n += 1
             outs.append(y)
-            if t.numel() == 0:
-                continue
-            x = _ortho_operand(t)
-            keep.append(x)
-            jobs.extend((x.data_ptr(), y.data_ptr(), *x.shape, *x.stride(), _ORTHO_DTYPES[t.dtype]))
-        lib = _lib.load()
-        addr, n = jobs.buffer_info()[0], len(keep)
-        need = lib.smel_orthogonalize_ws(addr, n)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=ts[0].device)
-        _lib.call("smel_orthogonalize", addr, n, int(steps), a, b, c, float(eps), _lib.ptr(ws), need, _lib.stream())
+        addr = jobs.buffer_info()[0]
+        need = _lib.load().smel_orthogonalize_ws(addr, n)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        _lib.call("smel_orthogonalize", addr, n, int(steps), a, b, c, float(eps), ws.data_ptr(), need, _lib.stream())
     return outs[0] if single else outs
 
 

@@ -384,90 +384,76 @@ def chunked_ce(h, head: LMHead, tgt, denom: float, token_chunk: int = TOKEN_CHUN
 
 
 def _balance_check(logits, topi, mask, offsets):
-    L.one_device(logits, topi, mask, offsets)
     if logits.dim() != 2 or logits.dtype not in _DT:
         raise ValueError(f"balance_loss takes bf16, fp16 or fp32 logits [T, E], got {tuple(logits.shape)} {logits.dtype}")
-    if topi.dim() != 2 or topi.shape[0] != logits.shape[0] or topi.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"balance_loss takes int64 or int32 picks [T, K] of the logits' {logits.shape[0]} tokens, got "
+    T = logits.shape[0]
+    if topi.dim() != 2 or topi.shape[0] != T or topi.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"balance_loss takes int64 or int32 picks [T, K] of the logits' {T} tokens, got "
                          f"{tuple(topi.shape)} {topi.dtype}")
-    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (logits.shape[0],)):
-        raise ValueError(f"balance_loss takes a bool mask [{logits.shape[0]}], got {tuple(mask.shape)} {mask.dtype}")
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (T,)):
+        raise ValueError(f"balance_loss takes a bool mask [{T}], got {tuple(mask.shape)} {mask.dtype}")
     if offsets is not None and (offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int64, torch.int32)):
         raise ValueError(f"balance_loss takes int64 or int32 offsets [S + 1], got {tuple(offsets.shape)} {offsets.dtype}")
+    L.one_device(logits, topi, mask, offsets)
 
 
-class _Balance:
-    """One call's operands, and the launches."""
+def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
+    """(loss, counts, what the backward takes). One allocation holds the backward's rows (16 bytes a token), its weights
+    and the workspace: a short batch is the host's time, and each allocation costs it as much as half a launch."""
+    T, E = z.shape
+    if not z.is_contiguous() and (E > 1 and z.stride(1) != 1 or T > 1 and z.stride(0) < E):
+        z = z.contiguous()
+    ldl = z.stride(0) if T > 1 else E
+    topi = topi.contiguous()
+    S = 1 if off is None else off.shape[0] - 1
+    rows_n = 16 * T if need_grad else 0
+    weights_n = (4 * (S * E + 1) + 15) & ~15
+    ws_n = L.load().smel_balance_ws_bytes(T, E, S)
+    mem = z.new_empty((rows_n + weights_n + ws_n) // z.element_size() + 8)
+    rows = mem.data_ptr()
+    weights = rows + rows_n
+    loss = torch.empty((), dtype=torch.float32, device=z.device)
+    counts = torch.empty((E,) if off is None else (S, E), dtype=torch.int64, device=z.device)
+    p = L.ptr
+    if mask is not None:
+        mask = mask.contiguous()
+    if off is not None:
+        off = off.contiguous()
+    dt = _DT[z.dtype]
+    L.call("smel_balance_fwd", z.data_ptr(), ldl, dt, topi.data_ptr(), topi.dtype is torch.int64, T, E, topi.shape[1],
+           p(mask), p(off), off is not None and off.dtype is torch.int64, S, coef, loss.data_ptr(), counts.data_ptr(),
+           rows if need_grad else None, weights, weights + weights_n, ws_n, L.stream())
+    return loss, counts, (z, mem, ldl, dt, T, E, S, rows, weights)
 
-    __slots__ = ("z", "T", "E", "ldl", "mask", "off", "S", "keep", "stats", "weights")
 
-    def __init__(self, logits, mask, offsets):
-        T, E = logits.shape
-        if logits.stride(1) != 1 and E > 1 or T > 1 and logits.stride(0) < E:
-            logits = logits.contiguous()
-        self.z, self.T, self.E = logits, T, E
-        self.ldl = logits.stride(0) if T > 1 else E
-        self.mask = mask.contiguous() if mask is not None else None
-        self.off = offsets.contiguous() if offsets is not None else None
-        self.S = 1 if offsets is None else offsets.numel() - 1
+def _balance_backward(ctx, go, _):
+    if go is None:
+        return None, None, None, None, None
+    z, mem = ctx.saved_tensors
+    ldl, dt, T, E, S, rows, weights = ctx.call
+    if go.dtype is not torch.float32 or go.device != z.device:
+        go = go.to(device=z.device, dtype=torch.float32)
+    dz = z.new_empty((T, E))
+    L.call("smel_balance_bwd", z.data_ptr(), ldl, dt, T, E, S, rows, weights, go.data_ptr(), dz.data_ptr(), L.stream())
+    return dz, None, None, None, None
 
-    def _common(self):
-        p = L.ptr
-        return p(self.mask), p(self.off), int(self.off is not None and self.off.dtype == torch.int64), self.S
 
-    def forward(self, topi, coef: float, need_grad: bool):
-        dev, T, E, S = self.z.device, self.T, self.E, self.S
-        topi = topi.contiguous()
-        mem = L.Carve()     # kept for the backward
-        self.weights = mem.take(4 * (S * E + 1))
-        self.stats = mem.take(16 * T) if need_grad else None
-        self.keep = mem
-        ws_n = L.load().smel_balance_ws_bytes(T, E, S)
-        tmp = L.Carve()
-        ws = (tmp if need_grad else mem).take(ws_n)
-        mem.alloc(dev)
-        if need_grad:
-            tmp.alloc(dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        counts = torch.empty((E,) if self.off is None else (S, E), dtype=torch.int64, device=dev)
-        p = L.ptr
-        L.call("smel_balance_fwd", p(self.z), self.ldl, _DT[self.z.dtype], p(topi), int(topi.dtype == torch.int64), T, E,
-               topi.shape[1], *self._common(), float(coef), p(loss), p(counts), p(self.stats), p(self.weights), p(ws), ws_n,
-               L.stream())
-        return loss, counts
-
-    def backward(self, go):
-        dz = torch.empty(self.T, self.E, dtype=self.z.dtype, device=self.z.device)
-        go = go.to(device=self.z.device, dtype=torch.float32).contiguous()
-        p = L.ptr
-        L.call("smel_balance_bwd", p(self.z), self.ldl, _DT[self.z.dtype], self.T, self.E, self.S, p(self.stats),
-               p(self.weights), p(go), p(dz), L.stream())
-        return dz
+_balance_backward_once = once_differentiable(_balance_backward)
 
 
 class _BalanceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topi, mask, offsets, coef):
-        b = _Balance(logits, mask, offsets)
-        with L.on_device_of(logits):
-            loss, counts = b.forward(topi, coef, True)
-        ctx.save_for_backward(b.z)     # autograd reports a change in place
-        ctx.b = b
-        b.z = b.mask = b.off = None
+        loss, counts, (z, mem, *call) = _balance_forward(logits, topi, mask, offsets, coef, True)
+        ctx.save_for_backward(z, mem)     # autograd reports logits that were changed in place
+        ctx.call = call
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, go, _):
-        if go is None:
-            return None, None, None, None, None
-        b = ctx.b
-        b.z, = ctx.saved_tensors
-        dz = b.backward(go)
-        b.z = None
-        return dz, None, None, None, None
+    def backward(ctx, go, dcounts):     # on the forward's device: autograd's thread has set it
+        return (_balance_backward_once if torch.is_grad_enabled() else _balance_backward)(ctx, go, dcounts)
 
 
 def balance_loss(logits, topi, mask=None, offsets=None, coef: float = 1.0):
@@ -478,13 +464,14 @@ def balance_loss(logits, topi, mask=None, offsets=None, coef: float = 1.0):
 
         loss = coef E sum_e c_e / (K n) P_e                    (coef for an even router)
 
-    ``mask`` [T] bool: the tokens that count (rows of others are not read: they may hold anything). ``offsets`` [S + 1]
+    ``mask`` [T] bool: the tokens that count (rows of others may hold anything). ``offsets`` [S + 1]
     (ascending, on the GPU): sequence s is the tokens offsets[s] to offsets[s + 1]; the loss is the mean of the losses of
     the sequences that have tokens, and tokens outside all of them count nowhere. Without any token the loss is 0. Picks
     outside [0, E) count nowhere. The gradient goes to the logits (zero rows where a token does not count); the counts
     are constants to it."""
     _balance_check(logits, topi, mask, offsets)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _BalanceFn.apply(logits, topi, mask, offsets, float(coef))
     with L.on_device_of(logits):
-        return _Balance(logits, mask, offsets).forward(topi, coef, False)
+        if torch.is_grad_enabled() and logits.requires_grad:
+            return _BalanceFn.apply(logits, topi, mask, offsets, float(coef))
+        loss, counts, _ = _balance_forward(logits, topi, mask, offsets, float(coef), False)
+    return loss, counts

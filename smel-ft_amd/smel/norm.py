@@ -172,7 +172,8 @@ def gated_rmsnorm(x, z, w, eps):
 _LN_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _ln_check(x, h, w, b):
+def _ln_refuse(x, h, w, b):
+    """Raises what is wrong with the call."""
     _lib.one_device(x, h, w, b)
     if x.dtype not in _LN_DTYPES:
         raise ValueError(f"layer norm takes bf16, fp16 or fp32 rows, got {x.dtype}")
@@ -184,79 +185,114 @@ def _ln_check(x, h, w, b):
         if t is not None and (t.dtype not in (x.dtype, torch.float32) or tuple(t.shape) != (x.shape[-1],)
                               or not t.is_contiguous()):
             raise ValueError(f"layer norm weights must be contiguous [{x.shape[-1]}] tensors of {x.dtype} or float32")
-    if w is not None and b is not None and w.dtype != b.dtype:
-        raise ValueError(f"layer norm's weight is {w.dtype} and its bias {b.dtype}")
+    raise ValueError(f"layer norm's weight is {w.dtype} and its bias {b.dtype}")
 
 
-def _ln_wtype(x, w, b) -> int:
-    t = w if w is not None else b
-    return _LN_DTYPES[x.dtype if t is None else t.dtype]
+def _ln_check(x, h, w, b) -> tuple:
+    """(columns, the rows' type code, the weights' type code) of a call that the kernels take; a small norm is the host's
+    time, so each tensor is looked at once."""
+    dt = _LN_DTYPES.get(x.dtype)
+    if dt is None or x.dim() == 0 or not x.is_cuda:
+        _ln_refuse(x, h, w, b)
+    n, dev = x.shape[-1], x.device
+    ok = 1 <= n <= MAX_COLS
+    if h is not None:
+        ok = ok and h.shape == x.shape and h.dtype is x.dtype and h.device == dev
+    wd = None
+    for t in (w, b):
+        if t is not None:
+            ok = ok and (wd is None or t.dtype is wd) and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() \
+                and t.device == dev
+            wd = t.dtype
+    wt = dt if wd is None or wd is x.dtype else 2
+    if not ok or (wt == 2 and wd is not None and wd is not torch.float32):
+        _ln_refuse(x, h, w, b)
+    return n, dt, wt
 
 
-def _ln_forward(x, h, w, b, eps):
-    """(rows the norm read, their pitch, s or None, y, stats)."""
+def _rows_of(x, n: int):
+    """(rows with unit column stride, their count, their pitch): x itself where it is packed."""
+    if x.is_contiguous():
+        return x, x.numel() // n, n
+    rows, pitch = _row_layout(x)
+    return rows, rows.shape[0], pitch
+
+
+def _stats_like(x, rows: int):
+    """8 bytes a row (its mean and rstd), in a tensor of x's type: the cheapest allocation on x's device."""
+    return x.new_empty(rows * (8 // x.element_size()))
+
+
+def _ln_forward(x, h, w, b, eps, n, dt, wt):
+    """(rows the norm read, their count and pitch, s or None, y, stats)."""
     if h is None:
-        x2, pitch = _row_layout(x)
-        h2 = s = None
+        x2, R, pitch = _rows_of(x, n)
+        h2 = s = sp = None
     else:
-        x2, h2 = _packed(x), _packed(h)
-        pitch = x2.shape[1]
-        s = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    R, n = x2.shape
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    stats = torch.empty(R, 2, device=x.device, dtype=torch.float32)
+        x2, h2 = x.contiguous(), h.contiguous()
+        R, pitch = x2.numel() // n, n
+        s = torch.empty_like(x2)
+        sp = s.data_ptr()
+    y = torch.empty_like(x2) if x2.is_contiguous() and x2.shape == x.shape else x.new_empty(x.shape)
+    stats = _stats_like(x, R)
     p = _lib.ptr
-    _lib.call("smel_layernorm_fwd", p(x2), p(h2), R, n, pitch, p(w), p(b), float(eps), _LN_DTYPES[x.dtype],
-              _ln_wtype(x, w, b), p(s), p(y), p(stats), _lib.stream())
-    return (x2 if h is None else s), pitch, s, y, stats
+    _lib.call("smel_layernorm_fwd", x2.data_ptr(), p(h2), R, n, pitch, p(w), p(b), eps, dt, wt, sp, y.data_ptr(),
+              stats.data_ptr(), _lib.stream())
+    return (x2 if h is None else s), R, pitch, s, y, stats
+
+
+def _ln_backward(ctx, *grads):
+    """dx (the same for both addends), dw and db, each only where it is asked for."""
+    rows, w, stats = ctx.saved_tensors
+    add, n, R, pitch, dt, wt, shape, wdt = ctx.call
+    ds, dy = grads if add else (None, grads[0])
+    if dy is None:      # the sum alone was used (or nothing)
+        return ds, ds if add else None, None, None, None, None
+    nx, nh, nw, nb = ctx.needs_input_grad[:4]
+    want_x = nx or nh
+    p = _lib.ptr
+    dy2 = dy.contiguous()
+    ds2 = ds.contiguous() if ds is not None and want_x else None
+    dx = rows.new_empty(shape) if want_x else None
+    dw = rows.new_empty(n, dtype=wdt) if nw else None
+    db = rows.new_empty(n, dtype=wdt) if nb else None
+    ws, ws_n = None, 0
+    if nw or nb:
+        ws_n = _lib.load().smel_layernorm_bwd_ws_floats(R, n)
+        ws = rows.new_empty(ws_n * (4 // rows.element_size()))
+    _lib.call("smel_layernorm_bwd", dy2.data_ptr(), rows.data_ptr(), R, n, pitch, p(w), stats.data_ptr(), p(ds2), dt, wt,
+              p(dx), p(dw), p(db), p(ws), ws_n, _lib.stream())
+    return dx, dx if add else None, dw, db, None, None
+
+
+_ln_backward_once = once_differentiable(_ln_backward)
 
 
 class _LayerNormFn(torch.autograd.Function):
-    """forward(x, h, w, b, eps): y, or (s, y) with the residual addend h. Saved: the rows that the norm read and two fp32
-    numbers a row."""
+    """forward(x, h, w, b, eps, the call's (columns, types)): y, or (s, y) with the residual addend h. Saved: the rows that
+    the norm read and two fp32 numbers a row."""
 
     @staticmethod
-    def forward(ctx, x, h, w, b, eps):
-        with _lib.on_device_of(x):
-            rows, ctx.pitch, s, y, stats = _ln_forward(x, h, w, b, eps)
+    def forward(ctx, x, h, w, b, eps, call):
+        n, dt, wt = call
+        rows, R, pitch, s, y, stats = _ln_forward(x, h, w, b, eps, n, dt, wt)
         ctx.save_for_backward(rows, w, stats)
-        ctx.add, ctx.wtype, ctx.like_b = h is not None, _ln_wtype(x, w, b), b is not None
+        ctx.call = (h is not None, n, R, pitch, dt, wt, x.shape, torch.float32 if wt == 2 else x.dtype)
         ctx.set_materialize_grads(False)
         return y if h is None else (s, y)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        ds, dy = grads if ctx.add else (None, grads[0])
-        if dy is None:      # the sum alone was used (or nothing)
-            return ds, ds if ctx.add else None, None, None, None
-        rows, w, stats = ctx.saved_tensors
-        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        want_w, want_b = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
-        n = rows.shape[-1]
-        R = stats.shape[0]
-        dev, p = rows.device, _lib.ptr
-        dy2 = _packed(dy)
-        ds2 = _packed(ds) if ds is not None and want_x else None
-        dx = torch.empty(dy.shape, device=dev, dtype=rows.dtype) if want_x else None
-        wdt = torch.float32 if ctx.wtype == 2 else rows.dtype
-        dw = torch.empty(n, device=dev, dtype=wdt) if want_w else None
-        db = torch.empty(n, device=dev, dtype=wdt) if want_b else None
-        ws, ws_n = None, 0
-        if want_w or want_b:
-            ws_n = _lib.load().smel_layernorm_bwd_ws_floats(R, n)
-            ws = torch.empty(max(ws_n, 1), device=dev, dtype=torch.float32)
-        _lib.call("smel_layernorm_bwd", p(dy2), p(rows), R, n, ctx.pitch, p(w), p(stats), p(ds2),
-                  _LN_DTYPES[rows.dtype], ctx.wtype, p(dx), p(dw), p(db), p(ws), ws_n, _lib.stream())
-        return dx, dx if ctx.add else None, dw, db, None
+    def backward(ctx, *grads):     # on the forward's device: autograd's thread has set it
+        return (_ln_backward_once if torch.is_grad_enabled() else _ln_backward)(ctx, *grads)
 
 
 def _ln(x, h, w, b, eps):
-    _ln_check(x, h, w, b)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, h, w, b)):
-        return _LayerNormFn.apply(x, h, w, b, eps)
+    call = _ln_check(x, h, w, b)
     with _lib.on_device_of(x):
-        _, _, s, y, _ = _ln_forward(x, h, w, b, eps)
+        if torch.is_grad_enabled() and (x.requires_grad or h is not None and h.requires_grad or w is not None and w.requires_grad
+                                        or b is not None and b.requires_grad):
+            return _LayerNormFn.apply(x, h, w, b, float(eps), call)
+        _, _, _, s, y, _ = _ln_forward(x, h, w, b, float(eps), *call)
     return y if h is None else (s, y)
 
 
