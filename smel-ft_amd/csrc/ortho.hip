@@ -212,6 +212,7 @@ struct Slice {
 
 // columns of an apply block's slice at most: two blocks on a CU
 constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt <= 4 ? 256 : 128; }
+constexpr int max_slice16(int nt) { return nt == 1 ? 1024 : nt == 2 ? 512 : nt == 4 ? 256 : 128; }   // of 16-bit types
 constexpr int slice_bytes(int nt) { return 16 * nt * (max_slice(nt) + 20) * 4; }
 
 // A gram block takes `per` slices, the next one on its way while one is multiplied (two buffers). Waves of a block: the
@@ -221,6 +222,10 @@ constexpr int slice_bytes(int nt) { return 16 * nt * (max_slice(nt) + 20) * 4; }
 constexpr int gram_slice(int nt) { return nt == 1 ? 512 : nt == 2 ? 256 : nt == 4 ? 128 : 64; }
 constexpr int gram_waves(int nt) { return nt == 8 ? 12 : WAVES; }
 constexpr int gram_tg(int nt) { return nt == 8 ? 12 : nt == 4 ? 2 : 1; }
+// At r = 128 a wave's three tiles share their operands: the 28 pairs of eight rows of tiles are eight triangles (the lines of the
+// affine plane of order 3 that miss a point: rows a, b, c give the tiles ab, ac, bc) and four pairs left over, each with its
+// rows' diagonal tiles. Half the LDS reads and conversions of three tiles of their own (36 x 128 x 2816: 50 -> 43 us).
+constexpr uint16_t GRAM_ROWS[12] = {0x012, 0x345, 0x036, 0x147, 0x156, 0x237, 0x057, 0x246, 0x677, 0x255, 0x044, 0x133};
 
 template <int NT, int DT>
 __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, double* __restrict__ part) {
@@ -235,14 +240,24 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int tg = wave % TG, kg = wave / TG;
   f64x4_t acc[TPW];
-  int ra[TPW], rb[TPW];
+  int ra[TPW], rb[TPW], tile[TPW];
+  const uint32_t rows = GRAM_ROWS[wave % 12];
+  const bool triangle = wave < 8;
 #pragma unroll
   for (int k = 0; k < TPW; ++k) {
     acc[k] = f64x4_t{0, 0, 0, 0};
     int t, u;
-    tile_of(tg * TPW + k, NT, t, u);
-    ra[k] = (16 * t + lo) * pitch + 4 * hi;
-    rb[k] = (16 * u + lo) * pitch + 4 * hi;
+    if constexpr (NT == 8) {   // ra: the three rows' operands
+      const int r[3] = {(int)(rows >> 8), (int)(rows >> 4 & 15), (int)(rows & 15)};
+      ra[k] = (16 * r[k] + lo) * pitch + 4 * hi;
+      t = r[k == 2];
+      u = triangle ? r[k == 0 ? 1 : 2] : r[k == 0 || k == 2];
+    } else {
+      tile_of(tg * TPW + k, NT, t, u);
+      ra[k] = (16 * t + lo) * pitch + 4 * hi;
+      rb[k] = (16 * u + lo) * pitch + 4 * hi;
+    }
+    tile[k] = tile_at(t, u, NT);
   }
   Slice<NT, DT, W, S> in;
   in.fetch(J, mat, s0 << lg, lg);
@@ -252,13 +267,37 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
     const float* const x = X + ((sl - s0) & 1) * BUF;
     if (sl + 1 < s1) in.fetch(J, mat, (sl + 1) << lg, lg);
     // 16 columns a step, four to a lane: which columns make one instruction's contraction does not matter
-    for (int j = 16 * kg; j < slice; j += 16 * KG)
+    if constexpr (NT == 8) {
+      for (int j = 0; j < slice; j += 16) {
+        const f32x4_t a = *(const f32x4_t*)(x + ra[0] + j), b = *(const f32x4_t*)(x + ra[1] + j);
+        if (triangle) {
+          const f32x4_t c = *(const f32x4_t*)(x + ra[2] + j);
 #pragma unroll
-      for (int k = 0; k < TPW; ++k) {
-        const f32x4_t a = *(const f32x4_t*)(x + ra[k] + j), b = *(const f32x4_t*)(x + rb[k] + j);
+          for (int m = 0; m < 4; ++m) {
+            const double am = a[m], bm = b[m], cm = c[m];
+            acc[0] = mfma64(am, bm, acc[0]);
+            acc[1] = mfma64(am, cm, acc[1]);
+            acc[2] = mfma64(bm, cm, acc[2]);
+          }
+        } else {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
+          for (int m = 0; m < 4; ++m) {
+            const double am = a[m], bm = b[m];
+            acc[0] = mfma64(am, bm, acc[0]);
+            acc[1] = mfma64(am, am, acc[1]);
+            acc[2] = mfma64(bm, bm, acc[2]);
+          }
+        }
       }
+    } else {
+      for (int j = 16 * kg; j < slice; j += 16 * KG)
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+          const f32x4_t a = *(const f32x4_t*)(x + ra[k] + j), b = *(const f32x4_t*)(x + rb[k] + j);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
+        }
+    }
     if (sl + 1 < s1) in.put(J.x_tall, lg, X + ((sl + 1 - s0) & 1) * BUF, pitch);
     __syncthreads();
   }
@@ -277,7 +316,7 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
   }
   if (kg == 0)
 #pragma unroll
-    for (int k = 0; k < TPW; ++k) *(f64x4_t*)(out + ((tg * TPW + k) * 64 + lane) * 4) = acc[k];
+    for (int k = 0; k < TPW; ++k) *(f64x4_t*)(out + (tile[k] * 64 + lane) * 4) = acc[k];
 }
 
 struct Steps {
@@ -579,13 +618,18 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
 }
 
 // The same for 16-bit results, whose rounding (2^-9, 2^-12) leaves room for fp32 sums: Q as three bf16 parts (24 bits), G's
-// bf16 values as they are and fp16 values as two bf16 parts, products on v_mfma_f32_16x16x16_bf16: 36 x 128 x 2816 bf16 took
+// bf16 values as they are and fp16 values as two bf16 parts, products on the bf16 matrix instruction: 36 x 128 x 2816 bf16 took
 // 80 us on the f64 instruction. The parts' products are added in fp32: off by at most 3 r 2^-24 of sum |q| |g|.
-// G's slice lies in LDS as pairs of rows: word [i / 2][j] = (i, i + 1), the operand's neighbours. Pitch slice + 8: the four
-// row pairs that 64 lanes read at 16 columns take the banks twice at most.
+// Of a tile's 16 rows (the contraction), lane l / 16 = h takes h, 4 + h, 8 + h and 12 + h: the order in which Q's tiles lie.
+// G's slice lies in LDS as words of the rows (i, i + 4): word [8 u + 4 k + h][j], rows 16 u + 8 k + h and + 4. Pitch slice + 36:
+// the four words' rows that 64 lanes read at 16 columns take the banks twice at most.
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
-SMEL_DEV f32x4_t mfma16(s16x4_t a, s16x4_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
-SMEL_DEV s16x4_t words(uint32_t a, uint32_t b) { return __builtin_bit_cast(s16x4_t, (u32x2_t{a, b})); }
+SMEL_DEV f32x4_t mfma16(u32x2_t a, u32x2_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, a), __builtin_bit_cast(s16x4_t, b), c, 0, 0, 0);
+}
+SMEL_DEV f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {   // two tiles' rows at once
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
 
 template <int NT>
 SMEL_DEV void load_pairs(const Job& J, int mat, int j0, int lg, uint32_t* X, int pitch) {
@@ -601,15 +645,17 @@ SMEL_DEV void load_pairs(const Job& J, int mat, int j0, int lg, uint32_t* X, int
       const int j = e / (16 * Q) * 16 + (e & 15), i = (e >> 4) % Q * 8;
       const u32x4_t v = ld_raw<0>(x + (int64_t)(j0 + j) * J.ld + i, j < nc ? J.r - i : 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) X[(i / 2 + k) * pitch + j] = v[k];
+      for (int h = 0; h < 4; ++h)
+        X[(i / 2 + h) * pitch + j] = (h & 1) ? v[h >> 1] >> 16 | (v[2 + (h >> 1)] & 0xffff0000u)
+                                             : (v[h >> 1] & 0xffffu) | v[2 + (h >> 1)] << 16;
     }
   } else {
     const int chunks = RP / 2 << (lg - 3);
 #pragma unroll 2
     for (int e = threadIdx.x; e < chunks; e += 64 * WAVES) {
-      const int p = e >> (lg - 3), j = (e << 3) & (slice - 1);
-      const uint16_t* const row = x + 2 * p * J.ld + j0 + j;
-      const u32x4_t a = ld_raw<0>(row, 2 * p < J.r ? nc - j : 0), b = ld_raw<0>(row + J.ld, 2 * p + 1 < J.r ? nc - j : 0);
+      const int p = e >> (lg - 3), j = (e << 3) & (slice - 1), i = (p >> 2) * 8 + (p & 3);
+      const uint16_t* const row = x + i * J.ld + j0 + j;
+      const u32x4_t a = ld_raw<0>(row, i < J.r ? nc - j : 0), b = ld_raw<0>(row + 4 * J.ld, i + 4 < J.r ? nc - j : 0);
       u32x4_t w[2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -648,68 +694,65 @@ template <int NT, int DT, bool SMALL>
 __global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps st, const double* __restrict__ in,
                                                           const double* __restrict__ qscale) {
   constexpr int CG = WAVES / NT;
-  __shared__ __attribute__((aligned(16))) uint32_t X[8 * NT * (max_slice(NT) + 8)];
-  const int slice = 1 << js.lg, pitch = slice + 8;
+  __shared__ __attribute__((aligned(16))) uint32_t X[8 * NT * (max_slice16(NT) + 36)];
+  const int slice = 1 << js.lg, pitch = slice + 36;
   const Job& J = js.j[find_job<BY_APPLY>(js, blockIdx.x)];
   const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = (lb % J.slices) << js.lg;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int t = wave % NT, cg = wave / NT;
   load_pairs<NT>(J, mat, j0, js.lg, X, pitch);
+  constexpr int K2 = NT == 1 ? 1 : 2;   // tiles of an instruction's contraction
+  typedef uint32_t word_t __attribute__((ext_vector_type(2 * K2)));
   float scale;
-  s16x4_t q[NT][3];   // parts of Q[16 t + lo][16 u + 4 hi + 0..3]
-  auto parts = [&](int u, const double (&v)[4]) {
+  word_t q[NT / K2][3];   // parts of Q[16 t + lo][16 u + 4 m + hi]
+  auto parts = [&](int u, f64x4_t v) {
     float r[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) r[k] = (float)v[k];
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       const uint32_t a = pack2bf(r[0], r[1]), b = pack2bf(r[2], r[3]);
-      q[u][p] = words(a, b);
+      q[u / K2][p][2 * (u % K2)] = a;
+      q[u / K2][p][2 * (u % K2) + 1] = b;
       r[0] -= bf_lo(a);
       r[1] -= bf_hi(a);
       r[2] -= bf_lo(b);
       r[3] -= bf_hi(b);
     }
   };
-  // element (4 hi + k, lo) of tile (u, t): register hi of lane (k, lo)
   if constexpr (SMALL) {
     __shared__ f64x4_t b[4 * NT * NT][64];
     __shared__ double tr[NT];
     scale = (float)steps_small<NT>(J, mat, st, in, b, tr);
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const double* const f = (const double*)b[(3 * NT + u) * NT + t];
-      parts(u, {f[lo * 4 + hi], f[(16 + lo) * 4 + hi], f[(32 + lo) * 4 + hi], f[(48 + lo) * 4 + hi]});
-    }
+    for (int u = 0; u < NT; ++u) parts(u, b[(3 * NT + u) * NT + t][lane]);
   } else {
     scale = (float)qscale[J.mat0 + mat];
     const double* const Q = in + (int64_t)(J.mat0 + mat) * (NT * NT * 256);
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const double* const f = Q + (u * NT + t) * 256;
-      parts(u, {f[lo * 4 + hi], f[(16 + lo) * 4 + hi], f[(32 + lo) * 4 + hi], f[(48 + lo) * 4 + hi]});
-    }
+    for (int u = 0; u < NT; ++u) parts(u, *(const f64x4_t*)(Q + ((u * NT + t) * 64 + lane) * 4));
     __syncthreads();
   }
   const int nc = min(slice, J.n - j0);
   uint16_t* const y = (uint16_t*)J.y + (int64_t)mat * J.r * J.n;
-  // acc += Q G (or its transpose) for column c of the lane
-  auto dot = [&](int u, int c, bool tall, f32x4_t acc) {
-    const uint32_t* const x = X + (8 * u + 2 * hi) * pitch + c;
-    const uint32_t w0 = x[0], w1 = x[pitch];
-    s16x4_t g, g2;
-    if constexpr (DT == 0) {
-      g = words(w0, w1);
-    } else {
-      const float f0 = to_f<2>(w0 & 0xffffu), f1 = to_f<2>(w0 >> 16), f2 = to_f<2>(w1 & 0xffffu), f3 = to_f<2>(w1 >> 16);
-      const uint32_t a = pack2bf(f0, f1), b = pack2bf(f2, f3);
-      g = words(a, b);
-      g2 = words(pack2bf(f0 - bf_lo(a), f1 - bf_hi(a)), pack2bf(f2 - bf_lo(b), f3 - bf_hi(b)));
+  // acc += Q G (or its transpose) over the tiles of instruction v, for column c of the lane
+  auto dot = [&](int v, int c, bool tall, f32x4_t acc) {
+    word_t g, g2;
+#pragma unroll
+    for (int k = 0; k < 2 * K2; ++k) {
+      const uint32_t w = X[(8 * K2 * v + 4 * k + hi) * pitch + c];
+      if constexpr (DT == 0) {
+        g[k] = w;
+      } else {
+        const float f0 = to_f<2>(w & 0xffffu), f1 = to_f<2>(w >> 16);
+        g[k] = pack2bf(f0, f1);
+        g2[k] = pack2bf(f0 - bf_lo(g[k]), f1 - bf_hi(g[k]));
+      }
     }
 #pragma unroll
     for (int p = 2; p >= 0; --p) {
-      if (DT == 2 && p < 2) acc = tall ? mfma16(q[u][p], g2, acc) : mfma16(g2, q[u][p], acc);
-      acc = tall ? mfma16(q[u][p], g, acc) : mfma16(g, q[u][p], acc);
+      if (DT == 2 && p < 2) acc = tall ? mfma16(q[v][p], g2, acc) : mfma16(g2, q[v][p], acc);
+      acc = tall ? mfma16(q[v][p], g, acc) : mfma16(g, q[v][p], acc);
     }
     return acc;
   };
@@ -717,7 +760,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps s
     for (int j = 16 * cg; j < nc; j += 16 * CG) {
       f32x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int u = 0; u < NT; ++u) acc = dot(u, j + lo, true, acc);
+      for (int v = 0; v < NT / K2; ++v) acc = dot(v, j + lo, true, acc);
       acc = acc * scale;
       const int i = 16 * t + 4 * hi;   // rows i + m, column j + lo
       if (j + lo < nc) st_run16<DT, 4>(y + (int64_t)(j0 + j + lo) * J.r + i, J.r - i, (const float*)&acc);
@@ -727,9 +770,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply16_kernel(Jobs js, Steps s
       f32x4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
       const int c = j + 8 * (lo >> 2) + (lo & 3);   // row 4 hi + m of the pair's results: columns 8 hi + m and 8 hi + 4 + m
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        acc[0] = dot(u, c, false, acc[0]);
-        acc[1] = dot(u, c + 4, false, acc[1]);
+      for (int v = 0; v < NT / K2; ++v) {
+        acc[0] = dot(v, c, false, acc[0]);
+        acc[1] = dot(v, c + 4, false, acc[1]);
       }
       acc[0] = acc[0] * scale;
       acc[1] = acc[1] * scale;
@@ -918,7 +961,7 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
   }
   // the largest slices that give most CUs a block, but at least 128 columns (each wave a block of 16); up to r = 32 every
   // block runs the steps, and two on a CU get in each other's way (a layer's 84 updates: 20.7 us with 780 blocks, 14.4 with 195)
-  int slice = max_slice(nt);
+  int slice = dt == 1 ? max_slice(nt) : max_slice16(nt);
   while (slice > 128 && cols / slice < 192) slice /= 2;
   p.js.lg = __builtin_ctz(slice);
   // gram: likewise, down to 64 columns at r > 64; then one round of blocks (two on a CU, one at r > 64, whose blocks fill it
