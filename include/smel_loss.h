@@ -101,7 +101,7 @@ int smel_ce_dequant8(const int8_t* q, const void* scale, int64_t R, int64_t C, i
  *   loss = coef / S' * sum_s E sum_e c[s][e] / (K n_s) * mean_t p[t][e]
  * (0 without any token). Rows that do not count may hold anything.
  * `dtype` of the logits [T][ldl]: 0 bf16, 1 fp32, 2 fp16; topi [T][K] contiguous, int64 or int32 by topi_i64.
- * 0 <= T <= 2^24, 1 <= E <= 512, 1 <= K <= 64, 1 <= S <= 2^24.
+ * 0 <= T <= 2^24, 1 <= E <= 512, 1 <= K <= 64, 1 <= S <= 2^22.
  * Writes loss (fp32), counts (int64 [S][E]) and, for the backward, row_stats ([T] of 16 bytes, aligned to them: the row's
  * maximum and 1 / its sum of exponentials (fp32), its sequence (int32, -1 where it does not count); may be null without a
  * backward) and weights (fp32 [S][E] and one more: coef E / (K n_s^2) (c[s][e] - sum_e c[s][e] / E), then

@@ -441,7 +441,7 @@ Ws ws_of(int64_t T, int64_t E, int64_t S) {
 int check(const char* name, const void* z, int64_t ldl, int dtype, int64_t T, int64_t E, int64_t S, const void* off) {
   SMEL_REQUIRE(T >= 0 && T <= (int64_t)1 << 24, SMEL_EUNSUPPORTED, "%s: T=%lld tokens, 0 to 2^24", name, (long long)T);
   SMEL_REQUIRE(E >= 1 && E <= MAX_E, SMEL_EUNSUPPORTED, "%s: E=%lld experts, 1 to %d", name, (long long)E, MAX_E);
-  SMEL_REQUIRE(S >= 1 && S <= (int64_t)1 << 24, SMEL_EUNSUPPORTED, "%s: S=%lld sequences, 1 to 2^24", name, (long long)S);
+  SMEL_REQUIRE(S >= 1 && S <= (int64_t)1 << 22, SMEL_EUNSUPPORTED, "%s: S=%lld sequences, 1 to 2^22", name, (long long)S);
   SMEL_REQUIRE(off || S == 1, SMEL_EINVAL, "%s: %lld sequences without offsets", name, (long long)S);
   SMEL_REQUIRE(dtype >= 0 && dtype <= 2, SMEL_EINVAL, "%s: dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", name, dtype);
   SMEL_REQUIRE(T == 0 || z, SMEL_EINVAL, "%s: null logits", name);

@@ -434,7 +434,7 @@ int64_t bwd_blocks(int64_t rows, int64_t cols) {
 template <int DT, int WT, int CPL, int BS>
 int launch_fwd(const LnArgs& p, hipStream_t stream) {
   const int64_t rpb = BS / p.lpr, blocks = (p.rows + rpb - 1) / rpb;
-  SMEL_REQUIRE(blocks < (int64_t)1 << 22, SMEL_EUNSUPPORTED, "layernorm_fwd: %lld rows is too many", (long long)p.rows);
+  SMEL_REQUIRE(blocks * BS < (int64_t)1 << 32, SMEL_EUNSUPPORTED, "layernorm_fwd: %lld rows is too many", (long long)p.rows);
   if (p.h) ln_fwd_kernel<DT, WT, CPL, BS, true><<<(unsigned)blocks, BS, 0, stream>>>(p);
   else ln_fwd_kernel<DT, WT, CPL, BS, false><<<(unsigned)blocks, BS, 0, stream>>>(p);
   return smel::launch_status();

@@ -423,18 +423,20 @@ def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
     L.call("smel_balance_fwd", z.data_ptr(), ldl, dt, topi.data_ptr(), topi.dtype is torch.int64, T, E, topi.shape[1],
            p(mask), p(off), off is not None and off.dtype is torch.int64, S, coef, loss.data_ptr(), counts.data_ptr(),
            rows if need_grad else None, weights, weights + weights_n, ws_n, L.stream())
-    return loss, counts, (z, mem, ldl, dt, T, E, S, rows, weights)
+    return loss, counts, (z, mem, dt, T, E, S, rows_n)
 
 
 def _balance_backward(ctx, go, _):
     if go is None:
         return None, None, None, None, None
     z, mem = ctx.saved_tensors
-    ldl, dt, T, E, S, rows, weights = ctx.call
+    dt, T, E, S, rows_n = ctx.call
+    ldl = z.stride(0) if T > 1 else E     # of what comes back: hooks on saved tensors may repack it
+    rows = mem.data_ptr()
     if go.dtype is not torch.float32 or go.device != z.device:
         go = go.to(device=z.device, dtype=torch.float32)
     dz = z.new_empty((T, E))
-    L.call("smel_balance_bwd", z.data_ptr(), ldl, dt, T, E, S, rows, weights, go.data_ptr(), dz.data_ptr(), L.stream())
+    L.call("smel_balance_bwd", z.data_ptr(), ldl, dt, T, E, S, rows, rows + rows_n, go.data_ptr(), dz.data_ptr(), L.stream())
     return dz, None, None, None, None
 
 

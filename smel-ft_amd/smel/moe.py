@@ -741,10 +741,10 @@ def route(x2d, gate_w, top_k, with_logits=False):
 
 class _RouteGemma4Fn(torch.autograd.Function):
     """route_gemma4 (smel/moe.py:170-180): topv differentiable w.r.t. h through the per-expert scale, the renorm, the
-    softmax, the router GEMM and the weightless RMSNorm."""
+    softmax, the router GEMM and the weightless RMSNorm; with_logits as in _RouteFn."""
 
     @staticmethod
-    def forward(ctx, h, scale, proj, pes, top_k, eps):
+    def forward(ctx, h, scale, proj, pes, top_k, eps, with_logits=False):
         T, H = h.shape
         E = proj.shape[0]
         dev = h.device
@@ -759,44 +759,51 @@ class _RouteGemma4Fn(torch.autograd.Function):
                L.ptr(probs), L.ptr(topv), L.ptr(topi), L.ptr(topi32), L.ptr(xn), L.ptr(rstd), L.ptr(lg), L.stream())
         ctx.save_for_backward(h, scale, proj, pes, probs, topi32, rstd)
         ctx.mark_non_differentiable(probs, topi)
-        return probs, topv, topi
+        ctx.set_materialize_grads(not with_logits)   # either gradient may be missing then
+        return (probs, topv, topi, lg[:, :E]) if with_logits else (probs, topv, topi)
 
     @staticmethod
-    def backward(ctx, dprobs, dtopv, dtopi):
-        if dtopv is None:
-            return None, None, None, None, None, None
+    def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
+        if dtopv is None and dlogits is None:
+            return None, None, None, None, None, None, None
         h, scale, proj, pes, probs, topi32, rstd = ctx.saved_tensors
         T, H = h.shape
         E, K = probs.shape[1], topi32.shape[1]
         dev = h.device
         wr = _router_ext_weight(proj, None)
-        dl = torch.empty(T, wr.R, dtype=torch.bfloat16, device=dev)
-        dw = dtopv.float().contiguous()
-        L.call("smel_route_bwd", L.ptr(dw), 1, None, L.ptr(probs), L.ptr(topi32), None, None, 0, T, K, E, T * K,
-               L.ptr(dl), wr.R, None, L.ptr(pes), L.stream())
+        if dtopv is None:
+            dl = torch.zeros(T, wr.R, dtype=torch.bfloat16, device=dev)
+        else:
+            dl = torch.empty(T, wr.R, dtype=torch.bfloat16, device=dev)
+            dw = dtopv.float().contiguous()
+            L.call("smel_route_bwd", L.ptr(dw), 1, None, L.ptr(probs), L.ptr(topi32), None, None, 0, T, K, E, T * K,
+                   L.ptr(dl), wr.R, None, L.ptr(pes), L.stream())
+        if dlogits is not None:
+            dl[:, :E] += dlogits
         dxn = _router_dx(dl, wr, T, dev, L.stream())
         dh = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
         L.call("smel_route_gemma4_prenorm_bwd", L.ptr(h), L.ptr(scale), L.ptr(rstd), L.ptr(dxn), T, H, L.ptr(dh),
                L.stream())
-        return dh, None, None, None, None, None
+        return dh, None, None, None, None, None, None
 
 
-def route_gemma4(h, W, top_k, eps):
+def route_gemma4(h, W, top_k, eps, with_logits=False):
     """Gemma 4 router on the residual stream (smel/moe.py:170-180) -> (probs fp32 [T,E], topv fp32 [T,K] =
     renormalised top-k x per_expert_scale, topi int64 [T,K]): weightless RMSNorm, x router.scale x H^-0.5, logits,
-    softmax, top-k, renorm, scale, as HIP kernels (differentiable w.r.t. h)."""
+    softmax, top-k, renorm, scale, as HIP kernels (differentiable w.r.t. h); with_logits: (..., logits) as in ``route``."""
     L.require_device(h)
+    k, eps, wl = int(top_k), float(eps), bool(with_logits)
     if h.dtype == torch.bfloat16 and _bf16_limit(h.shape[-1]) is not None:
-        return F32.RouteGemma4Fn.apply(h.float(), _f32_of(_bf16(W["router.scale"])).reshape(-1),
-                                       _f32_of(_bf16(W["router.proj.weight"])),
-                                       _f32_of(_bf16(W["router.per_expert_scale"])).reshape(-1), int(top_k), float(eps))
+        probs, topv, topi, *lg = F32.RouteGemma4Fn.apply(
+            h.float(), _f32_of(_bf16(W["router.scale"])).reshape(-1), _f32_of(_bf16(W["router.proj.weight"])),
+            _f32_of(_bf16(W["router.per_expert_scale"])).reshape(-1), k, eps, wl)
+        return (probs, topv, topi, *(t.to(h.dtype) for t in lg))
     if h.dtype == torch.float32:
         return F32.RouteGemma4Fn.apply(F32.f32(h), F32.f32(W["router.scale"], "router.scale").reshape(-1),
                                        F32.f32(W["router.proj.weight"], "router.proj.weight"),
-                                       F32.f32(W["router.per_expert_scale"], "router.per_expert_scale").reshape(-1),
-                                       int(top_k), float(eps))
+                                       F32.f32(W["router.per_expert_scale"], "router.per_expert_scale").reshape(-1), k, eps, wl)
     return _RouteGemma4Fn.apply(_bf16(h), _bf16(W["router.scale"]).reshape(-1), _bf16(W["router.proj.weight"]),
-                                _bf16(W["router.per_expert_scale"]).reshape(-1), int(top_k), float(eps))
+                                _bf16(W["router.per_expert_scale"]).reshape(-1), k, eps, wl)
 
 
 # ------------------------------------------------------------------------------------------------ fused layer

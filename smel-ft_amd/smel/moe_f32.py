@@ -290,10 +290,10 @@ def _router_bwd(dtopv, probs, topi32, w, pes, dlogits=None):
 
 class RouteGemma4Fn(torch.autograd.Function):
     """route_gemma4 (smel/moe.py:170-180) on fp32 tensors: weightless RMSNorm of h, x router.scale x fp32(H^-1/2),
-    logits, softmax, top-k, renorm, x per_expert_scale; differentiable w.r.t. h."""
+    logits, softmax, top-k, renorm, x per_expert_scale; differentiable w.r.t. h; with_logits as in RouteFn."""
 
     @staticmethod
-    def forward(ctx, h, scale, proj, pes, top_k, eps):
+    def forward(ctx, h, scale, proj, pes, top_k, eps, with_logits=False):
         T, H = h.shape
         E = proj.shape[0]
         dev = h.device
@@ -314,19 +314,20 @@ class RouteGemma4Fn(torch.autograd.Function):
         ctx.save_for_backward(h, scale, proj, pes, probs, topi32, rstd)
         ctx.hs = hs
         ctx.mark_non_differentiable(probs, topi)
-        return probs, topv, topi
+        ctx.set_materialize_grads(not with_logits)   # either gradient may be missing then
+        return (probs, topv, topi, logits) if with_logits else (probs, topv, topi)
 
     @staticmethod
-    def backward(ctx, dprobs, dtopv, dtopi):
-        if dtopv is None:
-            return None, None, None, None, None, None
+    def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
+        if dtopv is None and dlogits is None:
+            return None, None, None, None, None, None, None
         h, scale, proj, pes, probs, topi32, rstd = ctx.saved_tensors
         T, H = h.shape
-        dxn = _router_bwd(dtopv, probs, topi32, proj, pes)
+        dxn = _router_bwd(dtopv, probs, topi32, proj, pes, dlogits)
         dh = torch.empty(T, H, dtype=torch.float32, device=h.device)
         L.call("smel_route_prenorm_bwd_f32", L.ptr(h), L.ptr(scale), L.ptr(rstd), L.ptr(dxn), T, H, ctx.hs, L.ptr(dh),
                L.stream(), tag="route_f32_bwd")
-        return dh, None, None, None, None, None
+        return dh, None, None, None, None, None, None
 
 
 # ------------------------------------------------------------------------------------------------ routed experts

@@ -224,7 +224,7 @@ def _stats_like(x, rows: int):
 
 
 def _ln_forward(x, h, w, b, eps, n, dt, wt):
-    """(rows the norm read, their count and pitch, s or None, y, stats)."""
+    """(rows the norm read, their count, s or None, y, stats)."""
     if h is None:
         x2, R, pitch = _rows_of(x, n)
         h2 = s = sp = None
@@ -238,13 +238,14 @@ def _ln_forward(x, h, w, b, eps, n, dt, wt):
     p = _lib.ptr
     _lib.call("smel_layernorm_fwd", x2.data_ptr(), p(h2), R, n, pitch, p(w), p(b), eps, dt, wt, sp, y.data_ptr(),
               stats.data_ptr(), _lib.stream())
-    return (x2 if h is None else s), R, pitch, s, y, stats
+    return (x2 if h is None else s), R, s, y, stats
 
 
 def _ln_backward(ctx, *grads):
     """dx (the same for both addends), dw and db, each only where it is asked for."""
     rows, w, stats = ctx.saved_tensors
-    add, n, R, pitch, dt, wt, shape, wdt = ctx.call
+    add, n, R, dt, wt, shape, wdt = ctx.call
+    pitch = n if rows.is_contiguous() else rows.stride(0)     # of what comes back: hooks on saved tensors may repack it
     ds, dy = grads if add else (None, grads[0])
     if dy is None:      # the sum alone was used (or nothing)
         return ds, ds if add else None, None, None, None, None
@@ -275,9 +276,9 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, w, b, eps, call):
         n, dt, wt = call
-        rows, R, pitch, s, y, stats = _ln_forward(x, h, w, b, eps, n, dt, wt)
+        rows, R, s, y, stats = _ln_forward(x, h, w, b, eps, n, dt, wt)
         ctx.save_for_backward(rows, w, stats)
-        ctx.call = (h is not None, n, R, pitch, dt, wt, x.shape, torch.float32 if wt == 2 else x.dtype)
+        ctx.call = (h is not None, n, R, dt, wt, x.shape, torch.float32 if wt == 2 else x.dtype)
         ctx.set_materialize_grads(False)
         return y if h is None else (s, y)
 
@@ -292,7 +293,7 @@ def _ln(x, h, w, b, eps):
         if torch.is_grad_enabled() and (x.requires_grad or h is not None and h.requires_grad or w is not None and w.requires_grad
                                         or b is not None and b.requires_grad):
             return _LayerNormFn.apply(x, h, w, b, float(eps), call)
-        _, _, _, s, y, _ = _ln_forward(x, h, w, b, float(eps), *call)
+        _, _, s, y, _ = _ln_forward(x, h, w, b, float(eps), *call)
     return y if h is None else (s, y)
 
 

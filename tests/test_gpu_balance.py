@@ -280,3 +280,50 @@ def test_balance_refusals():
         zg.add_(1)
     with pytest.raises(RuntimeError):      # changed in place before the backward
         loss.backward()
+
+
+def test_balance_saved_tensors_moved():
+    """Hooks that take saved tensors to the host and back (repacked) change nothing, strided rows included; twice is the same."""
+    from smel.loss import balance_loss
+    z, topi = make(200, 48, 4, "bf16", 3)
+    wide = torch.zeros(200, 70, dtype=z.dtype, device=DEV)
+    wide[:, 11:59] = z.to(DEV)
+    off = torch.tensor([0, 30, 200], device=DEV)
+    for t in (z.to(DEV), wide[:, 11:59]):
+        zg = t.detach().requires_grad_(True)
+        loss, _ = balance_loss(zg, topi.to(DEV), offsets=off)
+        ref, = torch.autograd.grad(loss, zg, retain_graph=True)
+        assert torch.equal(ref, torch.autograd.grad(loss, zg)[0])
+        with torch.autograd.graph.save_on_cpu():
+            loss, _ = balance_loss(zg, topi.to(DEV), offsets=off)
+        assert torch.equal(ref, torch.autograd.grad(loss, zg)[0])
+
+
+@pytest.mark.parametrize("dt,H", [("bf16", 128), ("fp32", 128), ("bf16", 96)])
+def test_route_gemma4_logits_and_their_gradient(dt, H):
+    """The same routing as without; the logits' gradient alone and with topv's is the sum of the two alone, to the roundings of
+    dlogits' sum and of dx (the norm's backward mixes a row)."""
+    from smel.loss import balance_loss
+    from smel.moe import route_gemma4
+    T, E, K = 70, 16, 2
+    g = torch.Generator().manual_seed(11)
+    r = lambda *s: torch.randn(*s, generator=g)
+    W = {"router.scale": (1 + 0.1 * r(H)).to(DEV, DT[dt]), "router.proj.weight": r(E, H).to(DEV, DT[dt]),
+         "router.per_expert_scale": (1 + 0.1 * r(E)).to(DEV, DT[dt])}
+    h = (2 * r(T, H)).to(DEV, DT[dt])
+    plain = route_gemma4(h, W, K, 1e-6)
+    hg = h.detach().requires_grad_(True)
+    probs, topv, topi, lg = route_gemma4(hg, W, K, 1e-6, with_logits=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, (probs, topv, topi)))
+    half = torch.finfo(lg.dtype).eps / 2
+    soft = torch.softmax(lg.detach().double(), 1)
+    # probs are the softmax of the logits (of the unrounded ones where the bf16 rows run on the fp32 kernels)
+    assert ((probs.double() - soft).abs() <= soft * (64 * U + 4 * half * lg.detach().double().abs().amax(1, keepdim=True))).all()
+    loss, _ = balance_loss(lg, topi)
+    cot = r(T, K).to(DEV) * 1e-3
+    only_l, = torch.autograd.grad(loss, hg, retain_graph=True)
+    only_v, = torch.autograd.grad(topv, hg, cot, retain_graph=True)
+    both, = torch.autograd.grad((topv, loss), hg, (cot, torch.ones((), device=DEV)))
+    a, p, q = both.double(), only_l.double(), only_v.double()
+    scale = p.abs() + q.abs()
+    assert p.abs().max() > 0 and ((a - p - q).abs() <= 16 * half * (scale + scale.amax(1, keepdim=True))).all()

@@ -285,3 +285,31 @@ def test_layernorm_refusals():
     gx, = torch.autograd.grad(y, xg, torch.ones_like(y).requires_grad_(True), create_graph=True)
     with pytest.raises(RuntimeError):      # once differentiable
         gx.sum().backward()
+
+
+def test_layernorm_saved_tensors_moved():
+    """Hooks that take saved tensors to the host and back (repacked) change nothing, strided rows included."""
+    from smel.norm import add_layernorm, layernorm
+    x, h, w, b, dy, ds = (t.to(DEV) for t in make(40, 120, torch.bfloat16, torch.float32, 3))
+    for cut in (slice(None), slice(10, 110)):
+        xs = x[:, cut].detach().requires_grad_(True)
+        wg, bg = w[cut].clone().requires_grad_(True), b[cut].clone().requires_grad_(True)
+        ref = torch.autograd.grad(layernorm(xs, wg, bg, EPS), (xs, wg, bg), dy[:, cut])
+        with torch.autograd.graph.save_on_cpu():
+            y = layernorm(xs, wg, bg, EPS)
+        assert all(torch.equal(a, c) for a, c in zip(ref, torch.autograd.grad(y, (xs, wg, bg), dy[:, cut])))
+    hg = h.detach().requires_grad_(True)
+    ref, = torch.autograd.grad(add_layernorm(hg, x, w, b, EPS), hg, (ds, dy))
+    with torch.autograd.graph.save_on_cpu():
+        out = add_layernorm(hg, x, w, b, EPS)
+    assert torch.equal(ref, torch.autograd.grad(out, hg, (ds, dy))[0])
+
+
+def test_layernorm_backward_twice():
+    from smel.norm import layernorm
+    x, _, w, b, dy, _ = make(300, 96, torch.float16, torch.float16, 9)
+    xg, wg, bg = d(x), d(w), d(b)
+    y = layernorm(xg, wg, bg, EPS)
+    one = torch.autograd.grad(y, (xg, wg, bg), dy.to(DEV), retain_graph=True)
+    two = torch.autograd.grad(y, (xg, wg, bg), dy.to(DEV))
+    assert all(torch.equal(a, c) for a, c in zip(one, two))

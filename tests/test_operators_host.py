@@ -34,7 +34,7 @@ def test_balance_refusals():
     def f(z=16, ldl=16, dt=0, topi=16, T=100, E=16, K=2, off=16, S=3, loss=16, counts=16, stats=16, w=16, ws=16, n=need):
         return L.smel_balance_fwd(z, ldl, dt, topi, 1, T, E, K, None, off, 1, S, 1.0, loss, counts, stats, w, ws, n, None)
     g = lambda z=16, st=16, w=16, go=16, dz=16, E=16: L.smel_balance_bwd(z, 16, 0, 100, E, 3, st, w, go, dz, None)
-    assert f(E=513, ldl=513) == -2 and f(E=0) == -2 and f(T=-1) == -2 and f(T=(1 << 24) + 1) == -2 and f(S=0) == -2
+    assert f(E=513, ldl=513) == -2 and f(E=0) == -2 and f(T=-1) == -2 and f(T=(1 << 24) + 1) == -2 and f(S=0) == -2 and f(S=(1 << 22) + 1) == -2
     assert f(off=None) == -1 and f(dt=3) == -1 and f(ldl=15) == -1 and f(z=None) == -1 and f(topi=None) == -1
     assert f(K=0) == -2 and f(K=65) == -2 and f(loss=None) == -1 and f(counts=None) == -1 and f(w=None) == -1
     assert f(stats=8) == -1 and g(st=8) == -1
