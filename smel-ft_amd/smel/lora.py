@@ -155,33 +155,33 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
         return []
     if not ts[0].is_cuda:
         _lib.one_device(ts[0])
-    jobs, outs, keep, n = array("q"), [], [], 0
-    dev = ts[0].device
+    jobs, outs, keep = array("q"), [], []
+    add, dev = jobs.extend, ts[0].device
     with torch.no_grad(), _lib.on_device_of(ts[0]):
-        for t in ts:     # a layer has a dozen: about three microseconds each
+        for t in ts:     # a layer has a dozen: what each costs here is the call's time
+            shape = t.shape
             code = _ORTHO_DTYPES.get(t.dtype)
-            *lead, rows, cols = t.shape if t.dim() > 1 else (0, 0)
-            if code is None or t.dim() < 2:
-                raise ValueError(f"orthogonalize takes bf16, fp16 or fp32 matrices, got {tuple(t.shape)} {t.dtype}")
+            if code is None or len(shape) < 2:
+                raise ValueError(f"orthogonalize takes bf16, fp16 or fp32 matrices, got {tuple(shape)} {t.dtype}")
+            rows, cols = shape[-2], shape[-1]
             if rows > ORTHO_MAX_RANK and cols > ORTHO_MAX_RANK:
                 raise ValueError(f"orthogonalize takes matrices whose shorter side is at most {ORTHO_MAX_RANK}, got "
-                                 f"{tuple(t.shape)}")
+                                 f"{tuple(shape)}")
             if t.device != dev:
                 _lib.one_device(ts[0], t)
-            size = rows * cols
+            values, size = t.numel(), rows * cols
             if t.is_contiguous():
                 y = torch.empty_like(t)
-                if t.numel():
-                    jobs.extend((t.data_ptr(), y.data_ptr(), t.numel() // size, rows, cols, size, cols, 1, code))
-                    n += 1
+                if values:
+                    add((t.data_ptr(), y.data_ptr(), values // size, rows, cols, size, cols, 1, code))
             else:
-                y = t.new_empty(t.shape)
-                if t.numel():
+                y = t.new_empty(shape)
+                if values:
                     x = _ortho_operand(t)
                     keep.append(x)
-                    jobs.extend((x.data_ptr(), y.data_ptr(), *x.shape, *x.stride(), code))
-                    n += 1
+                    add((x.data_ptr(), y.data_ptr(), *x.shape, *x.stride(), code))
             outs.append(y)
+        n = len(jobs) // 9
         addr = jobs.buffer_info()[0]
         need = _lib.load().smel_orthogonalize_ws(addr, n)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
