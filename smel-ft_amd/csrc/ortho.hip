@@ -77,14 +77,6 @@ template <>
 struct Elem<1> {
   typedef float T;
 };
-template <int DT>
-SMEL_DEV void st_elem(typename Elem<DT>::T* p, double v) {
-  const float f = (float)v;
-  if constexpr (DT == 1) *p = f;
-  if constexpr (DT == 0) *p = f2bf(f);
-  if constexpr (DT == 2) *p = __builtin_bit_cast(uint16_t, (_Float16)f);
-}
-
 // the job of block (gram, apply) or matrix b; uniform
 enum { BY_GRAM, BY_APPLY, BY_MATRIX };
 template <int BY>
@@ -96,34 +88,18 @@ SMEL_DEV int find_job(const Jobs& js, int b) {
 
 typedef u32x4_t __attribute__((aligned(2))) u32x4_a2;
 typedef f32x4_t __attribute__((aligned(4))) f32x4_a4;
-// N (4 or 8) consecutive elements, `left` of them in range: 8- or 16-byte stores at any alignment
 typedef uint32_t __attribute__((ext_vector_type(2), aligned(2))) u32x2_a2;
-template <int DT, int N>
-SMEL_DEV void st_run(typename Elem<DT>::T* p, int left, const double* v) {
+// N (4 or 8) consecutive floats, `left` of them in range: 16-byte stores at any alignment
+template <int N>
+SMEL_DEV void st_run(float* p, int left, const double* v) {
   if (left >= N) {
-    if constexpr (DT == 1) {
 #pragma unroll
-      for (int k = 0; k < N; k += 4) *(f32x4_a4*)(p + k) = f32x4_t{(float)v[k], (float)v[k + 1], (float)v[k + 2], (float)v[k + 3]};
-    } else {
-      uint32_t w[N / 2];
-#pragma unroll
-      for (int k = 0; k < N / 2; ++k) {
-        if constexpr (DT == 0)
-          w[k] = pack2bf((float)v[2 * k], (float)v[2 * k + 1]);
-        else
-          w[k] = __builtin_bit_cast(uint16_t, (_Float16)(float)v[2 * k]) |
-                 (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(float)v[2 * k + 1]) << 16;
-      }
-      if constexpr (N == 8)
-        *(u32x4_a2*)p = u32x4_t{w[0], w[1], w[2], w[3]};
-      else
-        *(u32x2_a2*)p = u32x2_a2{w[0], w[1]};
-    }
+    for (int k = 0; k < N; k += 4) *(f32x4_a4*)(p + k) = f32x4_t{(float)v[k], (float)v[k + 1], (float)v[k + 2], (float)v[k + 3]};
     return;
   }
 #pragma unroll
   for (int k = 0; k < N; ++k)
-    if (k < left) st_elem<DT>(p + k, v[k]);
+    if (k < left) p[k] = (float)v[k];
 }
 
 template <int DT>
@@ -213,7 +189,6 @@ struct Slice {
 // columns of an apply block's slice at most: two blocks on a CU
 constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt <= 4 ? 256 : 128; }
 constexpr int max_slice16(int nt) { return nt == 1 ? 1024 : nt == 2 ? 512 : nt == 4 ? 256 : 128; }   // of 16-bit types
-constexpr int slice_bytes(int nt) { return 16 * nt * (max_slice(nt) + 20) * 4; }
 
 // A gram block takes `per` slices, the next one on its way while one is multiplied (two buffers). Waves of a block: the
 // upper tiles in TG groups, a group's columns dealt to the others. Three tiles a wave at r = 128: nine leave registers for two
@@ -330,8 +305,7 @@ SMEL_DEV int exp_of(double s) { return s > 0x1p64 && s < 0x1p1000 ? ilogb(s) - 6
 
 constexpr int TP = 17;   // doubles between the rows of a tile in LDS
 
-// waves of an iterate block, one to three upper tiles each
-constexpr int it_waves(int nt) { return nt == 4 ? 10 : 3; }
+constexpr int IT_WAVES = 10;   // of an iterate block: an upper tile each (r <= 64)
 
 // element (16 u + 4 m + l / 16, 16 t + l % 16) of a symmetric matrix in upper tiles: at + m * step
 SMEL_DEV int frag_at(int u, int t, int nt, int lo, int hi, int& step) {
@@ -343,101 +317,74 @@ SMEL_DEV int frag_at(int u, int t, int nt, int lo, int hi, int& step) {
   return tile_at(t, u, nt) * (16 * TP) + lo * TP + hi;
 }
 
-template <int NT>
-__global__ __launch_bounds__(64 * it_waves(NT)) void iterate_kernel(Jobs js, Steps st, const double* __restrict__ part,
-                                                                   double* __restrict__ Qout, double* __restrict__ qscale) {
-  constexpr int NTL = ntiles(NT), W = it_waves(NT), TPW = NTL / W;
-  static_assert(TPW * W == NTL, "tiles per wave");
-  __shared__ double buf0[NTL * 16 * TP], buf1[NTL * 16 * TP], trs[NT];
+// The steps of 32 < r <= 64, a block per matrix and a wave per upper tile; three barriers a step
+__global__ __launch_bounds__(64 * IT_WAVES) void iterate_kernel(Jobs js, Steps st, const double* __restrict__ part,
+                                                                double* __restrict__ Qout, double* __restrict__ qscale) {
+  constexpr int NT = 4, NTL = ntiles(NT), SIZE = NTL * 16 * TP;
+  static_assert(NTL == IT_WAVES, "a tile per wave");
+  __shared__ double bA[SIZE], bP[SIZE], bT[SIZE], bQ[SIZE], trs[NT];
   const Job& J = js.j[find_job<BY_MATRIX>(js, blockIdx.x)];
   const int mat = blockIdx.x - J.mat0;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
-  int tt[TPW], uu[TPW];
-  f64x4_t A[TPW], Q[TPW], P[TPW];
-#pragma unroll
-  for (int k = 0; k < TPW; ++k) {
-    tile_of(wave * TPW + k, NT, tt[k], uu[k]);
-    A[k] = f64x4_t{0, 0, 0, 0};
-    const double* p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + ((wave * TPW + k) * 64 + lane) * 4;
+  int t, u;
+  tile_of(wave, NT, t, u);
+  f64x4_t A = {0, 0, 0, 0}, eye;
+  const double* const p = part + (J.part0 + (int64_t)mat * J.parts) * (NTL * 256) + (wave * 64 + lane) * 4;
 #pragma unroll 8
-    for (int s = 0; s < J.parts; ++s) A[k] += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
-    if (tt[k] == uu[k]) {   // the tile's trace: row 4 m + hi, column lo
-      double d = 0;
+  for (int s = 0; s < J.parts; ++s) A += *(const f64x4_t*)(p + (int64_t)s * (NTL * 256));
+  double d = 0;   // the tile's trace: row 4 m + hi, column lo
 #pragma unroll
-      for (int m = 0; m < 4; ++m) d += 4 * m + hi == lo ? A[k][m] : 0.0;
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) d += __shfl_xor(d, o, 64);
-      if (lane == 0) trs[tt[k]] = d;
-    }
+  for (int m = 0; m < 4; ++m) {
+    eye[m] = t == u && 4 * m + hi == lo ? 1.0 : 0.0;
+    d += 4 * m + hi == lo ? A[m] : 0.0;
   }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) d += __shfl_xor(d, o, 64);
+  if (t == u && lane == 0) trs[t] = d;
   __syncthreads();
-  double tr = 0;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) tr += trs[t];
-  const double s = 1.0 / (sqrt(tr) + st.eps);
-#pragma unroll
-  for (int k = 0; k < TPW; ++k)
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      A[k][m] = A[k][m] * s * s;
-      Q[k][m] = tt[k] == uu[k] && 4 * m + hi == lo ? ldexp(s, -exp_of(s)) : 0.0;
-    }
+  const double s = 1.0 / (sqrt(((trs[0] + trs[1]) + trs[2]) + trs[3]) + st.eps);
+  const double sq = ldexp(s, -exp_of(s));
   if (threadIdx.x == 0) qscale[blockIdx.x] = ldexp(1.0, exp_of(s));
-  auto put = [&](double* buf, const f64x4_t* M) {
+  A = A * s * s;
+  f64x4_t Q = eye * sq;
+  auto put = [&](double* buf, f64x4_t M) {
 #pragma unroll
-    for (int k = 0; k < TPW; ++k)
-#pragma unroll
-      for (int m = 0; m < 4; ++m) buf[(wave * TPW + k) * (16 * TP) + (4 * m + hi) * TP + lo] = M[k][m];
+    for (int m = 0; m < 4; ++m) buf[wave * (16 * TP) + (4 * m + hi) * TP + lo] = M[m];
   };
-  auto product = [&](const double* M, const double* N, f64x4_t* out) {
+  auto product = [&](const double* M, const double* N) {
+    f64x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < TPW; ++k) {
-      f64x4_t acc = {0, 0, 0, 0};
+    for (int k = 0; k < NT; ++k) {
+      int sa, sb;
+      const int a = frag_at(k, t, NT, lo, hi, sa), b = frag_at(k, u, NT, lo, hi, sb);
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        int sa, sb;
-        const int a = frag_at(u, tt[k], NT, lo, hi, sa), b = frag_at(u, uu[k], NT, lo, hi, sb);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) acc = mfma64(M[a + m * sa], N[b + m * sb], acc);
-      }
-      out[k] = acc;
+      for (int m = 0; m < 4; ++m) acc = mfma64(M[a + m * sa], N[b + m * sb], acc);
     }
+    return acc;
   };
   for (int it = 0; it < st.steps; ++it) {
-    put(buf0, A);
-    __syncthreads();
-    f64x4_t S[TPW];
-    product(buf0, buf0, S);
-#pragma unroll
-    for (int k = 0; k < TPW; ++k)
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-        P[k][m] = st.b * A[k][m] + st.c * S[k][m] + (tt[k] == uu[k] && 4 * m + hi == lo ? st.a : 0.0);
-    put(buf1, P);
-    __syncthreads();
-    if (it + 1 < st.steps) {
-      product(buf0, buf1, S);   // A P
-      __syncthreads();
-      put(buf0, S);
-      __syncthreads();
-      product(buf0, buf1, A);   // A P P
-    }
-    __syncthreads();
-    put(buf0, Q);
-    __syncthreads();
-    product(buf0, buf1, Q);
-    __syncthreads();
+    const bool last = it + 1 == st.steps;
+    put(bA, A);
+    lds_barrier();
+    const f64x4_t P = st.b * A + st.c * product(bA, bA) + st.a * eye;
+    put(bP, P);
+    put(bQ, Q);
+    lds_barrier();
+    if (!last) put(bT, product(bA, bP));
+    Q = it == 0 ? P * sq : product(bP, bQ);
+    lds_barrier();
+    if (!last) A = product(bT, bP);
   }
-  // Q's tiles, both triangles, in the operand layout: tile (u, t) register m of lane l = Q[16 u + 4 m + hi][16 t + lo]
-  put(buf0, Q);
-  __syncthreads();
+  // Q's tiles, both triangles, in the operand layout: tile (k, t) register m of lane l = Q[16 k + 4 m + hi][16 t + lo]
+  put(bQ, Q);
+  lds_barrier();
   double* const out = Qout + (int64_t)blockIdx.x * (NT * NT * 256);
-  for (int k = wave; k < NT * NT; k += W) {
+  for (int k = wave; k < NT * NT; k += IT_WAVES) {
     int sa;
     const int a = frag_at(k / NT, k % NT, NT, lo, hi, sa);
     f64x4_t q;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) q[m] = buf0[a + m * sa];
+    for (int m = 0; m < 4; ++m) q[m] = bQ[a + m * sa];
     *(f64x4_t*)(out + (k * 64 + lane) * 4) = q;
   }
 }
@@ -547,17 +494,14 @@ SMEL_DEV double steps_small(const Job& J, int mat, const Steps& st, const double
   return ldexp(1.0, ex);
 }
 
-// Q G for a slice. SMALL: the steps run here, from the parts; else Q's tiles are read. A wave owns one tile of rows and every
+// Q G for a slice of fp32. SMALL: the steps run here, from the parts; else Q's tiles are read. A wave owns one tile of rows and every
 // CG-th pair of 16-column blocks. The columns of a pair (or, for a result whose short side is last, the rows of a tile) are
 // dealt to the instruction's rows so that a lane's registers are neighbours in memory.
-template <int NT, int DT, bool SMALL>
+template <int NT, bool SMALL>
 __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st, const double* __restrict__ in,
                                                         const double* __restrict__ qscale) {
-  static_assert(DT == 1, "16-bit types: apply16_kernel");
-  __shared__ __attribute__((aligned(16))) char smem[slice_bytes(NT)];
-  typedef typename Elem<DT>::T T;
   constexpr int CG = WAVES / NT;
-  float* const X = (float*)smem;
+  __shared__ __attribute__((aligned(16))) float X[16 * NT * (max_slice(NT) + 20)];
   const int slice = 1 << js.lg, pitch = slice + 20;
   const Job& J = js.j[find_job<BY_APPLY>(js, blockIdx.x)];
   const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = (lb % J.slices) << js.lg;
@@ -566,7 +510,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
   const int perm = 4 * (lo & 3) + (lo >> 2);   // row 4 m + hi of the result <- index 4 hi + m
   const int qlane = J.y_tall ? hi * 16 + perm : lane;
   {
-    Slice<NT, DT, WAVES, max_slice(NT)> in;
+    Slice<NT, 1, WAVES, max_slice(NT)> in;
     in.fetch(J, mat, j0, js.lg);
     in.put(J.x_tall, js.lg, X, pitch);
   }
@@ -588,7 +532,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
 #pragma unroll
   for (int u = 0; u < NT; ++u) q[u] = q[u] * scale;
   const int nc = min(slice, J.n - j0);
-  T* const y = (T*)J.y + (int64_t)mat * J.r * J.n;
+  float* const y = (float*)J.y + (int64_t)mat * J.r * J.n;
   if (J.y_tall) {
     for (int j = 16 * cg; j < nc; j += 16 * CG) {
       f64x4_t acc = {0, 0, 0, 0};
@@ -597,7 +541,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
 #pragma unroll
         for (int m = 0; m < 4; ++m) acc = mfma64(q[u][m], (double)X[(16 * u + 4 * m + hi) * pitch + j + lo], acc);
       const int i = 16 * t + 4 * hi;   // rows i + m, column j + lo
-      if (j + lo < nc) st_run<DT, 4>(y + (int64_t)(j0 + j + lo) * J.r + i, J.r - i, (const double*)&acc);
+      if (j + lo < nc) st_run<4>(y + (int64_t)(j0 + j + lo) * J.r + i, J.r - i, (const double*)&acc);
     }
   } else {
     for (int j = 32 * cg; j < nc; j += 32 * CG) {
@@ -612,7 +556,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
           acc[1] = mfma64((double)x[4], q[u][m], acc[1]);
         }
       const int i = 16 * t + lo, k = j + 8 * hi;   // row i, columns k to k + 7
-      if (i < J.r) st_run<DT, 8>(y + (int64_t)i * J.n + j0 + k, nc - k, (const double*)acc);
+      if (i < J.r) st_run<8>(y + (int64_t)i * J.n + j0 + k, nc - k, (const double*)acc);
     }
   }
 }
@@ -1056,7 +1000,7 @@ const double* run_big(const Plan& p, const Steps& st, const double* part, double
 
 template <int NT, int DT, bool SMALL>
 void run_apply(const Plan& p, const Steps& st, const double* in, const double* qscale, hipStream_t stream) {
-  if constexpr (DT == 1) apply_kernel<NT, DT, SMALL><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, st, in, qscale);
+  if constexpr (DT == 1) apply_kernel<NT, SMALL><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, st, in, qscale);
   else apply16_kernel<NT, DT, SMALL><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, st, in, qscale);
 }
 template <int NT, int DT>
@@ -1069,7 +1013,7 @@ int run(const Plan& p, const Steps& st, void* ws, hipStream_t stream) {
     run_apply<NT, DT, true>(p, st, part, nullptr, stream);
   } else if constexpr (NT == 4) {
     double* const qscale = rest + p.mats * NT * NT * 256;
-    iterate_kernel<NT><<<(unsigned)p.mats, 64 * it_waves(NT), 0, stream>>>(js, st, part, rest, qscale);
+    iterate_kernel<<<(unsigned)p.mats, 64 * IT_WAVES, 0, stream>>>(js, st, part, rest, qscale);
     run_apply<NT, DT, false>(p, st, rest, qscale, stream);
   } else {
     const double* qscale = nullptr;
