@@ -394,7 +394,10 @@ def _balance_check(logits, topi, mask, offsets):
         raise ValueError(f"balance_loss takes a bool mask [{T}], got {tuple(mask.shape)} {mask.dtype}")
     if offsets is not None and (offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int64, torch.int32)):
         raise ValueError(f"balance_loss takes int64 or int32 offsets [S + 1], got {tuple(offsets.shape)} {offsets.dtype}")
-    L.one_device(logits, topi, mask, offsets)
+    dev = logits.device
+    if not logits.is_cuda or topi.device != dev or mask is not None and mask.device != dev \
+            or offsets is not None and offsets.device != dev:
+        L.one_device(logits, topi, mask, offsets)
 
 
 def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
@@ -412,8 +415,8 @@ def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
     mem = z.new_empty((rows_n + weights_n + ws_n) // z.element_size() + 8)
     rows = mem.data_ptr()
     weights = rows + rows_n
-    loss = torch.empty((), dtype=torch.float32, device=z.device)
-    counts = torch.empty((E,) if off is None else (S, E), dtype=torch.int64, device=z.device)
+    loss = z.new_empty((), dtype=torch.float32)
+    counts = topi.new_empty((E,) if off is None else (S, E), dtype=torch.int64)
     p = L.ptr
     if mask is not None:
         mask = mask.contiguous()
@@ -474,6 +477,6 @@ def balance_loss(logits, topi, mask=None, offsets=None, coef: float = 1.0):
     _balance_check(logits, topi, mask, offsets)
     with L.on_device_of(logits):
         if torch.is_grad_enabled() and logits.requires_grad:
-            return _BalanceFn.apply(logits, topi, mask, offsets, float(coef))
+            return L.apply(_BalanceFn, logits, topi, mask, offsets, float(coef))
         loss, counts, _ = _balance_forward(logits, topi, mask, offsets, float(coef), False)
     return loss, counts

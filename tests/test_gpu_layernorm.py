@@ -313,3 +313,12 @@ def test_layernorm_backward_twice():
     one = torch.autograd.grad(y, (xg, wg, bg), dy.to(DEV), retain_graph=True)
     two = torch.autograd.grad(y, (xg, wg, bg), dy.to(DEV))
     assert all(torch.equal(a, c) for a, c in zip(one, two))
+
+
+def test_layernorm_functional_transforms_refused():
+    """torch.func's transforms have no rule for it and say so; ordinary calls go on after one."""
+    from smel.norm import layernorm
+    x, w = torch.randn(4, 8, device=DEV), torch.ones(8, device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: layernorm(t, w, None, EPS).sum())(x)
+    assert layernorm(x.requires_grad_(True), w, None, EPS).requires_grad
