@@ -327,3 +327,17 @@ def test_route_gemma4_logits_and_their_gradient(dt, H):
     a, p, q = both.double(), only_l.double(), only_v.double()
     scale = p.abs() + q.abs()
     assert p.abs().max() > 0 and ((a - p - q).abs() <= 16 * half * (scale + scale.amax(1, keepdim=True))).all()
+
+
+def test_balance_far_offsets():
+    """Rows whose offsets pass 2^31 elements: the same bits as packed ones."""
+    from smel.loss import balance_loss
+    z, topi = make(1100, 40, 4, "bf16", 9)
+    far = torch.zeros(1100, 1 << 21, dtype=torch.bfloat16, device=DEV)[:, 3:43]
+    far.copy_(z.to(DEV))
+    out = []
+    for t in (z.to(DEV), far):
+        zg = t.detach().requires_grad_(True)
+        loss, counts = balance_loss(zg, topi.to(DEV))
+        out.append((loss.detach(), counts, torch.autograd.grad(loss, zg)[0]))
+    assert all(torch.equal(p, q) for p, q in zip(*out))

@@ -322,3 +322,31 @@ def test_layernorm_functional_transforms_refused():
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: layernorm(t, w, None, EPS).sum())(x)
     assert layernorm(x.requires_grad_(True), w, None, EPS).requires_grad
+
+
+def test_layernorm_far_offsets():
+    """Rows whose offsets pass 2^31 elements: far apart in a view, and packed (two million rows): the same bits as alone."""
+    from smel.norm import layernorm
+    g = torch.Generator(device=DEV).manual_seed(1)
+    w, b = torch.randn(96, generator=g, device=DEV), torch.randn(96, generator=g, device=DEV)
+    far = torch.zeros(1100, 1 << 21, dtype=torch.bfloat16, device=DEV)[:, 5:101]
+    near = torch.randn(1100, 96, generator=g, device=DEV).bfloat16()
+    far.copy_(near)
+    dy = torch.randn(1100, 96, generator=g, device=DEV).bfloat16()
+
+    def grads(x, dy):
+        ts = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = layernorm(ts[0], ts[1], ts[2], EPS)
+        return [y.detach(), *torch.autograd.grad(y, ts, dy)]
+    assert all(torch.equal(p, q) for p, q in zip(grads(near, dy), grads(far, dy)))
+    del far
+    n, rows = 1024, (1 << 21) + 77
+    x = torch.zeros(rows, n, dtype=torch.float16, device=DEV)
+    some = torch.randn(100, n, generator=g, device=DEV).half()
+    x[:100] = x[-100:] = some       # the same rows before and behind 2^31 elements, of one call
+    xg = x.requires_grad_(True)
+    y = layernorm(xg, None, None, EPS)
+    dx, = torch.autograd.grad(y, xg, y.detach())
+    assert torch.equal(y[:100], y[-100:]) and torch.equal(dx[:100], dx[-100:])
+    assert not y[100:103].any() and not y[-101].any() and not dx[-101].any()
+    close(y[-100:], formula(some.cpu(), None, None, torch.zeros_like(some).cpu())["y"], "y")

@@ -185,3 +185,30 @@ def test_orthogonalize_refusals():
                 lambda: orthogonalize([x, x.long()])):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_orthogonalize_far_offsets():
+    """Matrices, rows and columns whose offsets pass 2^31 elements: the same bits as packed ones."""
+    from smel.lora import orthogonalize
+    big = torch.zeros(1100 << 21, dtype=torch.bfloat16, device=DEV)
+    G = make((3, 16, 700), "bf16", 4).to(DEV)
+    far = big.as_strided((3, 16, 700), (1 << 30, 1 << 21, 1))
+    far.copy_(G)
+    assert torch.equal(orthogonalize(far), orthogonalize(G))
+    H = make((16, 1000), "bf16", 5).to(DEV)
+    lines = big.as_strided((16, 1000), (1, 1 << 21))
+    lines.copy_(H)
+    assert torch.equal(orthogonalize(lines), orthogonalize(H))
+
+
+def test_orthogonalize_many_matrices():
+    """More matrices than a launch takes above rank 64, and many small ones: each as alone."""
+    from smel.lora import orthogonalize
+    G = make((300, 72, 80), "fp32", 6).to(DEV)
+    y = orthogonalize(G)
+    for k in (0, 255, 256, 299):
+        assert torch.equal(y[k], orthogonalize(G[k]))
+    close(y[[0, 255, 256, 299]], G[[0, 255, 256, 299]], "ends")
+    S = make((70000, 2, 5), "fp32", 7).to(DEV)
+    y = orthogonalize(S)
+    close(y[[0, 65535, 65536, 69999]], S[[0, 65535, 65536, 69999]], "ends")
