@@ -21,6 +21,8 @@ Structure here:
     up to 4096 rows (256 MB of bf16 terms at vocab_chunk 32768), where the GEMMs' row tiles fill the GPU. The rows are
     independent, so the results are those of the reference's chunking either way.
 The gradient is computed in the forward (lm_head is frozen) and handed back by the backward, as in the reference.
+
+``balance_loss``, at the end, is the router's: its loss and the picks per expert, with the gradient of the logits.
 """
 from __future__ import annotations
 
