@@ -249,12 +249,16 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
   __shared__ float join[WG && BS == 256 ? BS / 2 * CPL * 16 : 1];   // larger blocks are one row's
   const int lpr = p.lpr, n = p.cols, nch = (n + 7) >> 3;
   const int groups = BS / lpr, grp = threadIdx.x / lpr, li = threadIdx.x & (lpr - 1);
+  // the weights stay in registers, but for two chunks of fp32 (1024 threads leave 128 registers: they would spill)
+  constexpr bool HOLD = !(CPL == 2 && DT == 2);
   float w[CPL][8], dw[WG ? CPL * 8 : 1], db[WG ? CPL * 8 : 1];
-#pragma unroll
-  for (int k = 0; k < CPL; ++k) {
+  auto weights = [&](int k) {
     const int ck = li + lpr * k;
     weight8<WT>(ck < nch ? p.w : nullptr, 8 * ck, n, 1.f, w[k]);
-  }
+  };
+  if constexpr (HOLD)
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) weights(k);
   if constexpr (WG)
 #pragma unroll
     for (int i = 0; i < CPL * 8; ++i) dw[i] = db[i] = 0.f;
@@ -283,7 +287,8 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
     const bool live = row < p.rows;
     float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < CPL; ++k)
+    for (int k = 0; k < CPL; ++k) {
+      if constexpr (!HOLD) weights(k);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {   // d is zero past the row and past the last row
         const float d = b.d[k].at(j), xhat = (b.x[k].at(j) - b.mean) * b.rstd;
@@ -295,6 +300,7 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
           db[k * 8 + j] += d;
         }
       }
+    }
     row_sums(sums, lpr, rd);
     if (!live || !p.dx) return;
     const int64_t out = row * (int64_t)n;
@@ -303,6 +309,7 @@ __global__ __launch_bounds__(BS) void ln_bwd_kernel(LnArgs p) {
     for (int k = 0; k < CPL; ++k) {
       const int ck = li + lpr * k;
       if (ck >= nch) continue;
+      if constexpr (!HOLD) weights(k);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
