@@ -414,7 +414,7 @@ def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
     rows_n = 16 * T if need_grad else 0
     weights_n = (4 * (S * E + 1) + 15) & ~15
     ws_n = L.load().smel_balance_ws_bytes(T, E, S)
-    mem = z.new_empty((rows_n + weights_n + ws_n) // z.element_size() + 8)
+    mem = z.new_empty(rows_n + weights_n + ws_n, dtype=torch.uint8)
     rows = mem.data_ptr()
     weights = rows + rows_n
     loss = z.new_empty((), dtype=torch.float32)

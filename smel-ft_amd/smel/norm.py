@@ -218,11 +218,6 @@ def _rows_of(x, n: int):
     return rows, rows.shape[0], pitch
 
 
-def _stats_like(x, rows: int):
-    """8 bytes a row (its mean and rstd), in a tensor of x's type: the cheapest allocation on x's device."""
-    return x.new_empty(rows * (8 // x.element_size()))
-
-
 def _ln_forward(x, h, w, b, eps, n, dt, wt):
     """(rows the norm read, their count, s or None, y, stats)."""
     if h is None:
@@ -234,7 +229,7 @@ def _ln_forward(x, h, w, b, eps, n, dt, wt):
         s = torch.empty_like(x2)
         sp = s.data_ptr()
     y = torch.empty_like(x2) if x2.is_contiguous() and x2.shape == x.shape else x.new_empty(x.shape)
-    stats = _stats_like(x, R)
+    stats = x.new_empty(2 * R, dtype=torch.float32)     # a row's mean and rstd
     p = _lib.ptr
     _lib.call("smel_layernorm_fwd", x2.data_ptr(), p(h2), R, n, pitch, p(w), p(b), eps, dt, wt, sp, y.data_ptr(),
               stats.data_ptr(), _lib.stream())
@@ -260,7 +255,7 @@ def _ln_backward(ctx, *grads):
     ws, ws_n = None, 0
     if nw or nb:
         ws_n = _lib.load().smel_layernorm_bwd_ws_floats(R, n)
-        ws = rows.new_empty(ws_n * (4 // rows.element_size()))
+        ws = rows.new_empty(ws_n, dtype=torch.float32)
     _lib.call("smel_layernorm_bwd", dy2.data_ptr(), rows.data_ptr(), R, n, pitch, p(w), stats.data_ptr(), p(ds2), dt, wt,
               p(dx), p(dw), p(db), p(ws), ws_n, _lib.stream())
     return dx, dx if add else None, dw, db, None, None
