@@ -85,36 +85,66 @@ SMEL_DEV void st_run(typename El<DT>::T* row, int e0, int E, const float (&v)[N]
     if (e0 + i < E) row[e0 + i] = o[i];
 }
 
-// e^x (x <= 0 or NaN) on v_exp_f32: x log2(e) in two parts, so that the product's rounding does not grow with |x|; an expert
-// at -inf gives 0
+// e^x (x <= 0, -inf or NaN) on v_exp_f32: 2^h for h = x log2(e) as rounded, times e^d = 1 + d for what is left, d = x - h ln(2)
+// with ln(2) in two parts, so that h's rounding does not grow with |x|. At -inf, or where h overflows to it, d is anything
+// finite and the result 0.
 SMEL_DEV float exp_acc(float x) {
-  x = x < -200.f ? -200.f : x;
-  const float hi = x * 1.4426950408889634f;
-  const float lo = fmaf(x, 1.4426950408889634f, -hi) + x * 1.9259629911266175e-8f;
-  return __builtin_amdgcn_exp2f(hi) * fmaf(lo, 0.6931471805599453f, 1.f);
+  const float h = x * 1.4426950408889634f, e = __builtin_amdgcn_exp2f(h);
+  const float d = fmaf(-h, -1.9046543e-9f, fmaf(-h, 0.693147182464599609375f, x));
+  return fmaf(e, __builtin_amdgcn_fmed3f(d, -1.f, 1.f), e);
+}
+// 1 / x to its last bits (v_rcp_f32 and one Newton step; x: a row's sum of exponentials, 1 to 512 or NaN)
+SMEL_DEV float inverse(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, r, 1.f), r, r);
 }
 
-// Sum and maximum over the wave by DPP moves (six of about 8 cycles, where a shuffle through the LDS unit is about 64): rows of
-// 16 lanes, then across them; lane 63 holds the result. Lanes without a source add 0, or meet themselves.
-#define BAL_DPP(v, old, ctrl, rows) \
-  __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), ctrl, rows, 0xf, false))
-SMEL_DEV float sum64(float v) {
-  v += BAL_DPP(v, 0.f, 0x111, 0xf);   // row_shr:1, 2, 4, 8
-  v += BAL_DPP(v, 0.f, 0x112, 0xf);
-  v += BAL_DPP(v, 0.f, 0x114, 0xf);
-  v += BAL_DPP(v, 0.f, 0x118, 0xf);
-  v += BAL_DPP(v, 0.f, 0x142, 0xa);   // row_bcast:15 into rows 1 and 3
-  v += BAL_DPP(v, 0.f, 0x143, 0xc);   // row_bcast:31 into rows 2 and 3
-  return lane_get(v, 63);
+// Sums (or maxima) over the wave of B values at once, uniform. v_permlane32_swap hands two values' halves to each other, so that one
+// operation adds both (lanes 0-31: the first's, 32-63: the second's); v_permlane16_swap the same for rows of 16; then four
+// rotations within the rows. Four values take 10 operations, not the 24 of one after the other: a short row's share of the
+// forward is its instructions (4092 x 256 bf16 in nine sequences: 13 -> 11.3 us; 32768 fp32 rows: 13.4 -> 11.5).
+struct Sum {
+  SMEL_DEV static float of(float a, float b) { return a + b; }
+};
+struct Max {
+  SMEL_DEV static float of(float a, float b) { return fmaxf(a, b); }
+};
+template <class Op>
+SMEL_DEV float swap32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return Op::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-SMEL_DEV float max64(float v) {
-  v = fmaxf(v, BAL_DPP(v, v, 0x111, 0xf));
-  v = fmaxf(v, BAL_DPP(v, v, 0x112, 0xf));
-  v = fmaxf(v, BAL_DPP(v, v, 0x114, 0xf));
-  v = fmaxf(v, BAL_DPP(v, v, 0x118, 0xf));
-  v = fmaxf(v, BAL_DPP(v, v, 0x142, 0xa));
-  v = fmaxf(v, BAL_DPP(v, v, 0x143, 0xc));
-  return lane_get(v, 63);
+template <class Op>
+SMEL_DEV float swap16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return Op::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <class Op>
+SMEL_DEV float rotate16(float v) {   // over a row of 16, in every lane
+#define BAL_ROR(n) \
+  v = Op::of(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + n, 0xf, 0xf, true)))
+  BAL_ROR(8);
+  BAL_ROR(4);
+  BAL_ROR(2);
+  BAL_ROR(1);
+#undef BAL_ROR
+  return v;
+}
+template <class Op, int B>
+SMEL_DEV void over_wave(float (&v)[B]) {
+  static_assert(B == 2 || B == 4, "values at once");
+  if constexpr (B == 4) {   // rows of 16: values 0, 2, 1, 3
+    const float w = rotate16<Op>(swap16<Op>(swap32<Op>(v[0], v[1]), swap32<Op>(v[2], v[3])));
+    v[0] = lane_get(w, 0);
+    v[2] = lane_get(w, 16);
+    v[1] = lane_get(w, 32);
+    v[3] = lane_get(w, 48);
+  } else {
+    float w = swap32<Op>(v[0], v[1]);
+    w = rotate16<Op>(swap16<Op>(w, w));
+    v[0] = lane_get(w, 0);
+    v[1] = lane_get(w, 32);
+  }
 }
 
 struct Seqs {
@@ -234,27 +264,44 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
       float z[B][NE];
       bool keep[B];
 #pragma unroll
-      for (int k = 0; k < B; ++k) {   // a row that does not count may be read; nothing of it is used
+      for (int k = 0; k < B; ++k) {   // past the end: the last row again, with no share
         const int64_t t = min(t0 + k, e - 1);
-        keep[k] = t0 + k < e && !(a.mask && !a.mask[t]);
+        keep[k] = t0 + k < e;
         ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, -INFINITY, z[k]);
       }
+      if (a.mask)
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          const bool counts = a.mask[min(t0 + k, e - 1)];
+          keep[k] = keep[k] && counts;
+#pragma unroll
+          for (int i = 0; i < NE; ++i) z[k][i] = counts ? z[k][i] : 0.f;   // whatever it holds
+        }
+      float m[B], sum[B];
 #pragma unroll
       for (int k = 0; k < B; ++k) {
-        float m = z[k][0], sum = 0.f;
+        m[k] = z[k][0];
 #pragma unroll
-        for (int i = 1; i < NE; ++i) m = fmaxf(m, z[k][i]);
-        m = max64(m);
+        for (int i = 1; i < NE; ++i) m[k] = fmaxf(m[k], z[k][i]);
+      }
+      over_wave<Max>(m);
 #pragma unroll
-        for (int i = 0; i < NE; ++i) {
-          z[k][i] = e0 + i < a.E ? exp_acc(z[k][i] - m) : 0.f;
-          sum += z[k][i];
+      for (int k = 0; k < B; ++k) {
+        sum[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {   // experts past E are at -inf
+          z[k][i] = exp_acc(z[k][i] - m[k]);
+          sum[k] += z[k][i];
         }
-        const float r = 1.f / sum64(sum);
+      }
+      over_wave<Sum>(sum);
 #pragma unroll
-        for (int i = 0; i < NE; ++i) acc[i] = keep[k] ? fmaf(z[k][i], r, acc[i]) : acc[i];
+      for (int k = 0; k < B; ++k) {
+        const float r = inverse(sum[k]), share = keep[k] ? r : 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) acc[i] = fmaf(z[k][i], share, acc[i]);
         n += keep[k];
-        if (a.rows && lane == 0 && t0 + k < e) a.rows[t0 + k] = Row{m, r, keep[k] ? s : -1, 0};
+        if (a.rows && lane == 0 && t0 + k < e) a.rows[t0 + k] = Row{m[k], r, keep[k] ? s : -1, 0};
       }
     }
     while (i0 < e * a.K) {
@@ -381,7 +428,7 @@ __global__ __launch_bounds__(256) void bal_bwd_kernel(BalArgs a, const float* __
   for (int k = 0; k < B; ++k) {
     const int64_t t = min(t0 + k, a.T - 1);
     row[k] = a.rows[t];
-    ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, 0.f, z[k]);
+    ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, -INFINITY, z[k]);
   }
   if (a.q.S == 1) {
     ld_run<1, NE>(a.weights, e0, a.E, 0.f, v[0]);
@@ -393,18 +440,23 @@ __global__ __launch_bounds__(256) void bal_bwd_kernel(BalArgs a, const float* __
 #pragma unroll
     for (int k = 0; k < B; ++k) ld_run<1, NE>(a.weights + (int64_t)max(row[k].seq, 0) * a.E, e0, a.E, 0.f, v[k]);
   }
+  float dot[B];
+#pragma unroll
+  for (int k = 0; k < B; ++k) {
+    dot[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {   // past E: p = 0
+      z[k][i] = exp_acc(z[k][i] - row[k].m) * row[k].r;
+      dot[k] = fmaf(z[k][i], v[k][i], dot[k]);
+    }
+  }
+  over_wave<Sum>(dot);
 #pragma unroll
   for (int k = 0; k < B; ++k) {
     if (t0 + k >= a.T) break;
-    float p[NE], d[NE], dot = 0.f;
+    float d[NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      p[i] = exp_acc(z[k][i] - row[k].m) * row[k].r;
-      dot = e0 + i < a.E ? fmaf(p[i], v[k][i], dot) : dot;
-    }
-    dot = sum64(dot);
-#pragma unroll
-    for (int i = 0; i < NE; ++i) d[i] = row[k].seq >= 0 ? g * (p[i] * (v[k][i] - dot)) : 0.f;
+    for (int i = 0; i < NE; ++i) d[i] = row[k].seq >= 0 ? g * (z[k][i] * (v[k][i] - dot[k])) : 0.f;
     st_run<DT, NE>((T*)dz + (t0 + k) * a.E, e0, a.E, d);
   }
 }
