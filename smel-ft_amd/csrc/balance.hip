@@ -4,15 +4,16 @@
 // v only enters through differences, so its mean is taken out first: c_e - (sum c) / E is formed from whole numbers, and a
 // balanced router's gradient is zero instead of the rounding of two equal terms.
 //
-// Forward: a block of 16 waves takes a chunk of tokens and walks through the sequences in it; per sequence, each wave takes four
-// tokens at a time (their loads together: a chunk is short, so a row's latency counts), its lanes sum the softmax of NE
-// neighbouring experts each in registers, the picks are counted by integer adds in LDS, and the block writes both to slot
+// Forward: a block of 4 to 16 waves takes a chunk of tokens and walks through the sequences in it; per sequence, each wave takes
+// two to eight tokens at a time (their loads together: a chunk is short, so a row's latency counts), its lanes sum the softmax of
+// NE neighbouring experts each in registers, the picks are counted by integer adds in LDS, and the block writes both to slot
 // (chunk + sequence) of the workspace: along the tokens either number grows at every step, so slots are distinct and a
-// sequence's are consecutive. A second kernel (a block per sequence) adds a sequence's slots, a fixed set of them per thread in
-// order; a third joins the sequences' losses where there are several. A short batch of one sequence is one block's, and one
-// launch. Sums have a fixed order, integer adds have none that shows: results repeat bit for bit. The forward leaves with every
-// token what the backward needs to take it up again (maximum, 1 / sum, sequence or none): one pass, four rows a wave.
+// sequence's are consecutive. A second kernel adds a sequence's slots, a fixed set of them per thread in order; a third joins
+// the losses where there are several. A short batch of one sequence is one block's, and one launch. Sums have a fixed order,
+// integer adds have none that shows: results repeat bit for bit. The forward leaves with every token what the backward needs to
+// take it up again (maximum, 1 / sum, sequence or none): one pass over the rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/smel_loss.h"
 #include "abi_util.h"
@@ -130,10 +131,22 @@ SMEL_DEV float rotate16(float v) {   // over a row of 16, in every lane
 #undef BAL_ROR
   return v;
 }
-template <class Op, int B>
-SMEL_DEV void over_wave(float (&v)[B]) {
-  static_assert(B == 2 || B == 4, "values at once");
-  if constexpr (B == 4) {   // rows of 16: values 0, 2, 1, 3
+// over L lanes (16, 32 or 64), in each of them
+template <class Op, int L, int B>
+SMEL_DEV void over_lanes(float (&v)[B]) {
+  static_assert(L == 16 || B % 2 == 0, "values at once");
+  if constexpr (L == 16) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) v[k] = rotate16<Op>(v[k]);
+  } else if constexpr (L == 32) {
+#pragma unroll
+    for (int k = 0; k < B; k += 2) {   // rows of 16: v[k], v[k + 1], v[k], v[k + 1]
+      const uint32_t w = __float_as_uint(rotate16<Op>(swap16<Op>(v[k], v[k + 1])));
+      const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+      v[k] = __uint_as_float(r[0]);
+      v[k + 1] = __uint_as_float(r[1]);
+    }
+  } else if constexpr (B == 4) {   // rows of 16: values 0, 2, 1, 3
     const float w = rotate16<Op>(swap16<Op>(swap32<Op>(v[0], v[1]), swap32<Op>(v[2], v[3])));
     v[0] = lane_get(w, 0);
     v[2] = lane_get(w, 16);
@@ -146,6 +159,12 @@ SMEL_DEV void over_wave(float (&v)[B]) {
     v[1] = lane_get(w, 32);
   }
 }
+
+// A token's experts lie in L lanes, NE to each; a wave takes B runs of 64 / L tokens at a time.
+template <int NE_, int L_, int B_>
+struct Shape {
+  static constexpr int NE = NE_, L = L_, B = B_, RUN = 64 / L, TOKENS = RUN * B;
+};
 
 struct Seqs {
   const void* off;   // null: one sequence of all tokens
@@ -174,6 +193,10 @@ struct Row {      // what the backward takes a token up with
   int seq, pad;   // its sequence, -1 where it does not count
 };
 
+struct Num {      // of a slot
+  int32_t tokens, picks;   // that count (K T < 2^31)
+};
+
 struct BalArgs {
   const void* z;
   int64_t ldl, T;
@@ -186,52 +209,45 @@ struct BalArgs {
   Row* rows;       // null: no backward
   float* P;        // [slots][E]
   int32_t* C;      // [slots][E]
-  int32_t* N;      // [slots] counted tokens
+  Num* N;          // [slots]
   float* loss;
   int64_t* counts;
   float* weights;
-  float* seq_loss; // [S]
+  int parts;       // blocks of a sequence's sums
+  float* seq_loss; // [S][parts]
   int32_t* seq_n;  // [S]
 };
 
-template <int NE>
-constexpr int TB = NE == 8 ? 2 : 4;   // tokens of a wave at a time
-
-// A sequence's counts, weights and loss from expert x's picks c and sum P of the softmax, x < E in thread x; the sums over
-// the experts go through red and tot (a slot a wave). All threads of the block call it; the result is thread 0's.
-SMEL_DEV float finish_seq(const BalArgs& a, int s, int x, int64_t c, int64_t n, float P, float* red, long long* tot) {
-  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
-  const bool mine = x < a.E;
-  if (mine) a.counts[(int64_t)s * a.E + x] = c;
-  long long ct = mine ? c : 0;   // picks in range, over all experts
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) ct += __shfl_xor(ct, o, 64);
-  if ((threadIdx.x & 63) == 0) tot[wave] = ct;
-  __syncthreads();
-  ct = 0;
-  for (int k = 0; k < waves; ++k) ct += tot[k];
+// A sequence's counts and weights of expert x from its picks c and sum P of the softmax, x < E, and the share in the loss of
+// the block's experts; `in` counts the sequence's. All threads of the block call it (others with x >= E); the result, of red's
+// slot a wave, is thread 0's.
+SMEL_DEV float finish_seq(const BalArgs& a, int s, int x, int64_t c, Num in, float P, float* red) {
+  const int waves = blockDim.x >> 6;
+  const int64_t n = in.tokens;
   float l = 0.f;
-  if (mine) {
+  if (x < a.E) {
     const double scale = n > 0 ? (double)a.coef / ((double)a.K * (double)n * (double)n) : 0.0;
-    a.weights[(int64_t)s * a.E + x] = (float)((double)(c * a.E - ct) * scale);
+    a.counts[(int64_t)s * a.E + x] = c;
+    a.weights[(int64_t)s * a.E + x] = (float)((double)(c * a.E - in.picks) * scale);
     l = n > 0 ? (float)((double)(c * a.E) * scale) * P : 0.f;
   }
   l = wave_sum(l);
-  if ((threadIdx.x & 63) == 0) red[wave] = l;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = l;
   __syncthreads();
   for (int k = 1; k < waves; ++k) l = k == 1 ? red[0] + red[1] : l + red[k];
   return l;
 }
 
 // W waves. ONE: all tokens are this block's and one sequence: no slots, the loss at once
-template <int DT, int NE, int W, bool ONE>
+template <int DT, class SH, int W, bool ONE>
 __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
   typedef typename El<DT>::T T;
-  __shared__ float sp[W][64 * NE];
-  __shared__ int sc[MAX_E], sn;
+  constexpr int NE = SH::NE, L = SH::L, B = SH::B, RUN = SH::RUN;
+  __shared__ float sp[W][L * NE];
+  __shared__ int sc[MAX_E];
+  __shared__ Num sn;
   __shared__ float red[W];
-  __shared__ long long tot[W];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e0 = lane * NE;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sub = lane / L, e0 = lane % L * NE;
   const int64_t c0 = (int64_t)blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, a.T);
   if (a.rows && a.q.off) {   // tokens of no sequence
     for (int64_t t = c0 + threadIdx.x; t < c1; t += 64 * W) a.rows[t].seq = -1;
@@ -247,7 +263,7 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
       if (b >= e) continue;
     }
     for (int i = threadIdx.x; i < a.E; i += 64 * W) sc[i] = 0;
-    if (threadIdx.x == 0) sn = 0;
+    if (threadIdx.x == 0) sn = Num{0, 0};
     __syncthreads();
     auto pick = [&](int64_t i) -> int64_t {   // pick i of the block's, -1 where it counts nowhere
       if (i >= e * a.K || (a.mask && !a.mask[(uint32_t)i / (uint32_t)a.K])) return -1;   // T K < 2^31
@@ -259,20 +275,19 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < NE; ++i) acc[i] = 0.f;
-    constexpr int B = TB<NE>;
-    for (int64_t t0 = b + wave * B; t0 < e; t0 += W * B) {
+    for (int64_t t0 = b + wave * SH::TOKENS + sub; t0 < e + sub; t0 += W * SH::TOKENS) {   // uniform
       float z[B][NE];
       bool keep[B];
 #pragma unroll
       for (int k = 0; k < B; ++k) {   // past the end: the last row again, with no share
-        const int64_t t = min(t0 + k, e - 1);
-        keep[k] = t0 + k < e;
+        const int64_t t = min(t0 + k * RUN, e - 1);
+        keep[k] = t0 + k * RUN < e;
         ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, -INFINITY, z[k]);
       }
       if (a.mask)
 #pragma unroll
         for (int k = 0; k < B; ++k) {
-          const bool counts = a.mask[min(t0 + k, e - 1)];
+          const bool counts = a.mask[min(t0 + k * RUN, e - 1)];
           keep[k] = keep[k] && counts;
 #pragma unroll
           for (int i = 0; i < NE; ++i) z[k][i] = counts ? z[k][i] : 0.f;   // whatever it holds
@@ -284,7 +299,7 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
 #pragma unroll
         for (int i = 1; i < NE; ++i) m[k] = fmaxf(m[k], z[k][i]);
       }
-      over_wave<Max>(m);
+      over_lanes<Max, L>(m);
 #pragma unroll
       for (int k = 0; k < B; ++k) {
         sum[k] = 0.f;
@@ -294,24 +309,32 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
           sum[k] += z[k][i];
         }
       }
-      over_wave<Sum>(sum);
+      over_lanes<Sum, L>(sum);
 #pragma unroll
       for (int k = 0; k < B; ++k) {
         const float r = inverse(sum[k]), share = keep[k] ? r : 0.f;
 #pragma unroll
         for (int i = 0; i < NE; ++i) acc[i] = fmaf(z[k][i], share, acc[i]);
         n += keep[k];
-        if (a.rows && lane == 0 && t0 + k < e) a.rows[t0 + k] = Row{m[k], r, keep[k] ? s : -1, 0};
+        if (a.rows && e0 == 0 && t0 + k * RUN < e) a.rows[t0 + k * RUN] = Row{m[k], r, keep[k] ? s : -1, 0};
       }
     }
+    int picks = 0;   // the wave's, in its first lane, which leaves the loop last
     while (i0 < e * a.K) {
-      if (id >= 0 && id < a.E) atomicAdd(&sc[id], 1);
+      const bool in = id >= 0 && id < a.E;
+      if (in) atomicAdd(&sc[id], 1);
+      picks += __popcll(__ballot(in));
       i0 += 64 * W;
       id = pick(i0);
     }
-    if (lane == 0) atomicAdd(&sn, n);
+    if (e0 == 0) atomicAdd(&sn.tokens, n);
+    if (lane == 0) atomicAdd(&sn.picks, picks);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) sp[wave][e0 + i] = acc[i];
+    for (int i = 0; i < NE; ++i) {   // the wave's runs joined
+      if constexpr (L <= 32) acc[i] = swap32<Sum>(acc[i], acc[i]);
+      if constexpr (L <= 16) acc[i] = swap16<Sum>(acc[i], acc[i]);
+      if (sub == 0) sp[wave][e0 + i] = acc[i];
+    }
     __syncthreads();
     auto share = [&](int x) {
       float P = sp[0][x];
@@ -321,7 +344,7 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
     };
     if constexpr (ONE) {
       const int x = threadIdx.x;
-      const float l = finish_seq(a, 0, x, x < a.E ? sc[x] : 0, sn, x < a.E ? share(x) : 0.f, red, tot);
+      const float l = finish_seq(a, 0, x, x < a.E ? sc[x] : 0, sn, x < a.E ? share(x) : 0.f, red);
       if (x == 0) {
         *a.loss = l;
         a.weights[a.E] = 1.f;
@@ -338,31 +361,49 @@ __global__ __launch_bounds__(64 * W) void bal_fwd_kernel(BalArgs a) {
   }
 }
 
-// One sequence: its slots' sums, counts, weights and loss. Threads: columns of `1 << lgc` experts, the groups take every
+// A sequence's `1 << lgc` experts: its slots' sums, counts, weights and loss. The block's groups of as many threads take every
 // group-th slot each.
 template <int BS>
 __global__ __launch_bounds__(BS) void bal_seq_kernel(BalArgs a, int lgc) {
   __shared__ float sp[BS], red[BS / 64];
   __shared__ int sc[BS];
-  __shared__ long long tot[BS / 64];
-  __shared__ int sn;
-  const int s = blockIdx.x;
+  __shared__ Num sn;
+  const int s = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int64_t b = a.q.at(s), e = a.q.at(s + 1);
-  const int cols = 1 << lgc, groups = BS >> lgc, x = threadIdx.x & (cols - 1), g = threadIdx.x >> lgc;
+  const int cols = 1 << lgc, groups = BS >> lgc, col = threadIdx.x & (cols - 1), g = threadIdx.x >> lgc, x = (part << lgc) + col;
   const int64_t k0 = b / a.chunk + s, k1 = b < e ? (e - 1) / a.chunk + s : k0 - 1;
   float P = 0.f;
-  int c = 0;   // K T < 2^31
+  int c = 0;
+  constexpr int U = 8;   // slots at a time: each is a round trip to memory
   if (x < a.E)
-#pragma unroll 8
-    for (int64_t k = k0 + g; k <= k1; k += groups) {
-      P += a.P[k * a.E + x];
-      c += a.C[k * a.E + x];
+    for (int64_t k = k0 + g; k <= k1; k += U * groups) {
+      float p[U];
+      int q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = min(k + u * groups, k1) * a.E + x;
+        p[u] = a.P[i];
+        q[u] = a.C[i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = k + u * groups <= k1;
+        P += in ? p[u] : 0.f;
+        c += in ? q[u] : 0;
+      }
     }
   if (threadIdx.x < 64) {
-    int n = 0;
-    for (int64_t k = k0 + threadIdx.x; k <= k1; k += 64) n += a.N[k];
+    Num n{0, 0};
+    for (int64_t k = k0 + threadIdx.x; k <= k1; k += 64) {
+      const Num v = a.N[k];
+      n.tokens += v.tokens;
+      n.picks += v.picks;
+    }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
+    for (int o = 32; o >= 1; o >>= 1) {
+      n.tokens += __shfl_xor(n.tokens, o, 64);
+      n.picks += __shfl_xor(n.picks, o, 64);
+    }
     if (threadIdx.x == 0) sn = n;
   }
   sp[threadIdx.x] = P;
@@ -370,18 +411,17 @@ __global__ __launch_bounds__(BS) void bal_seq_kernel(BalArgs a, int lgc) {
   __syncthreads();
   if (g == 0)
     for (int k = 1; k < groups; ++k) {
-      P += sp[(k << lgc) + x];
-      c += sc[(k << lgc) + x];
+      P += sp[(k << lgc) + col];
+      c += sc[(k << lgc) + col];
     }
-  const int mine = g == 0 ? x : MAX_E;
-  const float l = finish_seq(a, s, mine, c, sn, P, red, tot);
+  const float l = finish_seq(a, s, g == 0 ? x : MAX_E, c, sn, P, red);
   if (threadIdx.x == 0) {
-    if (a.q.S == 1) {
+    if (a.q.S * a.parts == 1) {
       *a.loss = l;
       a.weights[a.E] = 1.f;
     } else {
-      a.seq_loss[s] = l;
-      a.seq_n[s] = sn > 0;
+      a.seq_loss[blockIdx.x] = l;
+      if (part == 0) a.seq_n[s] = sn.tokens > 0;
     }
   }
 }
@@ -391,10 +431,8 @@ __global__ __launch_bounds__(1024) void bal_join_kernel(BalArgs a) {
   __shared__ int cnt[16];
   float l = 0.f;
   int n = 0;
-  for (int s = threadIdx.x; s < a.q.S; s += 1024) {
-    l += a.seq_loss[s];
-    n += a.seq_n[s];
-  }
+  for (int s = threadIdx.x; s < a.q.S * a.parts; s += 1024) l += a.seq_loss[s];
+  for (int s = threadIdx.x; s < a.q.S; s += 1024) n += a.seq_n[s];
   l = wave_sum(l);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
@@ -414,19 +452,19 @@ __global__ __launch_bounds__(1024) void bal_join_kernel(BalArgs a) {
   }
 }
 
-template <int DT, int NE>
+template <int DT, class SH>
 __global__ __launch_bounds__(256) void bal_bwd_kernel(BalArgs a, const float* __restrict__ go, void* __restrict__ dz) {
   typedef typename El<DT>::T T;
-  constexpr int B = TB<NE>;
-  const int lane = threadIdx.x & 63, e0 = lane * NE;
-  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * B;
-  if (t0 >= a.T) return;
+  constexpr int NE = SH::NE, L = SH::L, B = SH::B, RUN = SH::RUN;
+  const int lane = threadIdx.x & 63, e0 = lane % L * NE;
+  const int64_t w0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * SH::TOKENS, t0 = w0 + lane / L;
+  if (w0 >= a.T) return;
   const float g = *go * a.weights[(int64_t)a.q.S * a.E];
   float z[B][NE], v[B][NE];
   Row row[B];
 #pragma unroll
   for (int k = 0; k < B; ++k) {
-    const int64_t t = min(t0 + k, a.T - 1);
+    const int64_t t = min(t0 + k * RUN, a.T - 1);
     row[k] = a.rows[t];
     ld_run<DT, NE>((const T*)a.z + t * a.ldl, e0, a.E, -INFINITY, z[k]);
   }
@@ -450,14 +488,14 @@ __global__ __launch_bounds__(256) void bal_bwd_kernel(BalArgs a, const float* __
       dot[k] = fmaf(z[k][i], v[k][i], dot[k]);
     }
   }
-  over_wave<Sum>(dot);
+  over_lanes<Sum, L>(dot);
 #pragma unroll
   for (int k = 0; k < B; ++k) {
-    if (t0 + k >= a.T) break;
+    if (t0 + k * RUN >= a.T) break;
     float d[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) d[i] = row[k].seq >= 0 ? g * (z[k][i] * (v[k][i] - dot[k])) : 0.f;
-    st_run<DT, NE>((T*)dz + (t0 + k) * a.E, e0, a.E, d);
+    st_run<DT, NE>((T*)dz + (t0 + k * RUN) * a.E, e0, a.E, d);
   }
 }
 
@@ -466,13 +504,23 @@ __global__ __launch_bounds__(256) void bal_bwd_kernel(BalArgs a, const float* __
 // Sequences of under 64 tokens on average: blocks of four waves and about four sequences (each costs a block a few round
 // trips to memory, so many blocks have to be under way: 131072 tokens in 4096 sequences 129 -> 40 us).
 bool short_seqs(int64_t T, int64_t S) { return S > 1 && S * 64 > T; }
-// tokens of a forward block: up to 256 blocks, 64 tokens at least (four for a wave)
+// To 2048 tokens on average: eight waves and chunks of 32, twice the blocks; a sequence's slots are few (517 x 256 bf16, with the
+// slots' sums: 9.9 -> 8.8 us; 4092 in nine sequences 16.9 -> 16.2; 8192 x 256 fp32 in 64: 23 -> 18, in one 11.9 -> 12.9)
+bool medium_seqs(int64_t T, int64_t S) { return T <= S * 2048; }
+// tokens of a forward block: up to 512 blocks, 256 of sixteen waves, four tokens for a wave at least
 int chunk_of(int64_t T, int64_t S) {
   if (short_seqs(T, S)) return (int)std::max<int64_t>(4, 4 * T / S);
+  if (medium_seqs(T, S)) return (int)std::max<int64_t>((T + 511) / 512, 32);
   return (int)std::max<int64_t>((T + 255) / 256, 64);
 }
 int64_t chunks_of(int64_t T, int64_t S) { return T ? (T + chunk_of(T, S) - 1) / chunk_of(T, S) : 0; }
 constexpr int64_t ONE_BLOCK = 192;   // tokens of one sequence that a block takes alone
+
+// Blocks of a sequence's sums: one, or where its slots are many, one for each 64 experts (256 slots of 512 experts: 19 us by one
+// CU, 6 by eight with 2 for the join; of 256: 10.2, or 5.7 and 2).
+int parts_of(int64_t T, int64_t E, int64_t S) {
+  return (chunks_of(T, S) + S) / S * E >= 1 << 16 ? (int)((E + 63) / 64) : 1;
+}
 
 struct Ws {
   int64_t P, C, N, loss, n, bytes;
@@ -484,8 +532,8 @@ Ws ws_of(int64_t T, int64_t E, int64_t S) {
   w.P = 0;
   w.C = up(slots * E * 4);
   w.N = w.C + up(slots * E * 4);
-  w.loss = w.N + up(slots * 4);
-  w.n = w.loss + up(S * 4);
+  w.loss = w.N + up(slots * 8);
+  w.n = w.loss + up(S * parts_of(T, E, S) * 4);
   w.bytes = w.n + up(S * 4);
   return w;
 }
@@ -505,14 +553,17 @@ template <int V>
 struct Int {
   static constexpr int value = V;
 };
-// f(dtype, experts a lane) as constants
+// f(dtype, shape) as constants: 16 bytes of a row to a lane, 16 lanes at least (131072 x 64 bf16, forward: 12 us, 64 lanes of an
+// expert each 21; 4092 x 256 in nine sequences: 9.7, 64 lanes of four 10.4; 32768 x 256 fp32 backward: 64 lanes of four 11.6,
+// 32 of eight 14); two or four rows' loads at a time (131072 x 64 in 4096 sequences: 33 us with two, 42 with four)
 template <class F>
 void pick(int dtype, int64_t E, F f) {
   auto by_e = [&](auto dt) {
-    if (E <= 64) f(dt, Int<1>{});
-    else if (E <= 128) f(dt, Int<2>{});
-    else if (E <= 256) f(dt, Int<4>{});
-    else f(dt, Int<8>{});
+    constexpr bool f32 = decltype(dt)::value == 1;
+    if (E <= 64) f(dt, Shape<4, 16, 2>{});
+    else if (E <= 128) f(dt, std::conditional_t<f32, Shape<4, 32, 4>, Shape<8, 16, 2>>{});
+    else if (E <= 256) f(dt, std::conditional_t<f32, Shape<4, 64, 4>, Shape<8, 32, 2>>{});
+    else f(dt, Shape<8, 64, 2>{});
   };
   if (dtype == 0) by_e(Int<0>{});
   else if (dtype == 1) by_e(Int<1>{});
@@ -557,29 +608,33 @@ extern "C" int smel_balance_fwd(const void* logits, int64_t ldl, int32_t dtype, 
   a.weights = weights;
   if (S == 1 && T <= ONE_BLOCK) {
     a.chunk = ONE_BLOCK;
-    pick(dtype, E, [&](auto dt, auto ne) {
-      bal_fwd_kernel<decltype(dt)::value, decltype(ne)::value, 16, true><<<1, 1024, 0, stream>>>(a);
+    pick(dtype, E, [&](auto dt, auto sh) {
+      bal_fwd_kernel<decltype(dt)::value, decltype(sh), 16, true><<<1, 1024, 0, stream>>>(a);
     });
     return smel::launch_status();
   }
   a.chunk = chunk_of(T, S);
   a.P = (float*)(base + w.P);
   a.C = (int32_t*)(base + w.C);
-  a.N = (int32_t*)(base + w.N);
+  a.N = (Num*)(base + w.N);
+  a.parts = parts_of(T, E, S);
   a.seq_loss = (float*)(base + w.loss);
   a.seq_n = (int32_t*)(base + w.n);
   if (T)
-    pick(dtype, E, [&](auto dt, auto ne) {
-      constexpr int d = decltype(dt)::value, m = decltype(ne)::value;
+    pick(dtype, E, [&](auto dt, auto sh) {
+      constexpr int d = decltype(dt)::value;
+      typedef decltype(sh) SH;
       const unsigned n = (unsigned)chunks_of(T, S);
-      if (short_seqs(T, S)) bal_fwd_kernel<d, m, 4, false><<<n, 256, 0, stream>>>(a);
-      else bal_fwd_kernel<d, m, 16, false><<<n, 1024, 0, stream>>>(a);
+      if (short_seqs(T, S)) bal_fwd_kernel<d, SH, 4, false><<<n, 256, 0, stream>>>(a);
+      else if (medium_seqs(T, S)) bal_fwd_kernel<d, SH, 8, false><<<n, 512, 0, stream>>>(a);
+      else bal_fwd_kernel<d, SH, 16, false><<<n, 1024, 0, stream>>>(a);
     });
   int lgc = 6;
-  while ((1 << lgc) < E) ++lgc;
-  if (S <= 512) bal_seq_kernel<1024><<<(unsigned)S, 1024, 0, stream>>>(a, lgc);
-  else bal_seq_kernel<512><<<(unsigned)S, 512, 0, stream>>>(a, lgc);
-  if (S > 1) bal_join_kernel<<<1, 1024, 0, stream>>>(a);
+  while (a.parts == 1 && (1 << lgc) < E) ++lgc;
+  const unsigned n = (unsigned)(S * a.parts);
+  if (n <= 512) bal_seq_kernel<1024><<<n, 1024, 0, stream>>>(a, lgc);
+  else bal_seq_kernel<512><<<n, 512, 0, stream>>>(a, lgc);
+  if (n > 1) bal_join_kernel<<<1, 1024, 0, stream>>>(a);
   return smel::launch_status();
 }
 
@@ -599,9 +654,10 @@ extern "C" int smel_balance_bwd(const void* logits, int64_t ldl, int32_t dtype, 
   a.q = Seqs{nullptr, 0, (int)S, T};
   a.rows = (Row*)const_cast<float*>(row_stats);
   a.weights = const_cast<float*>(weights);
-  pick(dtype, E, [&](auto dt, auto ne) {
-    constexpr int tokens = 4 * TB<decltype(ne)::value>;
-    bal_bwd_kernel<decltype(dt)::value, decltype(ne)::value><<<(unsigned)((T + tokens - 1) / tokens), 256, 0, stream>>>(a, go, dlogits);
+  pick(dtype, E, [&](auto dt, auto sh) {
+    typedef decltype(sh) SH;
+    constexpr int tokens = 4 * SH::TOKENS;
+    bal_bwd_kernel<decltype(dt)::value, SH><<<(unsigned)((T + tokens - 1) / tokens), 256, 0, stream>>>(a, go, dlogits);
   });
   return smel::launch_status();
 }

@@ -95,6 +95,20 @@ def test_balance_sequences_and_mask(ids, offs):
         check(zn, topi.to(ids), mask, offsets, 0.3, 2.0, offs)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,E,K,offsets", [(2048, 3, 1, None), (2049, 64, 6, None), (8231, 509, 3, None), (8231, 481, 2, [0, 8000, 8000, 8229]),
+                                           (16384, 512, 2, [9, 14000, 16384]), (4500, 130, 2, [5, 1300, 1333, 4499]),
+                                           (6000, 31, 2, list(range(0, 6001, 60)))])
+def test_balance_long(T, E, K, offsets, dt):
+    """On both sides of the sizes at which blocks, chunks and the number of blocks that add a sequence's slots change; ids out of
+    range count nowhere."""
+    z, topi = make(T, E, K, dt, T)
+    topi[::7, 0] = -1
+    topi[3::11, K - 1] = E
+    mask = torch.rand(T, generator=torch.Generator().manual_seed(E)) > 0.2
+    check(z, topi.int(), mask, offsets, 1.0, 3.0)
+
+
 def test_balance_nothing_counts():
     """No token, no counted token, only empty sequences: loss 0, counts 0, gradient 0."""
     z, topi = make(40, 16, 2, "bf16", 1)
