@@ -41,13 +41,13 @@ struct Job {
   int32_t batch, r, n;
   int32_t blk0, mat0;  // first block (gram, apply) and first matrix (iterate, Q)
   int32_t slices;      // of a matrix
-  int32_t gblk0, gslices, parts;   // gram: first block, slices and blocks of a matrix (each takes js.per slices)
+  int32_t gblk0, parts;   // gram: first block, blocks of a matrix (each takes js.per columns)
   int32_t x_tall;      // 1: the short side has the unit stride in x
   int32_t y_tall;      // 1: the short side is y's last
 };
 struct Jobs {
   int32_t n, lg;      // jobs; log2 of the columns of an apply block's slice (64 at least)
-  int32_t glg, per;   // log2 of the columns of a gram slice; slices of a gram block
+  int32_t glg, per;   // log2 of the columns of a gram slice; columns of a gram block, a multiple of 16
   Job j[MAX_JOBS];
 };
 static_assert(sizeof(Jobs) <= 3584, "kernel arguments");
@@ -151,11 +151,11 @@ struct Slice {
   // row and column of chunk e (lines along i: 16 lanes take a chunk of 16 lines)
   SMEL_DEV static int row(bool tall, int e, int lg) { return tall ? (e >> 4) % (RP / V) * V : e >> (lg - LV); }
   SMEL_DEV static int col(bool tall, int e, int lg) { return tall ? e / (16 * RP / V) * 16 + (e & 15) : (e << LV) & ((1 << lg) - 1); }
-  SMEL_DEV void fetch(const Job& J, int mat, int j0, int lg) {
+  SMEL_DEV void fetch(const Job& J, int mat, int j0, int end, int lg) {
     const int slice = 1 << lg;
     typedef typename Elem<DT>::T T;
     const T* const x = (const T*)J.x + mat * J.xb;
-    const int nc = min(slice, J.n - j0);
+    const int nc = min(slice, end - j0);
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
       const int e = threadIdx.x + q * 64 * W;
@@ -190,10 +190,10 @@ struct Slice {
 constexpr int max_slice(int nt) { return nt == 1 ? 1024 : nt <= 4 ? 256 : 128; }
 constexpr int max_slice16(int nt) { return nt == 1 ? 1024 : nt == 2 ? 512 : nt == 4 ? 256 : 128; }   // of 16-bit types
 
-// A gram block takes `per` slices, the next one on its way while one is multiplied (two buffers). Waves of a block: the
+// A gram block takes `per` columns in slices, the next one on its way while one is multiplied (two buffers). Waves of a block: the
 // upper tiles in TG groups, a group's columns dealt to the others. Three tiles a wave at r = 128: nine leave registers for two
 // waves a SIMD, too few to cover the operands' latencies (36 x 128 x 2816: 65 us, three: 55; one round of blocks with the
-// loads ahead: see the plan's `per`).
+// loads ahead: see the plan's `per`; blocks of 416 columns, not of 448 in whole slices: 43 -> 41.6).
 constexpr int gram_slice(int nt) { return nt == 1 ? 512 : nt == 2 ? 256 : nt == 4 ? 128 : 64; }
 constexpr int gram_waves(int nt) { return nt == 8 ? 12 : WAVES; }
 constexpr int gram_tg(int nt) { return nt == 8 ? 12 : nt == 4 ? 2 : 1; }
@@ -211,7 +211,8 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
   __shared__ __attribute__((aligned(16))) float X[2 * BUF];
   const int lg = js.glg, slice = 1 << lg, pitch = slice + 20;
   const Job& J = js.j[find_job<BY_GRAM>(js, blockIdx.x)];
-  const int lb = blockIdx.x - J.gblk0, mat = lb / J.parts, s0 = lb % J.parts * js.per, s1 = min(s0 + js.per, J.gslices);
+  const int lb = blockIdx.x - J.gblk0, mat = lb / J.parts, c1 = min((lb % J.parts + 1) * js.per, J.n);
+  int c0 = lb % J.parts * js.per;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int tg = wave % TG, kg = wave / TG;
   f64x4_t acc[TPW];
@@ -235,15 +236,17 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
     tile[k] = tile_at(t, u, NT);
   }
   Slice<NT, DT, W, S> in;
-  in.fetch(J, mat, s0 << lg, lg);
+  in.fetch(J, mat, c0, c1, lg);
   in.put(J.x_tall, lg, X, pitch);
   __syncthreads();
-  for (int sl = s0; sl < s1; ++sl) {
-    const float* const x = X + ((sl - s0) & 1) * BUF;
-    if (sl + 1 < s1) in.fetch(J, mat, (sl + 1) << lg, lg);
+  for (int buf = 0; c0 < c1; c0 += slice, buf ^= 1) {
+    const float* const x = X + buf * BUF;
+    const bool more = c0 + slice < c1;
+    const int width = min(slice, c1 - c0);
+    if (more) in.fetch(J, mat, c0 + slice, c1, lg);
     // 16 columns a step, four to a lane: which columns make one instruction's contraction does not matter
     if constexpr (NT == 8) {
-      for (int j = 0; j < slice; j += 16) {
+      for (int j = 0; j < width; j += 16) {
         const f32x4_t a = *(const f32x4_t*)(x + ra[0] + j), b = *(const f32x4_t*)(x + ra[1] + j);
         if (triangle) {
           const f32x4_t c = *(const f32x4_t*)(x + ra[2] + j);
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
         }
       }
     } else {
-      for (int j = 16 * kg; j < slice; j += 16 * KG)
+      for (int j = 16 * kg; j < width; j += 16 * KG)
 #pragma unroll
         for (int k = 0; k < TPW; ++k) {
           const f32x4_t a = *(const f32x4_t*)(x + ra[k] + j), b = *(const f32x4_t*)(x + rb[k] + j);
@@ -273,7 +276,7 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
           for (int m = 0; m < 4; ++m) acc[k] = mfma64(a[m], b[m], acc[k]);
         }
     }
-    if (sl + 1 < s1) in.put(J.x_tall, lg, X + ((sl + 1 - s0) & 1) * BUF, pitch);
+    if (more) in.put(J.x_tall, lg, X + (buf ^ 1) * BUF, pitch);
     __syncthreads();
   }
   // the column groups' sums, in group order
@@ -511,7 +514,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void apply_kernel(Jobs js, Steps st,
   const int qlane = J.y_tall ? hi * 16 + perm : lane;
   {
     Slice<NT, 1, WAVES, max_slice(NT)> in;
-    in.fetch(J, mat, j0, js.lg);
+    in.fetch(J, mat, j0, J.n, js.lg);
     in.put(J.x_tall, js.lg, X, pitch);
   }
   f64x4_t q[NT];
@@ -914,16 +917,16 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
   while (gs > 128 && cols / gs < 512) gs /= 2;
   p.js.glg = __builtin_ctz(gs);
   const int64_t round = nt == 8 ? 256 : 512;
-  p.js.per = (int)std::max<int64_t>(1, cols / gs / round);
+  p.js.per = (int)std::max<int64_t>(gs, std::min<int64_t>(cols / round / 16 * 16, 1 << 30));
   for (;;) {
     int64_t blocks = 0;
     for (int k = 0; k < p.js.n; ++k) {
       const smel_ortho_job& j = jobs[taken[k].job];
       const int64_t n = j.rows < j.cols ? j.cols : j.rows;
-      blocks += taken[k].count * ((n + gs * p.js.per - 1) / (gs * p.js.per));
+      blocks += taken[k].count * ((n + p.js.per - 1) / p.js.per);
     }
     if (blocks <= round || blocks <= p.mats) break;   // or a block a matrix
-    ++p.js.per;
+    p.js.per += std::max(16, p.js.per / 256 * 16);
   }
   int64_t mats = 0;
   for (int k = 0; k < p.js.n; ++k) {
@@ -947,8 +950,7 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
       o.x_tall = wide;
     }
     o.slices = (o.n + slice - 1) / slice;
-    o.gslices = (o.n + gs - 1) / gs;
-    o.parts = (o.gslices + p.js.per - 1) / p.js.per;
+    o.parts = (o.n + p.js.per - 1) / p.js.per;
     o.blk0 = (int32_t)p.blocks;
     o.gblk0 = (int32_t)p.gblocks;
     o.mat0 = (int32_t)mats;
