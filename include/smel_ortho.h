@@ -24,11 +24,14 @@ typedef struct smel_ortho_job {
   int64_t dtype;
 } smel_ortho_job;
 
-/* Bytes of the workspace that smel_orthogonalize needs for these jobs (-1 for jobs that it does not take). */
-int64_t smel_orthogonalize_ws(const smel_ortho_job* jobs, int32_t n_jobs);
+/* Bytes of the workspace that smel_orthogonalize needs for these jobs, steps and a (-1 for jobs that it does not take). */
+int64_t smel_orthogonalize_ws(const smel_ortho_job* jobs, int32_t n_jobs, int32_t steps, double a);
 
 /* Every matrix G of every job: X = G / (|G|_F + eps), then `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X, to y.
- * 0 <= steps <= 64. ws: device memory of ws_bytes bytes, 16-byte aligned, not shared with a call that may run at the
+ * 0 <= steps <= 64: up to K steps, the most with a^(2 K) <= 2^24 (6 of the usual coefficients), on the r x r matrices of the short
+ * side, G being read twice; up to 2 K in two such passes, more as the formula itself, step by step, the matrices kept in 64 bits in
+ * the workspace: the result is the formula's in 64 bits in each (directions that G lacks then hold a^steps times its rounding, as
+ * there: from about 28 steps on, anything of their size). ws: device memory of ws_bytes bytes, 16-byte aligned, not shared with a call that may run at the
  * same time. */
 int smel_orthogonalize(const smel_ortho_job* jobs, int32_t n_jobs, int32_t steps, double a, double b, double c,
                        double eps, void* ws, int64_t ws_bytes, hipStream_t stream);

@@ -2,12 +2,18 @@
 //   X0 = G / (|G|_F + eps),   X <- P X  with  P = a I + b A + c A^2,  A = X X^T   (steps times)
 // With the short side r as rows, every P is a polynomial of A0 = X0 X0^T, so the P commute and are symmetric: the products
 // run on r x r matrices alone,  A <- P A P,  Q <- P Q,  and the result is  Q G  (Q starts as I / (|G|_F + eps)): G is read
-// for A0 and for the last product, whatever the number of steps.
+// for A0 and for the last product.
 //
 // A and Q are kept and multiplied in 64 bits (v_mfma_f64_16x16x4_f64). A holds the squares of the singular values: in 32
 // bits those under 2^-12 of the largest would drown in A's rounding, and the products blow such a value up by a = 3.4
 // each step (its square's error by a^2); in 64 bits the result is that of the formula to fp32's own rounding. The sums
 // of A0 run in 64 bits for the same reason; products of fp32 values are exact there.
+//
+// That growth bounds the steps of a pass. A singular value of zero is +-2^-53 in A0; a^(2 k) of it after k steps, and once a
+// negative one reaches about -1, P grows without end there (X X^T formed anew has no negative eigenvalues). So a pass takes K steps
+// with a^(2 K) <= 2^24 (6 of the usual coefficients: A is right to 2^-29 still); to 2 K steps run as two passes, X between them
+// in 64 bits; more as the formula itself on X in 64 bits, X <- a X + (b A + c A^2) X, A formed in each: null directions then
+// carry what the formula's own rounding leaves in them, and equal rows stay equal.
 //
 // The accumulator layout of the f64 instruction (register m of lane l: row 4 m + l / 16, column l % 16) is its layout of
 // the operand B at step m of a 16-long contraction, and of the operand A of a symmetric matrix: results are the next
@@ -299,8 +305,11 @@ __global__ __launch_bounds__(64 * gram_waves(NT)) void gram_kernel(Jobs js, doub
 
 struct Steps {
   int32_t steps;
+  int32_t normed;   // 1: the matrix is X already, no norm is taken out
   double a, b, c, eps;
 };
+// 1 / (|G|_F + eps) of a trace of A0
+SMEL_DEV double inv_norm(const Steps& st, double trace) { return st.normed ? 1.0 : 1.0 / (sqrt(trace) + st.eps); }
 
 // Q carries 1 / (|G|_F + eps) = s. Above 2^64 (only an update of tiny norm with eps near 0) a power of two stays out of it, so
 // that Q's bf16 parts stay in range; the last product multiplies it back in. exp_of(s): that power's exponent.
@@ -345,7 +354,7 @@ __global__ __launch_bounds__(64 * IT_WAVES) void iterate_kernel(Jobs js, Steps s
   for (int o = 32; o >= 1; o >>= 1) d += __shfl_xor(d, o, 64);
   if (t == u && lane == 0) trs[t] = d;
   __syncthreads();
-  const double s = 1.0 / (sqrt(((trs[0] + trs[1]) + trs[2]) + trs[3]) + st.eps);
+  const double s = inv_norm(st, ((trs[0] + trs[1]) + trs[2]) + trs[3]);
   const double sq = ldexp(s, -exp_of(s));
   if (threadIdx.x == 0) qscale[blockIdx.x] = ldexp(1.0, exp_of(s));
   A = A * s * s;
@@ -445,7 +454,7 @@ SMEL_DEV double steps_small(const Job& J, int mat, const Steps& st, const double
   double sum = tr[0];
 #pragma unroll
   for (int k = 1; k < NT; ++k) sum += tr[k];
-  const double s = 1.0 / (sqrt(sum) + st.eps);
+  const double s = inv_norm(st, sum);
   const int ex = exp_of(s);
   const double sq = ldexp(s, -ex);
   A = A * s * s;
@@ -820,7 +829,7 @@ __global__ __launch_bounds__(256, 2) void big_kernel(BigArgs g) {
     double tr = 0;
 #pragma unroll
     for (int i = 0; i < BIG; ++i) tr += g.tr[mat * BIG + i];
-    s = 1.0 / (sqrt(tr) + g.st.eps);
+    s = inv_norm(g.st, tr);
   }
   const double s2 = s * s;
   if constexpr (WHAT == BIG_P) {
@@ -843,6 +852,198 @@ __global__ __launch_bounds__(256, 2) void big_kernel(BigArgs g) {
       big_store(g.Q2 + base, t, u, lane, big_product(g.P + base, g.Q + base, t, u, lane), tile[wave]);
   } else {
     big_store(g.A + base, t, u, lane, big_product(g.T + base, g.P + base, t, u, lane), tile[wave]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ passes on X in 64 bits
+
+// X: a group's matrices one after the other, each as blocks [n / 16][16 NT rows][16 columns], zero past r and n: what the matrix
+// instruction takes of a block lies together.
+SMEL_DEV double* x64_of(const Jobs& js, int k, int mat, int nt, double* X) {
+  int64_t at = 0;
+  for (int q = 0; q < k; ++q) at += (int64_t)js.j[q].batch * ((js.j[q].n + 15) >> 4);
+  return X + (at + (int64_t)mat * ((js.j[k].n + 15) >> 4)) * (256 * nt);
+}
+
+// The parts of X X^T, as gram_kernel's: a block's columns, tiles dealt to the waves (at r = 128 as there). A tile's operand is 2 KB in
+// one piece, which the rows' other tiles find in the caches. Every element is one chain of products in column order, so equal rows
+// give equal elements. 36 x 128 x 2816: 51 us (27 of f64 products).
+constexpr int gram64_waves(int nt) { return nt == 8 ? 12 : nt == 4 ? 5 : ntiles(nt); }
+template <int NT>
+__global__ __launch_bounds__(64 * gram64_waves(NT)) void gram64_kernel(Jobs js, const double* __restrict__ X, double* __restrict__ part) {
+  constexpr int NTL = ntiles(NT), W = gram64_waves(NT), TPW = NTL / W;
+  static_assert(TPW * W == NTL, "tiles per wave");
+  const int k = find_job<BY_GRAM>(js, blockIdx.x);
+  const Job& J = js.j[k];
+  const int lb = blockIdx.x - J.gblk0, mat = lb / J.parts;
+  const int b0 = lb % J.parts * (js.per >> 4), b1 = min(b0 + (js.per >> 4), (J.n + 15) >> 4);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+  const double* const x = x64_of(js, k, mat, NT, const_cast<double*>(X)) + lo * 16 + hi * 4;
+  auto operand = [&](int64_t b, int tile) { return *(const f64x4_t*)(x + (b * NT + tile) * 256); };
+  f64x4_t acc[TPW];
+  int tile[TPW];
+#pragma unroll
+  for (int q = 0; q < TPW; ++q) acc[q] = f64x4_t{0, 0, 0, 0};
+  if constexpr (NT == 8) {
+    const uint32_t rows = GRAM_ROWS[wave];
+    const int ra = rows >> 8, rb = rows >> 4 & 15, rc = rows & 15;
+    if (wave < 8) {
+      tile[0] = tile_at(ra, rb, NT);
+      tile[1] = tile_at(ra, rc, NT);
+      tile[2] = tile_at(rb, rc, NT);
+      f64x4_t an = operand(b0, ra), bn = operand(b0, rb), cn = operand(b0, rc);
+      for (int j = b0; j < b1; ++j) {   // the next block's on their way
+        const f64x4_t a = an, b = bn, c = cn;
+        const int next = min(j + 1, b1 - 1);
+        an = operand(next, ra), bn = operand(next, rb), cn = operand(next, rc);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          acc[0] = mfma64(a[m], b[m], acc[0]);
+          acc[1] = mfma64(a[m], c[m], acc[1]);
+          acc[2] = mfma64(b[m], c[m], acc[2]);
+        }
+      }
+    } else {
+      tile[0] = tile_at(ra, rb, NT);
+      tile[1] = tile_at(ra, ra, NT);
+      tile[2] = tile_at(rb, rb, NT);
+      f64x4_t an = operand(b0, ra), bn = operand(b0, rb);
+      for (int j = b0; j < b1; ++j) {
+        const f64x4_t a = an, b = bn;
+        const int next = min(j + 1, b1 - 1);
+        an = operand(next, ra), bn = operand(next, rb);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          acc[0] = mfma64(a[m], b[m], acc[0]);
+          acc[1] = mfma64(a[m], a[m], acc[1]);
+          acc[2] = mfma64(b[m], b[m], acc[2]);
+        }
+      }
+    }
+  } else {
+    int t[TPW], u[TPW];
+#pragma unroll
+    for (int q = 0; q < TPW; ++q) {
+      tile[q] = wave * TPW + q;
+      tile_of(tile[q], NT, t[q], u[q]);
+    }
+    f64x4_t an[TPW], bn[TPW];
+#pragma unroll
+    for (int q = 0; q < TPW; ++q) an[q] = operand(b0, t[q]), bn[q] = operand(b0, u[q]);
+    for (int j = b0; j < b1; ++j) {
+      const int next = min(j + 1, b1 - 1);
+#pragma unroll
+      for (int q = 0; q < TPW; ++q) {
+        const f64x4_t a = an[q], b = bn[q];
+        an[q] = operand(next, t[q]), bn[q] = operand(next, u[q]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) acc[q] = mfma64(a[m], b[m], acc[q]);
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < TPW; ++q) *(f64x4_t*)(part + ((J.part0 + lb) * (int64_t)NTL + tile[q]) * 256 + lane * 4) = acc[q];
+}
+
+// the steps of r <= 32, a block per matrix: Q's tiles to memory
+template <int NT>
+__global__ __launch_bounds__(64 * WAVES) void steps_kernel(Jobs js, Steps st, const double* __restrict__ part,
+                                                           double* __restrict__ Qout, double* __restrict__ qscale) {
+  constexpr int N2 = NT * NT;
+  __shared__ f64x4_t b[4 * N2][64];
+  __shared__ double tr[NT];
+  const Job& J = js.j[find_job<BY_MATRIX>(js, blockIdx.x)];
+  const double scale = steps_small<NT>(J, blockIdx.x - J.mat0, st, part, b, tr);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave < N2) *(f64x4_t*)(Qout + ((int64_t)blockIdx.x * N2 + wave) * 256 + lane * 4) = b[3 * N2 + wave][lane];
+  if (threadIdx.x == 0) qscale[blockIdx.x] = scale;
+}
+
+enum { X64 = 3 };   // beside the types 0 to 2: the group's X
+SMEL_DEV double ld_as(const void* p, int64_t i, int dt) {
+  switch (dt) {
+    case 0: return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+    case 1: return ((const float*)p)[i];
+    case 2: return (float)((const _Float16*)p)[i];
+    default: return ((const double*)p)[i];
+  }
+}
+// A 16-bit value is rounded by way of fp32: off by 2^-16 (bf16), 2^-13 (fp16) of its half step more at most
+SMEL_DEV void st_as(void* p, int64_t i, int dt, double v) {
+  switch (dt) {
+    case 0: ((uint16_t*)p)[i] = f2bf((float)v); break;
+    case 1: ((float*)p)[i] = (float)v; break;
+    case 2: ((_Float16*)p)[i] = (_Float16)(float)v; break;
+    default: ((double*)p)[i] = v;
+  }
+}
+
+// alpha X + Q X from `in` (G's type, or X64) to `out` (the result's type, or X64: in place). A wave owns a tile of rows, whose part of
+// Q stays in registers, and every CG-th block of 16 columns; the block's columns pass through LDS, the next ones on their way while
+// some are multiplied. A register of a lane is the operand's and the result's element alike. 36 x 128 x 2816: 92 us, 41 of bytes;
+// a step of the formula 160 (390 with X in rows of n and Q read for every 16 columns by every wave).
+template <int NT>
+__global__ __launch_bounds__(64 * WAVES) void apply64_kernel(Jobs js, double alpha, const double* __restrict__ Q,
+                                                             const double* __restrict__ qscale, double* X, int in, int out) {
+  constexpr int CG = WAVES / NT, RP = 16 * NT, PER = 4;   // elements of a thread: CG RP 16 / (64 WAVES)
+  __shared__ double buf[2][CG * RP * 16];
+  const int k = find_job<BY_APPLY>(js, blockIdx.x);
+  const Job& J = js.j[k];
+  const int lb = blockIdx.x - J.blk0, mat = lb / J.slices, j0 = (lb % J.slices) << js.lg;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4, t = wave % NT, cg = wave / NT;
+  const int nc = min(1 << js.lg, J.n - j0);
+  double* const x64 = x64_of(js, k, mat, NT, X) + (int64_t)(j0 >> 4) * (RP * 16);
+  double v[PER];
+  // element e of CG column blocks from column c on: its place in LDS
+  auto place = [&](int q) {
+    const int e = threadIdx.x + q * 64 * WAVES;
+    return in != X64 && J.x_tall ? e / (RP * 16) * (RP * 16) + e % RP * 16 + e / RP % 16 : e;
+  };
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int at = place(q), i = at / 16 % RP, col = c + at / (RP * 16) * 16 + at % 16;
+      v[q] = 0;
+      if (in == X64) {
+        if (col < ((nc + 15) & ~15)) v[q] = x64[(int64_t)c * RP + at];
+      } else if (i < J.r && col < nc) {
+        const int64_t j = j0 + col;
+        v[q] = ld_as(J.x, mat * J.xb + (J.x_tall ? j * J.ld + i : i * J.ld + j), in);
+      }
+    }
+  };
+  fetch(0);
+  f64x4_t q[NT];
+  const double scale = qscale[J.mat0 + mat];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) q[u] = *(const f64x4_t*)(Q + (int64_t)(J.mat0 + mat) * (NT * NT * 256) + ((u * NT + t) * 64 + lane) * 4) * scale;
+  for (int c = 0, par = 0; c < nc; c += 16 * CG, par ^= 1) {
+    double* const b = buf[par];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) b[place(e)] = v[e];
+    __syncthreads();   // the buffers alternate: who reads b has passed the next barrier before it is written again
+    if (c + 16 * CG < nc) fetch(c + 16 * CG);
+    const int w = c + 16 * cg;
+    if (w >= nc) continue;
+    const double* const x = b + cg * (RP * 16);
+    f64x4_t acc = {0, 0, 0, 0}, own;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) acc = mfma64(q[u][m], x[(16 * u + 4 * m + hi) * 16 + lo], acc);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) own[m] = fma(alpha, x[(16 * t + 4 * m + hi) * 16 + lo], acc[m]);
+    if (out == X64) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) x64[(int64_t)w * RP + (16 * t + 4 * m + hi) * 16 + lo] = own[m];
+    } else {
+      const int64_t j = j0 + w + lo;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int64_t i = 16 * t + 4 * m + hi;
+        if (w + lo < nc && i < J.r) st_as(J.y, (int64_t)mat * J.r * J.n + (J.y_tall ? j * J.r + i : i * J.n + j), out, own[m]);
+      }
+    }
   }
 }
 
@@ -963,12 +1164,25 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
   return at;
 }
 
+// steps of a pass on the r x r matrices: their rounding grows by a^2 a step
+int pass_steps(double a) {
+  const double growth = std::max(1.0, a * a);
+  int k = 1;
+  for (double g = growth * growth; k < 64 && g <= 0x1p24; g *= growth) ++k;
+  return k;
+}
+
 int64_t part_bytes(const Plan& p, int nt) { return p.gblocks * ntiles(nt) * 2048; }
-int64_t ws_bytes_of(const Plan& p, int nt) {
+// of the r x r matrices beside Q's tiles and scale: none to r = 64
+int64_t q_bytes(const Plan& p, int nt) {
+  return nt == 8 ? p.mats * (5 * BIG_MAT + BIG + 1) * 8 : p.mats * (nt * nt * 256 + 1) * 8;
+}
+int64_t ws_bytes_of(const Plan& p, int nt, bool passes) {
   const int64_t parts = part_bytes(p, nt);
-  if (nt <= 2) return parts;
-  if (nt == 4) return parts + p.mats * (nt * nt * 256 + 1) * 8;
-  return parts + p.mats * (5 * BIG_MAT + BIG + 1) * 8;
+  if (!passes) return nt <= 2 ? parts : parts + q_bytes(p, nt);
+  int64_t blocks = 0;   // of X
+  for (int k = 0; k < p.js.n; ++k) blocks += (int64_t)p.js.j[k].batch * ((p.js.j[k].n + 15) >> 4);
+  return parts + (q_bytes(p, nt) + 31) / 32 * 32 + blocks * (256 * nt * 8);
 }
 
 // the steps above r = 64; returns where Q's tiles are
@@ -1000,6 +1214,21 @@ const double* run_big(const Plan& p, const Steps& st, const double* part, double
   return g.Q;
 }
 
+// Q's tiles from the parts: where they are, and their scale
+template <int NT>
+const double* run_steps(const Plan& p, const Steps& st, const double* part, double* rest, const double*& qscale,
+                        hipStream_t stream) {
+  if constexpr (NT == 8) {
+    return run_big(p, st, part, rest, qscale, stream);
+  } else {
+    double* const scale = rest + p.mats * NT * NT * 256;
+    if constexpr (NT == 4) iterate_kernel<<<(unsigned)p.mats, 64 * IT_WAVES, 0, stream>>>(p.js, st, part, rest, scale);
+    else steps_kernel<NT><<<(unsigned)p.mats, 64 * WAVES, 0, stream>>>(p.js, st, part, rest, scale);
+    qscale = scale;
+    return rest;
+  }
+}
+
 template <int NT, int DT, bool SMALL>
 void run_apply(const Plan& p, const Steps& st, const double* in, const double* qscale, hipStream_t stream) {
   if constexpr (DT == 1) apply_kernel<NT, SMALL><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, st, in, qscale);
@@ -1013,19 +1242,40 @@ int run(const Plan& p, const Steps& st, void* ws, hipStream_t stream) {
   gram_kernel<NT, DT><<<(unsigned)p.gblocks, 64 * gram_waves(NT), 0, stream>>>(js, part);
   if constexpr (NT <= 2) {
     run_apply<NT, DT, true>(p, st, part, nullptr, stream);
-  } else if constexpr (NT == 4) {
-    double* const qscale = rest + p.mats * NT * NT * 256;
-    iterate_kernel<<<(unsigned)p.mats, 64 * IT_WAVES, 0, stream>>>(js, st, part, rest, qscale);
-    run_apply<NT, DT, false>(p, st, rest, qscale, stream);
   } else {
     const double* qscale = nullptr;
-    const double* const Q = run_big(p, st, part, rest, qscale, stream);
+    const double* const Q = run_steps<NT>(p, st, part, rest, qscale, stream);
     run_apply<NT, DT, false>(p, st, Q, qscale, stream);
+  }
+  return smel::launch_status();
+}
+// More steps than a pass takes
+template <int NT, int DT>
+int run_passes(const Plan& p, const Steps& st, int most, void* ws, hipStream_t stream) {
+  double* const part = (double*)ws;
+  double* const rest = (double*)((char*)ws + part_bytes(p, NT));
+  double* const X = (double*)((char*)rest + (q_bytes(p, NT) + 31) / 32 * 32);
+  auto pass = [&](bool first, bool last, const Steps& s, double alpha) {
+    if (first) gram_kernel<NT, DT><<<(unsigned)p.gblocks, 64 * gram_waves(NT), 0, stream>>>(p.js, part);
+    else gram64_kernel<NT><<<(unsigned)p.gblocks, 64 * gram64_waves(NT), 0, stream>>>(p.js, X, part);
+    const double* qscale = nullptr;
+    const double* const Q = run_steps<NT>(p, s, part, rest, qscale, stream);
+    apply64_kernel<NT><<<(unsigned)p.blocks, 64 * WAVES, 0, stream>>>(p.js, alpha, Q, qscale, X, first ? DT : X64, last ? DT : X64);
+  };
+  if (st.steps <= 2 * most) {
+    pass(true, false, Steps{(st.steps + 1) / 2, 0, st.a, st.b, st.c, st.eps}, 0);
+    pass(false, true, Steps{st.steps / 2, 1, st.a, st.b, st.c, 0}, 0);
+  } else {   // X0, then a step each: Q = b A + c A^2
+    pass(true, false, Steps{0, 0, st.a, st.b, st.c, st.eps}, 0);
+    for (int it = 0; it < st.steps; ++it) pass(false, it + 1 == st.steps, Steps{1, 1, 0, st.b, st.c, 0}, st.a);
   }
   return smel::launch_status();
 }
 template <int NT>
 int run_dt(const Plan& p, int dt, const Steps& st, void* ws, hipStream_t stream) {
+  if (const int most = pass_steps(st.a); st.steps > most)
+    return dt == 0 ? run_passes<NT, 0>(p, st, most, ws, stream) : dt == 1 ? run_passes<NT, 1>(p, st, most, ws, stream)
+                                                                          : run_passes<NT, 2>(p, st, most, ws, stream);
   return dt == 0 ? run<NT, 0>(p, st, ws, stream) : dt == 1 ? run<NT, 1>(p, st, ws, stream) : run<NT, 2>(p, st, ws, stream);
 }
 
@@ -1050,10 +1300,10 @@ int each(const smel_ortho_job* jobs, int32_t n, F f) {
   return 0;
 }
 
-int64_t ws_need(const smel_ortho_job* jobs, int32_t n, int& rc) {
+int64_t ws_need(const smel_ortho_job* jobs, int32_t n, bool passes, int& rc) {
   int64_t need = 0;   // the groups run one after the other on one stream and share the workspace
   rc = each(jobs, n, [&](const Plan& p, int nt, int) {
-    need = std::max(need, ws_bytes_of(p, nt));
+    need = std::max(need, ws_bytes_of(p, nt, passes));
     return 0;
   });
   return need;
@@ -1061,10 +1311,10 @@ int64_t ws_need(const smel_ortho_job* jobs, int32_t n, int& rc) {
 
 }  // namespace
 
-extern "C" int64_t smel_orthogonalize_ws(const smel_ortho_job* jobs, int32_t n_jobs) {
+extern "C" int64_t smel_orthogonalize_ws(const smel_ortho_job* jobs, int32_t n_jobs, int32_t steps, double a) {
   if (check(jobs, n_jobs)) return -1;
   int rc = 0;
-  const int64_t need = ws_need(jobs, n_jobs, rc);
+  const int64_t need = ws_need(jobs, n_jobs, steps > pass_steps(a), rc);
   return rc ? -1 : need;
 }
 
@@ -1074,12 +1324,12 @@ extern "C" int smel_orthogonalize(const smel_ortho_job* jobs, int32_t n_jobs, in
   if (rc) return rc;
   SMEL_REQUIRE(steps >= 0 && steps <= 64, SMEL_EINVAL, "orthogonalize: %d steps (0 to 64)", steps);
   SMEL_REQUIRE(eps >= 0, SMEL_EINVAL, "orthogonalize: eps %g", eps);
-  const int64_t need = ws_need(jobs, n_jobs, rc);
+  const int64_t need = ws_need(jobs, n_jobs, steps > pass_steps(a), rc);
   if (rc) return rc;
   SMEL_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), SMEL_EINVAL,
                "orthogonalize: a workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", (long long)need,
                (long long)ws_bytes);
-  const Steps st{steps, a, b, c, eps};
+  const Steps st{steps, 0, a, b, c, eps};
   return each(jobs, n_jobs, [&](const Plan& p, int nt, int dt) {
     return nt == 1 ? run_dt<1>(p, dt, st, ws, stream) : nt == 2 ? run_dt<2>(p, dt, st, ws, stream)
            : nt == 4 ? run_dt<4>(p, dt, st, ws, stream) : run_dt<8>(p, dt, st, ws, stream);

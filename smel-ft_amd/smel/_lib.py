@@ -25,7 +25,7 @@ WSET_MERGE_SHORT = 8 # smel_wset.flags: gate_up forward, a full int4 tile also t
 WSET_MERGED_LIST = 16 # smel_wset.flags: gate_up forward on smel_dispatch's merged tile list (int4 tiles up to 160 rows)
 WSET_TILE32 = 32     # smel_wset.flags: a tile list of at most 32 rows a tile
 WSET_COL_CHUNK = 64  # smel_wset.flags: column blocks, not tiles, are spread over the XCDs
-ABI_VERSION = 25
+ABI_VERSION = 26
 
 vp, i64, i32, f32, f64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_double
 
@@ -174,7 +174,7 @@ SIGNATURES = {
     "smel_balance_fwd": (i32, [vp, i64, i32, vp, i32, i64, i64, i64, vp, vp, i32, i64, f32, vp, vp, vp, vp, vp, i64, vp]),
     "smel_balance_bwd": (i32, [vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp]),
     # include/smel_ortho.h
-    "smel_orthogonalize_ws": (i64, [vp, i32]),
+    "smel_orthogonalize_ws": (i64, [vp, i32, i32, f64]),
     "smel_orthogonalize": (i32, [vp, i32, i32, f64, f64, f64, f64, vp, i64, vp]),
     # include/smel_probe.h
     "smel_probe_mfma": (i32, [vp, i32, i32, vp]),

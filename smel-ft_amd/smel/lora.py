@@ -142,8 +142,9 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
     which moves every singular value towards 1 and keeps the singular vectors. ``update``: a tensor [..., m, n] (bf16,
     fp16, fp32; a factor's gradient or momentum) or a sequence of them, e.g. every factor's of a block, which go through
     few launches together; the shorter side (a LoRA's rank) is at most 128. Returns the same shapes and dtypes,
-    contiguous, without gradients. The products run on the rank's r x r matrices in 64 bits, so small singular values keep
-    their directions (include/smel_ortho.h)."""
+    contiguous, without gradients. The products run in 64 bits, up to 6 steps of these coefficients on the rank's r x r matrices
+    alone, so small singular values keep their directions; 7 to 12 steps take two such passes, more a pass over the update for
+    each (include/smel_ortho.h)."""
     single = isinstance(update, torch.Tensor)
     ts = (update,) if single else tuple(update)
     a, b, c = (float(v) for v in coeffs)
@@ -183,7 +184,7 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
             outs.append(y)
         n = len(jobs) // 9
         addr = jobs.buffer_info()[0]
-        need = _lib.load().smel_orthogonalize_ws(addr, n)
+        need = _lib.load().smel_orthogonalize_ws(addr, n, int(steps), a)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         _lib.call("smel_orthogonalize", addr, n, int(steps), a, b, c, float(eps), ws.data_ptr(), need, _lib.stream())
     return outs[0] if single else outs

@@ -85,3 +85,18 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="eps"):
         orthogonalize(x, eps=-1.0)
     assert orthogonalize([]) == []
+
+
+def test_orthogonalize_workspace_of_steps():
+    """Steps beyond a pass keep the matrices in the workspace: its size says so, and a call with less is refused."""
+    from array import array
+    L = _L()
+    for rows, cols in ((16, 2048), (24, 70), (2048, 60), (100, 129)):
+        job = array("q", (16, 16, 3, rows, cols, rows * cols, cols, 1, 1))
+        at = job.buffer_info()[0]
+        ws = lambda steps, a=3.4445: L.smel_orthogonalize_ws(at, 1, steps, a)
+        call = lambda steps, n: L.smel_orthogonalize(at, 1, steps, 3.4445, -4.0, 2.0, 1e-7, 16, n, None)
+        assert ws(0) == ws(6) and ws(6) + 3 * rows * cols * 8 <= ws(7) == ws(12) == ws(64)
+        assert ws(13, 1.875) == ws(6) and ws(14, 1.875) == ws(7) and ws(64, 1.0) == ws(6)
+        assert call(7, ws(7) - 1) == -1 and b"workspace" in L.smel_last_error()
+        assert call(6, ws(6) - 1) == -1
