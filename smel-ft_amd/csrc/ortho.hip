@@ -311,9 +311,13 @@ struct Steps {
 // 1 / (|G|_F + eps) of a trace of A0
 SMEL_DEV double inv_norm(const Steps& st, double trace) { return st.normed ? 1.0 : 1.0 / (sqrt(trace) + st.eps); }
 
-// Q carries 1 / (|G|_F + eps) = s. Above 2^64 (only an update of tiny norm with eps near 0) a power of two stays out of it, so
+// Q carries 1 / (|G|_F + eps) = s. Outside 2^-64 to 2^64 (an update of tiny norm with eps near 0, or of values near the type's
+// largest, whose s would leave its second and third bf16 part under their smallest value) a power of two stays out of it, so
 // that Q's bf16 parts stay in range; the last product multiplies it back in. exp_of(s): that power's exponent.
-SMEL_DEV int exp_of(double s) { return s > 0x1p64 && s < 0x1p1000 ? ilogb(s) - 64 : 0; }
+SMEL_DEV int exp_of(double s) {
+  if (s > 0x1p64 && s < 0x1p1000) return ilogb(s) - 64;
+  return s < 0x1p-64 && s > 0x1p-1000 ? ilogb(s) + 64 : 0;
+}
 
 constexpr int TP = 17;   // doubles between the rows of a tile in LDS
 
