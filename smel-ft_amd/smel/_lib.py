@@ -11,6 +11,7 @@ import ctypes
 import os
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # SMEL_MOE_LIB names another build of the same library (e.g. one compiled with different flags)
@@ -329,6 +330,12 @@ def on_device_of(t: torch.Tensor):
     if _device is not None and t.device.index == _device():
         return _HERE
     return torch.cuda.device(t.device)
+
+
+def forward_mode() -> bool:
+    """Whether a call may carry tangents (inside ``forward_ad.dual_level``). Such a call takes ``apply``, which refuses tangents (no
+    function here has a rule for them), whether or not an input requires a gradient."""
+    return getattr(_forward_ad, "_current_level", 0) >= 0
 
 
 _transforms_active = getattr(torch._C, "_are_functorch_transforms_active", None)

@@ -478,7 +478,7 @@ def balance_loss(logits, topi, mask=None, offsets=None, coef: float = 1.0):
     are constants to it."""
     _balance_check(logits, topi, mask, offsets)
     with L.on_device_of(logits):
-        if torch.is_grad_enabled() and logits.requires_grad:
+        if torch.is_grad_enabled() and logits.requires_grad or L.forward_mode():
             return L.apply(_BalanceFn, logits, topi, mask, offsets, float(coef))
         loss, counts, _ = _balance_forward(logits, topi, mask, offsets, float(coef), False)
     return loss, counts

@@ -286,7 +286,7 @@ def _ln(x, h, w, b, eps):
     call = _ln_check(x, h, w, b)
     with _lib.on_device_of(x):
         if torch.is_grad_enabled() and (x.requires_grad or h is not None and h.requires_grad or w is not None and w.requires_grad
-                                        or b is not None and b.requires_grad):
+                                        or b is not None and b.requires_grad) or _lib.forward_mode():
             return _lib.apply(_LayerNormFn, x, h, w, b, float(eps), call)
         _, _, s, y, _ = _ln_forward(x, h, w, b, float(eps), *call)
     return y if h is None else (s, y)

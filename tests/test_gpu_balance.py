@@ -355,3 +355,18 @@ def test_balance_far_offsets():
         loss, counts = balance_loss(zg, topi.to(DEV))
         out.append((loss.detach(), counts, torch.autograd.grad(loss, zg)[0]))
     assert all(torch.equal(p, q) for p, q in zip(*out))
+
+
+def test_balance_forward_mode_refused():
+    """A tangent is not dropped: forward mode has no rule and says so, with and without gradients."""
+    import torch.autograd.forward_ad as fw
+    from smel.loss import balance_loss
+    z, topi = make(20, 8, 2, "fp32", 3)
+    z, topi = z.to(DEV), topi.to(DEV)
+    with fw.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                balance_loss(fw.make_dual(z, torch.ones_like(z)), topi)
+        loss, counts = balance_loss(z, topi)
+    again, counts2 = balance_loss(z, topi)
+    assert torch.equal(loss, again) and torch.equal(counts, counts2) and not loss.requires_grad

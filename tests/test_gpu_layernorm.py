@@ -350,3 +350,19 @@ def test_layernorm_far_offsets():
     assert torch.equal(y[:100], y[-100:]) and torch.equal(dx[:100], dx[-100:])
     assert not y[100:103].any() and not y[-101].any() and not dx[-101].any()
     close(y[-100:], formula(some.cpu(), None, None, torch.zeros_like(some).cpu())["y"], "y")
+
+
+def test_layernorm_forward_mode_refused():
+    """A tangent is not dropped: forward mode has no rule and says so, with and without gradients."""
+    import torch.autograd.forward_ad as fw
+    from smel.norm import add_layernorm, layernorm
+    x, w = torch.randn(4, 8, device=DEV), torch.ones(8, device=DEV)
+    with fw.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for bad in (lambda d: layernorm(d(x), w, None, EPS), lambda d: layernorm(x, d(w), None, EPS),
+                            lambda d: layernorm(x, w, d(w), EPS), lambda d: add_layernorm(d(x), x, w, w, EPS)):
+                    with pytest.raises(NotImplementedError):
+                        bad(lambda t: fw.make_dual(t, torch.ones_like(t)))
+        plain = layernorm(x, w, None, EPS)      # without a tangent in the call
+    assert torch.equal(plain, layernorm(x, w, None, EPS)) and not plain.requires_grad
