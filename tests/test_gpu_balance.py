@@ -370,3 +370,29 @@ def test_balance_forward_mode_refused():
         loss, counts = balance_loss(z, topi)
     again, counts2 = balance_loss(z, topi)
     assert torch.equal(loss, again) and torch.equal(counts, counts2) and not loss.requires_grad
+
+
+@pytest.mark.parametrize("run", [5, 1 << 20])
+def test_balance_run_of_empty_sequences(run):
+    """Offsets that repeat, inside a chunk, at the start and at the end before a padded tail (a buffer of fixed length filled up with
+    its last value): nothing that a block walks through one by one. A walk takes a trip to memory for each."""
+    from smel.loss import balance_loss
+    T, E, K = 300, 16, 2
+    z, topi = make(T, E, K, "fp32", 5)
+    cuts = [0] * run + [40, 41, 41, 60] + [60] * run + [61, 130, 130, 130, 250] + [250] * run
+    used = [s for s in range(len(cuts) - 1) if cuts[s] < cuts[s + 1]]
+    wl, wc, wz, err = definition(z, topi, None, [0, 40, 41, 60, 61, 130, 250], 1.0, 1.0)
+    zg, off, ids = z.to(DEV).requires_grad_(True), torch.tensor(cuts, device=DEV), topi.to(DEV)
+    ms = []
+    for _ in range(2):
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        loss, counts = balance_loss(zg, ids, offsets=off)
+        e1.record()
+        torch.cuda.synchronize()
+        ms.append(e0.elapsed_time(e1))
+    dz, = torch.autograd.grad(loss, zg)
+    assert abs(loss.item() - wl.item()) <= 372 * U * wl.item()
+    assert torch.equal(counts[used].cpu(), wc) and counts.sum().item() == 250 * K
+    assert ((dz.cpu().double() - wz).abs() <= U * wz.abs() + err).all()
+    assert min(ms) < 100, ms      # 227 with a walk of 2^20 trips to memory, 10 without
