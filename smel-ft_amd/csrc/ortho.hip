@@ -23,6 +23,8 @@
 // inside (every block of a matrix runs them again: two launches in all), for r <= 64 iterate (a block per matrix) and apply,
 // and above that the products as launches of their own, a wave per tile (a block per matrix would leave most CUs idle: 128 x 128
 // products of 17 cost 130 us of one CU's matrix units). Nothing is atomic: results repeat bit for bit.
+#include <stddef.h>
+
 #include <algorithm>
 #include <utility>
 
@@ -34,6 +36,13 @@ namespace {
 
 typedef double f64x4_t __attribute__((ext_vector_type(4)));
 SMEL_DEV f64x4_t mfma64(double a, double b, f64x4_t c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+
+// the binding packs a job as nine 8-byte values in this order
+static_assert(sizeof(smel_ortho_job) == 72 && offsetof(smel_ortho_job, x) == 0 && offsetof(smel_ortho_job, y) == 8 &&
+                  offsetof(smel_ortho_job, batch) == 16 && offsetof(smel_ortho_job, rows) == 24 && offsetof(smel_ortho_job, cols) == 32 &&
+                  offsetof(smel_ortho_job, x_batch) == 40 && offsetof(smel_ortho_job, x_row) == 48 &&
+                  offsetof(smel_ortho_job, x_col) == 56 && offsetof(smel_ortho_job, dtype) == 64,
+              "layout of a job");
 
 constexpr int MAX_R = 128;
 constexpr int MAX_JOBS = 36;   // of one launch: the jobs travel as kernel arguments (under 4 KiB)

@@ -116,6 +116,8 @@ def lora_gate_up(x, w_gate_up, A_gate, B_gate, A_up, B_up, scale):
 
 _ORTHO_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 ORTHO_MAX_RANK = 128   # of the shorter side
+# a smel_ortho_job (include/smel_ortho.h) as orthogonalize packs it: 8 bytes each
+_ORTHO_JOB = ("x", "y", "batch", "rows", "cols", "x_batch", "x_row", "x_col", "dtype")
 
 
 def _ortho_operand(t: torch.Tensor):
@@ -182,7 +184,7 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
                     keep.append(x)
                     add((x.data_ptr(), y.data_ptr(), *x.shape, *x.stride(), code))
             outs.append(y)
-        n = len(jobs) // 9
+        n = len(jobs) // len(_ORTHO_JOB)
         addr = jobs.buffer_info()[0]
         need = _lib.load().smel_orthogonalize_ws(addr, n, int(steps), a)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)

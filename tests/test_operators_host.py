@@ -100,3 +100,20 @@ def test_orthogonalize_workspace_of_steps():
         assert ws(13, 1.875) == ws(6) and ws(14, 1.875) == ws(7) and ws(64, 1.0) == ws(6)
         assert call(7, ws(7) - 1) == -1 and b"workspace" in L.smel_last_error()
         assert call(6, ws(6) - 1) == -1
+
+
+def test_job_fields_match_header():
+    """The fields of smel_ortho_job, by name and order, are those that the binding packs, each of 8 bytes."""
+    import os
+    import re
+    from smel import lora
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "smel_ortho.h")).read(), flags=re.S)
+    body = re.search(r"typedef struct smel_ortho_job \{(.*?)\} smel_ortho_job;", src, re.S).group(1)
+    fields = []
+    for line in body.split(";"):
+        if line.strip():
+            m = re.fullmatch(r"\s*(?:const\s+)?(void\s*\*|int64_t)\s*(.+?)\s*", line, re.S)
+            assert m, line      # pointers and int64_t alone: 8 bytes, without gaps
+            fields += [f.strip() for f in m.group(2).split(",")]
+    assert tuple(fields) == lora._ORTHO_JOB
