@@ -366,3 +366,24 @@ def test_layernorm_forward_mode_refused():
                         bad(lambda t: fw.make_dual(t, torch.ones_like(t)))
         plain = layernorm(x, w, None, EPS)      # without a tangent in the call
     assert torch.equal(plain, layernorm(x, w, None, EPS)) and not plain.requires_grad
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,n", [(7001, 1100), (14001, 520), (4700, 2056), (2500, 4104), (1100, 8200)])
+def test_layernorm_backward_many_turns(rows, n, dt):
+    """Rows enough that every block of the backward goes through its rows' buffers more than once, with a part of a turn at the
+    end: blocks of 256, 512 and 1024 threads, several rows a block and one, four, two and one on their way."""
+    from smel.norm import add_layernorm, layernorm
+    x, h, w, b, dy, ds = make(rows, n, DT[dt], DT[dt], rows + n)
+    xg, wg, bg = d(x), d(w), d(b)
+    gr = torch.autograd.grad(layernorm(xg, wg, bg, EPS), (xg, wg, bg), dy.to(DEV))
+    want = formula(x, w, b, dy)
+    for name, t in zip(("dx", "dw", "db"), gr):
+        close(t, want[name], name)
+    if n > 2000:
+        return
+    s64 = (h.float() + x.float()).to(x.dtype)
+    gr = torch.autograd.grad(add_layernorm(d(h), xg, wg, bg, EPS), (xg, wg, bg), (ds.to(DEV), dy.to(DEV)))
+    want = formula(s64, w, b, dy, ds)
+    for name, t in zip(("dx", "dw", "db"), gr):
+        close(t, want[name], name)
