@@ -15,7 +15,7 @@ extern "C" {
 
 /* `batch` matrices x[b][i][j] at x + b x_batch + i x_row + j x_col (elements; x_row or x_col is 1 where that side has
  * more than one element), dtype 0 = bf16, 1 = fp32, 2 = fp16; y: the same matrices, contiguous [batch][rows][cols], of
- * x's dtype. min(rows, cols) <= 128. y overlaps no x of the call. */
+ * x's dtype. min(rows, cols) <= 128, the longer side under 2^29 (2^30 up to a short side of 32). y overlaps no x of the call. */
 typedef struct smel_ortho_job {
   const void* x;
   void* y;

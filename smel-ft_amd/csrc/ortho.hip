@@ -1095,6 +1095,7 @@ struct Cursor {
   int64_t mat;
 };
 constexpr int64_t MAX_MATS = 65536, BIG_MATS = 256;   // of a launch; its workspace is 0.6 MB a matrix above r = 64
+constexpr int64_t MAX_PIECES = 1 << 21;               // of 128 columns: a launch takes fewer than 2^32 threads
 
 // the next jobs of one (tiles a side, dtype) from `at` on, as many as a launch takes (a job's batch may be split)
 Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Plan& p) {
@@ -1104,7 +1105,7 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
     int job;
     int64_t mat, count;
   } taken[MAX_JOBS];
-  int64_t cols = 0;
+  int64_t cols = 0, pieces = 0;
   const int64_t most = nt == 8 ? BIG_MATS : MAX_MATS;
   while (at.job < n && p.js.n < MAX_JOBS && p.mats < most) {
     const smel_ortho_job& j = jobs[at.job];
@@ -1113,7 +1114,10 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
       at = Cursor{at.job + 1, 0};
       continue;
     }
-    const int64_t take = j.batch - at.mat < most - p.mats ? j.batch - at.mat : most - p.mats;
+    const int64_t of_one = ((j.rows < j.cols ? j.cols : j.rows) + 127) / 128;
+    if (pieces && pieces + of_one > MAX_PIECES) break;
+    const int64_t take = std::min({j.batch - at.mat, most - p.mats, std::max<int64_t>((MAX_PIECES - pieces) / of_one, 1)});
+    pieces += take * of_one;
     taken[p.js.n++] = Taken{at.job, at.mat, take};
     p.mats += take;
     cols += take * (j.rows < j.cols ? j.cols : j.rows);
@@ -1172,7 +1176,7 @@ Cursor fill(const smel_ortho_job* jobs, int32_t n, Cursor at, int nt, int dt, Pl
     mats += o.batch;
     p.blocks += (int64_t)o.batch * o.slices;
     p.gblocks += (int64_t)o.batch * o.parts;
-    if (p.blocks >= (int64_t)1 << 22) return Cursor{-1, 0};   // 768 threads each at most: a launch takes fewer than 2^32
+    if (p.blocks >= (int64_t)1 << 22) return Cursor{-1, 0};   // one matrix of 2^29 columns or more, r > 32
   }
   return at;
 }
@@ -1305,7 +1309,7 @@ int each(const smel_ortho_job* jobs, int32_t n, F f) {
       for (Cursor at{0, 0}; any[nt][dt] && at.job < n;) {
         Plan p;
         at = fill(jobs, n, at, nt, dt, p);
-        SMEL_REQUIRE(at.job >= 0, SMEL_EUNSUPPORTED, "orthogonalize: too many columns in one call");
+        SMEL_REQUIRE(at.job >= 0, SMEL_EUNSUPPORTED, "orthogonalize: a matrix has too many columns for one launch");
         if (p.js.n == 0) continue;
         const int rc = f(p, nt, dt);
         if (rc) return rc;

@@ -69,3 +69,13 @@ def test_layer_of_updates(dt):
     ts = [make(s, dt, i) for i, s in enumerate(shapes)]
     for t, y in zip(ts, orthogonalize([t.to(DEV) for t in ts])):
         close(y, t, tuple(t.shape))
+
+
+def test_columns_of_several_launches():
+    """2^32 columns in one call, from one row read 65536 times."""
+    from smel.lora import orthogonalize
+    row = make((1, 1, 65536), "bf16", 3)
+    y = orthogonalize(row.to(DEV).expand(65536, 1, 65536))
+    for k in (0, 4095, 4096, 32767, 32768, 65535):
+        close(y[k], row[0], k)
+    assert torch.equal(y[1:].amin(0), y[0]) and torch.equal(y[1:].amax(0), y[0])

@@ -117,3 +117,15 @@ def test_job_fields_match_header():
             assert m, line      # pointers and int64_t alone: 8 bytes, without gaps
             fields += [f.strip() for f in m.group(2).split(",")]
     assert tuple(fields) == lora._ORTHO_JOB
+
+
+def test_orthogonalize_takes_many_columns():
+    """Columns beyond what a launch's grid takes are split over launches, not refused; a side of 2^30 is the limit."""
+    from array import array
+    L = _L()
+
+    def ws(batch, rows, cols, dt=0):
+        job = array("q", (16, 16, batch, rows, cols, rows * cols, cols, 1, dt))
+        return L.smel_orthogonalize_ws(job.buffer_info()[0], 1, 5, 3.4445)
+    assert 0 < ws(65536, 1, 65536) and 0 < ws(1 << 20, 1 << 14, 3) and 0 < ws(256, 128, 1 << 21) and 0 < ws(3, 64, (1 << 29) + 1, 1)
+    assert 0 < ws(1, 16, (1 << 30) - 1) and ws(1, 16, 1 << 30) == -1
