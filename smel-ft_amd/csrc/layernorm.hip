@@ -3,7 +3,7 @@
 //   dw = sum over rows of dy xhat,  db = sum over rows of dy
 // and the norm after a residual add, s = round(h + x). fp32 math, one rounding per output. The variance is the mean of
 // the squared distances from the mean (the row is in registers, so a second sum over it costs no bytes): a row whose mean
-// is large against its spread loses nothing to cancellation.
+// is large against its spread loses the mean's own fp32 rounding, not the cancellation of two squares.
 //
 // Layout: a row is split into chunks of 8 elements and belongs to `lpr` threads (a power of two up to 64, or the whole
 // block); thread i of a row takes chunks i, i + lpr, .... Chunks are read and written as 16-byte accesses of element
@@ -14,8 +14,8 @@
 // registers and four rows (16-bit) on their way; the block's row groups are joined through LDS in a tree, the blocks' sums go
 // to the workspace and a second kernel adds them in block order. No atomics: every result repeats bit for bit. A chunk per
 // thread and a block per row, not a wave per row with four chunks: 209 registers there let two waves on a SIMD and every row
-// read the weights twice more (32749 x 2048 bf16: 119 us; a block per row 108, with four rows on their way 91).
-// HBM-bound: forward 4.9 TB/s, backward 4.4 TB/s at 32749 x 2048 bf16 (a copy reaches 5.55).
+// read the weights twice more (32749 x 2048 bf16: 119 us; a block per row 108, with four rows on their way 91; with nontemporal stores 87).
+// HBM-bound: forward 4.7 TB/s, backward 4.6 TB/s at 32749 x 2048 bf16 (a copy reaches 5.55).
 #include "../../include/smel_norm.h"
 #include "abi_util.h"
 #include "common.h"
@@ -104,8 +104,8 @@ SMEL_DEV Raw<DT> load8(const typename El<DT>::T* p, int e0, int n) {
   }
   return r;
 }
-// Nontemporal: the rows written are more than an L2 holds, and what is read again is the rows (32749 x 2048 bf16: forward 55.1 ->
-// 54.0 us, backward 87.2 -> 81.4; 4092 x 2048 with the add: 33.7 -> 31.0 both). KEEP: what the next kernel reads, the weights' sums
+// Nontemporal: the rows written are more than an L2 holds, and what is read again is the rows (32749 x 2048 bf16: forward 57.9 ->
+// 56.7 us, backward 92.6 -> 87.2; 4092 x 2048 with the add: 15.3 -> 14.4 and 18.9 -> 18.7). KEEP: what the next kernel reads, the weights' sums
 template <int DT, bool KEEP = false>
 SMEL_DEV void store8(typename El<DT>::T* p, int e0, int n, const Raw<DT>& r) {
   if (e0 + 8 <= n) {
@@ -409,7 +409,7 @@ struct Shape {
   int lpr, cpl, bs;
 };
 // Forward. Rows of 513 to 2048 columns: a wave each, whose four chunks a lane hide the latency without a barrier, or, where
-// there are under 4096 of them, a block each (23 x 2048: 5.6 -> 4.4 us; 32749 rows: 79 us, a wave each 55)
+// there are under 4096 of them, a block each (23 x 2048: 5.6 -> 4.4 us; 32749 rows: 79 us, a wave each 56)
 Shape fwd_shape(int64_t rows, int64_t cols) {
   const int nch = (int)((cols + 7) / 8);   // <= 2048
   Shape s{1, 1, 256};
@@ -432,8 +432,8 @@ Shape bwd_shape(int64_t cols) {
 int64_t bwd_blocks(int64_t rows, int64_t cols) {
   const Shape s = bwd_shape(cols);
   const int64_t turns = (rows + s.bs / s.lpr - 1) / (s.bs / s.lpr);
-  // three blocks a CU of 256 threads, two of 512, one of 1024, with two rows each at least. 32749 x 2048 bf16: 114 us with 512
-  // blocks, 93 with 768, 93 with 1024 (and 1 us more for their sums); 4092 x 2816 fp32: 36 with 384, 33 with 512, 44 with 640
+  // three blocks a CU of 256 threads, two of 512, one of 1024, with two rows each at least. 32749 x 2048 bf16: 112 us with 512
+  // blocks, 87 with 768, 79 with 1024 (and 0.7 us more for their sums; 4092 x 2048 with the add 18.7 and 4.5 with 768, 18.4 and 5.4); 4092 x 2816 fp32: 36 with 384, 33 with 512, 44 with 640
   const int64_t most = s.bs == 256 ? 768 : s.bs == 512 ? 512 : 256, g = (turns + 1) / 2;
   return g < most ? g : most;
 }
