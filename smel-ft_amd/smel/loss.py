@@ -402,9 +402,13 @@ def _balance_check(logits, topi, mask, offsets):
         L.one_device(logits, topi, mask, offsets)
 
 
+_KEPT_WS = 1 << 20     # bytes
+
+
 def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
     """(loss, counts, what the backward takes). One allocation holds the backward's rows (16 bytes a token), its weights
-    and the workspace: a short batch is the host's time, and each allocation costs it as much as half a launch."""
+    and a workspace of up to 1 MB: a short batch is the host's time, and each allocation costs it as much as half a launch. A larger
+    workspace is one of its own, which does not outlive the call (131072 tokens in 4096 sequences: 10 MB)."""
     T, E = z.shape
     if not z.is_contiguous() and (E > 1 and z.stride(1) != 1 or T > 1 and z.stride(0) < E):
         z = z.contiguous()
@@ -414,7 +418,12 @@ def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
     rows_n = 16 * T if need_grad else 0
     weights_n = (4 * (S * E + 1) + 15) & ~15
     ws_n = L.load().smel_balance_ws_bytes(T, E, S)
-    mem = z.new_empty(rows_n + weights_n + ws_n, dtype=torch.uint8)
+    if ws_n <= _KEPT_WS:
+        mem = z.new_empty(rows_n + weights_n + ws_n, dtype=torch.uint8)
+        ws = mem.data_ptr() + rows_n + weights_n
+    else:
+        mem, own = z.new_empty(rows_n + weights_n, dtype=torch.uint8), z.new_empty(ws_n, dtype=torch.uint8)
+        ws = own.data_ptr()
     rows = mem.data_ptr()
     weights = rows + rows_n
     loss = z.new_empty((), dtype=torch.float32)
@@ -427,7 +436,7 @@ def _balance_forward(z, topi, mask, off, coef: float, need_grad: bool):
     dt = _DT[z.dtype]
     L.call("smel_balance_fwd", z.data_ptr(), ldl, dt, topi.data_ptr(), topi.dtype is torch.int64, T, E, topi.shape[1],
            p(mask), p(off), off is not None and off.dtype is torch.int64, S, coef, loss.data_ptr(), counts.data_ptr(),
-           rows if need_grad else None, weights, weights + weights_n, ws_n, L.stream())
+           rows if need_grad else None, weights, ws, ws_n, L.stream())
     return loss, counts, (z, mem, dt, T, E, S, rows_n)
 
 

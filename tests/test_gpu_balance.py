@@ -396,3 +396,26 @@ def test_balance_run_of_empty_sequences(run):
     assert torch.equal(counts[used].cpu(), wc) and counts.sum().item() == 250 * K
     assert ((dz.cpu().double() - wz).abs() <= U * wz.abs() + err).all()
     assert min(ms) < 100, ms      # 227 with a walk of 2^20 trips to memory, 10 without
+
+
+@pytest.mark.parametrize("T,S", [(131072, 4096), (65536, 0)])
+def test_balance_keeps_what_the_backward_reads(T, S):
+    """Between forward and backward: 16 bytes a token, the weights of each sequence's experts, under 1 MB of the workspace, and the
+    results; not the slots of the sums (16 MB in the first case)."""
+    from smel.loss import balance_loss
+    E, K = 256, 2
+    z = torch.randn(T, E, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16().requires_grad_(True)
+    topi = z.detach().float().topk(K, dim=1).indices
+    off = torch.arange(0, T + 1, T // S, device=DEV) if S else None
+    warm = balance_loss(z, topi, offsets=off)
+    ref, = torch.autograd.grad(warm[0], z)
+    del warm
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss, counts = balance_loss(z, topi, offsets=off)
+    kept = torch.cuda.memory_allocated() - before
+    results = 8 * max(S, 1) * E + 4
+    assert kept <= 16 * T + 4 * (max(S, 1) * E + 1) + results + (1 << 20) + 4096, kept
+    # what the workspace's memory holds by then does not matter
+    torch.empty(64 << 20, dtype=torch.uint8, device=DEV).fill_(255)
+    assert torch.equal(torch.autograd.grad(loss, z)[0], ref)
