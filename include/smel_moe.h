@@ -407,6 +407,32 @@ int smel_lora_wgrad(const smel_wg_job* jobs, int32_t n_jobs, const int32_t* lora
                     const int32_t* order, const float* topv, const float* sgate, int64_t max_rows, float* ws,
                     int64_t ws_floats, hipStream_t stream);
 
+/* Router logits alone: logits[t][e] = bf16(x[t] . gate_w[e]) at a row stride of smel_route_ld(E, 0) elements (columns from E
+ * on are zero). x [T][H], gate_w [E][H] bf16, H a multiple of 64, E <= 512. */
+int smel_router_logits(const uint16_t* x, const uint16_t* gate_w, int64_t T, int64_t H, int64_t E, uint16_t* logits,
+                       hipStream_t stream);
+
+/* The choice of K experts for each token from its logits z [T][E] (row stride ldl; dtype 0 bf16, 1 fp16, 2 fp32), all in fp32:
+ *   s = sigmoid(z) (score 0) or softmax(z) (score 1);  c = s + bias (fp32 [E], may be null)
+ *   groups > 1: the E experts are `groups` runs of E / groups neighbours; a group counts with the sum of its group_best (1 or 2)
+ *   largest c, and only the top_groups best groups' experts can be picked
+ *   topi [T][K]: the K largest c, descending (equal ones, and equal groups: the lower index first; a NaN counts as -infinity)
+ *   topv [T][K]: w_k = scale s_k / (sum of the K + 1e-20) (renorm) or scale s_k, s_k = s[topi_k] without the bias
+ * The ids are always K different ones of [0, E), whatever the logits hold. A softmax row without a logit above -infinity has
+ * scores 0. scores (may be null): s [T][E]. stats (may be null; softmax with a backward): a row's maximum and 1 / sum, [T][2].
+ * E <= 512, K <= 16, groups <= 64, E % groups == 0, K <= top_groups E / groups, T <= 2^25. */
+int smel_select_experts(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t K, int32_t score,
+                        const float* bias, int64_t groups, int64_t top_groups, int32_t group_best, int32_t renorm, float scale,
+                        float* topv, int64_t* topi, float* scores, float* stats, hipStream_t stream);
+
+/* dlogits [T][ldd] (the logits' dtype, ldd >= E, zero from column E on) from dtopv [T][K] of smel_select_experts' topv; the picks are
+ * constants. ds_k = scale (d_k - sum_j d_j s_j / S) / S with S = sum of the K + 1e-20 (renorm) or scale d_k;
+ *   sigmoid: dz = ds_k s (1 - s) at the picks, 0 elsewhere;  softmax: dz_e = s_e (ds_e - sum_k ds_k s_k)
+ * An id outside [0, E) counts nowhere. stats: smel_select_experts' (softmax; null otherwise). */
+int smel_select_experts_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t K, int32_t score,
+                            int32_t renorm, float scale, const int64_t* topi, const float* dtopv, const float* stats,
+                            void* dlogits, int64_t ldd, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

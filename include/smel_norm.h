@@ -1,4 +1,4 @@
-/* C-ABI of the RMSNorm family around the MoE block and of layer norm (libsmel_moe.so, HIP for gfx950).
+/* C-ABI of the RMSNorm family around the MoE block, of layer norm and of the norms around a residual add (libsmel_moe.so, HIP for gfx950).
  *
  * Same conventions as smel_moe.h: raw device pointers, element counts and strides in elements, 0 on success or an
  * SMEL_E* / hipError_t code with the message in smel_last_error(), every kernel on `stream`, no allocation, no host
@@ -64,6 +64,33 @@ int64_t smel_layernorm_bwd_ws_floats(int64_t rows, int64_t cols);
 int smel_layernorm_bwd(const void* dy, const void* x, int64_t rows, int64_t cols, int64_t x_stride, const void* w,
                        const float* stats, const void* ds, int32_t dtype, int32_t wtype, void* dx, void* dw, void* db,
                        float* ws, int64_t ws_floats, hipStream_t stream);
+
+/* The norm behind a block, its gate, the residual add, the residual scale and the norm before the next block:
+ *   n = x r1 w1',  s = round(scale (h + g n)),  y = s r2 w2'        r1, r2 = 1 / sqrt(mean of squares + eps) of x and of s
+ * One call's arguments; fields that a call does not have are null or 0. Rows of `dtype` (0 bf16, 1 fp16, 2 fp32), 1 <= cols <= 16384;
+ * x, h at row strides x_stride, h_stride, everything else contiguous; any element alignment. w1, w2 (null: 1) and a gate per channel
+ * of `wtype` (the rows' dtype or 2); w' = 1 + w where plus_one. pre: with y (0: s alone). gate_kind 0 none, 1 [cols], 2 [rows] (of
+ * gate_type: the rows' dtype or 2), 3 [rows][cols] (the rows' dtype); gate_act 1: g = sigmoid(gate), 0: g = gate. The scale is
+ * scale_value, or the element at `scale` (of scale_type: the rows' dtype or 2). stats [rows][2]: r1, r2, written forward, read backward.
+ * Backward: dS = ds + r2 (q - shat mean(q shat)), q = dy w2', shat = s r2; dh = scale dS; dn = dh g;
+ *   dx = r1 (q1 - xhat mean(q1 xhat)), q1 = dn w1', xhat = x r1; dw1 = sum_r dn xhat, dw2 = sum_r dy shat;
+ *   dgate = dh n (times g (1 - g)), summed over what the gate is broadcast over; dscale = sum of dS (h + g n)
+ * ds, dy: either may be null; dy null: as without pre. dx, dh, dw1, dw2, dgate, dscale: each may be null (not computed); h is read for
+ * dscale alone. Sums in fp32 (dscale's in 64 bits) in a fixed
+ * order, one rounding per output. */
+typedef struct smel_sandwich {
+  const void *h, *x, *w1, *w2, *gate, *scale, *ds, *dy;
+  void *s, *y, *dh, *dx, *dw1, *dw2, *dgate, *dscale;
+  float* stats;
+  int64_t rows, cols, x_stride, h_stride;
+  float eps, scale_value;
+  int32_t dtype, wtype, gate_kind, gate_type, gate_act, scale_type, plus_one, pre;
+} smel_sandwich;
+
+int smel_sandwich_fwd(const smel_sandwich* call, hipStream_t stream);
+/* Floats of the workspace (8-byte aligned) of smel_sandwich_bwd for this call (0 where it needs none). */
+int64_t smel_sandwich_bwd_ws_floats(const smel_sandwich* call);
+int smel_sandwich_bwd(const smel_sandwich* call, float* ws, int64_t ws_floats, hipStream_t stream);
 
 #ifdef __cplusplus
 }

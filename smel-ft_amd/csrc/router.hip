@@ -524,6 +524,18 @@ extern "C" int smel_route_counted(const uint16_t* x, const uint16_t* gate_w, con
                     stream);
 }
 
+extern "C" int smel_router_logits(const uint16_t* x, const uint16_t* gate_w, int64_t T, int64_t H, int64_t E,
+                                  uint16_t* logits, hipStream_t stream) {
+  SMEL_REQUIRE(T >= 0 && H > 0 && E > 0, SMEL_EINVAL, "router_logits: bad sizes");
+  SMEL_REQUIRE(E <= MAXE, SMEL_EUNSUPPORTED, "router_logits: E=%lld > %d experts", (long long)E, MAXE);
+  SMEL_REQUIRE(H % 64 == 0, SMEL_EUNSUPPORTED, "router_logits: hidden %lld must be a multiple of 64", (long long)H);
+  SMEL_REQUIRE(T * H * 2 < (1ll << 31), SMEL_EUNSUPPORTED, "router_logits: x larger than 2 GiB");
+  if (T == 0) return 0;
+  SMEL_REQUIRE(x && gate_w && logits, SMEL_EINVAL, "router_logits: null pointer");
+  launch_logits(stream, x, gate_w, nullptr, (int)T, (int)H, (int)E, (int)smel_route_ld(E, 0), logits);
+  return smel::launch_status();
+}
+
 extern "C" int smel_route_logits(const uint16_t* logits, int64_t T, int64_t E, int64_t K, float* probs,
                                  uint16_t* topv, int64_t* topi, int32_t* topi32, hipStream_t stream) {
   SMEL_REQUIRE(T >= 0 && E > 0 && K > 0, SMEL_EINVAL, "route_logits: bad sizes");

@@ -1,0 +1,481 @@
+// The norm behind a block, its gate, the residual add and scale, and the norm before the next block, forward and backward:
+//   n = x r1 w1',  u = h + g n,  s = round(scale u),  y = s r2 w2'          (r1, r2: 1 / root mean square of x and of s)
+//   dS = ds + r2 (q - shat mean(q shat)), q = dy w2';  dh = scale dS;  dn = dh g;  dx = r1 (q1 - xhat mean(q1 xhat)), q1 = dn w1'
+//   dw1 = sum dn xhat, dw2 = sum dy shat, dgate = dh n (g'), dscale = sum dS u
+// fp32 math, one rounding per output; y is the norm of the rounded s, as the next block reads it.
+//
+// Both row sums of the backward are taken in one reduction: with e = ds + r2 q, v = g w1' xhat and m2 = mean(q shat),
+//   sum(v dS) = sum(v e) - r2 m2 sum(v shat)
+// so a row costs one barrier. A gate per token and the scale are factors of the whole row: they stay outside the sums.
+//
+// Layout: rows.h's chunks of 8, `lpr` threads a row (a power of two up to 64, or the block). Blocks of the backward walk over
+// the rows, the weights and their sums in registers; the blocks' sums are added by a second launch in block order.
+#include "../../include/smel_norm.h"
+#include "abi_util.h"
+#include "common.h"
+#include "rows.h"
+
+namespace {
+
+constexpr int MAX_COLS = 16384;
+enum { G_NONE = 0, G_CHANNEL = 1, G_TOKEN = 2, G_FULL = 3 };
+
+SMEL_DEV float gate_of(float z, int act) { return act ? 1.f / (1.f + expf(-z)) : z; }
+// dg/dz from z: s (1 - s) without the subtraction's loss
+SMEL_DEV float gate_slope(float z, int act) {
+  if (!act) return 1.f;
+  const float q = expf(-fabsf(z)), a = 1.f / (1.f + q);
+  return q * a * a;
+}
+// element i of rows' type DT, or of fp32
+template <int DT>
+SMEL_DEV float one_at(const void* p, int64_t i, bool f32) {
+  if (DT == 2 || f32) return ((const float*)p)[i];
+  if constexpr (DT != 2) return cvt<DT>(((const uint16_t*)p)[i]);
+  return 0.f;
+}
+
+struct SwArgs {
+  smel_sandwich c;
+  float* part;      // [blocks][nsum cols], then (8-byte aligned) a double a block for dscale
+  int lpr, nsum, at1, at2, atg;   // sums of a column: their number and places (-1: not wanted)
+};
+
+SMEL_DEV double* scale_parts(const SwArgs& a, int64_t blocks) {
+  return (double*)(a.part + ((blocks * a.nsum * a.c.cols + 1) & ~(int64_t)1));
+}
+SMEL_DEV double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// w' of a chunk
+template <int WT>
+SMEL_DEV void norm_weight8(const void* p, int e0, int n, int plus_one, float v[8]) {
+  weight8<WT>(p, e0, n, 1.f, v);
+  if (plus_one && p)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += 1.f;
+}
+
+template <int DT, int WT, int CPL, int BS>
+__global__ __launch_bounds__(BS) void sandwich_fwd_kernel(SwArgs a) {
+  typedef typename El<DT>::T T;
+  __shared__ float red[2][16];
+  const smel_sandwich& p = a.c;
+  const int lpr = a.lpr, n = (int)p.cols, nch = (n + 7) >> 3;
+  const int64_t row = (int64_t)blockIdx.x * (BS / lpr) + threadIdx.x / lpr;
+  const int li = threadIdx.x & (lpr - 1);
+  const bool live = row < p.rows;
+  const int64_t r = live ? row : 0, out = r * (int64_t)n;
+  Raw<DT> X[CPL], H[CPL], G[CPL];
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) {
+    const int ck = li + lpr * k;
+    X[k] = H[k] = G[k] = Raw<DT>{};
+    if (live && ck < nch) {
+      X[k] = load8<DT>((const T*)p.x + r * p.x_stride, 8 * ck, n);
+      H[k] = load8<DT>((const T*)p.h + r * p.h_stride, 8 * ck, n);
+      if (p.gate_kind == G_FULL) G[k] = load8<DT>((const T*)p.gate + out, 8 * ck, n);
+    }
+  }
+  const float scale = p.scale ? one_at<DT>(p.scale, 0, p.scale_type == 2) : p.scale_value;
+  const float tg = p.gate_kind == G_TOKEN ? gate_of(one_at<DT>(p.gate, r, p.gate_type == 2), p.gate_act) : 1.f;
+  float ss[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < CPL; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss[0] = fmaf(X[k].at(j), X[k].at(j), ss[0]);   // zero past the row
+  row_sums(ss, lpr, red[0]);
+  const float r1 = 1.f / sqrtf(ss[0] / (float)n + p.eps);
+  ss[0] = 0.f;
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) {
+    const int ck = li + lpr * k;
+    if (!live || ck >= nch) continue;
+    float w[8], g[8], v[8];
+    norm_weight8<WT>(p.w1, 8 * ck, n, p.plus_one, w);
+    if (p.gate_kind == G_CHANNEL) {
+      weight8<WT>(p.gate, 8 * ck, n, 1.f, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = gate_of(g[j], p.gate_act);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = p.gate_kind == G_FULL ? gate_of(G[k].at(j), p.gate_act) : tg;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = scale * fmaf(g[j], X[k].at(j) * r1 * w[j], H[k].at(j));
+    H[k].set(v);
+    store8<DT>((T*)p.s + out, 8 * ck, n, H[k]);
+    if (p.pre)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (8 * ck + j < n) ss[0] = fmaf(H[k].at(j), H[k].at(j), ss[0]);
+  }
+  float r2 = 0.f;
+  if (p.pre) {
+    row_sums(ss, lpr, red[1]);
+    r2 = 1.f / sqrtf(ss[0] / (float)n + p.eps);
+  }
+  if (!live) return;
+  if (li == 0) {
+    p.stats[2 * row] = r1;
+    p.stats[2 * row + 1] = r2;
+  }
+  if (!p.pre) return;
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) {
+    const int ck = li + lpr * k;
+    if (ck >= nch) continue;
+    float w[8], v[8];
+    norm_weight8<WT>(p.w2, 8 * ck, n, p.plus_one, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = H[k].at(j) * r2 * w[j];
+    Raw<DT> o;
+    o.set(v);
+    store8<DT>((T*)p.y + out, 8 * ck, n, o);
+  }
+}
+
+template <int DT, int WT, int CPL, int BS, bool WG>
+__global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
+  typedef typename El<DT>::T T;
+  __shared__ float red[2][48];
+  __shared__ float join[WG && BS == 256 ? BS / 2 * CPL * 24 : 1];   // larger blocks are one row's
+  __shared__ double joins[16];
+  const smel_sandwich& p = a.c;
+  const int lpr = a.lpr, n = (int)p.cols, nch = (n + 7) >> 3;
+  const int groups = BS / lpr, grp = threadIdx.x / lpr, li = threadIdx.x & (lpr - 1);
+  const bool pre = p.dy != nullptr;
+  const float scale = p.scale ? one_at<DT>(p.scale, 0, p.scale_type == 2) : p.scale_value;
+  float sums[WG ? CPL * 24 : 1];   // of a chunk's columns: dw1, dw2, dgate
+  double usum = 0;                 // of dS u: its terms cancel, and a block has thousands of them
+  if constexpr (WG)
+#pragma unroll
+    for (int i = 0; i < CPL * 24; ++i) sums[i] = 0.f;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  // every thread of the block takes the same number of turns (row_sums has a barrier); the sums' buffers alternate: a row's
+  // readers are done before the next but one writes
+  int par = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < p.rows; r0 += step, par ^= 1) {
+    const int64_t row = r0 + grp;
+    const bool live = row < p.rows;
+    const int64_t r = live ? row : 0, out = r * (int64_t)n;
+    Raw<DT> X[CPL], S[CPL], D[CPL], Y[CPL], G[CPL];
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {
+      const int ck = li + lpr * k;
+      X[k] = S[k] = D[k] = Y[k] = G[k] = Raw<DT>{};
+      if (live && ck < nch) {
+        X[k] = load8<DT>((const T*)p.x + r * p.x_stride, 8 * ck, n);
+        if (p.ds) D[k] = load8<DT>((const T*)p.ds + out, 8 * ck, n);
+        if (pre) {
+          S[k] = load8<DT>((const T*)p.s + out, 8 * ck, n);
+          Y[k] = load8<DT>((const T*)p.dy + out, 8 * ck, n);
+        }
+        if (p.gate_kind == G_FULL) G[k] = load8<DT>((const T*)p.gate + out, 8 * ck, n);
+      }
+    }
+    const float r1 = live ? p.stats[2 * row] : 0.f, r2 = live && pre ? p.stats[2 * row + 1] : 0.f;
+    const float tz = p.gate_kind == G_TOKEN && live ? one_at<DT>(p.gate, row, p.gate_type == 2) : 0.f;
+    const float tg = p.gate_kind == G_TOKEN ? gate_of(tz, p.gate_act) : 1.f;
+    float abc[3] = {0.f, 0.f, 0.f};
+    float w1[8], w2[8], g[8];
+    auto weights = [&](int k) {   // of chunk k; g: the gate's value but a token's
+      const int ck = li + lpr * k;
+      norm_weight8<WT>(ck < nch ? p.w1 : nullptr, 8 * ck, n, p.plus_one, w1);
+      if (pre) norm_weight8<WT>(ck < nch ? p.w2 : nullptr, 8 * ck, n, p.plus_one, w2);
+      else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w2[j] = 0.f;
+      if (p.gate_kind == G_CHANNEL) weight8<WT>(ck < nch ? p.gate : nullptr, 8 * ck, n, 1.f, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        g[j] = p.gate_kind == G_CHANNEL ? gate_of(g[j], p.gate_act) : p.gate_kind == G_FULL ? gate_of(G[k].at(j), p.gate_act) : 1.f;
+    };
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {
+      weights(k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {   // x and s are zero past the row and past the last row
+        const float q = Y[k].at(j) * w2[j], sh = S[k].at(j) * r2, v = g[j] * w1[j] * (X[k].at(j) * r1);
+        abc[0] = fmaf(q, sh, abc[0]);
+        abc[1] = fmaf(v, fmaf(r2, q, D[k].at(j)), abc[1]);
+        abc[2] = fmaf(v, sh, abc[2]);
+      }
+    }
+    row_sums(abc, lpr, red[par]);
+    const float m2 = r2 * (abc[0] / (float)n), vd = scale * (abc[1] - m2 * abc[2]);   // vd = sum of dh w1' xhat (g)
+    const float m1 = tg * vd / (float)n;
+    if (!live) continue;
+    if (p.gate_kind == G_TOKEN && p.dgate && li == 0) {
+      const float d = vd * gate_slope(tz, p.gate_act);
+      if (DT == 2 || p.gate_type == 2) ((float*)p.dgate)[row] = d;
+      else if constexpr (DT != 2) ((T*)p.dgate)[row] = (T)enc<DT>(d);
+    }
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {
+      const int ck = li + lpr * k;
+      if (ck >= nch) continue;
+      weights(k);
+      float dh[8], dx[8], dg[8], u[8], us = 0.f;
+      if (p.dscale) {
+        const Raw<DT> H = load8<DT>((const T*)p.h + r * p.h_stride, 8 * ck, n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = H.at(j);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float sh = S[k].at(j) * r2, xh = X[k].at(j) * r1;
+        const float ds = fmaf(r2, Y[k].at(j) * w2[j], D[k].at(j)) - m2 * sh;
+        dh[j] = scale * ds;
+        const float dn = dh[j] * g[j] * tg;
+        dx[j] = r1 * (dn * w1[j] - xh * m1);
+        dg[j] = dh[j] * xh * w1[j];
+        if (p.dscale && 8 * ck + j < n) us = fmaf(ds, fmaf(g[j] * tg, xh * w1[j], u[j]), us);
+        if constexpr (WG) {
+          sums[k * 24 + j] = fmaf(dn, xh, sums[k * 24 + j]);
+          sums[k * 24 + 8 + j] = fmaf(Y[k].at(j), sh, sums[k * 24 + 8 + j]);
+          sums[k * 24 + 16 + j] += dg[j];
+        }
+      }
+      usum += (double)us;
+      Raw<DT> o;
+      if (p.dh) {
+        o.set(dh);
+        store8<DT>((T*)p.dh + out, 8 * ck, n, o);
+      }
+      if (p.dx) {
+        o.set(dx);
+        store8<DT>((T*)p.dx + out, 8 * ck, n, o);
+      }
+      if (p.gate_kind == G_FULL && p.dgate) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dg[j] *= gate_slope(G[k].at(j), p.gate_act);
+        o.set(dg);
+        store8<DT>((T*)p.dgate + out, 8 * ck, n, o);
+      }
+    }
+  }
+  if (p.dscale) {   // the block's sum of dS u
+    usum = wave_sum64(usum);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) joins[threadIdx.x >> 6] = usum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < BS / 64; ++w) usum += joins[w];
+      scale_parts(a, gridDim.x)[blockIdx.x] = usum;
+    }
+  }
+  if constexpr (WG) {
+    for (int half = groups / 2; half >= 1; half /= 2) {
+      __syncthreads();
+      if (grp >= half && grp < 2 * half)
+#pragma unroll
+        for (int i = 0; i < CPL * 24; ++i) join[((grp - half) * lpr + li) * (CPL * 24) + i] = sums[i];
+      __syncthreads();
+      if (grp < half)
+#pragma unroll
+        for (int i = 0; i < CPL * 24; ++i) sums[i] += join[(grp * lpr + li) * (CPL * 24) + i];
+    }
+    if (grp == 0) {
+      float* const o = a.part + (int64_t)blockIdx.x * a.nsum * n;
+      const int at[3] = {a.at1, a.at2, a.atg};
+#pragma unroll
+      for (int k = 0; k < CPL; ++k) {
+        const int e = 8 * (li + lpr * k);
+        if (e >= n) continue;
+        if (p.gate_kind == G_CHANNEL && p.gate_act) {
+          float z[8];
+          weight8<WT>(p.gate, e, n, 1.f, z);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sums[k * 24 + 16 + j] *= gate_slope(z[j], 1);
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          if (at[i] < 0) continue;
+          Raw<2> v;
+          v.set(sums + k * 24 + 8 * i);
+          store8<2, true>(o + (int64_t)at[i] * n, e, n, v);
+        }
+      }
+    }
+  }
+}
+
+// columns of part [blocks][nsum n] summed: a wave's lanes take 64 columns, the 16 waves a 16th of the blocks each; the last block
+// adds the blocks' sums for dscale
+template <int DT, int WT>
+__global__ __launch_bounds__(1024) void sandwich_wsum_kernel(SwArgs a, int blocks) {
+  __shared__ float red[16][64];
+  const smel_sandwich& p = a.c;
+  const int n = (int)p.cols, cols = a.nsum * n, wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const int c = blockIdx.x * 64 + l;
+  const bool last = p.dscale && blockIdx.x == gridDim.x - 1;
+  if (last) {   // a wave's work
+    if (wave != 0) return;
+    const double* const u = scale_parts(a, blocks);
+    double v = 0;
+    for (int r = l; r < blocks; r += 64) v += u[r];
+    v = wave_sum64(v);
+    if (l != 0) return;
+    if (DT == 2 || p.scale_type == 2) ((float*)p.dscale)[0] = (float)v;
+    else if constexpr (DT != 2) ((uint16_t*)p.dscale)[0] = (uint16_t)enc<DT>((float)v);
+    return;
+  }
+  float v = 0.f;
+  if (c < cols)
+#pragma unroll 8
+    for (int r = wave; r < blocks; r += 16) v += a.part[(int64_t)r * cols + c];
+  red[wave][l] = v;
+  __syncthreads();
+  if (wave != 0 || c >= cols) return;
+  for (int k = 1; k < 16; ++k) v += red[k][l];
+  const int which = c / n, e = c - which * n;
+  void* const o = which == a.at1 ? p.dw1 : which == a.at2 ? p.dw2 : p.dgate;
+  if constexpr (WT == 2)
+    ((float*)o)[e] = v;
+  else
+    ((uint16_t*)o)[e] = (uint16_t)enc<WT>(v);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+struct Shape {
+  int lpr, cpl, bs;
+};
+Shape fwd_shape(int64_t cols) {
+  const int nch = (int)((cols + 7) / 8);   // <= 2048
+  Shape s{1, 1, 256};
+  while (s.lpr < nch && s.lpr < 64) s.lpr *= 2;
+  if (nch > 64) s.lpr = 256;
+  if (nch > 1024) s.lpr = s.bs = 1024;
+  while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 4
+  return s;
+}
+// a chunk per thread where 1024 threads reach
+Shape bwd_shape(int64_t cols) {
+  const int nch = (int)((cols + 7) / 8);
+  Shape s{1, 1, 256};
+  while (s.lpr < nch && s.lpr < 1024) s.lpr *= 2;
+  if (s.lpr > 256) s.bs = s.lpr;
+  while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 2
+  return s;
+}
+int64_t bwd_blocks(int64_t rows, int64_t cols) {
+  const Shape s = bwd_shape(cols);
+  const int64_t turns = (rows + s.bs / s.lpr - 1) / (s.bs / s.lpr);
+  const int64_t most = s.bs == 256 ? 768 : s.bs == 512 ? 512 : 256;
+  return turns < most ? turns : most;
+}
+
+template <int DT, int WT, int CPL, int BS>
+int launch_fwd(const SwArgs& a, hipStream_t stream) {
+  const int64_t rpb = BS / a.lpr, blocks = (a.c.rows + rpb - 1) / rpb;
+  SMEL_REQUIRE(blocks * BS < (int64_t)1 << 32, SMEL_EUNSUPPORTED, "sandwich_fwd: %lld rows is too many", (long long)a.c.rows);
+  sandwich_fwd_kernel<DT, WT, CPL, BS><<<(unsigned)blocks, BS, 0, stream>>>(a);
+  return smel::launch_status();
+}
+template <int DT, int WT, int CPL, int BS>
+int launch_bwd(const SwArgs& a, hipStream_t stream) {
+  const unsigned blocks = (unsigned)bwd_blocks(a.c.rows, a.c.cols);
+  if (a.nsum) sandwich_bwd_kernel<DT, WT, CPL, BS, true><<<blocks, BS, 0, stream>>>(a);
+  else sandwich_bwd_kernel<DT, WT, CPL, BS, false><<<blocks, BS, 0, stream>>>(a);
+  return smel::launch_status();
+}
+template <int DT, int WT>
+struct Launch {
+  static int fwd(SwArgs& a, hipStream_t st) {
+    const Shape s = fwd_shape(a.c.cols);
+    a.lpr = s.lpr;
+    if (s.bs == 1024) return launch_fwd<DT, WT, 2, 1024>(a, st);
+    return s.cpl == 1 ? launch_fwd<DT, WT, 1, 256>(a, st) : s.cpl == 2 ? launch_fwd<DT, WT, 2, 256>(a, st)
+                                                                       : launch_fwd<DT, WT, 4, 256>(a, st);
+  }
+  static int bwd(SwArgs& a, hipStream_t st) {
+    int64_t blocks = 0;
+    if (a.c.rows > 0) {
+      const Shape s = bwd_shape(a.c.cols);
+      a.lpr = s.lpr;
+      const int rc = s.bs == 256   ? launch_bwd<DT, WT, 1, 256>(a, st)
+                     : s.bs == 512 ? launch_bwd<DT, WT, 1, 512>(a, st)
+                     : s.cpl == 1  ? launch_bwd<DT, WT, 1, 1024>(a, st)
+                                   : launch_bwd<DT, WT, 2, 1024>(a, st);
+      if (rc) return rc;
+      blocks = bwd_blocks(a.c.rows, a.c.cols);
+    }
+    const int64_t wb = (a.nsum * a.c.cols + 63) / 64 + (a.c.dscale ? 1 : 0);
+    if (!wb) return 0;
+    sandwich_wsum_kernel<DT, WT><<<(unsigned)wb, 1024, 0, st>>>(a, (int)blocks);
+    return smel::launch_status();
+  }
+};
+template <typename F>
+int by_type(const smel_sandwich& c, F f) {
+  if (c.dtype == 2) return f(Launch<2, 2>());
+  if (c.dtype == 0) return c.wtype == 2 ? f(Launch<0, 2>()) : f(Launch<0, 0>());
+  return c.wtype == 2 ? f(Launch<1, 2>()) : f(Launch<1, 1>());
+}
+
+int check(const char* name, const smel_sandwich* c) {
+  SMEL_REQUIRE(c, SMEL_EINVAL, "%s: null call", name);
+  SMEL_REQUIRE(c->rows >= 0 && c->cols >= 1, SMEL_EINVAL, "%s: bad sizes rows=%lld cols=%lld", name, (long long)c->rows,
+               (long long)c->cols);
+  SMEL_REQUIRE(c->cols <= MAX_COLS, SMEL_EUNSUPPORTED, "%s: %lld columns, at most %d", name, (long long)c->cols, MAX_COLS);
+  SMEL_REQUIRE(c->rows <= 1 || (c->x_stride >= c->cols && (!c->h || c->h_stride >= c->cols)), SMEL_EINVAL,
+               "%s: row strides %lld, %lld < cols %lld", name, (long long)c->x_stride, (long long)c->h_stride, (long long)c->cols);
+  SMEL_REQUIRE(c->dtype >= 0 && c->dtype <= 2, SMEL_EINVAL, "%s: dtype %d (0 = bf16, 1 = fp16, 2 = fp32)", name, c->dtype);
+  SMEL_REQUIRE(c->wtype == c->dtype || c->wtype == 2, SMEL_EINVAL, "%s: weights of type %d with rows of type %d", name, c->wtype,
+               c->dtype);
+  SMEL_REQUIRE(c->gate_kind >= 0 && c->gate_kind <= 3 && (c->gate_kind == 0 || c->gate || c->rows == 0), SMEL_EINVAL,
+               "%s: gate kind %d", name, c->gate_kind);
+  SMEL_REQUIRE(c->gate_kind != G_TOKEN || c->gate_type == c->dtype || c->gate_type == 2, SMEL_EINVAL, "%s: gate of type %d", name,
+               c->gate_type);
+  SMEL_REQUIRE(!c->scale || c->scale_type == c->dtype || c->scale_type == 2, SMEL_EINVAL, "%s: scale of type %d", name, c->scale_type);
+  return 0;
+}
+void places(SwArgs& a) {
+  const bool on[3] = {a.c.dw1 != nullptr, a.c.dw2 != nullptr, a.c.dgate && a.c.gate_kind == G_CHANNEL};
+  int at[3];
+  for (int i = 0; i < 3; ++i) at[i] = on[i] ? a.nsum++ : -1;
+  a.at1 = at[0];
+  a.at2 = at[1];
+  a.atg = at[2];
+}
+
+}  // namespace
+
+extern "C" int smel_sandwich_fwd(const smel_sandwich* call, hipStream_t stream) {
+  const int rc = check("sandwich_fwd", call);
+  if (rc) return rc;
+  if (call->rows == 0) return 0;
+  SMEL_REQUIRE(call->x && call->h && call->s && call->stats && (!call->pre || call->y), SMEL_EINVAL, "sandwich_fwd: null pointer");
+  SwArgs a{};
+  a.c = *call;
+  return by_type(a.c, [&](auto l) { return decltype(l)::fwd(a, stream); });
+}
+
+extern "C" int64_t smel_sandwich_bwd_ws_floats(const smel_sandwich* call) {
+  if (check("sandwich_bwd", call) || call->rows == 0) return 0;
+  SwArgs a{};
+  a.c = *call;
+  places(a);
+  const int64_t blocks = bwd_blocks(a.c.rows, a.c.cols);
+  return blocks * a.nsum * a.c.cols + (a.c.dscale ? 2 * blocks + 1 : 0);
+}
+
+extern "C" int smel_sandwich_bwd(const smel_sandwich* call, float* ws, int64_t ws_floats, hipStream_t stream) {
+  const int rc = check("sandwich_bwd", call);
+  if (rc) return rc;
+  SMEL_REQUIRE(call->rows == 0 || (call->x && call->stats && (!call->dy || call->s) && (!call->dscale || call->h)), SMEL_EINVAL,
+               "sandwich_bwd: null pointer");
+  const int64_t need = smel_sandwich_bwd_ws_floats(call);
+  SMEL_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 8 == 0 && ws_floats >= need), SMEL_EINVAL,
+               "sandwich_bwd: an aligned workspace of %lld floats is needed (got %lld)", (long long)need, (long long)ws_floats);
+  SwArgs a{};
+  a.c = *call;
+  a.part = ws;
+  places(a);
+  return by_type(a.c, [&](auto l) { return decltype(l)::bwd(a, stream); });
+}

@@ -1,5 +1,5 @@
 """ctypes binding of libsmel_moe.so (the C-ABI declared in include/smel_moe.h, smel_f32.h, smel_norm.h, smel_stream.h,
-smel_loss.h and smel_ortho.h).
+smel_loss.h, smel_ortho.h and smel_clip.h).
 
 The library is the only compute path: if it is missing, or no GPU is visible, calls raise instead of falling back to
 anything else. Tensors go in as raw device pointers; every call runs on torch's current HIP stream.
@@ -26,7 +26,7 @@ WSET_MERGE_SHORT = 8 # smel_wset.flags: gate_up forward, a full int4 tile also t
 WSET_MERGED_LIST = 16 # smel_wset.flags: gate_up forward on smel_dispatch's merged tile list (int4 tiles up to 160 rows)
 WSET_TILE32 = 32     # smel_wset.flags: a tile list of at most 32 rows a tile
 WSET_COL_CHUNK = 64  # smel_wset.flags: column blocks, not tiles, are spread over the XCDs
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 vp, i64, i32, f32, f64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_double
 
@@ -80,6 +80,14 @@ class H2DRegion(ctypes.Structure):
     _fields_ = [("dst", vp), ("src", vp), ("bytes", i64)]
 
 
+class Sandwich(ctypes.Structure):
+    """smel_sandwich of include/smel_norm.h."""
+    _fields_ = [(n, vp) for n in ("h", "x", "w1", "w2", "gate", "scale", "ds", "dy", "s", "y", "dh", "dx", "dw1", "dw2", "dgate",
+                                  "dscale", "stats")] + \
+               [(n, i64) for n in ("rows", "cols", "x_stride", "h_stride")] + [("eps", f32), ("scale_value", f32)] + \
+               [(n, i32) for n in ("dtype", "wtype", "gate_kind", "gate_type", "gate_act", "scale_type", "plus_one", "pre")]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "smel_last_error": (ctypes.c_char_p, []),
@@ -97,6 +105,9 @@ SIGNATURES = {
     "smel_route_counted": (i32, [vp, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "smel_route_ld": (i64, [i64, i32]),
     "smel_route_logits": (i32, [vp, i64, i64, i64, vp, vp, vp, vp, vp]),
+    "smel_router_logits": (i32, [vp, vp, i64, i64, i64, vp, vp]),
+    "smel_select_experts": (i32, [vp, i64, i32, i64, i64, i64, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp, vp, vp]),
+    "smel_select_experts_bwd": (i32, [vp, i64, i32, i64, i64, i64, i32, i32, f32, vp, vp, vp, vp, i64, vp]),
     "smel_dispatch": (i32, [vp, i32, i64, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp]),
     "smel_dispatch_counted": (i32, [vp, i32, i64, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp,
                                     vp]),
@@ -151,6 +162,9 @@ SIGNATURES = {
     "smel_layernorm_fwd": (i32, [vp, vp, i64, i64, i64, vp, vp, f32, i32, i32, vp, vp, vp, vp]),
     "smel_layernorm_bwd_ws_floats": (i64, [i64, i64]),
     "smel_layernorm_bwd": (i32, [vp, vp, i64, i64, i64, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64, vp]),
+    "smel_sandwich_fwd": (i32, [ctypes.POINTER(Sandwich), vp]),
+    "smel_sandwich_bwd_ws_floats": (i64, [ctypes.POINTER(Sandwich)]),
+    "smel_sandwich_bwd": (i32, [ctypes.POINTER(Sandwich), vp, i64, vp]),
     # include/smel_stream.h
     "smel_event_create": (i32, [ctypes.POINTER(vp)]),
     "smel_event_destroy": (i32, [vp]),
@@ -177,6 +191,10 @@ SIGNATURES = {
     # include/smel_ortho.h
     "smel_orthogonalize_ws": (i64, [vp, i32, i32, f64]),
     "smel_orthogonalize": (i32, [vp, i32, i32, f64, f64, f64, f64, vp, i64, vp]),
+    # include/smel_clip.h
+    "smel_clip_ws": (i64, [vp, i32]),
+    "smel_grad_norm": (i32, [vp, i32, i32, vp, vp, i64, vp]),
+    "smel_clip_grads": (i32, [vp, i32, i32, f64, f64, vp, vp, i64, vp]),
     # include/smel_probe.h
     "smel_probe_mfma": (i32, [vp, i32, i32, vp]),
     "smel_probe_read": (i32, [vp, i64, vp, i32, vp]),

@@ -5,7 +5,8 @@ B [.., out, r] zero), so adapters written by either load into the other.
 
 The MoE layer never multiplies these factors in Python: smel.moe lays them out as a 32-wide K-extension of the
 grouped-GEMM kernels. ``lora_linear`` / ``lora_gate_up`` are the dense helpers of the API (torch ops);
-``orthogonalize`` makes the factors' updates orthogonal on the GPU (include/smel_ortho.h).
+``orthogonalize`` makes the factors' updates orthogonal on the GPU (include/smel_ortho.h), ``clip_grads`` scales the gradients
+down to a global norm (include/smel_clip.h).
 """
 from __future__ import annotations
 
@@ -190,6 +191,98 @@ def orthogonalize(update, steps: int = 5, coeffs=(3.4445, -4.7750, 2.0315), eps:
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         _lib.call("smel_orthogonalize", addr, n, int(steps), a, b, c, float(eps), ws.data_ptr(), need, _lib.stream())
     return outs[0] if single else outs
+
+
+# ------------------------------------------------------------------------------------------------ the gradients' norm
+
+_CLIP_JOB = ("in", "out", "n", "dtype")      # a smel_clip_job (include/smel_clip.h): 8 bytes each
+_NORM_TYPES = {2.0: 0, math.inf: 1}
+
+
+def _flat(t: torch.Tensor) -> bool:
+    """Whether t's values fill t.numel() elements of memory from its first on, in whatever order of dimensions."""
+    at = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def _clip_call(grads, max_norm, norm_type, eps, inplace):
+    """(the scaled tensors, the norm) of grads; max_norm None: the norm alone."""
+    what = "grad_norm" if max_norm is None else "clip_grads"
+    ts = (grads,) if isinstance(grads, torch.Tensor) else tuple(grads)
+    kind = _NORM_TYPES.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"{what} takes norm_type 2 or inf, got {norm_type}")
+    if max_norm is not None and not max_norm >= 0:
+        raise ValueError(f"{what}: max_norm must not be negative, got {max_norm}")
+    if not eps >= 0:
+        raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    first = next((t for t in ts if t is not None), None)
+    if first is None:
+        return list(ts), torch.zeros((), dtype=torch.float32)
+    if not first.is_cuda:
+        _lib.one_device(first)
+    jobs, outs, keep, back = array("q"), [], [], []
+    add, dev = jobs.extend, first.device
+    scaled = max_norm is not None
+    with torch.no_grad(), _lib.on_device_of(first):
+        for t in ts:     # a block has hundreds: what each costs here is the call's time
+            if t is None:
+                outs.append(None)
+                continue
+            code = _ORTHO_DTYPES.get(t.dtype)
+            if code is None or t.layout is not torch.strided:
+                raise ValueError(f"{what} takes bf16, fp16 or fp32 tensors, got {t.dtype} {t.layout}")
+            if t.device != dev:
+                _lib.one_device(first, t)
+            x = t
+            if not t.is_contiguous() and not _flat(t):
+                x = t.contiguous()
+                keep.append(x)
+                if inplace:
+                    back.append((t, x))
+            y = x if inplace or not scaled else torch.empty_like(x)
+            add((x.data_ptr(), y.data_ptr(), x.numel(), code))
+            outs.append(t if inplace else y)
+        n = len(jobs) // len(_CLIP_JOB)
+        addr = jobs.buffer_info()[0]
+        need = _lib.load().smel_clip_ws(addr, n)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        if scaled:
+            _lib.call("smel_clip_grads", addr, n, kind, float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                      _lib.stream())
+        else:
+            _lib.call("smel_grad_norm", addr, n, kind, norm.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream())
+        for t, x in back:
+            t.copy_(x)
+        if inplace:     # what autograd kept of them is out of date
+            torch.autograd.graph.increment_version([t for t in ts if t is not None])
+    return outs, norm
+
+
+def grad_norm(grads, norm_type: float = 2.0):
+    """The norm of all values of all tensors together (an fp32 scalar on their GPU; no host synchronisation): norm_type 2
+    (sums in 64 bits) or inf (the largest magnitude). ``grads``: a tensor or a sequence (bf16, fp16, fp32; None entries are passed
+    over). A NaN anywhere gives NaN."""
+    return _clip_call(grads, None, norm_type, 0.0, False)[1]
+
+
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6):
+    """(clipped, norm): every tensor times min(1, max_norm / (norm + eps)) with ``norm`` the norm of all of them together, as
+    ``grad_norm`` gives it; new tensors of the same shapes and dtypes, without gradients (None stays None), one tensor for one tensor.
+    A norm that is infinite or NaN gives what the product with that factor gives."""
+    outs, norm = _clip_call(grads, max_norm, norm_type, eps, False)
+    return (outs[0] if isinstance(grads, torch.Tensor) else outs), norm
+
+
+def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6):
+    """``clip_grads`` in place; returns the norm before. Tensors that are within the norm already are not written. The tensors must not
+    overlap (one given twice is refused)."""
+    return _clip_call(grads, max_norm, norm_type, eps, True)[1]
 
 
 class LayerLoRA(nn.Module):

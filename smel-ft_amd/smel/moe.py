@@ -26,6 +26,7 @@ from collections import OrderedDict
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import moe_f32 as F32
@@ -804,6 +805,151 @@ def route_gemma4(h, W, top_k, eps, with_logits=False):
                                        F32.f32(W["router.per_expert_scale"], "router.per_expert_scale").reshape(-1), k, eps, wl)
     return _RouteGemma4Fn.apply(_bf16(h), _bf16(W["router.scale"]).reshape(-1), _bf16(W["router.proj.weight"]),
                                 _bf16(W["router.per_expert_scale"]).reshape(-1), k, eps, wl)
+
+
+# ------------------------------------------------------------------------------------------------ chosen by scores, bias and groups
+
+_SCORES = {"sigmoid": 0, "softmax": 1}
+_SEL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _select_check(logits, top_k, score, bias, groups, top_groups, group_best):
+    if not logits.is_cuda:
+        L.one_device(logits)
+    if logits.dim() != 2 or logits.dtype not in _SEL_DTYPES:
+        raise ValueError(f"select_experts takes bf16, fp16 or fp32 logits [T, E], got {tuple(logits.shape)} {logits.dtype}")
+    E = logits.shape[1]
+    if score not in _SCORES:
+        raise ValueError(f"score is 'sigmoid' or 'softmax', got {score!r}")
+    if bias is not None:
+        if not bias.is_floating_point() or tuple(bias.shape) != (E,):
+            raise ValueError(f"select_experts takes a floating bias [{E}], got {tuple(bias.shape)} {bias.dtype}")
+        if bias.device != logits.device:
+            L.one_device(logits, bias)
+    if groups < 1 or E % groups:
+        raise ValueError(f"{E} experts make no {groups} groups of equal size")
+    if not 1 <= top_groups <= groups or not 1 <= top_k <= top_groups * (E // groups):
+        raise ValueError(f"{top_groups} of {groups} groups of {E // groups} experts give no {top_k} picks")
+    if group_best not in (1, 2):
+        raise ValueError(f"a group counts with its best 1 or 2, got {group_best}")
+
+
+def _select_forward(z, bias, k, score, groups, top_groups, best, renorm, scale, with_scores, train):
+    """(topv, topi, scores or None, what the backward takes)."""
+    T, E = z.shape
+    if not z.is_contiguous() and (E > 1 and z.stride(1) != 1 or T > 1 and z.stride(0) < E):
+        z = z.contiguous()
+    if bias is not None:
+        bias = bias.detach().to(torch.float32).contiguous()
+    topv = z.new_empty((T, k), dtype=torch.float32)
+    topi = z.new_empty((T, k), dtype=torch.int64)
+    scores = z.new_empty((T, E), dtype=torch.float32) if with_scores else None
+    stats = z.new_empty(2 * T, dtype=torch.float32) if train and score else None
+    L.call("smel_select_experts", z.data_ptr(), z.stride(0) if T > 1 else E, _SEL_DTYPES[z.dtype], T, E, k, score, L.ptr(bias), groups,
+           top_groups, best, renorm, scale, topv.data_ptr(), topi.data_ptr(), L.ptr(scores), L.ptr(stats), L.stream())
+    return topv, topi, scores, (z, stats)
+
+
+def _select_backward(ctx, dtopv, *_):
+    rest = (None,) * 9
+    if dtopv is None:
+        return None, *rest
+    z, topi, stats = ctx.saved_tensors
+    score, renorm, scale = ctx.call
+    T, E = z.shape
+    dtopv = dtopv.to(torch.float32).contiguous()
+    dz = z.new_empty((T, E))
+    L.call("smel_select_experts_bwd", z.data_ptr(), z.stride(0) if T > 1 else E, _SEL_DTYPES[z.dtype], T, E, topi.shape[1], score, renorm,
+           scale, topi.data_ptr(), dtopv.data_ptr(), L.ptr(stats), dz.data_ptr(), E, L.stream())
+    return dz, *rest
+
+
+_select_backward_once = once_differentiable(_select_backward)
+
+
+class _SelectFn(torch.autograd.Function):
+    """select_experts: topv differentiable w.r.t. the logits, the picks constants."""
+
+    @staticmethod
+    def forward(ctx, z, bias, *args):
+        topv, topi, scores, (z, stats) = _select_forward(z, bias, *args, True)
+        ctx.save_for_backward(z, topi, stats)
+        ctx.call = (args[1], args[5], args[6])
+        ctx.set_materialize_grads(False)
+        if scores is None:
+            ctx.mark_non_differentiable(topi)
+            return topv, topi
+        ctx.mark_non_differentiable(topi, scores)
+        return topv, topi, scores
+
+    @staticmethod
+    def backward(ctx, *grads):     # on the forward's device: autograd's thread has set it
+        return (_select_backward_once if torch.is_grad_enabled() else _select_backward)(ctx, *grads)
+
+
+def select_experts(logits, top_k, score="sigmoid", bias=None, groups=1, top_groups=1, group_best=2, renorm=True, scale=1.0,
+                   with_scores=False):
+    """The experts of each token from its router logits [T, E] (bf16, fp16, fp32): (topv fp32 [T, K], topi int64 [T, K]), with
+    ``with_scores`` also the scores fp32 [T, E].
+
+    scores s: the logits' sigmoid or softmax. Picked by c = s + bias (``bias`` [E] steers the load and is no part of the weights):
+    the E experts are ``groups`` runs of neighbours, a group counts with the sum of its ``group_best`` largest c, the ``top_groups``
+    best groups stay, and of their experts the K largest c are picked, descending (ties: the lower index). topv: the picks' s, over
+    their sum (``renorm``), times ``scale``. Differentiable w.r.t. the logits through topv. At most 512 experts, 64 groups, K = 16.
+    Whatever the logits hold (a padded row's NaN too), topi are K different experts."""
+    k, groups, top_groups, group_best = int(top_k), int(groups), int(top_groups), int(group_best)
+    _select_check(logits, k, score, bias, groups, top_groups, group_best)
+    args = (k, _SCORES[score], groups, top_groups, group_best, bool(renorm), float(scale), bool(with_scores))
+    with L.on_device_of(logits):
+        if torch.is_grad_enabled() and logits.requires_grad or L.forward_mode():
+            return L.apply(_SelectFn, logits, bias, *args)
+        topv, topi, scores, _ = _select_forward(logits, bias, *args, False)
+    return (topv, topi, scores) if with_scores else (topv, topi)
+
+
+class _RouterLogitsFn(torch.autograd.Function):
+    """x W_r^T rounded to bf16 (route's logits), differentiable w.r.t. x."""
+
+    @staticmethod
+    def forward(ctx, x, gate_w):
+        T, H = x.shape
+        E = gate_w.shape[0]
+        lg = torch.empty(T, L.load().smel_route_ld(E, 0), dtype=torch.bfloat16, device=x.device)
+        L.call("smel_router_logits", L.ptr(x), L.ptr(gate_w), T, H, E, L.ptr(lg), L.stream())
+        ctx.save_for_backward(gate_w)
+        return lg[:, :E]
+
+    @staticmethod
+    def backward(ctx, dlogits):
+        gate_w, = ctx.saved_tensors
+        T, E = dlogits.shape
+        wr = _router_ext_weight(gate_w, None)
+        if wr.R != E:
+            dl = torch.zeros(T, wr.R, dtype=torch.bfloat16, device=dlogits.device)
+            dl[:, :E] = dlogits
+        else:
+            dl = dlogits.contiguous()
+        return _router_dx(dl, wr, T, dlogits.device, L.stream()), None
+
+
+def _router_logits(x2d, gate_w):
+    if x2d.dtype == torch.float32:
+        return F32.RouterLogitsFn.apply(F32.f32(x2d), F32.f32(gate_w, "gate_w"))
+    if _bf16_limit(x2d.shape[-1]) is not None:
+        return F32.RouterLogitsFn.apply(_bf16(x2d).float(), _f32_of(_bf16(gate_w))).to(x2d.dtype)
+    return _RouterLogitsFn.apply(_bf16(x2d), _bf16(gate_w))
+
+
+def route_grouped(x2d, gate_w, top_k, score="sigmoid", bias=None, groups=1, top_groups=1, group_best=2, renorm=True, scale=1.0,
+                  with_logits=False):
+    """``route`` with the choice of ``select_experts``: (scores fp32 [T, E], topv fp32 [T, K], topi int64 [T, K]), with_logits:
+    (..., logits [T, E]), differentiable w.r.t. x2d; what ``routed_experts`` and the stats hook take. bf16 (logits rounded to bf16, as
+    ``route``'s) or fp32 activations."""
+    L.require_device(x2d, gate_w)
+    with L.on_device_of(x2d):
+        logits = _router_logits(x2d, gate_w)
+        topv, topi, scores = select_experts(logits, top_k, score, bias, groups, top_groups, group_best, renorm, scale, True)
+    return (scores, topv, topi, logits) if with_logits else (scores, topv, topi)
 
 
 # ------------------------------------------------------------------------------------------------ fused layer

@@ -288,6 +288,28 @@ def _router_bwd(dtopv, probs, topi32, w, pes, dlogits=None):
     return dx
 
 
+class RouterLogitsFn(torch.autograd.Function):
+    """x W_r^T on fp32 tensors (fp32 MFMA), differentiable w.r.t. x."""
+
+    @staticmethod
+    def forward(ctx, x, gate_w):
+        T, E = x.shape[0], gate_w.shape[0]
+        tl, _, _ = dense_tiles(T, x.device)
+        logits = torch.empty(T, E, dtype=torch.float32, device=x.device)
+        gmm(_dense(gate_w), 0, tl, x, x.shape[1], logits, E, tag="route_f32")
+        ctx.save_for_backward(gate_w)
+        return logits
+
+    @staticmethod
+    def backward(ctx, dlogits):
+        gate_w, = ctx.saved_tensors
+        T, (E, H) = dlogits.shape[0], gate_w.shape
+        tl, _, _ = dense_tiles(T, dlogits.device)
+        dx = torch.empty(T, H, dtype=torch.float32, device=dlogits.device)
+        gmm(_dense(gate_w), 1, tl, dlogits.contiguous(), E, dx, H, tag="route_f32_bwd")
+        return dx, None
+
+
 class RouteGemma4Fn(torch.autograd.Function):
     """route_gemma4 (smel/moe.py:170-180) on fp32 tensors: weightless RMSNorm of h, x router.scale x fp32(H^-1/2),
     logits, softmax, top-k, renorm, x per_expert_scale; differentiable w.r.t. h; with_logits as in RouteFn."""

@@ -1,12 +1,14 @@
 """RMSNorm family of the frozen layers around the MoE block, and layer norm with trained weights, on the HIP kernels of
-libsmel_moe.so (include/smel_norm.h): one launch forward, one backward (layer norm: two, the second adds up the weights'
-gradients).
+libsmel_moe.so (include/smel_norm.h): one launch forward, one backward (with trained weights: two, the second adds up the
+weights' gradients).
 
   rmsnorm(x, w, eps, plus_one)          y = x * rstd * (1 + w) (Qwen3.5/3.6), x * rstd * w (Gemma 4), x * rstd (w None)
   add_rmsnorm(h, x, w, eps, plus_one)   s = h + x (the residual add), y = rmsnorm(s)
   gated_rmsnorm(x, z, w, eps)           y = w * norm(x) * silu(z)  (output norm of Gated DeltaNet)
   layernorm(x, w, b, eps)               y = (x - mean) * rstd * w + b
   add_layernorm(h, x, w, b, eps)        s = h + x, y = layernorm(s)
+  post_rmsnorm(h, x, w, eps, plus_one, gate, gate_act, scale)             s = scale (h + gate rmsnorm(x)): behind a block
+  sandwich_rmsnorm(h, x, w_post, w_pre, eps, plus_one, gate, gate_act, scale)    the same s, and y = rmsnorm(s) before the next
 
 Of the RMSNorm functions the API is the reference's smel/norm.py:252-275 (``supported``, ``ENABLED``, ``MAX_COLS`` and the three functions,
 same arguments and return values). Their weights are frozen, so backward gives dx (and dz) only, as there.
@@ -21,6 +23,8 @@ question as the reference's (16-bit rows on the GPU, frozen contiguous weights o
 columns), so a caller that routes other cases to its own torch code keeps doing so.
 """
 from __future__ import annotations
+
+import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -301,3 +305,178 @@ def layernorm(x, w, b, eps):
 def add_layernorm(h, x, w, b, eps):
     """(h + x, layernorm(h + x)): the residual add, rounded to the stream's dtype, and the norm after it."""
     return _ln(x, h, w, b, eps)
+
+
+# ------------------------------------------------------------------------------------------------ around the residual add
+
+_GATE_NONE, _GATE_CHANNEL, _GATE_TOKEN, _GATE_FULL = 0, 1, 2, 3
+_GATE_ACTS = {None: 0, "sigmoid": 1}
+
+
+def _sw_refuse(h, x, w1, w2, gate, scale):
+    """Raises what is wrong with the call."""
+    _lib.one_device(x, h, w1, w2, gate, scale)
+    if x.dtype not in _LN_DTYPES:
+        raise ValueError(f"the norms around a residual add take bf16, fp16 or fp32 rows, got {x.dtype}")
+    if x.dim() == 0 or not 1 <= x.shape[-1] <= MAX_COLS:
+        raise ValueError(f"the norms around a residual add take rows of 1 to {MAX_COLS} columns, got shape {tuple(x.shape)}")
+    if h.shape != x.shape or h.dtype != x.dtype:
+        raise ValueError(f"the stream and the block's output differ: {tuple(h.shape)} {h.dtype} and {tuple(x.shape)} {x.dtype}")
+    n = x.shape[-1]
+    for t in (w1, w2):
+        if t is not None and (t.dtype not in (x.dtype, torch.float32) or tuple(t.shape) != (n,) or not t.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous [{n}] tensors of {x.dtype} or float32")
+    if gate is not None:
+        token, full = (*x.shape[:-1], 1), tuple(x.shape)
+        if tuple(gate.shape) not in ((n,), token, full):
+            raise ValueError(f"a gate has shape [{n}], {list(token)} or {list(full)}, got {tuple(gate.shape)}")
+        if gate.dtype not in (x.dtype, torch.float32) or gate.dtype != x.dtype and tuple(gate.shape) == full and full not in ((n,), token):
+            raise ValueError(f"a gate of {gate.dtype} with rows of {x.dtype}")
+    if scale is not None and (scale.numel() != 1 or scale.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f"the scale is a number or one element of {x.dtype} or float32, got {tuple(scale.shape)} {scale.dtype}")
+    raise ValueError("norm weights and a gate per channel must have one dtype")
+
+
+def _sw_check(h, x, w1, w2, gate, scale) -> tuple:
+    """(columns, the rows' type code, the weights' type code, the gate's kind) of a call that the kernels take."""
+    dt = _LN_DTYPES.get(x.dtype)
+    if dt is None or x.dim() == 0 or not x.is_cuda:
+        _sw_refuse(h, x, w1, w2, gate, scale)
+    n, dev, shape = x.shape[-1], x.device, x.shape
+    ok = 1 <= n <= MAX_COLS and h.shape == shape and h.dtype is x.dtype and h.device == dev
+    kind, wd = _GATE_NONE, None
+    weights = (w1, w2)
+    if gate is not None:
+        ok = ok and gate.device == dev and (gate.dtype is x.dtype or gate.dtype is torch.float32)
+        if gate.dim() == 1 and gate.shape[0] == n:      # of one row: whichever, they are the same
+            kind, weights = _GATE_CHANNEL, (w1, w2, gate.contiguous() if ok else None)
+        elif gate.shape == shape and (n != 1 or gate.dtype is x.dtype):
+            kind = _GATE_FULL
+            ok = ok and gate.dtype is x.dtype
+        else:
+            kind = _GATE_TOKEN
+            ok = ok and gate.dim() == x.dim() and gate.shape[-1] == 1 and gate.shape[:-1] == shape[:-1]
+    for t in weights:
+        if t is not None:
+            ok = ok and (wd is None or t.dtype is wd) and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() \
+                and t.device == dev
+            wd = t.dtype
+    wt = dt if wd is None or wd is x.dtype else 2
+    if scale is not None:
+        ok = ok and scale.device == dev and scale.numel() == 1 and (scale.dtype is x.dtype or scale.dtype is torch.float32)
+    if not ok or (wt == 2 and wd is not None and wd is not torch.float32):
+        _sw_refuse(h, x, w1, w2, gate, scale)
+    return n, dt, wt, kind
+
+
+def _sw_call(n, dt, wt, kind, act, plus_one, eps, w1, w2, gate, scale, scale_value):
+    """The call's part that forward and backward share."""
+    c, p = _lib.Sandwich(), _lib.ptr
+    c.w1, c.w2, c.gate, c.scale = p(w1), p(w2), p(gate), p(scale)
+    c.cols, c.eps, c.scale_value = n, eps, scale_value
+    c.dtype, c.wtype, c.gate_kind, c.gate_act, c.plus_one = dt, wt, kind, act, plus_one
+    c.gate_type = 2 if gate is not None and gate.dtype is torch.float32 else dt
+    c.scale_type = 2 if scale is not None and scale.dtype is torch.float32 else dt
+    return c
+
+
+def _sw_forward(h, x, w1, w2, gate, scale, pre, rest):
+    """(the rows of x, s, y or None, stats, the contiguous gate)."""
+    n, dt, wt, kind, act, plus_one, eps, scale_value = rest
+    if gate is not None:
+        gate = gate.contiguous()
+    c = _sw_call(n, dt, wt, kind, act, plus_one, eps, w1, w2, gate, scale, scale_value)
+    x2, R, c.x_stride = _rows_of(x, n)
+    h2, _, c.h_stride = _rows_of(h, n)
+    s = x.new_empty(x.shape)
+    y = x.new_empty(x.shape) if pre else None
+    stats = x.new_empty(2 * R, dtype=torch.float32)     # a row's two reciprocal root mean squares
+    c.x, c.h, c.s, c.y, c.stats = x2.data_ptr(), h2.data_ptr(), s.data_ptr(), _lib.ptr(y), stats.data_ptr()
+    c.rows, c.pre = R, pre
+    _lib.call("smel_sandwich_fwd", ctypes.byref(c), _lib.stream())
+    return x2, s, y, stats, gate
+
+
+def _sw_backward(ctx, ds, dy=None):
+    """Gradients of h, x, w1, w2, gate and scale, each only where it is asked for."""
+    x2, s, h, w1, w2, gate, scale, stats = ctx.saved_tensors
+    pre, R, shape, rest = ctx.call
+    n, dt, wt, kind, act, plus_one, eps, scale_value = rest
+    nh, nx, nw1, nw2, ng, nsc = ctx.needs_input_grad[:6]
+    none = (None, None, None)
+    if ds is None and dy is None:
+        return (None,) * 6 + none
+    c = _sw_call(n, dt, wt, kind, act, plus_one, eps, w1, w2, gate, scale, scale_value)
+    c.rows, c.x_stride = R, n if x2.is_contiguous() else x2.stride(0)     # of what comes back: hooks on saved tensors may repack it
+    ds2 = ds.contiguous() if ds is not None else None
+    dy2 = dy.contiguous() if dy is not None else None
+    p, new = _lib.ptr, x2.new_empty
+    passed = dy is None and scale is None and scale_value == 1.0     # the stream's gradient goes through as it is
+    dh = ds if passed else new(shape) if nh else None
+    dx = new(shape) if nx else None
+    dw1 = torch.empty_like(w1) if nw1 else None
+    dw2 = torch.empty_like(w2) if nw2 else None
+    dg = torch.empty_like(gate) if ng else None
+    dsc = torch.empty_like(scale) if nsc else None
+    c.x, c.s, c.ds, c.dy, c.stats = x2.data_ptr(), p(s), p(ds2), p(dy2), stats.data_ptr()
+    c.dh, c.dx, c.dw1, c.dw2, c.dgate, c.dscale = None if passed else p(dh), p(dx), p(dw1), p(dw2), p(dg), p(dsc)
+    if nsc:
+        h2, _, c.h_stride = _rows_of(h, n)
+        c.h = h2.data_ptr()
+    ws, ws_n = None, _lib.load().smel_sandwich_bwd_ws_floats(ctypes.byref(c))
+    if ws_n:
+        ws = new(ws_n, dtype=torch.float32)
+    if nx or nw1 or nw2 or ng or nsc or not passed and nh:
+        _lib.call("smel_sandwich_bwd", ctypes.byref(c), p(ws), ws_n, _lib.stream())
+    return (dh if nh else None, dx, dw1, dw2, dg, dsc) + none
+
+
+_sw_backward_once = once_differentiable(_sw_backward)
+
+
+class _SandwichFn(torch.autograd.Function):
+    """forward(h, x, w1, w2, gate, scale, pre, keep h, the call's numbers): s, or (s, y) with ``pre``. Saved: x's rows, s (pre), the
+    gate, two fp32 numbers a row, and h for a trained scale."""
+
+    @staticmethod
+    def forward(ctx, h, x, w1, w2, gate, scale, pre, rest, _):
+        x2, s, y, stats, gate = _sw_forward(h, x, w1, w2, gate, scale, pre, rest)
+        ctx.save_for_backward(x2, s if pre else None, h if ctx.needs_input_grad[5] else None, w1, w2, gate, scale, stats)
+        ctx.call = (pre, stats.shape[0] // 2, x.shape, rest)
+        ctx.set_materialize_grads(False)
+        return (s, y) if pre else s
+
+    @staticmethod
+    def backward(ctx, *grads):     # on the forward's device: autograd's thread has set it
+        return (_sw_backward_once if torch.is_grad_enabled() else _sw_backward)(ctx, *grads)
+
+
+def _sandwich(h, x, w1, w2, eps, plus_one, gate, gate_act, scale, pre):
+    act = _GATE_ACTS.get(gate_act)
+    if act is None:
+        raise ValueError(f"gate_act is None or 'sigmoid', got {gate_act!r}")
+    value = 1.0
+    if scale is not None and not isinstance(scale, torch.Tensor):
+        scale, value = None, float(scale)
+    rest = (*_sw_check(h, x, w1, w2, gate, scale), act, bool(plus_one), float(eps), value)
+    with _lib.on_device_of(x):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, x, w1, w2, gate, scale)) or _lib.forward_mode():
+            return _lib.apply(_SandwichFn, h, x, w1, w2, gate, scale, pre, rest, None)
+        _, s, y, _, _ = _sw_forward(h, x, w1, w2, gate, scale, pre, rest)
+    return (s, y) if pre else s
+
+
+def post_rmsnorm(h, x, w, eps, plus_one=False, gate=None, gate_act=None, scale=None):
+    """scale (h + gate rmsnorm(x)): the norm behind a block, its gate, the residual add and the residual scale, rounded once.
+
+    h, x [..., n]: the residual stream and the block's output, bf16, fp16 or fp32 rows of any stride. w [n] (None: 1; 1 + w with
+    ``plus_one``), of the rows' dtype or fp32. gate: a value per channel [n] (the weights' dtype), per token [..., 1] (the rows' dtype
+    or fp32) or per element [..., n] (the rows' dtype); ``gate_act`` "sigmoid": the gate's sigmoid. scale: a number or one element on
+    the GPU. Backward gives every gradient that is asked for: of h, x, w, the gate and the scale."""
+    return _sandwich(h, x, w, None, eps, plus_one, gate, gate_act, scale, False)
+
+
+def sandwich_rmsnorm(h, x, w_post, w_pre, eps, plus_one=False, gate=None, gate_act=None, scale=None):
+    """(s, y): s = ``post_rmsnorm(h, x, w_post, ...)`` and y = rmsnorm(s) with w_pre, the norm before the next block (of the rounded
+    s, as the next block would read it). w_pre None: weight 1."""
+    return _sandwich(h, x, w_post, w_pre, eps, plus_one, gate, gate_act, scale, True)
