@@ -21,7 +21,9 @@ struct SelArgs {
   float *topv, *scores, *stats;
   int64_t* topi;
   int64_t ldl, T;
-  int E, K, score, groups, top_groups, best, renorm;
+  int E, K, score, best, renorm, drop;
+  int parts, size, lg, per;   // groups, experts of one; log2 of a group's lanes; experts of a lane
+  int top_groups;
   float scale;
 };
 
@@ -32,6 +34,16 @@ SMEL_DEV float logit_at(const void* z, int64_t at) {
   else
     return cvt<DT>(((const uint16_t*)z)[at]);
 }
+// 8 values kept in the caches for the next kernel (rows.h's stores pass them by)
+template <int DT>
+SMEL_DEV void keep8(typename El<DT>::T* p, int e0, int n, const Raw<DT>& r) {
+  if constexpr (DT == 2) {
+    store8<2, true>(p, e0, n, r);
+  } else {
+    if (e0 + 8 <= n) *(u32x4_a2*)(p + e0) = r.q[0];
+    else store8<DT>(p, e0, n, r);
+  }
+}
 // order-preserving form of a choice, above 0: -infinity and NaN are 0x007fffff
 SMEL_DEV uint32_t order_of(float c) {
   if (!(c > -INFINITY)) return 0x007fffffu;
@@ -39,115 +51,187 @@ SMEL_DEV uint32_t order_of(float c) {
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 SMEL_DEV float choice_of(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
-SMEL_DEV uint64_t wave_max_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint64_t u = __shfl_xor(v, o, 64);
-    v = v > u ? v : u;
+// Reductions over the LT (16 or 64) lanes of a token, every lane gets the result. Within 16 lanes by DPP moves: a row's halves and
+// quads are exchanged until all agree.
+template <int CTRL>
+SMEL_DEV uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+SMEL_DEV float dpp(float v) {
+  return __uint_as_float(dpp<CTRL>(__float_as_uint(v)));
+}
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
+template <int LT, typename T, typename F>
+SMEL_DEV T over_lanes(T v, F f) {
+  v = f(v, dpp<XOR1>(v));
+  v = f(v, dpp<XOR2>(v));
+  v = f(v, dpp<HALF_MIRROR>(v));
+  v = f(v, dpp<MIRROR>(v));
+  if (LT == 64) {
+    v = f(v, __shfl_xor(v, 16, 64));
+    v = f(v, __shfl_xor(v, 32, 64));
   }
   return v;
 }
-SMEL_DEV float sigmoid_of(float z) { return 1.f / (1.f + expf(-z)); }
+template <int LT>
+SMEL_DEV float sum_lanes(float v) {
+  return over_lanes<LT>(v, [](float a, float b) { return a + b; });
+}
+template <int LT>
+SMEL_DEV uint32_t max_lanes(uint32_t v) {
+  if constexpr (LT == 64) return wave_max_u32(v);
+  return over_lanes<LT>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+SMEL_DEV float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.f + expf(-z)); }
 
-// a wave per token, expert l + 64 j in lane l
-template <int DT>
-__global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
-  constexpr int NPL = MAXE / 64;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= p.T) return;
-  const int l = lane_id();
-  float s[NPL];
-  float m = -INFINITY;
+// n (<= N) values from p on, zeros behind; all of them at once where there are N
+template <int DT, int N>
+SMEL_DEV void run_of(const void* base, int64_t at, int n, float v[N]) {
+  typedef typename El<DT>::T T;
+  const T* const p = (const T*)base + at;
+  if constexpr (N > 1) {
+    if (n == N) {
+      typedef T __attribute__((ext_vector_type(N < 8 ? N : 8), aligned(sizeof(T)))) vec;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) {
-    const int e = l + 64 * j;
-    s[j] = e < p.E ? logit_at<DT>(p.z, t * p.ldl + e) : -INFINITY;
-    m = fmaxf(m, s[j]);
+      for (int i = 0; i < (N + 7) / 8; ++i) {
+        const vec q = ((const vec*)p)[i];
+#pragma unroll
+        for (int j = 0; j < (N < 8 ? N : 8); ++j) {
+          if constexpr (DT == 2) v[8 * i + j] = q[j];
+          else v[8 * i + j] = cvt<DT>((uint32_t)q[j]);
+        }
+      }
+      return;
+    }
   }
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = j < n ? logit_at<DT>(p, j) : 0.f;
+}
+
+// LT lanes a token (four tokens a wave, or one). A group's experts lie in LT / 2^k lanes next to each other, N of them at most in a
+// lane, in the order of their indices; without groups to drop, all experts are one. Each lane sorts its own, so a pick is the largest
+// of the lanes' heads: the maximum by DPP moves, the lowest lane that holds it (the lowest index: ties), and that lane goes on to its
+// next. Bound by instructions: about 25 for a pick, 15 for a score, 5 for each of a lane's N (N - 1) / 2 comparisons.
+template <int DT, int LT, int N>
+__global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
+  const int l = lane_id(), li = l & (LT - 1), base = l & ~(LT - 1);
+  const int64_t t = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / LT) + l / LT;
+  const bool live = t < p.T;
+  const int64_t row = live ? t : p.T - 1;
+  const int grp = li >> p.lg, q = li & ((1 << p.lg) - 1);
+  const int e0 = grp * p.size + q * p.per;
+  const int n = grp < p.parts ? min(max(p.size - q * p.per, 0), p.per) : 0;
+  float s[N], bias[N];
+  run_of<DT, N>(p.z, row * p.ldl + e0, n, s);
+  if (p.bias) run_of<2, N>(p.bias, e0, n, bias);
+  float m = 0.f, inv = 0.f;
   if (p.score == 0) {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) s[j] = sigmoid_of(s[j]);
+    for (int j = 0; j < N; ++j) s[j] = sigmoid_of(s[j]);
   } else {
-    m = wave_max(m);
-    const float base = m > -INFINITY ? m : 0.f;
+    m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) m = fmaxf(m, s[j]);
+    m = over_lanes<LT>(m, [](float a, float b) { return fmaxf(a, b); });
+    if (!(m > -INFINITY)) m = 0.f;
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-      s[j] = l + 64 * j < p.E ? expf(s[j] - base) : 0.f;
-      sum += s[j];
+    for (int j = 0; j < N; ++j) {
+      s[j] = expf(s[j] - m);
+      if (j < n) sum += s[j];
     }
-    sum = wave_sum(sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    sum = sum_lanes<LT>(sum);
+    inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) s[j] *= inv;
-    if (p.stats && l == 0) {
-      p.stats[2 * t] = base;
+    for (int j = 0; j < N; ++j) s[j] *= inv;
+    if (p.stats && live && li == 0) {
+      p.stats[2 * t] = m;
       p.stats[2 * t + 1] = inv;
     }
   }
-  uint64_t key[NPL];
+  if (p.scores && live)
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) {
-    const int e = l + 64 * j;
-    key[j] = 0;
-    if (e < p.E) {
-      if (p.scores) p.scores[t * p.E + e] = s[j];
-      key[j] = (uint64_t)order_of(p.bias ? s[j] + p.bias[e] : s[j]) << 32 | (0xffffffffu - (uint32_t)e);
-    }
+    for (int j = 0; j < N; ++j)
+      if (j < n) p.scores[t * p.E + e0 + j] = s[j];
+  uint32_t key[N], at[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    key[j] = j < n ? order_of(p.bias ? s[j] + bias[j] : s[j]) : 0u;
+    at[j] = j;
   }
-  const int size = p.E / p.groups;
-  if (p.top_groups < p.groups) {
-    uint64_t mine = 0;   // lane g keeps group g's value
-    for (int g = 0; g < p.groups; ++g) {
-      uint64_t first = 0, second = 0;
+  // descending, equal ones in order
 #pragma unroll
-      for (int j = 0; j < NPL; ++j)
-        if ((l + 64 * j) / size == g && key[j] > first) first = key[j];
-      first = wave_max_u64(first);
+  for (int i = 1; i < N; ++i)
 #pragma unroll
-      for (int j = 0; j < NPL; ++j)
-        if ((l + 64 * j) / size == g && key[j] != first && key[j] > second) second = key[j];
-      second = wave_max_u64(second);
-      float v = choice_of(first >> 32);
-      if (p.best == 2 && size > 1) v += choice_of(second >> 32);
-      if (l == g) mine = (uint64_t)order_of(v) << 32 | (0xffffffffu - (uint32_t)g);
+    for (int j = N - 1; j >= i; --j) {
+      const bool up = key[j] > key[j - 1];
+      const uint32_t hi = max(key[j], key[j - 1]), lo = min(key[j], key[j - 1]);
+      const uint32_t ah = up ? at[j] : at[j - 1], al = up ? at[j - 1] : at[j];
+      key[j - 1] = hi;
+      key[j] = lo;
+      at[j - 1] = ah;
+      at[j] = al;
     }
-    uint64_t kept = 0;
-    for (int k = 0; k < p.top_groups; ++k) {
-      const uint64_t b = wave_max_u64(mine);
-      const int g = (int)(0xffffffffu - (uint32_t)b);
-      kept |= 1ull << g;
-      if (l == g) mine = 0;
+  if (p.drop) {   // groups
+    float c1 = key[0] ? choice_of(key[0]) : -INFINITY, c2 = -INFINITY;
+    if constexpr (N > 1) c2 = key[1] ? choice_of(key[1]) : -INFINITY;
+    auto join = [&](float d1, float d2) {
+      c2 = fmaxf(fminf(c1, d1), fmaxf(c2, d2));
+      c1 = fmaxf(c1, d1);
+    };
+    if (p.lg > 0) join(dpp<XOR1>(c1), dpp<XOR1>(c2));
+    if (p.lg > 1) join(dpp<XOR2>(c1), dpp<XOR2>(c2));
+    if (p.lg > 2) join(dpp<HALF_MIRROR>(c1), dpp<HALF_MIRROR>(c2));
+    if (p.lg > 3) join(dpp<MIRROR>(c1), dpp<MIRROR>(c2));
+    if (p.lg > 4) join(__shfl_xor(c1, 16, 64), __shfl_xor(c2, 16, 64));
+    const uint32_t value = grp < p.parts ? order_of(p.best == 2 && p.size > 1 ? c1 + c2 : c1) : 0u;
+    int rank = 0;
+    for (int g = 0; g < p.parts; ++g) {
+      uint32_t v;
+      if constexpr (LT == 64) v = (uint32_t)lane_get((int)value, g << p.lg);
+      else v = __shfl(value, base + (g << p.lg), 64);
+      rank += v > value || (v == value && g < grp);
     }
+    if (rank >= p.top_groups)
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (l + 64 * j < p.E && !(kept >> ((l + 64 * j) / size) & 1)) key[j] = 0;
+      for (int j = 0; j < N; ++j) key[j] = 0u;
   }
-  float w = 0.f, sum = 0.f;   // lane k keeps pick k
-  int id = 0;
+  // the order of a lane's experts, four bits each
+  uint64_t next = 0;
+#pragma unroll
+  for (int j = N - 1; j >= 0; --j) next = next << 4 | at[j];
+  int id = 0;   // lane k of a token keeps pick k
   for (int k = 0; k < p.K; ++k) {
-    uint64_t best = 0;
+    const uint32_t best = max_lanes<LT>(key[0]);
+    const uint64_t who = __ballot(key[0] == best);
+    const int head = e0 + (int)(next & 15);
+    int w, e;
+    if constexpr (LT == 64) {
+      w = __builtin_ctzll(who);
+      e = lane_get(head, w);
+    } else {
+      w = __builtin_ctz((uint32_t)(who >> base) & 0xffffu);
+      e = __shfl(head, base + w, 64);
+    }
+    if (li == k) id = e;
+    if (li == w) {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) best = best > key[j] ? best : key[j];
-    best = wave_max_u64(best);
-    const int e = (int)(0xffffffffu - (uint32_t)best);
-    float v = 0.f;
-#pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (l + 64 * j == e) {
-        v = s[j];
-        key[j] = 0;
-      }
-    v = __shfl(v, e & 63, 64);
-    sum += v;
-    if (l == k) {
-      w = v;
-      id = e;
+      for (int j = 0; j + 1 < N; ++j) key[j] = key[j + 1];
+      key[N - 1] = 0u;
+      next >>= 4;
     }
   }
-  if (l < p.K) {
-    p.topv[t * p.K + l] = p.renorm ? p.scale * w / (sum + SUM_EPS) : p.scale * w;
-    p.topi[t * p.K + l] = id;
+  float w = 0.f;
+  if (li < p.K) {
+    const float z = logit_at<DT>(p.z, row * p.ldl + id);
+    w = p.score == 0 ? sigmoid_of(z) : expf(z - m) * inv;
+  }
+  const float sum = sum_lanes<16>(w);   // K <= 16
+  if (live && li < p.K) {
+    p.topv[t * p.K + li] = p.renorm ? p.scale * w / (sum + SUM_EPS) : p.scale * w;
+    p.topi[t * p.K + li] = id;
   }
 }
 
@@ -157,54 +241,92 @@ struct SelBwdArgs {
   const float *dtopv, *stats;
   void* dz;
   int64_t ldl, ldd, T;
-  int E, K, score, renorm;
+  int E, K, score, renorm, lpr;
   float scale;
 };
 
+// lpr lanes a token, 8 columns each: lane k works out pick k's gradient and puts it into the row in LDS, each lane writes its columns.
+// A row's lanes are of one wave, whose LDS accesses take effect in order. Bound by the bytes of dz (softmax: and of z).
 template <int DT>
 __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
   typedef typename El<DT>::T T;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= p.T) return;
-  const int l = lane_id();
-  const float m = p.score ? p.stats[2 * t] : 0.f, inv = p.score ? p.stats[2 * t + 1] : 0.f;
+  __shared__ __attribute__((aligned(16))) float rows[256 * 8];
+  const int lpr = p.lpr, li = threadIdx.x & (lpr - 1);
+  const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  const bool live = t < p.T;
+  const int64_t row = live ? t : p.T - 1;
+  float* const mine = rows + (threadIdx.x / lpr) * (8 * lpr);
+  Raw<DT> z{};
+  if (p.score && 8 * li < p.E) z = load8<DT>((const T*)p.z + row * p.ldl, 8 * li, p.E);
+  f32x4_t* const own = (f32x4_t*)(mine + 8 * li);
+  own[0] = own[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float m = p.score ? p.stats[2 * row] : 0.f, inv = p.score ? p.stats[2 * row + 1] : 0.f;
   int id = -1;
-  float d = 0.f, s = 0.f, slope = 0.f;   // lane k: pick k
-  if (l < p.K) {
-    const int64_t e = p.topi[t * p.K + l];
+  float d = 0.f, s = 0.f, slope = 1.f;   // lane k: pick k
+  if (li < p.K) {
+    const int64_t e = p.topi[row * p.K + li];
     if (e >= 0 && e < p.E) {
       id = (int)e;
-      d = p.scale * p.dtopv[t * p.K + l];
-      const float z = logit_at<DT>(p.z, t * p.ldl + id);
+      d = p.scale * p.dtopv[row * p.K + li];
+      const float zk = logit_at<DT>(p.z, row * p.ldl + id);
       if (p.score == 0) {
-        s = sigmoid_of(z);
-        const float q = expf(-fabsf(z));
-        slope = q / ((1.f + q) * (1.f + q));
+        s = sigmoid_of(zk);
+        const float q = expf(-fabsf(zk)), a = __builtin_amdgcn_rcpf(1.f + q);
+        slope = q * a * a;
       } else {
-        s = expf(z - m) * inv;
+        s = expf(zk - m) * inv;
       }
     }
   }
+  auto sum = [&](float v) {
+    for (int o = 1; o < lpr; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+  };
   if (p.renorm) {
-    const float S = wave_sum(s) + SUM_EPS, dot = wave_sum(d * s);
+    const float S = sum(s) + SUM_EPS, dot = sum(d * s);
     d = (d - dot / S) / S;
   }
-  const float all = p.score ? wave_sum(d * s) : 0.f;
-  if (p.score == 0) d *= slope;
-  for (int e = l; e < p.ldd; e += 64) {
-    float g = 0.f;
-    for (int k = 0; k < p.K; ++k) {
-      const int ik = lane_get(id, k);
-      const float dk = lane_get(d, k);
-      if (ik == e) g += dk;
-    }
-    float v = g;
-    if (p.score) v = e < p.E ? expf(logit_at<DT>(p.z, t * p.ldl + e) - m) * inv * (g - all) : 0.f;
-    if constexpr (DT == 2)
-      ((T*)p.dz)[t * p.ldd + e] = v;
-    else
-      ((T*)p.dz)[t * p.ldd + e] = (T)enc<DT>(v);
+  const float all = p.score ? sum(d * s) : 0.f;
+  if (id >= 0) atomicAdd(&mine[id], d * slope);
+  if (!live) return;
+  const f32x4_t a = own[0], b = own[1];
+  float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  if (p.score)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 8 * li + j < p.E ? expf(z.at(j) - m) * inv * (v[j] - all) : 0.f;
+  Raw<DT> o;
+  o.set(v);
+  T* const out = (T*)p.dz + t * p.ldd;
+  const int n = (int)(p.ldd < 8 * lpr ? p.ldd : 8 * lpr);
+  if (8 * li < n) keep8<DT>(out, 8 * li, n, o);
+  for (int64_t e = 8 * lpr + li; e < p.ldd; e += lpr) out[e] = T(0);
+}
+
+// A lane's experts with lt lanes a token: their most, and log2 of the lanes of a group
+int lane_plan(SelArgs& p, int lt) {
+  int lanes = lt;
+  p.lg = lt == 64 ? 6 : 4;
+  for (int g = 1; g < p.parts; g *= 2) {
+    lanes /= 2;
+    --p.lg;
   }
+  if (lanes == 0) return 1 << 20;
+  return p.per = (p.size + lanes - 1) / lanes;
+}
+template <int DT, int LT, int N>
+int launch_plan(const SelArgs& p, hipStream_t stream) {
+  constexpr int64_t TOKENS = 4 * (64 / LT);
+  select_kernel<DT, LT, N><<<(unsigned)((p.T + TOKENS - 1) / TOKENS), 256, 0, stream>>>(p);
+  return smel::launch_status();
+}
+template <int DT>
+int launch_select(SelArgs& p, hipStream_t stream) {
+  const int n = lane_plan(p, 64);
+  if (n <= 1) return launch_plan<DT, 64, 1>(p, stream);
+  if (n <= 2) return launch_plan<DT, 64, 2>(p, stream);
+  if (n <= 4) return launch_plan<DT, 64, 4>(p, stream);
+  if (n <= 8) return launch_plan<DT, 64, 8>(p, stream);
+  return launch_plan<DT, 64, 16>(p, stream);
 }
 
 int check(const char* name, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t K, int32_t score) {
@@ -233,13 +355,26 @@ extern "C" int smel_select_experts(const void* logits, int64_t ldl, int32_t dtyp
   SMEL_REQUIRE(group_best == 1 || group_best == 2, SMEL_EINVAL, "select_experts: group_best %d (1 or 2)", group_best);
   if (T == 0) return 0;
   SMEL_REQUIRE(logits && topv && topi, SMEL_EINVAL, "select_experts: null pointer");
-  const SelArgs p{logits, bias,       topv,     scores,     stats,           topi,       ldl,    T,
-                  (int)E, (int)K, score, (int)groups, (int)top_groups, group_best, renorm, scale};
-  const dim3 g((unsigned)((T + 3) / 4)), b(256);
-  if (dtype == 0) select_kernel<0><<<g, b, 0, stream>>>(p);
-  else if (dtype == 1) select_kernel<1><<<g, b, 0, stream>>>(p);
-  else select_kernel<2><<<g, b, 0, stream>>>(p);
-  return smel::launch_status();
+  SelArgs p{};
+  p.z = logits;
+  p.bias = bias;
+  p.topv = topv;
+  p.scores = scores;
+  p.stats = stats;
+  p.topi = topi;
+  p.ldl = ldl;
+  p.T = T;
+  p.E = (int)E;
+  p.K = (int)K;
+  p.score = score;
+  p.best = group_best;
+  p.renorm = renorm;
+  p.drop = top_groups < groups;
+  p.parts = p.drop ? (int)groups : 1;
+  p.size = p.E / p.parts;
+  p.top_groups = (int)top_groups;
+  p.scale = scale;
+  return dtype == 0 ? launch_select<0>(p, stream) : dtype == 1 ? launch_select<1>(p, stream) : launch_select<2>(p, stream);
 }
 
 extern "C" int smel_select_experts_bwd(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t K,
@@ -250,8 +385,11 @@ extern "C" int smel_select_experts_bwd(const void* logits, int64_t ldl, int32_t 
   SMEL_REQUIRE(ldd >= E && ldd < (1 << 20), SMEL_EINVAL, "select_experts_bwd: row stride %lld for %lld experts", (long long)ldd, (long long)E);
   if (T == 0) return 0;
   SMEL_REQUIRE(logits && topi && dtopv && dlogits && (score == 0 || stats), SMEL_EINVAL, "select_experts_bwd: null pointer");
-  const SelBwdArgs p{logits, topi, dtopv, stats, dlogits, ldl, ldd, T, (int)E, (int)K, score, renorm, scale};
-  const dim3 g((unsigned)((T + 3) / 4)), b(256);
+  int lpr = 1;
+  while (lpr < 64 && (8 * lpr < E || lpr < K)) lpr *= 2;   // 8 lpr >= E, lpr >= K
+  const SelBwdArgs p{logits, topi, dtopv, stats, dlogits, ldl, ldd, T, (int)E, (int)K, score, renorm, lpr, scale};
+  const int64_t tokens = 256 / lpr;
+  const dim3 g((unsigned)((T + tokens - 1) / tokens)), b(256);
   if (dtype == 0) select_bwd_kernel<0><<<g, b, 0, stream>>>(p);
   else if (dtype == 1) select_bwd_kernel<1><<<g, b, 0, stream>>>(p);
   else select_bwd_kernel<2><<<g, b, 0, stream>>>(p);
