@@ -109,10 +109,19 @@ SMEL_DEV void run_of(const void* base, int64_t at, int n, float v[N]) {
   for (int j = 0; j < N; ++j) v[j] = j < n ? logit_at<DT>(p, j) : 0.f;
 }
 
+template <int N>
+struct Order {
+  typedef uint32_t T;
+};
+template <>
+struct Order<16> {
+  typedef uint64_t T;
+};
+
 // LT lanes a token (four tokens a wave, or one). A group's experts lie in LT / 2^k lanes next to each other, N of them at most in a
 // lane, in the order of their indices; without groups to drop, all experts are one. Each lane sorts its own, so a pick is the largest
 // of the lanes' heads: the maximum by DPP moves, the lowest lane that holds it (the lowest index: ties), and that lane goes on to its
-// next. Bound by instructions: about 25 for a pick, 15 for a score, 5 for each of a lane's N (N - 1) / 2 comparisons.
+// next. Bound by instructions: about 22 for a pick, 15 for a score, 5 for each of a lane's N (N - 1) / 2 comparisons.
 template <int DT, int LT, int N>
 __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   const int l = lane_id(), li = l & (LT - 1), base = l & ~(LT - 1);
@@ -166,13 +175,12 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   for (int i = 1; i < N; ++i)
 #pragma unroll
     for (int j = N - 1; j >= i; --j) {
-      const bool up = key[j] > key[j - 1];
-      const uint32_t hi = max(key[j], key[j - 1]), lo = min(key[j], key[j - 1]);
-      const uint32_t ah = up ? at[j] : at[j - 1], al = up ? at[j - 1] : at[j];
-      key[j - 1] = hi;
-      key[j] = lo;
-      at[j - 1] = ah;
-      at[j] = al;
+      const uint32_t k1 = key[j], k0 = key[j - 1], a1 = at[j], a0 = at[j - 1];
+      const bool up = k1 > k0;
+      key[j - 1] = max(k1, k0);
+      key[j] = min(k1, k0);
+      at[j - 1] = up ? +a1 : +a0;   // of values: a conditional of the variables themselves is one of addresses
+      at[j] = up ? +a0 : +a1;
     }
   if (p.drop) {   // groups
     float c1 = key[0] ? choice_of(key[0]) : -INFINITY, c2 = -INFINITY;
@@ -199,7 +207,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
       for (int j = 0; j < N; ++j) key[j] = 0u;
   }
   // the order of a lane's experts, four bits each
-  uint64_t next = 0;
+  typename Order<N>::T next = 0;
 #pragma unroll
   for (int j = N - 1; j >= 0; --j) next = next << 4 | at[j];
   int id = 0;   // lane k of a token keeps pick k
@@ -207,15 +215,16 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
     const uint32_t best = max_lanes<LT>(key[0]);
     const uint64_t who = __ballot(key[0] == best);
     const int head = e0 + (int)(next & 15);
-    int w, e;
+    int w;
     if constexpr (LT == 64) {
       w = __builtin_ctzll(who);
-      e = lane_get(head, w);
+      const int e = lane_get(head, w);
+      if (li == k) id = e;
     } else {
       w = __builtin_ctz((uint32_t)(who >> base) & 0xffffu);
-      e = __shfl(head, base + w, 64);
+      const int e = __shfl(head, base + w, 64);
+      if (li == k) id = e;
     }
-    if (li == k) id = e;
     if (li == w) {
 #pragma unroll
       for (int j = 0; j + 1 < N; ++j) key[j] = key[j + 1];
@@ -321,6 +330,14 @@ int launch_plan(const SelArgs& p, hipStream_t stream) {
 }
 template <int DT>
 int launch_select(SelArgs& p, hipStream_t stream) {
+  // Four tokens a wave share a pick's instructions, but wait for each other and sort longer lists. us of the kernel, a token a wave and
+  // four: 64 experts 4092 tokens 3.4, 3.3, 65536 tokens 21, 12; 128 experts 517 tokens 3.0, 3.9, 4092 4.1, 4.1, 65536 32, 21; lists of
+  // 16 (256 experts) 65536 tokens 43, 78
+  if (p.T >= 4096) {
+    const int m = lane_plan(p, 16);
+    if (m <= 4) return launch_plan<DT, 16, 4>(p, stream);
+    if (m <= 8) return launch_plan<DT, 16, 8>(p, stream);
+  }
   const int n = lane_plan(p, 64);
   if (n <= 1) return launch_plan<DT, 64, 1>(p, stream);
   if (n <= 2) return launch_plan<DT, 64, 2>(p, stream);

@@ -109,7 +109,9 @@ SHAPES = [  # T, E, K, groups, kept
     (1, 1, 1, 1, 1), (1, 256, 8, 8, 4), (3, 2, 1, 2, 1), (5, 7, 3, 1, 1), (23, 64, 4, 1, 1), (70, 96, 6, 3, 2), (33, 100, 5, 4, 2),
     (129, 128, 8, 1, 1), (40, 160, 8, 8, 3), (517, 256, 8, 8, 4), (66, 256, 16, 1, 1), (31, 300, 9, 12, 5), (20, 511, 16, 1, 1),
     (57, 512, 10, 16, 4), (19, 495, 7, 33, 9), (9, 64, 5, 64, 20), (17, 510, 3, 2, 1), (14, 512, 16, 64, 2), (301, 63, 2, 9, 9),
-    (1, 512, 16, 1, 1), (2050, 24, 2, 2, 1)]
+    (1, 512, 16, 1, 1), (2050, 24, 2, 2, 1),
+    (4096, 64, 6, 1, 1), (4097, 64, 16, 8, 3), (4098, 37, 3, 1, 1), (4099, 128, 8, 1, 1), (5003, 100, 9, 4, 3), (4100, 120, 7, 15, 5),
+    (4111, 16, 4, 16, 9), (4103, 34, 2, 17, 3), (4102, 102, 16, 17, 7), (4101, 2, 1, 1, 1)]
 
 
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
