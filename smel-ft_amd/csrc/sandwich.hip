@@ -10,45 +10,9 @@
 //
 // Layout: rows.h's chunks of 8, `lpr` threads a row (a power of two up to 64, or the block). Blocks of the backward walk over
 // the rows, the weights and their sums in registers; the blocks' sums are added by a second launch in block order.
-#include "../../include/smel_norm.h"
-#include "abi_util.h"
-#include "common.h"
-#include "rows.h"
+#include "sandwich.h"
 
 namespace {
-
-constexpr int MAX_COLS = 16384;
-enum { G_NONE = 0, G_CHANNEL = 1, G_TOKEN = 2, G_FULL = 3 };
-
-SMEL_DEV float gate_of(float z, int act) { return act ? 1.f / (1.f + expf(-z)) : z; }
-// dg/dz from z: s (1 - s) without the subtraction's loss
-SMEL_DEV float gate_slope(float z, int act) {
-  if (!act) return 1.f;
-  const float q = expf(-fabsf(z)), a = 1.f / (1.f + q);
-  return q * a * a;
-}
-// element i of rows' type DT, or of fp32
-template <int DT>
-SMEL_DEV float one_at(const void* p, int64_t i, bool f32) {
-  if (DT == 2 || f32) return ((const float*)p)[i];
-  if constexpr (DT != 2) return cvt<DT>(((const uint16_t*)p)[i]);
-  return 0.f;
-}
-
-struct SwArgs {
-  smel_sandwich c;
-  float* part;      // [blocks][nsum cols], then (8-byte aligned) a double a block for dscale
-  int lpr, nsum, at1, at2, atg;   // sums of a column: their number and places (-1: not wanted)
-};
-
-SMEL_DEV double* scale_parts(const SwArgs& a, int64_t blocks) {
-  return (double*)(a.part + ((blocks * a.nsum * a.c.cols + 1) & ~(int64_t)1));
-}
-SMEL_DEV double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 
 // w' of a chunk
 template <int WT>
@@ -138,172 +102,6 @@ __global__ __launch_bounds__(BS) void sandwich_fwd_kernel(SwArgs a) {
   }
 }
 
-template <int DT, int WT, int CPL, int BS, bool WG>
-__global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
-  typedef typename El<DT>::T T;
-  __shared__ float red[2][48];
-  __shared__ float join[WG && BS == 256 ? BS / 2 * CPL * 24 : 1];   // larger blocks are one row's
-  __shared__ double joins[16];
-  const smel_sandwich& p = a.c;
-  const int lpr = a.lpr, n = (int)p.cols, nch = (n + 7) >> 3;
-  const int groups = BS / lpr, grp = threadIdx.x / lpr, li = threadIdx.x & (lpr - 1);
-  const bool pre = p.dy != nullptr;
-  const float scale = p.scale ? one_at<DT>(p.scale, 0, p.scale_type == 2) : p.scale_value;
-  float sums[WG ? CPL * 24 : 1];   // of a chunk's columns: dw1, dw2, dgate
-  double usum = 0;                 // of dS u: its terms cancel, and a block has thousands of them
-  if constexpr (WG)
-#pragma unroll
-    for (int i = 0; i < CPL * 24; ++i) sums[i] = 0.f;
-  const int64_t step = (int64_t)gridDim.x * groups;
-  // every thread of the block takes the same number of turns (row_sums has a barrier); the sums' buffers alternate: a row's
-  // readers are done before the next but one writes
-  int par = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < p.rows; r0 += step, par ^= 1) {
-    const int64_t row = r0 + grp;
-    const bool live = row < p.rows;
-    const int64_t r = live ? row : 0, out = r * (int64_t)n;
-    Raw<DT> X[CPL], S[CPL], D[CPL], Y[CPL], G[CPL];
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      const int ck = li + lpr * k;
-      X[k] = S[k] = D[k] = Y[k] = G[k] = Raw<DT>{};
-      if (live && ck < nch) {
-        X[k] = load8<DT>((const T*)p.x + r * p.x_stride, 8 * ck, n);
-        if (p.ds) D[k] = load8<DT>((const T*)p.ds + out, 8 * ck, n);
-        if (pre) {
-          S[k] = load8<DT>((const T*)p.s + out, 8 * ck, n);
-          Y[k] = load8<DT>((const T*)p.dy + out, 8 * ck, n);
-        }
-        if (p.gate_kind == G_FULL) G[k] = load8<DT>((const T*)p.gate + out, 8 * ck, n);
-      }
-    }
-    const float r1 = live ? p.stats[2 * row] : 0.f, r2 = live && pre ? p.stats[2 * row + 1] : 0.f;
-    const float tz = p.gate_kind == G_TOKEN && live ? one_at<DT>(p.gate, row, p.gate_type == 2) : 0.f;
-    const float tg = p.gate_kind == G_TOKEN ? gate_of(tz, p.gate_act) : 1.f;
-    float abc[3] = {0.f, 0.f, 0.f};
-    float w1[8], w2[8], g[8];
-    auto weights = [&](int k) {   // of chunk k; g: the gate's value but a token's
-      const int ck = li + lpr * k;
-      norm_weight8<WT>(ck < nch ? p.w1 : nullptr, 8 * ck, n, p.plus_one, w1);
-      if (pre) norm_weight8<WT>(ck < nch ? p.w2 : nullptr, 8 * ck, n, p.plus_one, w2);
-      else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w2[j] = 0.f;
-      if (p.gate_kind == G_CHANNEL) weight8<WT>(ck < nch ? p.gate : nullptr, 8 * ck, n, 1.f, g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        g[j] = p.gate_kind == G_CHANNEL ? gate_of(g[j], p.gate_act) : p.gate_kind == G_FULL ? gate_of(G[k].at(j), p.gate_act) : 1.f;
-    };
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      weights(k);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {   // x and s are zero past the row and past the last row
-        const float q = Y[k].at(j) * w2[j], sh = S[k].at(j) * r2, v = g[j] * w1[j] * (X[k].at(j) * r1);
-        abc[0] = fmaf(q, sh, abc[0]);
-        abc[1] = fmaf(v, fmaf(r2, q, D[k].at(j)), abc[1]);
-        abc[2] = fmaf(v, sh, abc[2]);
-      }
-    }
-    row_sums(abc, lpr, red[par]);
-    const float m2 = r2 * (abc[0] / (float)n), vd = scale * (abc[1] - m2 * abc[2]);   // vd = sum of dh w1' xhat (g)
-    const float m1 = tg * vd / (float)n;
-    if (!live) continue;
-    if (p.gate_kind == G_TOKEN && p.dgate && li == 0) {
-      const float d = vd * gate_slope(tz, p.gate_act);
-      if (DT == 2 || p.gate_type == 2) ((float*)p.dgate)[row] = d;
-      else if constexpr (DT != 2) ((T*)p.dgate)[row] = (T)enc<DT>(d);
-    }
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      const int ck = li + lpr * k;
-      if (ck >= nch) continue;
-      weights(k);
-      float dh[8], dx[8], dg[8], u[8], us = 0.f;
-      if (p.dscale) {
-        const Raw<DT> H = load8<DT>((const T*)p.h + r * p.h_stride, 8 * ck, n);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = H.at(j);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float sh = S[k].at(j) * r2, xh = X[k].at(j) * r1;
-        const float ds = fmaf(r2, Y[k].at(j) * w2[j], D[k].at(j)) - m2 * sh;
-        dh[j] = scale * ds;
-        const float dn = dh[j] * g[j] * tg;
-        dx[j] = r1 * (dn * w1[j] - xh * m1);
-        dg[j] = dh[j] * xh * w1[j];
-        if (p.dscale && 8 * ck + j < n) us = fmaf(ds, fmaf(g[j] * tg, xh * w1[j], u[j]), us);
-        if constexpr (WG) {
-          sums[k * 24 + j] = fmaf(dn, xh, sums[k * 24 + j]);
-          sums[k * 24 + 8 + j] = fmaf(Y[k].at(j), sh, sums[k * 24 + 8 + j]);
-          sums[k * 24 + 16 + j] += dg[j];
-        }
-      }
-      usum += (double)us;
-      Raw<DT> o;
-      if (p.dh) {
-        o.set(dh);
-        store8<DT>((T*)p.dh + out, 8 * ck, n, o);
-      }
-      if (p.dx) {
-        o.set(dx);
-        store8<DT>((T*)p.dx + out, 8 * ck, n, o);
-      }
-      if (p.gate_kind == G_FULL && p.dgate) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dg[j] *= gate_slope(G[k].at(j), p.gate_act);
-        o.set(dg);
-        store8<DT>((T*)p.dgate + out, 8 * ck, n, o);
-      }
-    }
-  }
-  if (p.dscale) {   // the block's sum of dS u
-    usum = wave_sum64(usum);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) joins[threadIdx.x >> 6] = usum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < BS / 64; ++w) usum += joins[w];
-      scale_parts(a, gridDim.x)[blockIdx.x] = usum;
-    }
-  }
-  if constexpr (WG) {
-    for (int half = groups / 2; half >= 1; half /= 2) {
-      __syncthreads();
-      if (grp >= half && grp < 2 * half)
-#pragma unroll
-        for (int i = 0; i < CPL * 24; ++i) join[((grp - half) * lpr + li) * (CPL * 24) + i] = sums[i];
-      __syncthreads();
-      if (grp < half)
-#pragma unroll
-        for (int i = 0; i < CPL * 24; ++i) sums[i] += join[(grp * lpr + li) * (CPL * 24) + i];
-    }
-    if (grp == 0) {
-      float* const o = a.part + (int64_t)blockIdx.x * a.nsum * n;
-      const int at[3] = {a.at1, a.at2, a.atg};
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        const int e = 8 * (li + lpr * k);
-        if (e >= n) continue;
-        if (p.gate_kind == G_CHANNEL && p.gate_act) {
-          float z[8];
-          weight8<WT>(p.gate, e, n, 1.f, z);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) sums[k * 24 + 16 + j] *= gate_slope(z[j], 1);
-        }
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          if (at[i] < 0) continue;
-          Raw<2> v;
-          v.set(sums + k * 24 + 8 * i);
-          store8<2, true>(o + (int64_t)at[i] * n, e, n, v);
-        }
-      }
-    }
-  }
-}
-
 // columns of part [blocks][nsum n] summed: a wave's lanes take 64 columns, the 16 waves a 16th of the blocks each; the last block
 // adds the blocks' sums for dscale
 template <int DT, int WT>
@@ -342,9 +140,6 @@ __global__ __launch_bounds__(1024) void sandwich_wsum_kernel(SwArgs a, int block
 
 // ------------------------------------------------------------------------------------------------ host
 
-struct Shape {
-  int lpr, cpl, bs;
-};
 Shape fwd_shape(int64_t cols) {
   const int nch = (int)((cols + 7) / 8);   // <= 2048
   Shape s{1, 1, 256};
@@ -354,34 +149,11 @@ Shape fwd_shape(int64_t cols) {
   while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 4
   return s;
 }
-// a chunk per thread where 1024 threads reach
-Shape bwd_shape(int64_t cols) {
-  const int nch = (int)((cols + 7) / 8);
-  Shape s{1, 1, 256};
-  while (s.lpr < nch && s.lpr < 1024) s.lpr *= 2;
-  if (s.lpr > 256) s.bs = s.lpr;
-  while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 2
-  return s;
-}
-int64_t bwd_blocks(int64_t rows, int64_t cols) {
-  const Shape s = bwd_shape(cols);
-  const int64_t turns = (rows + s.bs / s.lpr - 1) / (s.bs / s.lpr);
-  const int64_t most = s.bs == 256 ? 768 : s.bs == 512 ? 512 : 256;
-  return turns < most ? turns : most;
-}
-
 template <int DT, int WT, int CPL, int BS>
 int launch_fwd(const SwArgs& a, hipStream_t stream) {
   const int64_t rpb = BS / a.lpr, blocks = (a.c.rows + rpb - 1) / rpb;
   SMEL_REQUIRE(blocks * BS < (int64_t)1 << 32, SMEL_EUNSUPPORTED, "sandwich_fwd: %lld rows is too many", (long long)a.c.rows);
   sandwich_fwd_kernel<DT, WT, CPL, BS><<<(unsigned)blocks, BS, 0, stream>>>(a);
-  return smel::launch_status();
-}
-template <int DT, int WT, int CPL, int BS>
-int launch_bwd(const SwArgs& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)bwd_blocks(a.c.rows, a.c.cols);
-  if (a.nsum) sandwich_bwd_kernel<DT, WT, CPL, BS, true><<<blocks, BS, 0, stream>>>(a);
-  else sandwich_bwd_kernel<DT, WT, CPL, BS, false><<<blocks, BS, 0, stream>>>(a);
   return smel::launch_status();
 }
 template <int DT, int WT>
@@ -396,12 +168,7 @@ struct Launch {
   static int bwd(SwArgs& a, hipStream_t st) {
     int64_t blocks = 0;
     if (a.c.rows > 0) {
-      const Shape s = bwd_shape(a.c.cols);
-      a.lpr = s.lpr;
-      const int rc = s.bs == 256   ? launch_bwd<DT, WT, 1, 256>(a, st)
-                     : s.bs == 512 ? launch_bwd<DT, WT, 1, 512>(a, st)
-                     : s.cpl == 1  ? launch_bwd<DT, WT, 1, 1024>(a, st)
-                                   : launch_bwd<DT, WT, 2, 1024>(a, st);
+      const int rc = DT == 0 ? smel::sandwich_bwd_bf16(a, st) : DT == 1 ? smel::sandwich_bwd_f16(a, st) : smel::sandwich_bwd_f32(a, st);
       if (rc) return rc;
       blocks = bwd_blocks(a.c.rows, a.c.cols);
     }
