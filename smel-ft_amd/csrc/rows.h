@@ -127,14 +127,15 @@ SMEL_DEV void weight8(const void* p, int e0, int n, float one, float v[8]) {
   for (int j = 0; j < 8; ++j) v[j] = r.at(j);
 }
 
-// sums over the lpr threads of a row: xor butterfly over its lanes, then the row's waves in order. red: 16 floats a value
-template <int N>
+// sums over the lpr threads of a row: xor butterfly over its lanes, then the row's waves in order. red: 16 floats a value. lpr is a
+// power of two, or the whole block's threads (ONE: its only row)
+template <int N, bool ONE = false>
 SMEL_DEV void row_sums(float (&v)[N], int lpr, float* red) {
   for (int o = 1; o < lpr && o < 64; o <<= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
   if (lpr > 64) {
-    const int wave = threadIdx.x >> 6, nw = lpr >> 6, w0 = wave & ~(nw - 1);
+    const int wave = threadIdx.x >> 6, nw = lpr >> 6, w0 = ONE ? 0 : wave & ~(nw - 1);
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) red[i * 16 + wave] = v[i];

@@ -69,18 +69,22 @@ SMEL_DEV double wave_sum64(double v) {
 struct Shape {
   int lpr, cpl, bs;
 };
-// a chunk per thread where 1024 threads reach
+// The threads of a row: a power of two up to 256, several rows a block; above 2048 columns the block, as many waves as it needs. A
+// chunk per thread, two above 8192 columns. bs: the kernel's most threads.
 Shape bwd_shape(int64_t cols) {
   const int nch = (int)((cols + 7) / 8);
-  Shape s{1, 1, 256};
-  while (s.lpr < nch && s.lpr < 1024) s.lpr *= 2;
-  if (s.lpr > 256) s.bs = s.lpr;
-  while (s.cpl * s.lpr < nch) s.cpl *= 2;   // <= 2
+  Shape s{1, nch > 1024 ? 2 : 1, 256};
+  if (nch <= 256) {
+    while (s.lpr < nch) s.lpr *= 2;
+    return s;
+  }
+  s.lpr = ((nch + s.cpl - 1) / s.cpl + 63) / 64 * 64;
+  s.bs = s.lpr <= 512 && s.cpl == 1 ? 512 : 1024;
   return s;
 }
-int64_t bwd_blocks(int64_t rows, int64_t cols) {
+int64_t bwd_blocks(int64_t rows, int64_t cols, bool sums) {
   const Shape s = bwd_shape(cols);
-  const int64_t turns = (rows + s.bs / s.lpr - 1) / (s.bs / s.lpr);
+  const int64_t rpb = s.bs == 256 ? 256 / s.lpr : 1, turns = (rows + rpb - 1) / rpb;
   const int64_t most = s.bs == 256 ? 768 : s.bs == 512 ? 512 : 256;
   return turns < most ? turns : most;
 }

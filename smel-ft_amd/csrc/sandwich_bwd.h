@@ -15,14 +15,15 @@ SMEL_DEV void chunk_weight8(int wtype, const void* p, int e0, int n, int plus_on
 }
 
 template <int DT, int CPL, int BS, int GK, bool PRE, bool WG>
-__global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
+__global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwArgs a) {
   typedef typename El<DT>::T T;
   __shared__ float red[2][48];
   __shared__ float join[WG && BS == 256 ? BS / 2 * CPL * 24 : 1];   // larger blocks are one row's
   __shared__ double joins[16];
   const smel_sandwich& p = a.c;
   const int lpr = a.lpr, n = (int)p.cols, nch = (n + 7) >> 3;
-  const int groups = BS / lpr, grp = threadIdx.x / lpr, li = threadIdx.x & (lpr - 1);
+  constexpr bool ONE = BS > 256;      // a row a block, of as many waves as it needs
+  const int groups = ONE ? 1 : BS / lpr, grp = ONE ? 0 : threadIdx.x / lpr, li = ONE ? threadIdx.x : threadIdx.x & (lpr - 1);
   const float scale = p.scale ? one_at<DT>(p.scale, 0, p.scale_type == 2) : p.scale_value;
   // the weights stay in registers where a thread has one chunk
   constexpr bool HOLD = CPL == 1;
@@ -43,12 +44,10 @@ __global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
   if constexpr (WG)
 #pragma unroll
     for (int i = 0; i < CPL * 24; ++i) sums[i] = 0.f;
-  // PF rows on their way: buffer f is refilled as soon as its row is done with, PF - 1 rows before it is used again
-  constexpr int PF = CPL == 2 || (DT == 2 && BS == 1024) ? 1 : 2;
   struct Row {
     Raw<DT> x[CPL], d[CPL], s[PRE ? CPL : 1], y[PRE ? CPL : 1], g[GK == G_FULL ? CPL : 1];
     float r1, r2, tz;
-  } buf[PF];
+  };
   auto fetch = [&](Row& b, int64_t row) {
     const bool ok = row < p.rows;
     const int64_t r = ok ? row : 0, out = r * (int64_t)n;
@@ -103,7 +102,7 @@ __global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
         }
       }
     }
-    row_sums(abc, lpr, rd);
+    row_sums<PRE ? 3 : 1, ONE>(abc, lpr, rd);
     const float m2 = PRE ? b.r2 * (abc[PRE ? 1 : 0] / (float)n) : 0.f;
     const float vd = scale * (PRE ? abc[0] - m2 * abc[PRE ? 2 : 0] : abc[0]);   // the sum of dh w1' xhat (g)
     const float m1 = tg * vd / (float)n;
@@ -165,28 +164,21 @@ __global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
       }
     }
   };
-  const int64_t step = (int64_t)gridDim.x * groups, first = (int64_t)blockIdx.x * groups;
-#pragma unroll
-  for (int f = 0; f < PF; ++f) fetch(buf[f], first + f * step + grp);
   // every thread of the block takes the same number of turns (row_sums has a barrier); the sums' buffers alternate: a row's
   // readers are done before the next but one writes
   int par = 0;
-  for (int64_t r0 = first; r0 < p.rows; r0 += PF * step)
-#pragma unroll
-    for (int f = 0; f < PF; ++f) {
-      const int64_t row = r0 + f * step;
-      if (row >= p.rows) break;
-      one(buf[f], row + grp, red[par]);
-      par ^= 1;
-      fetch(buf[f], row + PF * step + grp);
-    }
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < p.rows; r0 += (int64_t)gridDim.x * groups, par ^= 1) {
+    Row b;
+    fetch(b, r0 + grp);
+    one(b, r0 + grp, red[par]);
+  }
   if (p.dscale) {   // the block's sum of dS u
     usum = wave_sum64(usum);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) joins[threadIdx.x >> 6] = usum;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < BS / 64; ++w) usum += joins[w];
+      for (int w = 1; w < (int)blockDim.x >> 6; ++w) usum += joins[w];
       scale_parts(a, gridDim.x)[blockIdx.x] = usum;
     }
   }
@@ -228,9 +220,9 @@ __global__ __launch_bounds__(BS) void sandwich_bwd_kernel(SwArgs a) {
 
 template <int DT, int CPL, int BS, int GK, bool PRE>
 int launch_bwd_sums(const SwArgs& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)bwd_blocks(a.c.rows, a.c.cols);
-  if (a.nsum) sandwich_bwd_kernel<DT, CPL, BS, GK, PRE, true><<<blocks, BS, 0, stream>>>(a);
-  else sandwich_bwd_kernel<DT, CPL, BS, GK, PRE, false><<<blocks, BS, 0, stream>>>(a);
+  const unsigned blocks = (unsigned)bwd_blocks(a.c.rows, a.c.cols, a.nsum || a.c.dscale);
+  if (a.nsum) sandwich_bwd_kernel<DT, CPL, BS, GK, PRE, true><<<blocks, BS == 256 ? 256 : a.lpr, 0, stream>>>(a);
+  else sandwich_bwd_kernel<DT, CPL, BS, GK, PRE, false><<<blocks, BS == 256 ? 256 : a.lpr, 0, stream>>>(a);
   return smel::launch_status();
 }
 template <int DT, int CPL, int BS, int GK>
