@@ -2,7 +2,7 @@
 //
 // The tensors travel as kernel arguments, a table a launch; a block takes chunks of their values, wherever they lie in the list. Squares
 // are summed in 64 bits: no value of 32 bits over- or underflows there, and the sum of 2^28 squares keeps its last fp32 bit. A block's
-// sum goes to the workspace, one block adds them in order: no atomics, the same bits every time.
+// sum goes to the workspace, and whoever needs the norm adds those in order: no atomics, the same bits every time.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -50,33 +50,56 @@ SMEL_DEV void each_chunk(const Jobs& js, F f) {
   }
 }
 
+// A chunk's values in registers, all of them on their way at once: thread i has the 8 from 8 i on, 8 (256 + i) on, .... Zeros behind n.
+constexpr int TURNS = CHUNK / (8 * 256);
+template <int DT>
+struct Chunk {
+  Raw<DT> r[TURNS];
+  SMEL_DEV void load(const void* in, int64_t at, int n) {
+    const typename El<DT>::T* const p = (const typename El<DT>::T*)in + at;
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+      const int e = 8 * (256 * k + (int)threadIdx.x);
+      r[k] = Raw<DT>{};
+      if (e < n) r[k] = load8<DT>(p, e, n);
+    }
+  }
+};
 template <int DT>
 SMEL_DEV double squares(const void* in, int64_t at, int n) {
-  const typename El<DT>::T* const p = (const typename El<DT>::T*)in + at;
+  Chunk<DT> c;
+  c.load(in, at, n);
   double v = 0;
-  for (int e = 8 * threadIdx.x; e < n; e += 8 * 256) {
-    const Raw<DT> r = load8<DT>(p, e, n);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v = __builtin_fma((double)r.at(j), (double)r.at(j), v);
-  }
+  for (int k = 0; k < TURNS; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v = __builtin_fma((double)c.r[k].at(j), (double)c.r[k].at(j), v);
   return v;
 }
 template <int DT>
 SMEL_DEV uint32_t largest(const void* in, int64_t at, int n) {   // bits of |x|: NaN is above infinity
-  const typename El<DT>::T* const p = (const typename El<DT>::T*)in + at;
+  Chunk<DT> c;
+  c.load(in, at, n);
   uint32_t v = 0;
-  for (int e = 8 * threadIdx.x; e < n; e += 8 * 256) {
-    const Raw<DT> r = load8<DT>(p, e, n);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v = max(v, __float_as_uint(fabsf(r.at(j))));
-  }
+  for (int k = 0; k < TURNS; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v = max(v, __float_as_uint(fabsf(c.r[k].at(j))));
   return v;
 }
 
-SMEL_DEV double wave_sum64(double v) {
+template <bool INF>
+SMEL_DEV double joined(double a, double b) {
+  return INF ? (b > a || b != b ? b : a) : a + b;     // the largest, NaN above all; or the sum
+}
+// of the 256 threads' v, in a fixed order, for all of them
+template <bool INF>
+SMEL_DEV double block_total(double v, double* red) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  for (int o = 32; o >= 1; o >>= 1) v = joined<INF>(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return joined<INF>(joined<INF>(red[0], red[1]), joined<INF>(red[2], red[3]));
 }
 
 template <bool INF>
@@ -90,52 +113,56 @@ __global__ __launch_bounds__(256) void norm_parts_kernel(Jobs js, double* __rest
     else
       v += e.dtype == 0 ? squares<0>(e.in, at, n) : e.dtype == 1 ? squares<2>(e.in, at, n) : squares<1>(e.in, at, n);
   });
-  if constexpr (INF) {
-    m = wave_max_u32(m);
-    v = (double)__uint_as_float(m);
-  } else {
-    v = wave_sum64(v);
-  }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int k = 1; k < 4; ++k) v = INF ? (red[k] > v || red[k] != red[k] ? red[k] : v) : v + red[k];
-  part[blockIdx.x] = v;
+  if constexpr (INF) v = (double)__uint_as_float(m);
+  v = block_total<INF>(v, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = v;
 }
 
-// the norm from the parts [n], and the factor behind it: part[n]
+// the parts [n] as one, eight loads at a time
 template <bool INF>
-__global__ __launch_bounds__(256) void norm_total_kernel(double* __restrict__ part, int n, double max_norm, double eps,
-                                                         float* __restrict__ norm) {
-  __shared__ double red[256];
+SMEL_DEV double parts_total(const double* __restrict__ part, int n, double* red) {
   double v = 0;
-  for (int i = threadIdx.x; i < n; i += 256) v = INF ? (part[i] > v || part[i] != part[i] ? part[i] : v) : v + part[i];
-  red[threadIdx.x] = v;
-  __syncthreads();
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += 256) v = joined<INF>(v, part[i]);
+  return block_total<INF>(v, red);
+}
+// one part of many, or (norm given) the norm itself
+template <bool INF>
+__global__ __launch_bounds__(256) void norm_total_kernel(const double* __restrict__ part, int n, double* __restrict__ total,
+                                                         float* __restrict__ norm) {
+  __shared__ double red[4];
+  const double v = parts_total<INF>(part, n, red);
   if (threadIdx.x != 0) return;
-  for (int i = 1; i < 256; ++i) v = INF ? (red[i] > v || red[i] != red[i] ? red[i] : v) : v + red[i];
-  if (!INF) v = sqrt(v);
-  *norm = (float)v;
-  const double c = max_norm / (v + eps);
-  part[n] = c >= 1.0 ? 1.0 : c;     // NaN stays
+  if (norm) *norm = (float)(INF ? v : sqrt(v));
+  else *total = v;
 }
 
 template <int DT>
 SMEL_DEV void scaled(const Entry& en, int64_t at, int n, float c) {
   typedef typename El<DT>::T T;
-  const T* const p = (const T*)en.in + at;
   T* const o = (T*)en.out + at;
-  for (int e = 8 * threadIdx.x; e < n; e += 8 * 256) {
-    Raw<DT> r = load8<DT>(p, e, n);
+  Chunk<DT> x;
+  x.load(en.in, at, n);
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    const int e = 8 * (256 * k + (int)threadIdx.x);
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = r.at(j) * c;
-    r.set(v);
-    store8<DT>(o, e, n, r);
+    for (int j = 0; j < 8; ++j) v[j] = x.r[k].at(j) * c;
+    x.r[k].set(v);
+    if (e < n) store8<DT>(o, e, n, x.r[k]);
   }
 }
-__global__ __launch_bounds__(256) void scale_kernel(Jobs js, const double* __restrict__ factor) {
-  const float c = (float)*factor;
+// Every block adds up the parts itself (a few kilobytes from the L2): a launch less, and no wait for it
+template <bool INF>
+__global__ __launch_bounds__(256) void scale_kernel(Jobs js, const double* __restrict__ part, int n_parts, double max_norm, double eps,
+                                                    float* __restrict__ norm) {
+  __shared__ double red[4];
+  double v = parts_total<INF>(part, n_parts, red);
+  if (!INF) v = sqrt(v);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+  const double f = max_norm / (v + eps);
+  const float c = f >= 1.0 ? 1.f : (float)f;     // NaN stays
   each_chunk(js, [&](const Entry& e, int64_t at, int n) {
     if (c == 1.f && e.in == e.out) return;
     if (e.dtype == 0) scaled<0>(e, at, n, c);
@@ -234,8 +261,8 @@ int each(const smel_clip_job* jobs, int32_t n, F f) {
   return 0;
 }
 
-int norm_launches(const char* name, const smel_clip_job* jobs, int32_t n, int32_t type, double max_norm, double eps, float* norm,
-                  void* ws, int64_t ws_bytes, int64_t& parts, hipStream_t stream) {
+int parts_launches(const char* name, const smel_clip_job* jobs, int32_t n, int32_t type, float* norm, void* ws, int64_t ws_bytes,
+                   int64_t& parts, hipStream_t stream) {
   SMEL_REQUIRE(type == 0 || type == 1, SMEL_EINVAL, "%s: norm type %d (0 = 2-norm, 1 = largest magnitude)", name, type);
   SMEL_REQUIRE(norm, SMEL_EINVAL, "%s: null pointer", name);
   const int64_t need = smel_clip_ws(jobs, n);
@@ -243,16 +270,17 @@ int norm_launches(const char* name, const smel_clip_job* jobs, int32_t n, int32_
                "%s: an aligned workspace of %lld bytes is needed (got %lld)", name, (long long)need, (long long)ws_bytes);
   double* const part = (double*)ws;
   parts = 0;
-  const int rc = each(jobs, n, [&](const Jobs& js) {
+  return each(jobs, n, [&](const Jobs& js) {
     const int64_t b = blocks_of(js);
     if (type) norm_parts_kernel<true><<<(unsigned)b, 256, 0, stream>>>(js, part + parts);
     else norm_parts_kernel<false><<<(unsigned)b, 256, 0, stream>>>(js, part + parts);
     parts += b;
     return smel::launch_status();
   });
-  if (rc) return rc;
-  if (type) norm_total_kernel<true><<<1, 256, 0, stream>>>(part, (int)parts, max_norm, eps, norm);
-  else norm_total_kernel<false><<<1, 256, 0, stream>>>(part, (int)parts, max_norm, eps, norm);
+}
+int total_launch(int32_t type, const double* part, int64_t parts, double* total, float* norm, hipStream_t stream) {
+  if (type) norm_total_kernel<true><<<1, 256, 0, stream>>>(part, (int)parts, total, norm);
+  else norm_total_kernel<false><<<1, 256, 0, stream>>>(part, (int)parts, total, norm);
   return smel::launch_status();
 }
 
@@ -273,7 +301,8 @@ extern "C" int smel_grad_norm(const smel_clip_job* jobs, int32_t n_jobs, int32_t
   const int rc = check("grad_norm", jobs, n_jobs);
   if (rc) return rc;
   int64_t parts;
-  return norm_launches("grad_norm", jobs, n_jobs, norm_type, 1.0, 0.0, norm, ws, ws_bytes, parts, stream);
+  const int rl = parts_launches("grad_norm", jobs, n_jobs, norm_type, norm, ws, ws_bytes, parts, stream);
+  return rl ? rl : total_launch(norm_type, (double*)ws, parts, nullptr, norm, stream);
 }
 
 extern "C" int smel_clip_grads(const smel_clip_job* jobs, int32_t n_jobs, int32_t norm_type, double max_norm, double eps, float* norm,
@@ -284,11 +313,22 @@ extern "C" int smel_clip_grads(const smel_clip_job* jobs, int32_t n_jobs, int32_
   rc = apart(jobs, n_jobs);
   if (rc) return rc;
   int64_t parts;
-  rc = norm_launches("clip_grads", jobs, n_jobs, norm_type, max_norm, eps, norm, ws, ws_bytes, parts, stream);
+  rc = parts_launches("clip_grads", jobs, n_jobs, norm_type, norm, ws, ws_bytes, parts, stream);
   if (rc) return rc;
-  const double* const factor = (const double*)ws + parts;
+  double* part = (double*)ws;
+  int64_t n_parts = parts;
+  if (parts == 0 || parts > 4 * MOST_BLOCKS) {   // nothing to scale, or more than every block should read
+    rc = total_launch(norm_type, part, parts, part + parts, parts ? nullptr : norm, stream);
+    if (rc) return rc;
+    part += parts;
+    n_parts = 1;
+  }
+  float* to = norm;     // of the first launch
   return each(jobs, n_jobs, [&](const Jobs& js) {
-    scale_kernel<<<(unsigned)blocks_of(js), 256, 0, stream>>>(js, factor);
+    const unsigned b = (unsigned)blocks_of(js);
+    if (norm_type) scale_kernel<true><<<b, 256, 0, stream>>>(js, part, (int)n_parts, max_norm, eps, to);
+    else scale_kernel<false><<<b, 256, 0, stream>>>(js, part, (int)n_parts, max_norm, eps, to);
+    to = nullptr;
     return smel::launch_status();
   });
 }

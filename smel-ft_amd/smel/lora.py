@@ -226,17 +226,17 @@ def _clip_call(grads, max_norm, norm_type, eps, inplace):
     if not first.is_cuda:
         _lib.one_device(first)
     jobs, outs, keep, back = array("q"), [], [], []
-    add, dev = jobs.extend, first.device
-    scaled = max_norm is not None
+    add, put, codes, index, like = jobs.extend, outs.append, _ORTHO_DTYPES, first.get_device(), torch.empty_like
+    copies = max_norm is not None and not inplace
     with torch.no_grad(), _lib.on_device_of(first):
         for t in ts:     # a block has hundreds: what each costs here is the call's time
             if t is None:
-                outs.append(None)
+                put(None)
                 continue
-            code = _ORTHO_DTYPES.get(t.dtype)
+            code = codes.get(t.dtype)
             if code is None or t.layout is not torch.strided:
                 raise ValueError(f"{what} takes bf16, fp16 or fp32 tensors, got {t.dtype} {t.layout}")
-            if t.device != dev:
+            if t.get_device() != index:
                 _lib.one_device(first, t)
             x = t
             if not t.is_contiguous() and not _flat(t):
@@ -244,19 +244,23 @@ def _clip_call(grads, max_norm, norm_type, eps, inplace):
                 keep.append(x)
                 if inplace:
                     back.append((t, x))
-            y = x if inplace or not scaled else torch.empty_like(x)
-            add((x.data_ptr(), y.data_ptr(), x.numel(), code))
-            outs.append(t if inplace else y)
+            at = x.data_ptr()
+            if copies:
+                x = like(x)
+                add((at, x.data_ptr(), x.numel(), code))
+                put(x)
+            else:
+                add((at, at, x.numel(), code))
+                put(t)
         n = len(jobs) // len(_CLIP_JOB)
         addr = jobs.buffer_info()[0]
         need = _lib.load().smel_clip_ws(addr, n)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        if scaled:
-            _lib.call("smel_clip_grads", addr, n, kind, float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), ws.numel(),
+        ws, norm = first.new_empty(need, dtype=torch.uint8), first.new_empty((), dtype=torch.float32)
+        if max_norm is not None:
+            _lib.call("smel_clip_grads", addr, n, kind, float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), need,
                       _lib.stream())
         else:
-            _lib.call("smel_grad_norm", addr, n, kind, norm.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream())
+            _lib.call("smel_grad_norm", addr, n, kind, norm.data_ptr(), ws.data_ptr(), need, _lib.stream())
         for t, x in back:
             t.copy_(x)
         if inplace:     # what autograd kept of them is out of date
