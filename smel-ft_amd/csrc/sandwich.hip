@@ -14,15 +14,18 @@
 
 namespace {
 
-// w' of a chunk
+// A chunk's weights as stored, or ones
 template <int WT>
-SMEL_DEV void norm_weight8(const void* p, int e0, int n, int plus_one, float v[8]) {
-  weight8<WT>(p, e0, n, 1.f, v);
-  if (plus_one && p)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += 1.f;
+SMEL_DEV Raw<WT> stored8(const void* p, int e0, int n) {
+  if (p) return load8<WT>((const typename El<WT>::T*)p, e0, n);
+  const float one[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+  Raw<WT> r;
+  r.set(one);
+  return r;
 }
 
+// Weights are loaded with the row where a thread has one or two chunks of it: a lone row waits for one round trip to memory instead of
+// three.
 template <int DT, int WT, int CPL>
 __global__ __launch_bounds__(CPL == 4 ? 512 : 256) void sandwich_fwd_kernel(SwArgs a) {
   typedef typename El<DT>::T T;
@@ -34,11 +37,19 @@ __global__ __launch_bounds__(CPL == 4 ? 512 : 256) void sandwich_fwd_kernel(SwAr
   const int li = ONE ? threadIdx.x : threadIdx.x & (lpr - 1);
   const bool live = row < p.rows;
   const int64_t r = live ? row : 0, out = r * (int64_t)n;
+  constexpr bool EARLY = CPL <= 2;
+  const float add1 = p.plus_one && p.w1 ? 1.f : 0.f, add2 = p.plus_one && p.w2 ? 1.f : 0.f;
   Raw<DT> X[CPL], H[CPL], G[CPL];
+  Raw<WT> W1[EARLY ? CPL : 1], W2[EARLY ? CPL : 1], GC[EARLY ? CPL : 1];
 #pragma unroll
   for (int k = 0; k < CPL; ++k) {
     const int ck = li + lpr * k;
     X[k] = H[k] = G[k] = Raw<DT>{};
+    if (EARLY && ck < nch) {
+      W1[EARLY ? k : 0] = stored8<WT>(p.w1, 8 * ck, n);
+      if (p.pre) W2[EARLY ? k : 0] = stored8<WT>(p.w2, 8 * ck, n);
+      if (p.gate_kind == G_CHANNEL) GC[EARLY ? k : 0] = stored8<WT>(p.gate, 8 * ck, n);
+    }
     if (live && ck < nch) {
       X[k] = load8<DT>((const T*)p.x + r * p.x_stride, 8 * ck, n);
       H[k] = load8<DT>((const T*)p.h + r * p.h_stride, 8 * ck, n);
@@ -59,18 +70,18 @@ __global__ __launch_bounds__(CPL == 4 ? 512 : 256) void sandwich_fwd_kernel(SwAr
   for (int k = 0; k < CPL; ++k) {
     const int ck = li + lpr * k;
     if (!live || ck >= nch) continue;
-    float w[8], g[8], v[8];
-    norm_weight8<WT>(p.w1, 8 * ck, n, p.plus_one, w);
+    float g[8], v[8];
+    const Raw<WT> w = EARLY ? W1[EARLY ? k : 0] : stored8<WT>(p.w1, 8 * ck, n);
     if (p.gate_kind == G_CHANNEL) {
-      weight8<WT>(p.gate, 8 * ck, n, 1.f, g);
+      const Raw<WT> c = EARLY ? GC[EARLY ? k : 0] : stored8<WT>(p.gate, 8 * ck, n);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = gate_of(g[j], p.gate_act);
+      for (int j = 0; j < 8; ++j) g[j] = gate_of(c.at(j), p.gate_act);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[j] = p.gate_kind == G_FULL ? gate_of(G[k].at(j), p.gate_act) : tg;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = scale * fmaf(g[j], X[k].at(j) * r1 * w[j], H[k].at(j));
+    for (int j = 0; j < 8; ++j) v[j] = scale * fmaf(g[j], X[k].at(j) * r1 * (w.at(j) + add1), H[k].at(j));
     H[k].set(v);
     store8<DT>((T*)p.s + out, 8 * ck, n, H[k]);
     if (p.pre)
@@ -93,10 +104,10 @@ __global__ __launch_bounds__(CPL == 4 ? 512 : 256) void sandwich_fwd_kernel(SwAr
   for (int k = 0; k < CPL; ++k) {
     const int ck = li + lpr * k;
     if (ck >= nch) continue;
-    float w[8], v[8];
-    norm_weight8<WT>(p.w2, 8 * ck, n, p.plus_one, w);
+    float v[8];
+    const Raw<WT> w = EARLY ? W2[EARLY ? k : 0] : stored8<WT>(p.w2, 8 * ck, n);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = H[k].at(j) * r2 * w[j];
+    for (int j = 0; j < 8; ++j) v[j] = H[k].at(j) * r2 * (w.at(j) + add2);
     Raw<DT> o;
     o.set(v);
     store8<DT>((T*)p.y + out, 8 * ck, n, o);

@@ -388,8 +388,10 @@ def _sw_forward(h, x, w1, w2, gate, scale, pre, rest):
     c = _sw_call(n, dt, wt, kind, act, plus_one, eps, w1, w2, gate, scale, scale_value)
     x2, R, c.x_stride = _rows_of(x, n)
     h2, _, c.h_stride = _rows_of(h, n)
-    s = x.new_empty(x.shape)
-    y = x.new_empty(x.shape) if pre else None
+    if x2 is x:
+        s, y = torch.empty_like(x), torch.empty_like(x) if pre else None
+    else:
+        s, y = x.new_empty(x.shape), x.new_empty(x.shape) if pre else None
     stats = x.new_empty(2 * R, dtype=torch.float32)     # a row's two reciprocal root mean squares
     c.x, c.h, c.s, c.y, c.stats = x2.data_ptr(), h2.data_ptr(), s.data_ptr(), _lib.ptr(y), stats.data_ptr()
     c.rows, c.pre = R, pre
@@ -410,10 +412,11 @@ def _sw_backward(ctx, ds, dy=None):
     c.rows, c.x_stride = R, n if x2.is_contiguous() else x2.stride(0)     # of what comes back: hooks on saved tensors may repack it
     ds2 = ds.contiguous() if ds is not None else None
     dy2 = dy.contiguous() if dy is not None else None
-    p, new = _lib.ptr, x2.new_empty
+    p = _lib.ptr
+    new = (lambda: torch.empty_like(x2)) if x2.shape == shape and x2.is_contiguous() else (lambda: x2.new_empty(shape))
     passed = dy is None and scale is None and scale_value == 1.0     # the stream's gradient goes through as it is
-    dh = ds if passed else new(shape) if nh else None
-    dx = new(shape) if nx else None
+    dh = ds if passed else new() if nh else None
+    dx = new() if nx else None
     dw1 = torch.empty_like(w1) if nw1 else None
     dw2 = torch.empty_like(w2) if nw2 else None
     dg = torch.empty_like(gate) if ng else None
@@ -425,7 +428,7 @@ def _sw_backward(ctx, ds, dy=None):
         c.h = h2.data_ptr()
     ws, ws_n = None, _lib.load().smel_sandwich_bwd_ws_floats(ctypes.byref(c))
     if ws_n:
-        ws = new(ws_n, dtype=torch.float32)
+        ws = x2.new_empty(ws_n, dtype=torch.float32)
     if nx or nw1 or nw2 or ng or nsc or not passed and nh:
         _lib.call("smel_sandwich_bwd", ctypes.byref(c), p(ws), ws_n, _lib.stream())
     return (dh if nh else None, dx, dw1, dw2, dg, dsc) + none
@@ -460,7 +463,9 @@ def _sandwich(h, x, w1, w2, eps, plus_one, gate, gate_act, scale, pre):
         scale, value = None, float(scale)
     rest = (*_sw_check(h, x, w1, w2, gate, scale), act, bool(plus_one), float(eps), value)
     with _lib.on_device_of(x):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, x, w1, w2, gate, scale)) or _lib.forward_mode():
+        if torch.is_grad_enabled() and (h.requires_grad or x.requires_grad or w1 is not None and w1.requires_grad
+                                        or w2 is not None and w2.requires_grad or gate is not None and gate.requires_grad
+                                        or scale is not None and scale.requires_grad) or _lib.forward_mode():
             return _lib.apply(_SandwichFn, h, x, w1, w2, gate, scale, pre, rest, None)
         _, s, y, _, _ = _sw_forward(h, x, w1, w2, gate, scale, pre, rest)
     return (s, y) if pre else s
