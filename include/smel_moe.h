@@ -419,7 +419,8 @@ int smel_router_logits(const uint16_t* x, const uint16_t* gate_w, int64_t T, int
  *   topi [T][K]: the K largest c, descending (equal ones, and equal groups: the lower index first; a NaN counts as -infinity)
  *   topv [T][K]: w_k = scale s_k / (sum of the K + 1e-20) (renorm) or scale s_k, s_k = s[topi_k] without the bias
  * The ids are always K different ones of [0, E), whatever the logits hold. A softmax row without a logit above -infinity has
- * scores 0. scores (may be null): s [T][E]. stats (may be null; softmax with a backward): a row's maximum and 1 / sum, [T][2].
+ * scores 0. scores (may be null): s [T][E]. stats (may be null; softmax with a backward): a row's maximum and the sum of e^(z - maximum)
+ * (infinity for such a row), [T][2].
  * E <= 512, K <= 16, groups <= 64, E % groups == 0, K <= top_groups E / groups, T <= 2^25. */
 int smel_select_experts(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E, int64_t K, int32_t score,
                         const float* bias, int64_t groups, int64_t top_groups, int32_t group_best, int32_t renorm, float scale,

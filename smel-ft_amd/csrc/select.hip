@@ -83,7 +83,9 @@ SMEL_DEV uint32_t max_lanes(uint32_t v) {
   if constexpr (LT == 64) return wave_max_u32(v);
   return over_lanes<LT>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
+// for the comparisons, and (rounded correctly but for e^-z) for the weights and their gradients
 SMEL_DEV float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.f + expf(-z)); }
+SMEL_DEV float weight_of(float z) { return 1.f / (1.f + expf(-z)); }
 
 // n (<= N) values from p on, zeros behind; all of them at once where there are N
 template <int DT, int N>
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   float s[N], bias[N];
   run_of<DT, N>(p.z, row * p.ldl + e0, n, s);
   if (p.bias) run_of<2, N>(p.bias, e0, n, bias);
-  float m = 0.f, inv = 0.f;
+  float m = 0.f, total = 1.f;
   if (p.score == 0) {
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = sigmoid_of(s[j]);
@@ -145,19 +147,26 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
       if (j < n) m = fmaxf(m, s[j]);
     m = over_lanes<LT>(m, [](float a, float b) { return fmaxf(a, b); });
     if (!(m > -INFINITY)) m = 0.f;
-    float sum = 0.f;
+    float sum = 0.f;   // by fours
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      s[j] = expf(s[j] - m);
-      if (j < n) sum += s[j];
+    for (int i = 0; i < N; i += 4) {
+      float four = 0.f;
+#pragma unroll
+      for (int j = i; j < (i + 4 < N ? i + 4 : N); ++j) {
+        s[j] = expf(s[j] - m);
+        if (j < n) four += s[j];
+      }
+      sum += four;
     }
     sum = sum_lanes<LT>(sum);
-    inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f) sum = INFINITY;     // no logit above -infinity: scores 0
+    total = sum;
+    const float inv = 1.f / sum;
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] *= inv;
     if (p.stats && live && li == 0) {
       p.stats[2 * t] = m;
-      p.stats[2 * t + 1] = inv;
+      p.stats[2 * t + 1] = sum;
     }
   }
   if (p.scores && live)
@@ -235,7 +244,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   float w = 0.f;
   if (li < p.K) {
     const float z = logit_at<DT>(p.z, row * p.ldl + id);
-    w = p.score == 0 ? sigmoid_of(z) : expf(z - m) * inv;
+    w = p.score == 0 ? weight_of(z) : expf(z - m) / total;
   }
   const float sum = sum_lanes<16>(w);   // K <= 16
   if (live && li < p.K) {
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
   if (p.score && 8 * li < p.E) z = load8<DT>((const T*)p.z + row * p.ldl, 8 * li, p.E);
   f32x4_t* const own = (f32x4_t*)(mine + 8 * li);
   own[0] = own[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const float m = p.score ? p.stats[2 * row] : 0.f, inv = p.score ? p.stats[2 * row + 1] : 0.f;
+  const float m = p.score ? p.stats[2 * row] : 0.f, total = p.score ? p.stats[2 * row + 1] : 1.f;
   int id = -1;
   float d = 0.f, s = 0.f, slope = 1.f;   // lane k: pick k
   if (li < p.K) {
@@ -279,11 +288,11 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
       d = p.scale * p.dtopv[row * p.K + li];
       const float zk = logit_at<DT>(p.z, row * p.ldl + id);
       if (p.score == 0) {
-        s = sigmoid_of(zk);
+        s = weight_of(zk);
         const float q = expf(-fabsf(zk)), a = __builtin_amdgcn_rcpf(1.f + q);
         slope = q * a * a;
       } else {
-        s = expf(zk - m) * inv;
+        s = expf(zk - m) / total;
       }
     }
   }
@@ -291,7 +300,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
     for (int o = 1; o < lpr; o <<= 1) v += __shfl_xor(v, o, 64);
     return v;
   };
-  if (p.renorm) {
+  if (p.renorm) {   // K = 1: the weight is a constant, and the difference what is left of d s / s
     const float S = sum(s) + SUM_EPS, dot = sum(d * s);
     d = (d - dot / S) / S;
   }
@@ -300,9 +309,11 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
   if (!live) return;
   const f32x4_t a = own[0], b = own[1];
   float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  if (p.score)
+  if (p.score) {
+    const float inv = 1.f / total;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 8 * li + j < p.E ? expf(z.at(j) - m) * inv * (v[j] - all) : 0.f;
+  }
   Raw<DT> o;
   o.set(v);
   T* const out = (T*)p.dz + t * p.ldd;
