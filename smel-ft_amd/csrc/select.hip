@@ -63,8 +63,8 @@ SMEL_DEV float dpp(float v) {
 }
 constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
 template <int LT, typename T, typename F>
-SMEL_DEV T over_lanes(T v, F f) {
-  v = f(v, dpp<XOR1>(v));
+SMEL_DEV T over_lanes(T v, F f, int from = 1) {   // from 2: pairs agree already
+  if (from < 2) v = f(v, dpp<XOR1>(v));
   v = f(v, dpp<XOR2>(v));
   v = f(v, dpp<HALF_MIRROR>(v));
   v = f(v, dpp<MIRROR>(v));
@@ -111,6 +111,36 @@ SMEL_DEV void run_of(const void* base, int64_t at, int n, float v[N]) {
   for (int j = 0; j < N; ++j) v[j] = j < n ? logit_at<DT>(p, j) : 0.f;
 }
 
+// The sum of a softmax's terms (n of a lane's N): neighbours in pairs, pairs of pairs, ...; from 128 experts on fours are added up one
+// after the other first. For powers of two up to 256 that is one order, however many lanes a token has: with one pick and
+// renormalised weights the gradient is nothing but the roundings of d s / s, and those do not change with the batch.
+template <int LT, int N>
+SMEL_DEV float row_total(const float (&s)[N], int n, int E) {
+  float v[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = j < n ? s[j] : 0.f;
+  if constexpr (N == 1) return sum_lanes<LT>(v[0]);
+  if constexpr (N == 2) {
+    float a = v[0] + v[1];
+    if (E >= 128) {   // the even lane of two goes on with the other's
+      const float c = dpp<XOR1>(v[0]), d = dpp<XOR1>(v[1]);
+      a = lane_id() & 1 ? (c + d + v[0]) + v[1] : (a + c) + d;
+      a = over_lanes<LT>(a, [](float p, float q) { return p + q; }, 2);
+      return a;
+    }
+    return sum_lanes<LT>(a);
+  }
+  float q[N / 4 > 0 ? N / 4 : 1];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    q[i] = E >= 128 ? ((v[4 * i] + v[4 * i + 1]) + v[4 * i + 2]) + v[4 * i + 3] : (v[4 * i] + v[4 * i + 1]) + (v[4 * i + 2] + v[4 * i + 3]);
+#pragma unroll
+  for (int o = 1; o < N / 4; o *= 2)
+#pragma unroll
+    for (int i = 0; i + o < N / 4; i += 2 * o) q[i] += q[i + o];
+  return sum_lanes<LT>(q[0]);
+}
+
 template <int N>
 struct Order {
   typedef uint32_t T;
@@ -147,18 +177,9 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
       if (j < n) m = fmaxf(m, s[j]);
     m = over_lanes<LT>(m, [](float a, float b) { return fmaxf(a, b); });
     if (!(m > -INFINITY)) m = 0.f;
-    float sum = 0.f;   // by fours
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      float four = 0.f;
-#pragma unroll
-      for (int j = i; j < (i + 4 < N ? i + 4 : N); ++j) {
-        s[j] = expf(s[j] - m);
-        if (j < n) four += s[j];
-      }
-      sum += four;
-    }
-    sum = sum_lanes<LT>(sum);
+    for (int j = 0; j < N; ++j) s[j] = expf(s[j] - m);
+    float sum = row_total<LT, N>(s, n, p.E);
     if (sum == 0.f) sum = INFINITY;     // no logit above -infinity: scores 0
     total = sum;
     const float inv = 1.f / sum;

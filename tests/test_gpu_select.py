@@ -443,3 +443,24 @@ def test_route_grouped_edges():
     assert scores.shape == (1, 16) and topi.shape == (1, 2) and torch.autograd.grad(topv.sum() + scores.sum() * 0, x)[0].shape == (1, 64)
     with pytest.raises(ValueError):
         route_grouped(x.cpu(), w, 2)
+
+
+@pytest.mark.parametrize("E,K", [(16, 1), (64, 1), (128, 3), (256, 8)])
+def test_rows_do_not_depend_on_the_batch(E, K):
+    """A token's results are the same bits alone and among many (powers of two of experts, whatever lanes a token gets)."""
+    z, bias, d = logits_of(4500, E, torch.float32, E)
+    for score in ("sigmoid", "softmax"):
+        for groups, kept in ((1, 1), (4, 2)):
+            many = run(z, bias, d[:, :K], K, score=score, groups=groups, top_groups=kept)
+            few = run(z[:70], bias, d[:70, :K], K, score=score, groups=groups, top_groups=kept)
+            assert all(torch.equal(a[:70], b) for a, b in zip(many, few))
+
+
+def test_one_renormalised_pick():
+    """K = 1 with renormalised weights: the weight is the scale, its gradient zero but for the rounding of d s / s."""
+    for score in ("sigmoid", "softmax"):
+        z, bias, d = logits_of(300, 64, torch.float32, 2)
+        topv, topi, dz = run(z, bias, d[:, :1], 1, score=score, scale=2.5)
+        close(topv, *(t.expand(300, 1) for t in (torch.tensor([[2.5]], dtype=torch.float64), torch.tensor([[8 * U]], dtype=torch.float64))), "topv")
+        s = scores64(z, score).gather(1, topi.cpu())
+        assert (dz.cpu().double().abs() <= 4 * U * 2.5 * d[:, :1].double().abs() / s * s.clamp(max=1)).all()
