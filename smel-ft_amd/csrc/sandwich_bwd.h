@@ -25,8 +25,10 @@ __global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwA
   constexpr bool ONE = BS > 256;      // a row a block, of as many waves as it needs
   const int groups = ONE ? 1 : BS / lpr, grp = ONE ? 0 : threadIdx.x / lpr, li = ONE ? threadIdx.x : threadIdx.x & (lpr - 1);
   const float scale = p.scale ? one_at<DT>(p.scale, 0, p.scale_type == 2) : p.scale_value;
-  // the weights stay in registers where a thread has one chunk
-  constexpr bool HOLD = CPL == 1;
+  // The weights stay in registers where a thread has one chunk, and so does the row. 1024 threads leave a thread of two chunks 128
+  // registers: the weights are read again after the row's sums, and 16-bit rows too, from the caches (4000 x 16384 bf16 with the
+  // weights' sums 363 -> 228 us; fp32 rows are kept: 507 us, read again 599)
+  constexpr bool HOLD = CPL == 1, KEEP = HOLD || DT == 2;
   float w1[8], w2[8], gc[8];
   auto weights = [&](int k) {
     const int ck = li + lpr * k;
@@ -44,71 +46,67 @@ __global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwA
   if constexpr (WG)
 #pragma unroll
     for (int i = 0; i < CPL * 24; ++i) sums[i] = 0.f;
-  struct Row {
-    Raw<DT> x[CPL], d[CPL], s[PRE ? CPL : 1], y[PRE ? CPL : 1], g[GK == G_FULL ? CPL : 1];
-    float r1, r2, tz;
+  struct Chunk {
+    Raw<DT> x, d, s, y, g;
   };
-  auto fetch = [&](Row& b, int64_t row) {
-    const bool ok = row < p.rows;
-    const int64_t r = ok ? row : 0, out = r * (int64_t)n;
-    b.r1 = ok ? p.stats[2 * row] : 0.f;
-    b.r2 = ok && PRE ? p.stats[2 * row + 1] : 0.f;
-    b.tz = GK == G_TOKEN && p.gate_kind == G_TOKEN && ok ? one_at<DT>(p.gate, row, p.gate_type == 2) : 0.f;
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      const int ck = li + lpr * k;
-      const bool in = ok && ck < nch;
-      b.x[k] = b.d[k] = Raw<DT>{};
-      if (in) b.x[k] = load8<DT>((const T*)p.x + r * p.x_stride, 8 * ck, n);
-      if (in && p.ds) b.d[k] = load8<DT>((const T*)p.ds + out, 8 * ck, n);
-      if constexpr (PRE) {
-        b.s[k] = b.y[k] = Raw<DT>{};
-        if (in) {
-          b.s[k] = load8<DT>((const T*)p.s + out, 8 * ck, n);
-          b.y[k] = load8<DT>((const T*)p.dy + out, 8 * ck, n);
-        }
-      }
-      if constexpr (GK == G_FULL) {
-        b.g[k] = Raw<DT>{};
-        if (in) b.g[k] = load8<DT>((const T*)p.gate + out, 8 * ck, n);
-      }
+  auto fetch = [&](Chunk& c, int64_t row, int k) {
+    const int ck = li + lpr * k;
+    const bool in = row < p.rows && ck < nch;
+    const int64_t r = in ? row : 0, out = r * (int64_t)n;
+    c.x = c.d = c.s = c.y = c.g = Raw<DT>{};
+    if (in) c.x = load8<DT>((const T*)p.x + r * p.x_stride, 8 * ck, n);
+    if (in && p.ds) c.d = load8<DT>((const T*)p.ds + out, 8 * ck, n);
+    if (PRE && in) {
+      c.s = load8<DT>((const T*)p.s + out, 8 * ck, n);
+      c.y = load8<DT>((const T*)p.dy + out, 8 * ck, n);
     }
+    if (GK == G_FULL && in) c.g = load8<DT>((const T*)p.gate + out, 8 * ck, n);
   };
-  auto one = [&](Row& b, int64_t row, float* rd) {
+  auto one = [&](int64_t row, float* rd) {
     const bool live = row < p.rows;
-    const float tg = GK == G_TOKEN && p.gate_kind == G_TOKEN ? gate_of(b.tz, p.gate_act) : 1.f;
-    float gv[GK == G_FULL ? 8 : 1], gs[GK == G_FULL ? 8 : 1];   // a chunk's gate and its slope: worked out once where they stay
-    auto gates = [&](int k) {
+    Chunk chunks[KEEP ? CPL : 1];
+    if constexpr (KEEP)
+#pragma unroll
+      for (int k = 0; k < CPL; ++k) fetch(chunks[k], row, k);
+    const float r1 = live ? p.stats[2 * row] : 0.f, r2 = live && PRE ? p.stats[2 * row + 1] : 0.f;
+    const bool token = GK == G_TOKEN && p.gate_kind == G_TOKEN;
+    const float tz = token && live ? one_at<DT>(p.gate, row, p.gate_type == 2) : 0.f;
+    const float tg = token ? gate_of(tz, p.gate_act) : 1.f;
+    float gv[GK == G_FULL ? 8 : 1], gs[GK == G_FULL ? 8 : 1];   // a chunk's gate and its slope
+    auto gates = [&](const Chunk& c) {
       if constexpr (GK == G_FULL)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) gv[j] = gate_of(b.g[k].at(j), p.gate_act, gs[j]);
+        for (int j = 0; j < 8; ++j) gv[j] = gate_of(c.g.at(j), p.gate_act, gs[j]);
     };
     auto gate = [&](int j) { return GK == G_CHANNEL ? gc[j] : GK == G_FULL ? gv[j] : 1.f; };
     float abc[PRE ? 3 : 1] = {};
 #pragma unroll
     for (int k = 0; k < CPL; ++k) {
+      Chunk& c = chunks[KEEP ? k : 0];
+      if constexpr (!KEEP) fetch(c, row, k);
       if constexpr (!HOLD) weights(k);
-      gates(k);
+      gates(c);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {   // x and s are zero past the row and past the last row
-        const float v = gate(j) * w1[j] * (b.x[k].at(j) * b.r1);
+        const float v = gate(j) * w1[j] * (c.x.at(j) * r1);
         if constexpr (PRE) {
-          const float q = b.y[k].at(j) * w2[j], sh = b.s[k].at(j) * b.r2;
-          abc[0] = fmaf(v, fmaf(b.r2, q, b.d[k].at(j)), abc[0]);
+          const float q = c.y.at(j) * w2[j], sh = c.s.at(j) * r2;
+          abc[0] = fmaf(v, fmaf(r2, q, c.d.at(j)), abc[0]);
           abc[1] = fmaf(q, sh, abc[1]);
           abc[2] = fmaf(v, sh, abc[2]);
         } else {
-          abc[0] = fmaf(v, b.d[k].at(j), abc[0]);
+          abc[0] = fmaf(v, c.d.at(j), abc[0]);
         }
       }
     }
     row_sums<PRE ? 3 : 1, ONE>(abc, lpr, rd);
-    const float m2 = PRE ? b.r2 * (abc[PRE ? 1 : 0] / (float)n) : 0.f;
+    if constexpr (!KEEP) asm volatile("" ::: "memory");     // the chunks are read again, not kept
+    const float m2 = PRE ? r2 * (abc[PRE ? 1 : 0] / (float)n) : 0.f;
     const float vd = scale * (PRE ? abc[0] - m2 * abc[PRE ? 2 : 0] : abc[0]);   // the sum of dh w1' xhat (g)
     const float m1 = tg * vd / (float)n;
     if (!live) return;
-    if (GK == G_TOKEN && p.gate_kind == G_TOKEN && p.dgate && li == 0) {
-      const float d = vd * gate_slope(b.tz, p.gate_act);
+    if (token && p.dgate && li == 0) {
+      const float d = vd * gate_slope(tz, p.gate_act);
       if (DT == 2 || p.gate_type == 2) ((float*)p.dgate)[row] = d;
       else if constexpr (DT != 2) ((T*)p.dgate)[row] = (T)enc<DT>(d);
     }
@@ -117,9 +115,11 @@ __global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwA
     for (int k = 0; k < CPL; ++k) {
       const int ck = li + lpr * k;
       if (ck >= nch) continue;
+      Chunk& c = chunks[KEEP ? k : 0];
+      if constexpr (!KEEP) fetch(c, row, k);
       if constexpr (!HOLD) {
         weights(k);
-        gates(k);
+        gates(c);
       }
       float dh[8], dx[8], dg[8], u[8], us = 0.f;
       if (p.dscale) {
@@ -129,20 +129,20 @@ __global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwA
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float g = gate(j), xh = b.x[k].at(j) * b.r1;
-        float ds = b.d[k].at(j), sh = 0.f;
+        const float g = gate(j), xh = c.x.at(j) * r1;
+        float ds = c.d.at(j), sh = 0.f;
         if constexpr (PRE) {
-          sh = b.s[k].at(j) * b.r2;
-          ds = fmaf(b.r2, b.y[k].at(j) * w2[j], ds) - m2 * sh;
+          sh = c.s.at(j) * r2;
+          ds = fmaf(r2, c.y.at(j) * w2[j], ds) - m2 * sh;
         }
         dh[j] = scale * ds;
         const float dn = dh[j] * g * tg;
-        dx[j] = b.r1 * (dn * w1[j] - xh * m1);
+        dx[j] = r1 * (dn * w1[j] - xh * m1);
         dg[j] = dh[j] * xh * w1[j];
         if (p.dscale && 8 * ck + j < n) us = fmaf(ds, fmaf(g * tg, xh * w1[j], u[j]), us);
         if constexpr (WG) {
           sums[k * 24 + j] = fmaf(dn, xh, sums[k * 24 + j]);
-          if constexpr (PRE) sums[k * 24 + 8 + j] = fmaf(b.y[k].at(j), sh, sums[k * 24 + 8 + j]);
+          if constexpr (PRE) sums[k * 24 + 8 + j] = fmaf(c.y.at(j), sh, sums[k * 24 + 8 + j]);
           if constexpr (GK == G_CHANNEL) sums[k * 24 + 16 + j] += dg[j];
         }
       }
@@ -168,9 +168,7 @@ __global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwA
   // readers are done before the next but one writes
   int par = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < p.rows; r0 += (int64_t)gridDim.x * groups, par ^= 1) {
-    Row b;
-    fetch(b, r0 + grp);
-    one(b, r0 + grp, red[par]);
+    one(r0 + grp, red[par]);
   }
   if (p.dscale) {   // the block's sum of dS u
     usum = wave_sum64(usum);
