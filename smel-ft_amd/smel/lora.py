@@ -240,6 +240,8 @@ def _clip_call(grads, max_norm, norm_type, eps, inplace):
                 _lib.one_device(first, t)
             x = t
             if not t.is_contiguous() and not _flat(t):
+                if inplace and 0 in t.stride() and any(st == 0 and size > 1 for st, size in zip(t.stride(), t.shape)):
+                    raise ValueError(f"{what} in place: a tensor of shape {tuple(t.shape)} and strides {t.stride()} overlaps itself")
                 x = t.contiguous()
                 keep.append(x)
                 if inplace:
@@ -285,7 +287,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6
 
 def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6):
     """``clip_grads`` in place; returns the norm before. Tensors that are within the norm already are not written. The tensors must not
-    overlap (one given twice is refused)."""
+    overlap (dense ones that do, one given twice among them, are refused before anything is written; strided ones go through copies).
+    Autograd sees the change, as of any in-place operation."""
     return _clip_call(grads, max_norm, norm_type, eps, True)[1]
 
 

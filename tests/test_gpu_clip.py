@@ -231,5 +231,7 @@ def test_refusals():
     for bad in (lambda: clip_grads_([x, x], 1.0), lambda: clip_grads_([x[:60], x[59:]], 1.0), lambda: clip_grads_([x, x[10:20]], 1.0)):
         with pytest.raises(SmelError, match="overlap"):
             bad()
+    with pytest.raises(ValueError, match="overlaps itself"):
+        clip_grads_([x, torch.ones(1, 5, device=DEV).expand(7, 5)], 1.0)
     assert torch.equal(x, torch.ones(100, device=DEV))
     clip_grads_([x[:60], x[60:]], 1.0)
