@@ -82,7 +82,7 @@ Shape bwd_shape(int64_t cols) {
   s.bs = s.lpr <= 512 && s.cpl == 1 ? 512 : 1024;
   return s;
 }
-int64_t bwd_blocks(int64_t rows, int64_t cols, bool sums) {
+int64_t bwd_blocks(int64_t rows, int64_t cols) {
   const Shape s = bwd_shape(cols);
   const int64_t rpb = s.bs == 256 ? 256 / s.lpr : 1, turns = (rows + rpb - 1) / rpb;
   const int64_t most = s.bs == 256 ? 768 : s.bs == 512 ? 512 : 256;

@@ -188,7 +188,7 @@ struct Launch {
     if (a.c.rows > 0) {
       const int rc = DT == 0 ? smel::sandwich_bwd_bf16(a, st) : DT == 1 ? smel::sandwich_bwd_f16(a, st) : smel::sandwich_bwd_f32(a, st);
       if (rc) return rc;
-      blocks = bwd_blocks(a.c.rows, a.c.cols, true);
+      blocks = bwd_blocks(a.c.rows, a.c.cols);
     }
     const int64_t wb = (a.nsum * a.c.cols + 63) / 64 + (a.c.dscale ? 1 : 0);
     if (!wb) return 0;
@@ -246,7 +246,7 @@ extern "C" int64_t smel_sandwich_bwd_ws_floats(const smel_sandwich* call) {
   SwArgs a{};
   a.c = *call;
   places(a);
-  const int64_t blocks = bwd_blocks(a.c.rows, a.c.cols, true);
+  const int64_t blocks = bwd_blocks(a.c.rows, a.c.cols);
   return blocks * a.nsum * a.c.cols + (a.c.dscale ? 2 * blocks + 1 : 0);
 }
 

@@ -218,7 +218,7 @@ __global__ __launch_bounds__(BS, BS == 256 ? 3 : 4) void sandwich_bwd_kernel(SwA
 
 template <int DT, int CPL, int BS, int GK, bool PRE>
 int launch_bwd_sums(const SwArgs& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)bwd_blocks(a.c.rows, a.c.cols, a.nsum || a.c.dscale);
+  const unsigned blocks = (unsigned)bwd_blocks(a.c.rows, a.c.cols);
   if (a.nsum) sandwich_bwd_kernel<DT, CPL, BS, GK, PRE, true><<<blocks, BS == 256 ? 256 : a.lpr, 0, stream>>>(a);
   else sandwich_bwd_kernel<DT, CPL, BS, GK, PRE, false><<<blocks, BS == 256 ? 256 : a.lpr, 0, stream>>>(a);
   return smel::launch_status();

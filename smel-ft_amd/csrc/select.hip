@@ -276,6 +276,13 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   }
 }
 
+// Order of a wave's LDS accesses for its lanes that exchange values there: the hardware keeps it, the compiler must too
+SMEL_DEV void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 struct SelBwdArgs {
   const void* z;
   const int64_t* topi;
@@ -287,7 +294,7 @@ struct SelBwdArgs {
 };
 
 // lpr lanes a token, 8 columns each: lane k works out pick k's gradient and puts it into the row in LDS, each lane writes its columns.
-// A row's lanes are of one wave, whose LDS accesses take effect in order. Bound by the bytes of dz (softmax: and of z).
+// A row's lanes are of one wave. Bound by the bytes of dz (softmax: and of z).
 template <int DT>
 __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
   typedef typename El<DT>::T T;
@@ -301,6 +308,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
   if (p.score && 8 * li < p.E) z = load8<DT>((const T*)p.z + row * p.ldl, 8 * li, p.E);
   f32x4_t* const own = (f32x4_t*)(mine + 8 * li);
   own[0] = own[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  wave_lds_order();
   const float m = p.score ? p.stats[2 * row] : 0.f, total = p.score ? p.stats[2 * row + 1] : 1.f;
   int id = -1;
   float d = 0.f, s = 0.f, slope = 1.f;   // lane k: pick k
@@ -329,6 +337,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
   }
   const float all = p.score ? sum(d * s) : 0.f;
   if (id >= 0) atomicAdd(&mine[id], d * slope);
+  wave_lds_order();
   if (!live) return;
   const f32x4_t a = own[0], b = own[1];
   float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};

@@ -923,6 +923,8 @@ class _RouterLogitsFn(torch.autograd.Function):
     def backward(ctx, dlogits):
         gate_w, = ctx.saved_tensors
         T, E = dlogits.shape
+        if T == 0:
+            return dlogits.new_empty(0, gate_w.shape[1]), None
         wr = _router_ext_weight(gate_w, None)
         if wr.R != E:
             dl = torch.zeros(T, wr.R, dtype=torch.bfloat16, device=dlogits.device)

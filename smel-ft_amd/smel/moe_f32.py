@@ -294,9 +294,10 @@ class RouterLogitsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_w):
         T, E = x.shape[0], gate_w.shape[0]
-        tl, _, _ = dense_tiles(T, x.device)
         logits = torch.empty(T, E, dtype=torch.float32, device=x.device)
-        gmm(_dense(gate_w), 0, tl, x, x.shape[1], logits, E, tag="route_f32")
+        if T:
+            tl, _, _ = dense_tiles(T, x.device)
+            gmm(_dense(gate_w), 0, tl, x, x.shape[1], logits, E, tag="route_f32")
         ctx.save_for_backward(gate_w)
         return logits
 
@@ -304,9 +305,10 @@ class RouterLogitsFn(torch.autograd.Function):
     def backward(ctx, dlogits):
         gate_w, = ctx.saved_tensors
         T, (E, H) = dlogits.shape[0], gate_w.shape
-        tl, _, _ = dense_tiles(T, dlogits.device)
         dx = torch.empty(T, H, dtype=torch.float32, device=dlogits.device)
-        gmm(_dense(gate_w), 1, tl, dlogits.contiguous(), E, dx, H, tag="route_f32_bwd")
+        if T:
+            tl, _, _ = dense_tiles(T, dlogits.device)
+            gmm(_dense(gate_w), 1, tl, dlogits.contiguous(), E, dx, H, tag="route_f32_bwd")
         return dx, None
 
 

@@ -235,3 +235,19 @@ def test_refusals():
         clip_grads_([x, torch.ones(1, 5, device=DEV).expand(7, 5)], 1.0)
     assert torch.equal(x, torch.ones(100, device=DEV))
     clip_grads_([x[:60], x[60:]], 1.0)
+
+
+def test_parts_of_many_launches():
+    """More parts than every block of the scaling adds up itself (8192): they go through a launch of their own."""
+    from smel.lora import clip_grads, grad_norm
+    g = torch.Generator(device=DEV).manual_seed(3)
+    flat = 1e-3 * torch.randn(600, 140001, generator=g, device=DEV).bfloat16()
+    ts = list(flat.unbind(0))
+    n = float(torch.sqrt(flat.double().square().sum()))
+    for kind, want in ((2.0, n), (math.inf, float(flat.abs().max()))):
+        out, norm = clip_grads(ts, want / 4, kind)
+        assert abs(float(norm) - want) <= 1.01 * U * want and torch.equal(norm, grad_norm(ts, kind))
+        c = (want / 4) / (want + 1e-6)
+        ref = flat.double() * c
+        tol = (2.0 ** -8 * (1 + 2 ** -8) + 3 * U) * ref.abs() + TINY[torch.bfloat16]
+        assert ((torch.stack(out).double() - ref).abs() <= tol).all()

@@ -464,3 +464,13 @@ def test_one_renormalised_pick():
         close(topv, *(t.expand(300, 1) for t in (torch.tensor([[2.5]], dtype=torch.float64), torch.tensor([[8 * U]], dtype=torch.float64))), "topv")
         s = scores64(z, score).gather(1, topi.cpu())
         assert (dz.cpu().double().abs() <= 4 * U * 2.5 * d[:, :1].double().abs() / s * s.clamp(max=1)).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_route_grouped_without_tokens(dt):
+    from smel.moe import route_grouped
+    x = torch.empty(0, 128, device=DEV, dtype=DT[dt], requires_grad=True)
+    w = torch.randn(64, 128, device=DEV).to(DT[dt])
+    scores, topv, topi = route_grouped(x, w, 4, groups=4, top_groups=2)
+    assert scores.shape == (0, 64) and topv.shape == topi.shape == (0, 4)
+    assert torch.autograd.grad(topv, x, torch.empty_like(topv))[0].shape == (0, 128)
