@@ -71,7 +71,7 @@ int smel_layernorm_bwd(const void* dy, const void* x, int64_t rows, int64_t cols
  * x, h at row strides x_stride, h_stride, everything else contiguous; any element alignment. w1, w2 (null: 1) and a gate per channel
  * of `wtype` (the rows' dtype or 2); w' = 1 + w where plus_one. pre: with y (0: s alone). gate_kind 0 none, 1 [cols], 2 [rows] (of
  * gate_type: the rows' dtype or 2), 3 [rows][cols] (the rows' dtype); gate_act 1: g = sigmoid(gate), 0: g = gate. The scale is
- * scale_value, or the element at `scale` (of scale_type: the rows' dtype or 2). stats [rows][2]: r1, r2, written forward, read backward.
+ * scale_value, or the element at `scale` (of scale_type: the rows' dtype or 2). stats [rows][2]: r1, r2, written forward (null: not), read backward.
  * Backward: dS = ds + r2 (q - shat mean(q shat)), q = dy w2', shat = s r2; dh = scale dS; dn = dh g;
  *   dx = r1 (q1 - xhat mean(q1 xhat)), q1 = dn w1', xhat = x r1; dw1 = sum_r dn xhat, dw2 = sum_r dy shat;
  *   dgate = dh n (times g (1 - g)), summed over what the gate is broadcast over; dscale = sum of dS (h + g n)

@@ -56,7 +56,6 @@ SMEL_DEV float one_at(const void* p, int64_t i, bool f32) {
   return 0.f;
 }
 
-
 SMEL_DEV double* scale_parts(const SwArgs& a, int64_t blocks) {
   return (double*)(a.part + ((blocks * a.nsum * a.c.cols + 1) & ~(int64_t)1));
 }

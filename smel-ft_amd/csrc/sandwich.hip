@@ -98,7 +98,7 @@ __global__ __launch_bounds__(CPL == 4 ? 512 : 256) void sandwich_fwd_kernel(SwAr
     r2 = 1.f / sqrtf(ss[0] / (float)n + p.eps);
   }
   if (!live) return;
-  if (li == 0) {
+  if (p.stats && li == 0) {
     p.stats[2 * row] = r1;
     p.stats[2 * row + 1] = r2;
   }
@@ -235,7 +235,7 @@ extern "C" int smel_sandwich_fwd(const smel_sandwich* call, hipStream_t stream) 
   const int rc = check("sandwich_fwd", call);
   if (rc) return rc;
   if (call->rows == 0) return 0;
-  SMEL_REQUIRE(call->x && call->h && call->s && call->stats && (!call->pre || call->y), SMEL_EINVAL, "sandwich_fwd: null pointer");
+  SMEL_REQUIRE(call->x && call->h && call->s && (!call->pre || call->y), SMEL_EINVAL, "sandwich_fwd: null pointer");
   SwArgs a{};
   a.c = *call;
   return by_type(a.c, [&](auto l) { return decltype(l)::fwd(a, stream); });

@@ -813,25 +813,36 @@ _SCORES = {"sigmoid": 0, "softmax": 1}
 _SEL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _select_check(logits, top_k, score, bias, groups, top_groups, group_best):
-    if not logits.is_cuda:
-        L.one_device(logits)
+def _select_refuse(logits, top_k, score, bias, groups, top_groups, group_best):
+    """Raises what is wrong with the call."""
+    L.one_device(logits, bias)
     if logits.dim() != 2 or logits.dtype not in _SEL_DTYPES:
         raise ValueError(f"select_experts takes bf16, fp16 or fp32 logits [T, E], got {tuple(logits.shape)} {logits.dtype}")
     E = logits.shape[1]
     if score not in _SCORES:
         raise ValueError(f"score is 'sigmoid' or 'softmax', got {score!r}")
-    if bias is not None:
-        if not bias.is_floating_point() or tuple(bias.shape) != (E,):
-            raise ValueError(f"select_experts takes a floating bias [{E}], got {tuple(bias.shape)} {bias.dtype}")
-        if bias.device != logits.device:
-            L.one_device(logits, bias)
+    if bias is not None and (not bias.is_floating_point() or tuple(bias.shape) != (E,)):
+        raise ValueError(f"select_experts takes a floating bias [{E}], got {tuple(bias.shape)} {bias.dtype}")
     if groups < 1 or E % groups:
         raise ValueError(f"{E} experts make no {groups} groups of equal size")
     if not 1 <= top_groups <= groups or not 1 <= top_k <= top_groups * (E // groups):
         raise ValueError(f"{top_groups} of {groups} groups of {E // groups} experts give no {top_k} picks")
-    if group_best not in (1, 2):
-        raise ValueError(f"a group counts with its best 1 or 2, got {group_best}")
+    raise ValueError(f"a group counts with its best 1 or 2, got {group_best}")
+
+
+def _select_check(logits, top_k, score, bias, groups, top_groups, group_best) -> int:
+    """The score's code of a call that the kernels take; a few tokens are the host's time, so each argument is looked at once."""
+    sc = _SCORES.get(score)
+    ok = sc is not None and logits.is_cuda and logits.dtype in _SEL_DTYPES and logits.dim() == 2
+    if ok:
+        E = logits.shape[1]
+        ok = groups >= 1 and E % groups == 0 and 1 <= top_groups <= groups and 1 <= top_k <= top_groups * (E // groups) \
+            and 1 <= group_best <= 2
+        if bias is not None:
+            ok = ok and bias.dim() == 1 and bias.shape[0] == E and bias.is_floating_point() and bias.device == logits.device
+    if not ok:
+        _select_refuse(logits, top_k, score, bias, groups, top_groups, group_best)
+    return sc
 
 
 def _select_forward(z, bias, k, score, groups, top_groups, best, renorm, scale, with_scores, train):
@@ -839,7 +850,7 @@ def _select_forward(z, bias, k, score, groups, top_groups, best, renorm, scale, 
     T, E = z.shape
     if not z.is_contiguous() and (E > 1 and z.stride(1) != 1 or T > 1 and z.stride(0) < E):
         z = z.contiguous()
-    if bias is not None:
+    if bias is not None and (bias.dtype is not torch.float32 or not bias.is_contiguous()):
         bias = bias.detach().to(torch.float32).contiguous()
     topv = z.new_empty((T, k), dtype=torch.float32)
     topi = z.new_empty((T, k), dtype=torch.int64)
@@ -898,8 +909,8 @@ def select_experts(logits, top_k, score="sigmoid", bias=None, groups=1, top_grou
     their sum (``renorm``), times ``scale``. Differentiable w.r.t. the logits through topv. At most 512 experts, 64 groups, K = 16.
     Whatever the logits hold (a padded row's NaN too), topi are K different experts."""
     k, groups, top_groups, group_best = int(top_k), int(groups), int(top_groups), int(group_best)
-    _select_check(logits, k, score, bias, groups, top_groups, group_best)
-    args = (k, _SCORES[score], groups, top_groups, group_best, bool(renorm), float(scale), bool(with_scores))
+    sc = _select_check(logits, k, score, bias, groups, top_groups, group_best)
+    args = (k, sc, groups, top_groups, group_best, bool(renorm), float(scale), bool(with_scores))
     with L.on_device_of(logits):
         if torch.is_grad_enabled() and logits.requires_grad or L.forward_mode():
             return L.apply(_SelectFn, logits, bias, *args)

@@ -380,8 +380,8 @@ def _sw_call(n, dt, wt, kind, act, plus_one, eps, w1, w2, gate, scale, scale_val
     return c
 
 
-def _sw_forward(h, x, w1, w2, gate, scale, pre, rest):
-    """(the rows of x, s, y or None, stats, the contiguous gate)."""
+def _sw_forward(h, x, w1, w2, gate, scale, pre, rest, train):
+    """(the rows of x, s, y or None, stats or None, the contiguous gate)."""
     n, dt, wt, kind, act, plus_one, eps, scale_value = rest
     if gate is not None:
         gate = gate.contiguous()
@@ -392,8 +392,8 @@ def _sw_forward(h, x, w1, w2, gate, scale, pre, rest):
         s, y = torch.empty_like(x), torch.empty_like(x) if pre else None
     else:
         s, y = x.new_empty(x.shape), x.new_empty(x.shape) if pre else None
-    stats = x.new_empty(2 * R, dtype=torch.float32)     # a row's two reciprocal root mean squares
-    c.x, c.h, c.s, c.y, c.stats = x2.data_ptr(), h2.data_ptr(), s.data_ptr(), _lib.ptr(y), stats.data_ptr()
+    stats = x.new_empty(2 * R, dtype=torch.float32) if train else None     # a row's two reciprocal root mean squares
+    c.x, c.h, c.s, c.y, c.stats = x2.data_ptr(), h2.data_ptr(), s.data_ptr(), _lib.ptr(y), _lib.ptr(stats)
     c.rows, c.pre = R, pre
     _lib.call("smel_sandwich_fwd", ctypes.byref(c), _lib.stream())
     return x2, s, y, stats, gate
@@ -443,7 +443,7 @@ class _SandwichFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, x, w1, w2, gate, scale, pre, rest, _):
-        x2, s, y, stats, gate = _sw_forward(h, x, w1, w2, gate, scale, pre, rest)
+        x2, s, y, stats, gate = _sw_forward(h, x, w1, w2, gate, scale, pre, rest, True)
         ctx.save_for_backward(x2, s if pre else None, h if ctx.needs_input_grad[5] else None, w1, w2, gate, scale, stats)
         ctx.call = (pre, stats.shape[0] // 2, x.shape, rest)
         ctx.set_materialize_grads(False)
@@ -467,7 +467,7 @@ def _sandwich(h, x, w1, w2, eps, plus_one, gate, gate_act, scale, pre):
                                         or w2 is not None and w2.requires_grad or gate is not None and gate.requires_grad
                                         or scale is not None and scale.requires_grad) or _lib.forward_mode():
             return _lib.apply(_SandwichFn, h, x, w1, w2, gate, scale, pre, rest, None)
-        _, s, y, _, _ = _sw_forward(h, x, w1, w2, gate, scale, pre, rest)
+        _, s, y, _, _ = _sw_forward(h, x, w1, w2, gate, scale, pre, rest, False)
     return (s, y) if pre else s
 
 

@@ -54,10 +54,10 @@ def test_sandwich_refusals():
         assert g(rows=-1) == -1 and g(cols=0) == -1 and g(cols=16385, x_stride=1 << 20, h_stride=1 << 20) == -2
         assert g(x_stride=63) == -1 and g(h_stride=63) == -1 and g(dtype=3) == -1 and g(dtype=0, wtype=1) == -1 and g(dtype=2, wtype=0) == -1
         assert g(gate_kind=4) == -1 and g(gate_kind=1) == -1 and g(gate_kind=2, gate=16, gate_type=1) == -1
-        assert g(scale=16, scale_type=1) == -1 and g(x=None) == -1 and g(stats=None) == -1
+        assert g(scale=16, scale_type=1) == -1 and g(x=None) == -1
     assert f(h=None) == -1 and f(s=None) == -1 and f(y=None) == -1
     assert f(rows=0, x=None) == 0
-    assert b(s=None) == -1 and b(dscale=16, h=None) == -1
+    assert b(s=None) == -1 and b(stats=None) == -1 and b(dscale=16, h=None) == -1
     assert L.smel_sandwich_fwd(None, None) == -1 and L.smel_sandwich_bwd(None, None, 0, None) == -1
     need = lambda **kw: L.smel_sandwich_bwd_ws_floats(ctypes.byref(_call(**kw)))  # noqa: E731
     assert need() == 0 and need(rows=0, dw1=16) == 0 and need(cols=0) == 0
