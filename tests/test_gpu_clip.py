@@ -251,3 +251,16 @@ def test_parts_of_many_launches():
         ref = flat.double() * c
         tol = (2.0 ** -8 * (1 + 2 ** -8) + 3 * U) * ref.abs() + TINY[torch.bfloat16]
         assert ((torch.stack(out).double() - ref).abs() <= tol).all()
+
+
+def test_scalars_and_parameters():
+    """0-dimensional tensors, parameters (the results carry no gradient), and gradients that are neighbours in one buffer."""
+    from smel.lora import clip_grads, clip_grads_
+    ts = [torch.tensor(3.0, device=DEV), torch.nn.Parameter(torch.full((4,), 2.0, device=DEV))]
+    out, norm = clip_grads(ts, 1.0)
+    check([t.detach() for t in ts], out, norm, 1.0)
+    assert out[0].shape == () and not isinstance(out[1], torch.nn.Parameter)
+    flat = torch.arange(1.0, 1001.0, device=DEV)
+    want, n1 = clip_grads([flat], 5.0)
+    assert torch.equal(clip_grads_(list(flat.split([1, 7, 500, 492])), 5.0), n1)
+    assert torch.equal(flat, want[0])

@@ -473,3 +473,39 @@ def test_far_offsets():
     got = grads(*(big(v) for v in some), w=None)
     for a, b in zip(got, alone):
         assert torch.equal(a[:100], b) and torch.equal(a[-100:], b) and not a[100:103].any() and not a[-101].any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_one_tensor_in_several_places(dt):
+    """The stream, the block's output and the gate may be one tensor: its gradient is the sum of theirs (each rounded once, and the
+    sums rounded: three half steps of the parts)."""
+    t, ds, dy = make(33, 260, DT[dt], DT[dt], 21)
+    x = t["x"]
+    apart = dev({**t, "h": x.clone(), "x": x.clone(), "gate": x.clone()})
+    out = call(apart, True, True, False)
+    parts = torch.autograd.grad(out, [apart[k] for k in ("h", "x", "gate")], (ds.to(DEV), dy.to(DEV)))
+    xg = x.to(DEV).requires_grad_(True)
+    one = {**dev(t), "h": xg, "x": xg, "gate": xg}
+    same = call(one, True, True, False)
+    assert all(torch.equal(a, b) for a, b in zip(out, same))
+    dx, = torch.autograd.grad(same, xg, (ds.to(DEV), dy.to(DEV)))
+    size = sum(p.double().abs() for p in parts)
+    assert ((dx.double() - sum(p.double() for p in parts)).abs() <= 3 * half(x.dtype) * size).all()
+
+
+def test_one_column():
+    """Rows of one column: a gate of [rows, 1] is one per element of the rows' dtype, one per token in fp32."""
+    for dt in DT.values():
+        for gate_dt in (dt, torch.float32):
+            t, ds, dy = make(50, 1, dt, dt, 3, "token", "tensor", gate_dt=gate_dt)
+            check(t, ds, dy, True, True, False)
+
+
+def test_four_dimensions():
+    from smel.norm import sandwich_rmsnorm
+    g = torch.Generator().manual_seed(5)
+    h, x = (torch.randn(2, 3, 4, 72, generator=g).bfloat16().to(DEV) for _ in range(2))
+    gate = torch.randn(2, 3, 4, 1, generator=g).bfloat16().to(DEV)
+    s, y = sandwich_rmsnorm(h, x, None, None, EPS, gate=gate)
+    s2, y2 = sandwich_rmsnorm(h.view(24, 72), x.view(24, 72), None, None, EPS, gate=gate.view(24, 1))
+    assert s.shape == y.shape == h.shape and torch.equal(s.view(24, 72), s2) and torch.equal(y.view(24, 72), y2)
