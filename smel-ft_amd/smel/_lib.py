@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 
 import torch
@@ -365,3 +366,31 @@ def apply(fn, *args):
     if _transforms_active is None or _transforms_active():
         return fn.apply(*args)
     return super(torch.autograd.Function, fn).apply(*args)
+
+
+class _Once(torch.autograd.Function):
+    """A backward's results as they are, behind a node that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, _, *ts):
+        return ts
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("smel functions can be differentiated once: they have no second derivative")
+
+
+def once(backward):
+    """``backward`` of a torch.autograd.Function for ``create_graph``: its results raise when they are differentiated again. torch's
+    own once_differentiable lets them go as constants where the incoming gradient is one (a sum's), and a penalty on them is lost."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        outs = out if isinstance(out, tuple) else (out,)
+        ts = [t for t in outs if t is not None]
+        marked = iter(_Once.apply(torch.zeros((), requires_grad=True), *ts) if ts else ())
+        return tuple(None if t is None else next(marked) for t in outs)
+    return run

@@ -27,7 +27,6 @@ The gradient is computed in the forward (lm_head is frozen) and handed back by t
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .quant import dequant_int8_rows, quantize_int8_rows
@@ -454,9 +453,6 @@ def _balance_backward(ctx, go, _):
     return dz, None, None, None, None
 
 
-_balance_backward_once = once_differentiable(_balance_backward)
-
-
 class _BalanceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topi, mask, offsets, coef):
@@ -467,9 +463,7 @@ class _BalanceFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return loss, counts
 
-    @staticmethod
-    def backward(ctx, go, dcounts):     # on the forward's device: autograd's thread has set it
-        return (_balance_backward_once if torch.is_grad_enabled() else _balance_backward)(ctx, go, dcounts)
+    backward = staticmethod(L.once(_balance_backward))     # on the forward's device: autograd's thread has set it
 
 
 def balance_loss(logits, topi, mask=None, offsets=None, coef: float = 1.0):

@@ -26,7 +26,6 @@ from collections import OrderedDict
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import moe_f32 as F32
@@ -875,9 +874,6 @@ def _select_backward(ctx, dtopv, *_):
     return dz, *rest
 
 
-_select_backward_once = once_differentiable(_select_backward)
-
-
 class _SelectFn(torch.autograd.Function):
     """select_experts: topv differentiable w.r.t. the logits, the picks constants."""
 
@@ -893,9 +889,7 @@ class _SelectFn(torch.autograd.Function):
         ctx.mark_non_differentiable(topi, scores)
         return topv, topi, scores
 
-    @staticmethod
-    def backward(ctx, *grads):     # on the forward's device: autograd's thread has set it
-        return (_select_backward_once if torch.is_grad_enabled() else _select_backward)(ctx, *grads)
+    backward = staticmethod(L.once(_select_backward))     # on the forward's device: autograd's thread has set it
 
 
 def select_experts(logits, top_k, score="sigmoid", bias=None, groups=1, top_groups=1, group_best=2, renorm=True, scale=1.0,

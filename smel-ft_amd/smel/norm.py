@@ -27,7 +27,6 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -265,9 +264,6 @@ def _ln_backward(ctx, *grads):
     return dx, dx if add else None, dw, db, None, None
 
 
-_ln_backward_once = once_differentiable(_ln_backward)
-
-
 class _LayerNormFn(torch.autograd.Function):
     """forward(x, h, w, b, eps, the call's (columns, types)): y, or (s, y) with the residual addend h. Saved: the rows that
     the norm read and two fp32 numbers a row."""
@@ -281,9 +277,7 @@ class _LayerNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return y if h is None else (s, y)
 
-    @staticmethod
-    def backward(ctx, *grads):     # on the forward's device: autograd's thread has set it
-        return (_ln_backward_once if torch.is_grad_enabled() else _ln_backward)(ctx, *grads)
+    backward = staticmethod(_lib.once(_ln_backward))     # on the forward's device: autograd's thread has set it
 
 
 def _ln(x, h, w, b, eps):
@@ -434,9 +428,6 @@ def _sw_backward(ctx, ds, dy=None):
     return (dh if nh else None, dx, dw1, dw2, dg, dsc) + none
 
 
-_sw_backward_once = once_differentiable(_sw_backward)
-
-
 class _SandwichFn(torch.autograd.Function):
     """forward(h, x, w1, w2, gate, scale, pre, keep h, the call's numbers): s, or (s, y) with ``pre``. Saved: x's rows, s (pre), the
     gate, two fp32 numbers a row, and h for a trained scale."""
@@ -449,9 +440,7 @@ class _SandwichFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return (s, y) if pre else s
 
-    @staticmethod
-    def backward(ctx, *grads):     # on the forward's device: autograd's thread has set it
-        return (_sw_backward_once if torch.is_grad_enabled() else _sw_backward)(ctx, *grads)
+    backward = staticmethod(_lib.once(_sw_backward))     # on the forward's device: autograd's thread has set it
 
 
 def _sandwich(h, x, w1, w2, eps, plus_one, gate, gate_act, scale, pre):
