@@ -925,6 +925,7 @@ class _RouterLogitsFn(torch.autograd.Function):
         return lg[:, :E]
 
     @staticmethod
+    @L.once
     def backward(ctx, dlogits):
         gate_w, = ctx.saved_tensors
         T, E = dlogits.shape

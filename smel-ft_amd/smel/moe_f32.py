@@ -302,6 +302,7 @@ class RouterLogitsFn(torch.autograd.Function):
         return logits
 
     @staticmethod
+    @L.once
     def backward(ctx, dlogits):
         gate_w, = ctx.saved_tensors
         T, (E, H) = dlogits.shape[0], gate_w.shape
