@@ -361,6 +361,7 @@ class _ChunkedCE(torch.autograd.Function):
         return total
 
     @staticmethod
+    @L.once
     def backward(ctx, go):
         g = ctx.grad
         ctx.grad = None

@@ -690,6 +690,7 @@ class _RouteFn(torch.autograd.Function):
         return (probs, topv, topi, lg[:, :E]) if with_logits else (probs, topv, topi)
 
     @staticmethod
+    @L.once
     def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
         probs, topi32, gate_w = ctx.saved_tensors
         T, E = probs.shape
@@ -763,6 +764,7 @@ class _RouteGemma4Fn(torch.autograd.Function):
         return (probs, topv, topi, lg[:, :E]) if with_logits else (probs, topv, topi)
 
     @staticmethod
+    @L.once
     def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
         if dtopv is None and dlogits is None:
             return None, None, None, None, None, None, None
@@ -1373,6 +1375,7 @@ class _MoELayerFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @L.once
     def backward(ctx, dout):
         c = ctx.c
         split = getattr(c, "split", None)
@@ -1408,6 +1411,7 @@ class _RoutedFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @L.once
     def backward(ctx, dout):
         c = ctx.c
         dx, dtopv, grads = _backward_pipeline(c, dout, router=None)
@@ -1624,6 +1628,7 @@ class _MLPFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @L.once
     def backward(ctx, dy):
         sv, (w_gu_t, w_dn_t), lora = ctx.sv, ctx.w, ctx.lora
         ones = torch.ones(sv.x.shape[0], dtype=torch.float32, device=dy.device)   # row weight 1
@@ -1854,6 +1859,7 @@ class FrozenExpertsFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @L.once
     def backward(ctx, dy):
         if ctx.plan_f32 is not None:
             keep, ctx.plan_f32 = ctx.plan_f32, None

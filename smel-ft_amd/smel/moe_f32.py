@@ -262,6 +262,7 @@ class RouteFn(torch.autograd.Function):
         return (probs, topv, topi, logits) if with_logits else (probs, topv, topi)
 
     @staticmethod
+    @L.once
     def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
         if dtopv is None and dlogits is None:
             return None, None, None, None
@@ -343,6 +344,7 @@ class RouteGemma4Fn(torch.autograd.Function):
         return (probs, topv, topi, logits) if with_logits else (probs, topv, topi)
 
     @staticmethod
+    @L.once
     def backward(ctx, dprobs, dtopv, dtopi, dlogits=None):
         if dtopv is None and dlogits is None:
             return None, None, None, None, None, None, None
@@ -412,6 +414,7 @@ class RoutedFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @L.once
     def backward(ctx, dout):
         sv, ys, tv, inv, offsets, tl, w_gu, w_dn, lw, s, I, _hold, ex, lora, T, K = ctx.keep
         ctx.keep = None
@@ -462,6 +465,7 @@ class MLPFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @L.once
     def backward(ctx, dy):
         sv, tl, offs, jobs, I, w_gu, w_dn, split, lw, s, lora, act_name, _hold = ctx.keep
         ctx.keep = None
@@ -493,6 +497,7 @@ class GateAddFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @L.once
     def backward(ctx, dout):
         y, sl, w_sg = ctx.saved_tensors
         T, H = y.shape

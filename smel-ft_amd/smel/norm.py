@@ -103,6 +103,7 @@ class _NormFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_lib.once
     def backward(ctx, *grads):
         p, stream = _lib.ptr, _lib.stream()
         if ctx.kind == _RMS:
