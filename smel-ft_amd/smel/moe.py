@@ -668,6 +668,13 @@ def _bank_sources(fz):
 # ------------------------------------------------------------------------------------------------ router
 
 
+def _router_check(x, w):
+    """The rows and the router's weight of a call: [T, H] and [E, H] on one GPU."""
+    L.one_device(x, w)
+    if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1]:
+        raise ValueError(f"a router takes rows [T, H] and a router weight [E, H], got {tuple(x.shape)} and {tuple(w.shape)}")
+
+
 class _RouteFn(torch.autograd.Function):
     """route (smel/moe.py:162-167) with topv differentiable w.r.t. x through the router softmax; with_logits: the rounded
     logits as a fourth result, differentiable too (their gradient joins topv's before the router GEMM's backward)."""
@@ -731,7 +738,7 @@ def route(x2d, gate_w, top_k, with_logits=False):
     """smel/moe.py:162-167 -> (probs fp32 [T,E], topv [T,K] renormalised in the logits' dtype, topi int64 [T,K]).
     bf16 or fp32 activations (the fp32 path: every product an fp32 MFMA). with_logits: (..., logits [T,E] in the
     activations' dtype), differentiable w.r.t. x2d, for losses on the router (``smel.loss.balance_loss``)."""
-    L.require_device(x2d, gate_w)
+    _router_check(x2d, gate_w)
     if x2d.dtype == torch.float32:
         return F32.RouteFn.apply(F32.f32(x2d), F32.f32(gate_w, "gate_w"), int(top_k), bool(with_logits))
     if _bf16_limit(x2d.shape[-1]) is not None:
@@ -793,7 +800,11 @@ def route_gemma4(h, W, top_k, eps, with_logits=False):
     """Gemma 4 router on the residual stream (smel/moe.py:170-180) -> (probs fp32 [T,E], topv fp32 [T,K] =
     renormalised top-k x per_expert_scale, topi int64 [T,K]): weightless RMSNorm, x router.scale x H^-0.5, logits,
     softmax, top-k, renorm, scale, as HIP kernels (differentiable w.r.t. h); with_logits: (..., logits) as in ``route``."""
-    L.require_device(h)
+    _router_check(h, W["router.proj.weight"])
+    for name, n in (("router.scale", h.shape[1]), ("router.per_expert_scale", W["router.proj.weight"].shape[0])):
+        L.one_device(h, W[name])
+        if W[name].numel() != n:
+            raise ValueError(f"{name} holds {W[name].numel()} values, {n} are needed")
     k, eps, wl = int(top_k), float(eps), bool(with_logits)
     if h.dtype == torch.bfloat16 and _bf16_limit(h.shape[-1]) is not None:
         probs, topv, topi, *lg = F32.RouteGemma4Fn.apply(
@@ -955,7 +966,7 @@ def route_grouped(x2d, gate_w, top_k, score="sigmoid", bias=None, groups=1, top_
     """``route`` with the choice of ``select_experts``: (scores fp32 [T, E], topv fp32 [T, K], topi int64 [T, K]), with_logits:
     (..., logits [T, E]), differentiable w.r.t. x2d; what ``routed_experts`` and the stats hook take. bf16 (logits rounded to bf16, as
     ``route``'s) or fp32 activations."""
-    L.require_device(x2d, gate_w)
+    _router_check(x2d, gate_w)
     with L.on_device_of(x2d):
         logits = _router_logits(x2d, gate_w)
         topv, topi, scores = select_experts(logits, top_k, score, bias, groups, top_groups, group_best, renorm, scale, True)
