@@ -357,6 +357,12 @@ def forward_mode() -> bool:
     return getattr(_forward_ad, "_current_level", 0) >= 0
 
 
+def refuse_tangents(what: str, ts):
+    """Raises where a tensor carries a tangent, for functions that autograd does not see."""
+    if forward_mode() and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{what} has no rule for forward mode, and a tensor carries a tangent")
+
+
 _transforms_active = getattr(torch._C, "_are_functorch_transforms_active", None)
 
 

@@ -225,6 +225,7 @@ def _clip_call(grads, max_norm, norm_type, eps, inplace):
         return list(ts), torch.zeros((), dtype=torch.float32)
     if not first.is_cuda:
         _lib.one_device(first)
+    _lib.refuse_tangents(what, ts)
     jobs, outs, keep, back = array("q"), [], [], []
     add, put, codes, index, like = jobs.extend, outs.append, _ORTHO_DTYPES, first.get_device(), torch.empty_like
     copies = max_norm is not None and not inplace
