@@ -343,7 +343,8 @@ def _sw_check(h, x, w1, w2, gate, scale) -> tuple:
     weights = (w1, w2)
     if gate is not None:
         ok = ok and gate.device == dev and (gate.dtype is x.dtype or gate.dtype is torch.float32)
-        if gate.dim() == 1 and gate.shape[0] == n:      # of one row: whichever, they are the same
+        # of one row without leading dimensions: per channel where its dtype is the weights', whose gate that has to be
+        if gate.dim() == 1 and gate.shape[0] == n and (x.dim() > 1 or all(w is None or w.dtype is gate.dtype for w in weights)):
             kind, weights = _GATE_CHANNEL, (w1, w2, gate.contiguous() if ok else None)
         elif gate.shape == shape and (n != 1 or gate.dtype is x.dtype):
             kind = _GATE_FULL
@@ -466,7 +467,8 @@ def post_rmsnorm(h, x, w, eps, plus_one=False, gate=None, gate_act=None, scale=N
 
     h, x [..., n]: the residual stream and the block's output, bf16, fp16 or fp32 rows of any stride. w [n] (None: 1; 1 + w with
     ``plus_one``), of the rows' dtype or fp32. gate: a value per channel [n] (the weights' dtype), per token [..., 1] (the rows' dtype
-    or fp32) or per element [..., n] (the rows' dtype); ``gate_act`` "sigmoid": the gate's sigmoid. scale: a number or one element on
+    or fp32) or per element [..., n] (the rows' dtype); of a lone row [n], a gate [n] is the one whose dtype it has. ``gate_act``
+    "sigmoid": the gate's sigmoid. scale: a number or one element on
     the GPU. Backward gives every gradient that is asked for: of h, x, w, the gate and the scale."""
     return _sandwich(h, x, w, None, eps, plus_one, gate, gate_act, scale, False)
 
