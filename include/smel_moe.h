@@ -417,7 +417,8 @@ int smel_router_logits(const uint16_t* x, const uint16_t* gate_w, int64_t T, int
  *   groups > 1: the E experts are `groups` runs of E / groups neighbours; a group counts with the sum of its group_best (1 or 2)
  *   largest c, and only the top_groups best groups' experts can be picked
  *   topi [T][K]: the K largest c, descending (equal ones, and equal groups: the lower index first; a NaN counts as -infinity)
- *   topv [T][K]: w_k = scale s_k / (sum of the K + 1e-20) (renorm) or scale s_k, s_k = s[topi_k] without the bias
+ *   topv [T][K]: w_k = scale s_k / (sum of the K + 1e-20) (renorm) or scale s_k, s_k = s[topi_k] without the bias: the numbers that
+ *   were compared, and that `scores` holds, bit for bit (a sigmoid below 2^-126 is 0)
  * The ids are always K different ones of [0, E), whatever the logits hold. A softmax row without a logit above -infinity has
  * scores 0. scores (may be null): s [T][E]. stats (may be null; softmax with a backward): a row's maximum and the sum of e^(z - maximum)
  * (infinity for such a row), [T][2].

@@ -85,9 +85,21 @@ SMEL_DEV uint32_t max_lanes(uint32_t v) {
   if constexpr (LT == 64) return wave_max_u32(v);
   return over_lanes<LT>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
-// for the comparisons, and (rounded correctly but for e^-z) for the weights and their gradients
-SMEL_DEV float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.f + expf(-z)); }
-SMEL_DEV float weight_of(float z) { return 1.f / (1.f + expf(-z)); }
+// One score for the comparisons, the scores handed out, the weights and their gradients: the lower index of a tie and the weights'
+// order are those of the numbers that a caller sees. Both are the rounded quotient in a few instructions (32768 tokens of 256 experts,
+// events: 27.6 us, with divisions 28.0, with two scores, the compared ones from the bare reciprocal, 27.1).
+// 1 / (1 + e^-z): one step of Newton's on the hardware's reciprocal is the quotient for every d below 2^126 (all 2^23 mantissas
+// compared at seven exponents); 0 from there on, z < -87.3. An infinite d must not meet the reciprocal's 0; NaN stays NaN in r.
+SMEL_DEV float sigmoid_of(float z) {
+  const float d = 1.f + expf(-z), r = __builtin_amdgcn_rcpf(d);
+  return fmaf(fmaf(-fminf(d, 0x1.fffffep127f), r, 1.f), r, r);
+}
+// e / den from den's rounded reciprocal (the quotient's bits from e = 2^-100 on); den: a softmax's sum, or for a row without a logit above -infinity (e = 0) one
+SMEL_DEV float share_of(float e, float den, float inv) {
+  const float q = e * inv;
+  return fmaf(fmaf(-q, den, e), inv, q);
+}
+SMEL_DEV float den_of(float total) { return total == INFINITY ? 1.f : total; }
 
 // n (<= N) values from p on, zeros behind; all of them at once where there are N
 template <int DT, int N>
@@ -168,7 +180,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   float s[N], bias[N];
   run_of<DT, N>(p.z, row * p.ldl + e0, n, s);
   if (p.bias) run_of<2, N>(p.bias, e0, n, bias);
-  float m = 0.f, total = 1.f;
+  float m = 0.f, den = 1.f, inv = 1.f;
   if (p.score == 0) {
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = sigmoid_of(s[j]);
@@ -183,10 +195,10 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
     for (int j = 0; j < N; ++j) s[j] = expf(s[j] - m);
     float sum = row_total<LT, N>(s, n, p.E);
     if (sum == 0.f) sum = INFINITY;     // no logit above -infinity: scores 0
-    total = sum;
-    const float inv = 1.f / sum;
+    den = den_of(sum);
+    inv = 1.f / den;
 #pragma unroll
-    for (int j = 0; j < N; ++j) s[j] *= inv;
+    for (int j = 0; j < N; ++j) s[j] = share_of(s[j], den, inv);
     if (p.stats && live && li == 0) {
       p.stats[2 * t] = m;
       p.stats[2 * t + 1] = sum;
@@ -267,7 +279,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelArgs p) {
   float w = 0.f;
   if (li < p.K) {
     const float z = logit_at<DT>(p.z, row * p.ldl + id);
-    w = p.score == 0 ? weight_of(z) : expf(z - m) / total;
+    w = p.score == 0 ? sigmoid_of(z) : share_of(expf(z - m), den, inv);
   }
   const float sum = sum_lanes<16>(w);   // K <= 16
   if (live && li < p.K) {
@@ -319,11 +331,12 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelBwdArgs p) {
       d = p.scale * p.dtopv[row * p.K + li];
       const float zk = logit_at<DT>(p.z, row * p.ldl + id);
       if (p.score == 0) {
-        s = weight_of(zk);
+        s = sigmoid_of(zk);
         const float q = expf(-fabsf(zk)), a = __builtin_amdgcn_rcpf(1.f + q);
         slope = q * a * a;
       } else {
-        s = expf(zk - m) / total;
+        const float den = den_of(total);
+        s = share_of(expf(zk - m), den, 1.f / den);
       }
     }
   }
