@@ -260,7 +260,7 @@ def _clip_call(grads, max_norm, norm_type, eps, inplace):
         need = _lib.load().smel_clip_ws(addr, n)
         ws, norm = first.new_empty(need, dtype=torch.uint8), first.new_empty((), dtype=torch.float32)
         if max_norm is not None:
-            _lib.call("smel_clip_grads", addr, n, kind, float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), need,
+            _lib.call("smel_clip_grads", addr, n, kind, max_norm, float(eps), norm.data_ptr(), ws.data_ptr(), need,
                       _lib.stream())
         else:
             _lib.call("smel_grad_norm", addr, n, kind, norm.data_ptr(), ws.data_ptr(), need, _lib.stream())
@@ -282,7 +282,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6
     """(clipped, norm): every tensor times min(1, max_norm / (norm + eps)) with ``norm`` the norm of all of them together, as
     ``grad_norm`` gives it; new tensors of the same shapes and dtypes, without gradients (None stays None), one tensor for one tensor.
     A norm that is infinite or NaN gives what the product with that factor gives."""
-    outs, norm = _clip_call(grads, max_norm, norm_type, eps, False)
+    outs, norm = _clip_call(grads, float(max_norm), norm_type, eps, False)
     return (outs[0] if isinstance(grads, torch.Tensor) else outs), norm
 
 
@@ -290,7 +290,7 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-
     """``clip_grads`` in place; returns the norm before. Tensors that are within the norm already are not written. The tensors must not
     overlap (dense ones that do, one given twice among them, are refused before anything is written; strided ones go through copies).
     Autograd sees the change, as of any in-place operation."""
-    return _clip_call(grads, max_norm, norm_type, eps, True)[1]
+    return _clip_call(grads, float(max_norm), norm_type, eps, True)[1]
 
 
 class LayerLoRA(nn.Module):
