@@ -8,7 +8,7 @@
 //   sum(v dS) = sum(v e) - r2 m2 sum(v shat)
 // so a row costs one barrier. A gate per token and the scale are factors of the whole row: they stay outside the sums.
 //
-// Layout: rows.h's chunks of 8, `lpr` threads a row (a power of two up to 64, or the block). Blocks of the backward walk over
+// Layout: rows.h's chunks of 8, `lpr` threads a row (a power of two, forward up to 64, backward up to 256, or the block). Blocks of the backward walk over
 // the rows, the weights and their sums in registers; the blocks' sums are added by a second launch in block order. No atomics: every
 // result repeats bit for bit.
 // HBM-bound, us at 32749 x 2048 bf16 (a tensor: 134 MB; a copy reaches 5.4 TB/s): forward 95 to 101 (5.3 to 5.6 TB/s), with a gate per

@@ -272,9 +272,9 @@ def _clip_call(grads, max_norm, norm_type, eps, inplace):
 
 
 def grad_norm(grads, norm_type: float = 2.0):
-    """The norm of all values of all tensors together (an fp32 scalar on their GPU; no host synchronisation): norm_type 2
-    (sums in 64 bits) or inf (the largest magnitude). ``grads``: a tensor or a sequence (bf16, fp16, fp32; None entries are passed
-    over). A NaN anywhere gives NaN."""
+    """The norm of all values of all tensors together (an fp32 scalar on their GPU, on the host where there is no tensor; a constant to
+    autograd; no host synchronisation): norm_type 2 (sums in 64 bits) or inf (the largest magnitude). ``grads``: a tensor or a sequence
+    (bf16, fp16, fp32; None entries are passed over). A NaN anywhere gives NaN."""
     return _clip_call(grads, None, norm_type, 0.0, False)[1]
 
 
@@ -287,8 +287,9 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6
 
 
 def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6):
-    """``clip_grads`` in place; returns the norm before. Tensors that are within the norm already are not written. The tensors must not
-    overlap (dense ones that do, one given twice among them, are refused before anything is written; strided ones go through copies).
+    """``clip_grads`` in place; returns the norm before. Dense tensors that are within the norm already are not written. The tensors must
+    not overlap (dense ones that do, one given twice among them, are refused before anything is written; strided ones go through
+    copies, and get their own values back where the factor is 1).
     Autograd sees the change, as of any in-place operation."""
     return _clip_call(grads, float(max_norm), norm_type, eps, True)[1]
 
