@@ -100,3 +100,17 @@ def test_weights_are_the_scores(dt):
         assert torch.equal(topv, 4 * s.gather(1, topi)) and (topv[:, 1:] <= topv[:, :-1]).all()
         topv = select_experts(z.to(DEV), 8, score)[0]
         assert (topv[:, 1:] <= topv[:, :-1]).all()
+
+
+def test_not_a_number_stays():
+    """A NaN logit's sigmoid is NaN (and counts as -infinity), a softmax row with one, or with an infinity, is NaN throughout; all else
+    is a number. Infinite and far logits have the scores 0 and 1."""
+    from smel.moe import select_experts
+    for T in (40, 4101):
+        z, _, _, _, _ = inputs("special", T, 64, 9)
+        topv, topi, s = (t.cpu() for t in select_experts(z.to(DEV), 4, renorm=False, with_scores=True))
+        assert torch.equal(s.isnan(), z.isnan()) and (s[z < -104] == 0).all() and (s[z > 17] == 1).all() and (s[z == 0] == 0.5).all()
+        some = (~z.isnan()).sum(1) >= 4
+        assert not topv[some].isnan().any() and topv[z.isnan().all(1)].isnan().all()
+        s = select_experts(z.to(DEV), 4, "softmax", with_scores=True)[2].cpu()
+        assert torch.equal(s.isnan(), (z.isnan() | (z == math.inf)).any(1, keepdim=True).expand(T, 64))
