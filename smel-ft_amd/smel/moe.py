@@ -1727,7 +1727,7 @@ def _shared_weights(W: dict, store: dict | None = None):
 def moe_forward(x2d, W, ex: LayerExperts, top_k: int, lora_layer=None, stats=None):
     """x2d [N, H] (already post-attention-normed) -> [N, H] bf16 (smel/moe.py:255-263): router, stats hook, routed
     experts and the shared expert, fused into one forward/backward pipeline."""
-    L.require_device(x2d)
+    _router_check(x2d, W["mlp.gate.weight"])
     if x2d.dtype == torch.float32:
         return _moe_forward_f32(x2d, W, ex, top_k, lora_layer, stats)
     _check_bank(ex)

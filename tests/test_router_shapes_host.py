@@ -41,3 +41,12 @@ def test_devices():
     for f in (moe.route, moe.route_grouped):
         with pytest.raises(ValueError, match="one call on cuda:0 and cuda:1"):
             f(_On("cuda:0"), _On("cuda:1"), 2)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_layer(monkeypatch, dt):
+    monkeypatch.setattr(_lib, "require_device", lambda *ts: None)
+    monkeypatch.setattr(_lib, "one_device", lambda *ts: None)
+    for H in (64, 256):
+        with pytest.raises(ValueError, match="router weight"):
+            moe.moe_forward(torch.empty(4, 128, dtype=dt, **M), {"mlp.gate.weight": torch.empty(16, H, dtype=dt, **M)}, None, 2)
